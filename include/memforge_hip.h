@@ -282,6 +282,47 @@ int mf_paged_attention_kv_write(const void* q, int64_t q_stride_row, int64_t q_s
                                 int64_t num_merges, const int32_t* device_counts,
                                 float* partials, int64_t partials_floats, mf_stream_t stream);
 
+/* Attention with scored keys: what mf_paged_attention, _counted and _kv_write
+ * compute, with the scores of row r, query head h and key k (of sequence s)
+ *     t = scale * q.k
+ *     t = softcap * tanh(t / softcap)                    softcap > 0
+ *     t = t - slopes[h] * |positions[r] - k|             slopes non-NULL
+ * and with key k visible to row r when k < kv_lens[s], k >= first_keys[s]
+ * (NULL: 0), and k <= positions[r] or k < prefix_lens[s] (NULL: 0). A row that
+ * sees no key gets zeros. Keys below first_keys[s] and from kv_lens[s] on may
+ * hold anything, NaN included. A document mask runs each document's rows as a
+ * sequence of their own over the same block table, first_keys the document's
+ * first position; rows before the prefix's end see the whole prefix.
+ * softcap: finite, 0 for none; so small or large against the scale that their
+ * quotient leaves fp32's normal numbers is MF_ERR_ARG. slopes: fp32[num_q_heads],
+ * first_keys / prefix_lens: int32 per sequence, all on the device.
+ * slot_mapping non-NULL: the new rows are written in the same call, as
+ * mf_paged_attention_kv_write does (pool_lens and row_map are NULL then);
+ * device_counts non-NULL: the counts are capacities, as in
+ * mf_paged_attention_counted. Plans are mf_attention_plan_device's; a plan made
+ * without a device (mf_attention_plan) may leave out tiles that only a prefix
+ * makes visible. Where first_keys is set, an item's ranges may start at the tile
+ * of its sequence's first key. No counterpart in the reference, whose attention
+ * is the plain one. */
+typedef struct mf_scoring {
+    float softcap;
+    const float* slopes;
+    const int32_t* first_keys;
+    const int32_t* prefix_lens;
+} mf_scoring;
+int mf_paged_attention_scored(const mf_scoring* scoring, const void* q, int64_t q_stride_row, int64_t q_stride_head,
+                              void* out, int64_t out_stride_row, int64_t out_stride_head, int dtype, void* k_pool,
+                              void* v_pool, int64_t pool_stride_block, int64_t pool_stride_slot,
+                              int64_t pool_stride_head, int block_size, const int32_t* block_tables,
+                              int64_t block_table_stride, const int32_t* cu_seqlens, const int32_t* kv_lens,
+                              const int64_t* positions, const int32_t* row_map, const int32_t* pool_lens,
+                              const void* new_k, const void* new_v, int64_t new_stride_row, int64_t new_stride_head,
+                              const int64_t* slot_mapping, int64_t num_new_rows, int64_t num_slots, int num_q_heads,
+                              int num_kv_heads, int head_dim, float scale, const int32_t* plan_items,
+                              int64_t num_items_narrow, int64_t num_items_wide, const int32_t* plan_merges,
+                              int64_t num_merges, const int32_t* device_counts, float* partials,
+                              int64_t partials_floats, mf_stream_t stream);
+
 /* mf_paged_attention without a partials buffer or merge counters, so that
  * the call allocates nothing. No counterpart in the reference: it is for
  * callers that cannot allocate device memory (code under HIP graph capture,

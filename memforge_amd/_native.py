@@ -10,6 +10,7 @@ runs on the MI355X or not at all.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from collections import OrderedDict
 from dataclasses import dataclass
@@ -68,6 +69,10 @@ _SIGNATURES = {
     "mf_paged_attention_kv_write": (_c_int, [
         _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_int, _vp, _vp, _c_i64, _c_i64, _c_i64,
         _c_int, _vp, _c_i64, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64,
+        _c_int, _c_int, _c_int, _c_f32, _vp, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp, _c_i64, _vp]),
+    "mf_paged_attention_scored": (_c_int, [
+        _vp, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_int, _vp, _vp, _c_i64, _c_i64, _c_i64,
+        _c_int, _vp, _c_i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64,
         _c_int, _c_int, _c_int, _c_f32, _vp, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp, _c_i64, _vp]),
     "mf_paged_attention_noalloc": (_c_int, [
         _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_int, _vp, _vp, _c_i64, _c_i64, _c_i64,
@@ -389,6 +394,63 @@ def upload(parts: Sequence[np.ndarray], device) -> List[torch.Tensor]:
     return _views(buf, arrs, offs)
 
 
+# ------------------------------------------------------------ scored attention
+
+class _ScoringStruct(ctypes.Structure):
+    _fields_ = [("softcap", _c_f32), ("slopes", _vp), ("first_keys", _vp), ("prefix_lens", _vp)]
+
+
+@dataclass(frozen=True)
+class Scoring:
+    """What a model does to the scores of its attention (mf_scoring), for
+    ``paged_attention`` and ``paged_attention_kv_write``:
+
+    * ``softcap``: scores t become ``softcap * tanh(t / softcap)``; 0 for none.
+    * ``slopes`` (fp32, one per query head): then ``slopes[h] * |position - key|``
+      is subtracted.
+    * ``first_keys`` (int32, one per sequence of the call): keys before it are not
+      seen. A document mask runs every document's rows as a sequence of their own
+      over the same block table.
+    * ``prefix_lens`` (int32, one per sequence): keys before it are seen by every
+      row, those after the row's position too (from ``first_keys`` on).
+
+    A row that sees no key gets zeros. Plans for masked calls are made with the
+    same ``first_keys`` and ``prefix_lens`` as host lists (``plan_attention``)."""
+
+    softcap: float = 0.0
+    slopes: Optional[torch.Tensor] = None
+    first_keys: Optional[torch.Tensor] = None
+    prefix_lens: Optional[torch.Tensor] = None
+
+    def __post_init__(self):
+        cap = 0.0 if self.softcap is None else float(self.softcap)
+        if not 0.0 <= cap < float("inf"):
+            raise ValueError(f"softcap must be finite and not negative, got {self.softcap}")
+        object.__setattr__(self, "softcap", cap)
+
+    @property
+    def active(self) -> bool:
+        return self.softcap > 0.0 or self.slopes is not None or self.first_keys is not None \
+            or self.prefix_lens is not None
+
+    def struct(self, num_q_heads: int, num_seqs: int, device: torch.device) -> _ScoringStruct:
+        """The C structure, its tensors checked against the call."""
+        for name, x, dt, n in (("slopes", self.slopes, torch.float32, num_q_heads),
+                               ("first_keys", self.first_keys, torch.int32, num_seqs),
+                               ("prefix_lens", self.prefix_lens, torch.int32, num_seqs)):
+            if x is None:
+                continue
+            if x.dtype != dt or not x.is_contiguous() or x.numel() != n:
+                raise TypeError(f"{name} must be a contiguous {dt} tensor of {n}, got {x.dtype} {tuple(x.shape)}")
+            if x.device != device:
+                raise ValueError(f"{name} is on {x.device}, the query on {device}")
+        return _ScoringStruct(self.softcap, _ptr(self.slopes), _ptr(self.first_keys), _ptr(self.prefix_lens))
+
+
+def _scored(scoring: Optional[Scoring]) -> Optional[Scoring]:
+    return scoring if scoring is not None and scoring.active else None
+
+
 # ---------------------------------------------------------------- attention
 
 @dataclass
@@ -516,19 +578,47 @@ _PLAN_CACHE: "OrderedDict[tuple, tuple]" = OrderedDict()
 PLAN_CACHE_SIZE = 64
 
 
+def _plan_from_first_keys(plan, cu_seqlens: Sequence[int], kv_lens: Sequence[int], first_keys: Sequence[int]):
+    """``plan(kv_lens)``'s arrays for sequences whose keys before ``first_keys``
+    no row sees: planned as contexts that begin at the first key's 16-key tile,
+    then moved there. A sequence all of whose keys are hidden keeps its last
+    tile, so that its rows are written (with zeros)."""
+    kv = np.asarray(kv_lens, dtype=np.int64)
+    tile = np.clip(np.asarray(first_keys, dtype=np.int64), 0, np.maximum(kv - 1, 0)) // 16
+    items, merges, counts = plan((kv - 16 * tile).tolist())
+    items = items.copy()
+    live = items[:, 9] > 0
+    at = tile[items[:, 0]] * live
+    items[:, 4] += at.astype(np.int32)
+    items[:, 5] += at.astype(np.int32)
+    items[:, 10] += (16 * at).astype(np.int32)
+    return items, merges, counts
+
+
 def plan_host(cu_seqlens: Sequence[int], kv_lens: Sequence[int], num_q_heads: int, num_kv_heads: int,
               head_dim: int, dtype: torch.dtype, device=None, partition_tiles: int = 0,
-              decode_slices: bool = False) -> Tuple[np.ndarray, np.ndarray, np.ndarray, bool]:
+              decode_slices: bool = False, first_keys: Optional[Sequence[int]] = None,
+              prefix_lens: Optional[Sequence[int]] = None,
+              kv_bits: int = 16) -> Tuple[np.ndarray, np.ndarray, np.ndarray, bool]:
     """Host plan arrays (items or slices, merges, counts) and whether they are
     a slice plan. With ``decode_slices`` (the caller's launch has 16-token
     blocks, no row map and no in-flight keys) a decode step large enough to
     fill the GPU on ``device`` more than once gets a slice plan; every other
-    call, and an explicit ``partition_tiles``, the per-range plan."""
+    call, and an explicit ``partition_tiles``, the per-range plan.
+    ``first_keys`` / ``prefix_lens`` (per sequence): the masks of a scored call
+    (``Scoring``); tiles below a sequence's first key are not planned. ``kv_bits``:
+    4 for a pool held in 4 bits."""
     on_gpu = partition_tiles <= 0 and device is not None and torch.device(device).type == "cuda"
-    slices = decode_slices and on_gpu
+    masked = first_keys is not None or prefix_lens is not None
+    for name, x in (("first_keys", first_keys), ("prefix_lens", prefix_lens)):
+        if x is not None and len(x) != len(kv_lens):
+            raise ValueError(f"{len(x)} {name} for {len(kv_lens)} sequences")
+    slices = decode_slices and on_gpu and not masked and kv_bits == 16
     cus = device_cus(device) if on_gpu else 0
+    firsts = None if first_keys is None else tuple(int(x) for x in first_keys)
+    prefixes = None if prefix_lens is None else tuple(int(x) for x in prefix_lens)
     key = (tuple(int(x) for x in cu_seqlens), tuple(int(x) for x in kv_lens), num_q_heads, num_kv_heads,
-           head_dim, dtype, partition_tiles, cus, slices)
+           head_dim, dtype, partition_tiles, cus, slices, firsts, prefixes, kv_bits)
     hit = _PLAN_CACHE.get(key)
     if hit is not None:
         _PLAN_CACHE.move_to_end(key)
@@ -537,8 +627,12 @@ def plan_host(cu_seqlens: Sequence[int], kv_lens: Sequence[int], num_q_heads: in
     if made is not None:
         out = (*made, True)
     else:
-        out = (*plan_attention_host(cu_seqlens, kv_lens, num_q_heads, num_kv_heads, head_dim, dtype,
-                                    partition_tiles, cus), False)
+        def plan(lens):
+            return plan_attention_host(cu_seqlens, lens, num_q_heads, num_kv_heads, head_dim, dtype,
+                                       partition_tiles, cus)
+
+        out = (*(plan(kv_lens) if firsts is None else _plan_from_first_keys(plan, cu_seqlens, kv_lens, firsts)),
+               False)
     for a in out[:3]:
         a.flags.writeable = False
     _PLAN_CACHE[key] = out
@@ -549,10 +643,13 @@ def plan_host(cu_seqlens: Sequence[int], kv_lens: Sequence[int], num_q_heads: in
 
 def plan_attention(cu_seqlens: Sequence[int], kv_lens: Sequence[int], num_q_heads: int,
                    num_kv_heads: int, head_dim: int, dtype: torch.dtype, device,
-                   partition_tiles: int = 0, decode_slices: bool = False) -> AttentionPlan:
+                   partition_tiles: int = 0, decode_slices: bool = False,
+                   first_keys: Optional[Sequence[int]] = None, prefix_lens: Optional[Sequence[int]] = None,
+                   kv_bits: int = 16) -> AttentionPlan:
     """A plan for ``paged_attention`` (``plan_host``, then one upload)."""
     items, merges, counts, sliced = plan_host(cu_seqlens, kv_lens, num_q_heads, num_kv_heads, head_dim, dtype,
-                                              device, partition_tiles, decode_slices)
+                                              device, partition_tiles, decode_slices, first_keys, prefix_lens,
+                                              kv_bits)
     dev_items, dev_merges = upload(plan_upload_parts(items, merges), device)
     return plan_from_parts(items, merges, counts, dev_items, dev_merges, sliced)
 
@@ -659,8 +756,11 @@ def paged_attention(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: PoolView
                     new_k_rows: Optional[torch.Tensor] = None,
                     new_v_rows: Optional[torch.Tensor] = None,
                     partials: Optional[torch.Tensor] = None,
-                    counters: Optional[torch.Tensor] = None, fused_merge: bool = False) -> None:
+                    counters: Optional[torch.Tensor] = None, fused_merge: bool = False,
+                    scoring: Optional[Scoring] = None) -> None:
     """Varlen paged attention into ``out_rows`` ((rows, Hq, D) views, device).
+    ``scoring``: capped, biased or masked scores (mf_paged_attention_scored;
+    per-range plans, no fused merge).
 
     Split-K partitions are merged by a separate merge kernel; with
     ``fused_merge`` the attention kernel merges them itself (the last partition
@@ -677,6 +777,12 @@ def paged_attention(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: PoolView
         if t.dtype != dt or not t.is_contiguous():
             raise TypeError(f"{name} must be a contiguous {dt} tensor")
     Hq, D = q_rows.shape[1], q_rows.shape[2]
+    if _scored(scoring) is not None:
+        if fused_merge:
+            raise ValueError("scored attention takes no fused merge")
+        return _paged_attention_scored(scoring, q_rows, out_rows, pool, block_tables, cu_seqlens, kv_lens, positions,
+                                       plan, scale, num_kv_heads, row_map, pool_lens, new_k_rows, new_v_rows,
+                                       partials=partials)
     if isinstance(plan, CountedPlan):
         return _paged_attention_counted(q_rows, out_rows, pool, block_tables, cu_seqlens, kv_lens, positions,
                                         plan, scale, num_kv_heads, row_map, pool_lens, new_k_rows, new_v_rows)
@@ -724,11 +830,64 @@ def paged_attention(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: PoolView
     ), "mf_paged_attention")
 
 
+class _Plan:
+    """A plan's launch arguments: counts or capacities, the live counts and the partials."""
+
+    __slots__ = ("narrow", "wide", "merges", "counts", "partials")
+
+    def __init__(self, plan, device, partials: Optional[torch.Tensor] = None):
+        if isinstance(plan, CountedPlan):
+            self.narrow, self.wide, self.merges = plan.cap_narrow, plan.cap_wide, plan.cap_merges
+            self.counts, self.partials = plan.counts, plan.partials
+            return
+        if plan.sliced:
+            raise ValueError("scored attention takes per-range plans (mf_attention_plan)")
+        self.narrow, self.wide, self.merges = plan.n_narrow, plan.n_wide, plan.n_merges
+        self.counts = None
+        self.partials = partials if partials is not None else _WORKSPACE.partials(plan.partials_floats, device)
+        if self.partials is not None and self.partials.numel() < plan.partials_floats:
+            raise ValueError(f"the plan needs {plan.partials_floats} partial floats, got {self.partials.numel()}")
+
+
+def _on(device: torch.device):
+    """The device's context, entered only when another device is current."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _paged_attention_scored(scoring: Scoring, q_rows, out_rows, pool, block_tables, cu_seqlens, kv_lens, positions,
+                            plan, scale, num_kv_heads, row_map=None, pool_lens=None, nk=None, nv=None,
+                            slot_mapping=None, partials=None) -> None:
+    if pool_lens is not None:
+        if nk is None or nv is None:
+            raise ValueError("pool_lens needs the in-flight new_k_rows/new_v_rows")
+        require_device(pool_lens, nk, nv)
+        if not same_layout(nk, nv):
+            raise ValueError("in-flight K and V rows must share strides")
+    dev = q_rows.device
+    p = _Plan(plan, dev, partials)
+    mods = scoring.struct(q_rows.shape[1], kv_lens.numel(), dev)
+    bt_stride = block_tables.shape[1] if block_tables.dim() == 2 else 0
+    with _on(dev):
+        _check(lib().mf_paged_attention_scored(
+            ctypes.addressof(mods), _ptr(q_rows), q_rows.stride(0), q_rows.stride(1),
+            _ptr(out_rows), out_rows.stride(0), out_rows.stride(1),
+            dtype_code(q_rows.dtype), _ptr(pool.k), _ptr(pool.v),
+            pool.stride_block, pool.stride_slot, pool.stride_head, pool.block_size,
+            _ptr(block_tables), bt_stride, _ptr(cu_seqlens), _ptr(kv_lens), _ptr(positions),
+            _ptr(row_map), _ptr(pool_lens), _ptr(nk), _ptr(nv),
+            nk.stride(0) if nk is not None else 0, nk.stride(1) if nk is not None else 0,
+            _ptr(slot_mapping), slot_mapping.numel() if slot_mapping is not None else 0, pool.num_slots,
+            q_rows.shape[1], num_kv_heads, q_rows.shape[2], float(scale),
+            _ptr(plan.items), p.narrow, p.wide, _ptr(plan.merges), p.merges, _ptr(p.counts),
+            _ptr(p.partials), p.partials.numel() if p.partials is not None else 0, _stream(dev),
+        ), "mf_paged_attention_scored")
+
+
 def paged_attention_kv_write(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: PoolView,
                              block_tables: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
                              positions: torch.Tensor, plan, scale: float, num_kv_heads: int,
                              new_k_rows: torch.Tensor, new_v_rows: torch.Tensor,
-                             slot_mapping: torch.Tensor) -> None:
+                             slot_mapping: torch.Tensor, scoring: Optional[Scoring] = None) -> None:
     """One launch for a packed step's KV write and its attention
     (mf_paged_attention_kv_write): rows ``new_k_rows``/``new_v_rows``
     ((rows, Hkv, D) views in the pool's dtype) go to the pool through
@@ -737,7 +896,7 @@ def paged_attention_kv_write(q_rows: torch.Tensor, out_rows: torch.Tensor, pool:
     pool. Row cu_seqlens[s] + i must be sequence s's new token at position
     kv_lens[s] - q_len[s] + i. ``plan`` is an AttentionPlan or a CountedPlan
     (graph capture). Same pool contents and output as ``kv_write`` followed by
-    ``paged_attention``."""
+    ``paged_attention`` (with the same ``scoring``)."""
     _rows_ok(q_rows, "q_rows")
     _rows_ok(out_rows, "out_rows")
     _rows_ok(new_k_rows, "new_k_rows")
@@ -769,6 +928,10 @@ def paged_attention_kv_write(q_rows: torch.Tensor, out_rows: torch.Tensor, pool:
         held = plan.items_host[: n_narrow + n_wide]
         if held.shape[0] and int((held[:, 8] + held[:, 9]).max()) > T:
             raise ValueError(f"the plan's sequences reach past the {T} new rows")
+    if _scored(scoring) is not None:
+        return _paged_attention_scored(scoring, q_rows, out_rows, pool, block_tables, cu_seqlens, kv_lens, positions,
+                                       plan, scale, num_kv_heads, nk=new_k_rows, nv=new_v_rows,
+                                       slot_mapping=slot_mapping)
     _check(lib().mf_paged_attention_kv_write(
         _ptr(q_rows), q_rows.stride(0), q_rows.stride(1),
         _ptr(out_rows), out_rows.stride(0), out_rows.stride(1),
@@ -859,12 +1022,15 @@ def paged_attention_packed(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: P
                            offsets: Sequence[int], num_seqs: int, bt_stride: int, counts: np.ndarray,
                            scale: float, num_kv_heads: int, has_row_map: bool, has_pool_lens: bool,
                            new_k_rows: Optional[torch.Tensor] = None,
-                           new_v_rows: Optional[torch.Tensor] = None, sliced: bool = False) -> None:
+                           new_v_rows: Optional[torch.Tensor] = None, sliced: bool = False,
+                           softcap: float = 0.0, slopes: Optional[torch.Tensor] = None,
+                           has_first_keys: bool = False, has_prefix_lens: bool = False) -> None:
     """mf_paged_attention on index arrays that one ``upload`` placed in the
     device buffer ``buf`` at ``offsets`` (int32 words, as ``_layout`` gives
     them): the padded block tables, the plan's items, its merges, cu_seqlens
     followed by kv_lens (``num_seqs`` + 1 and ``num_seqs`` int32), the int64
-    positions, then the row map and the pool lengths when present. The caller
+    positions, then the row map, the pool lengths, the first keys and the prefix
+    lengths (a scored call's masks, int32 per sequence) when present. The caller
     built all of them, so only the tensors it did not build (query, output,
     pool, in-flight rows) are checked, and the launch takes addresses inside
     ``buf`` instead of building a tensor view per array. ``sliced``: the plan
@@ -903,6 +1069,25 @@ def paged_attention_packed(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: P
         return
     row_map = addr[5] if has_row_map else None
     pool_lens = addr[5 + int(has_row_map)] if has_pool_lens else None
+    if softcap or slopes is not None or has_first_keys or has_prefix_lens:
+        at = 5 + int(has_row_map) + int(has_pool_lens)
+        mods = Scoring(softcap, slopes).struct(q_rows.shape[1], num_seqs, dev)
+        mods.first_keys = addr[at] if has_first_keys else None
+        mods.prefix_lens = addr[at + int(has_first_keys)] if has_prefix_lens else None
+        with _on(dev):
+            _check(lib().mf_paged_attention_scored(
+                ctypes.addressof(mods), _ptr(q_rows), q_rows.stride(0), q_rows.stride(1),
+                _ptr(out_rows), out_rows.stride(0), out_rows.stride(1),
+                dtype_code(q_rows.dtype), _ptr(pool.k), _ptr(pool.v),
+                pool.stride_block, pool.stride_slot, pool.stride_head, pool.block_size,
+                addr[0], bt_stride, addr[3], addr[3] + 4 * (num_seqs + 1), addr[4],
+                row_map, pool_lens, _ptr(nk), _ptr(nv),
+                nk.stride(0) if nk is not None else 0, nk.stride(1) if nk is not None else 0, None, 0, 0,
+                q_rows.shape[1], num_kv_heads, q_rows.shape[2], float(scale),
+                addr[1], n_narrow, n_wide, addr[2], n_merges, None,
+                _ptr(partials), partials.numel() if partials is not None else 0, _stream(dev),
+            ), "mf_paged_attention_scored")
+        return
     _check(lib().mf_paged_attention(
         _ptr(q_rows), q_rows.stride(0), q_rows.stride(1),
         _ptr(out_rows), out_rows.stride(0), out_rows.stride(1),

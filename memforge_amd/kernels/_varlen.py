@@ -49,32 +49,50 @@ def run_varlen(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: nat.PoolView,
                tables: Sequence[Sequence[int]], seq_ids: Sequence[int], positions: Sequence[int],
                scale: Optional[float], num_kv_heads: int, kv_lens: Optional[Sequence[int]] = None,
                pool_lens: Optional[Sequence[int]] = None, new_k_rows: Optional[torch.Tensor] = None,
-               new_v_rows: Optional[torch.Tensor] = None) -> None:
+               new_v_rows: Optional[torch.Tensor] = None, softcap: Optional[float] = None,
+               slopes: Optional[torch.Tensor] = None, doc_starts: Optional[Sequence[int]] = None,
+               prefix_lens: Optional[Sequence[int]] = None) -> None:
     """Attention for packed rows in any order.
 
     q_rows / out_rows: (T, Hq, D) device views. Row r belongs to table
     ``seq_ids[r]`` and sees keys 0..positions[r]. ``kv_lens`` (per table)
     defaults to max position + 1 of that table's rows. With ``pool_lens`` the
     keys at or above pool_lens[s] are the in-flight rows of sequence s's own
-    query rows, in position order.
+    query rows, in position order. ``softcap`` and ``slopes`` (fp32 per query
+    head, on the device) score as ``nat.Scoring`` says; row r sees no key before
+    ``doc_starts[r]``, and every row of table s the keys before
+    ``prefix_lens[s]``.
     """
     dev = q_rows.device
     T, hq, d = q_rows.shape
+    scoring = nat.Scoring(softcap or 0.0, slopes)
+    if (doc_starts is not None or prefix_lens is not None) and pool_lens is not None:
+        raise ValueError("masked attention reads every key from the pool")
+    if doc_starts is not None and (len(doc_starts) != T or any(x < 0 for x in doc_starts)):
+        raise ValueError(f"doc_starts must be {T} positions, none negative")
+    if prefix_lens is not None and (len(prefix_lens) != len(tables) or any(x < 0 for x in prefix_lens)):
+        raise ValueError(f"prefix_lens must be {len(tables)} lengths, none negative")
     groups = {}
     order: List[int] = []
+    firsts: List[int] = []
     for r, s in enumerate(seq_ids):
-        if s not in groups:
-            groups[s] = []
+        key = s if doc_starts is None else (s, int(doc_starts[r]))
+        if key not in groups:
+            groups[key] = []
             order.append(s)
-        groups[s].append(r)
+            firsts.append(0 if doc_starts is None else key[1])
+        groups[key].append(r)
     row_map: List[int] = []
     cu = [0]
     kvl: List[int] = []
-    for s in order:
-        rows = sorted(groups[s], key=lambda r: positions[r])
+    prefixes: List[int] = []
+    for s, members in zip(order, groups.values()):
+        rows = sorted(members, key=lambda r: positions[r])
         row_map.extend(rows)
         cu.append(len(row_map))
-        kvl.append(kv_lens[s] if kv_lens is not None else max(positions[r] for r in rows) + 1)
+        prefixes.append(int(prefix_lens[s]) if prefix_lens is not None else 0)
+        kvl.append(kv_lens[s] if kv_lens is not None else max(max(positions[r] for r in rows) + 1, prefixes[-1]))
+    masked_first, masked_prefix = any(firsts), any(prefixes)
     identity = row_map == list(range(T))
     # every block id the kernel will read must address the pool
     bs, nblocks = pool.block_size, pool.num_blocks
@@ -92,9 +110,11 @@ def run_varlen(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: nat.PoolView,
         _check_ids(tables, order, need, nblocks)
     nat.require_device(q_rows, out_rows, pool.k)
     # a large decode step on 16-token blocks runs as one round of slices
-    sliceable = identity and pool_lens is None and pool.block_size == 16
+    sliceable = identity and pool_lens is None and pool.block_size == 16 and not scoring.active
     items, merges, counts, sliced = nat.plan_host(cu, kvl, hq, num_kv_heads, d, q_rows.dtype, dev,
-                                                  decode_slices=sliceable)
+                                                  decode_slices=sliceable,
+                                                  first_keys=firsts if masked_first else None,
+                                                  prefix_lens=prefixes if masked_prefix else None)
     # tables, plan, cu/kv lengths, positions, row map and pool lengths cross
     # to the device in one copy (none when the same bytes crossed before on
     # this stream), and the launch addresses them inside that one buffer
@@ -105,10 +125,15 @@ def run_varlen(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: nat.PoolView,
         parts.append(np.asarray(row_map, dtype=np.int32))
     if pool_lens is not None:
         parts.append(np.asarray([pool_lens[s] for s in order], dtype=np.int32))
+    if masked_first:
+        parts.append(np.asarray(firsts, dtype=np.int32))
+    if masked_prefix:
+        parts.append(np.asarray(prefixes, dtype=np.int32))
     buf, offsets = nat.upload_packed_cached(parts, dev)
     nat.paged_attention_packed(
         q_rows, out_rows, pool, buf, offsets, len(order), tables_host.shape[1], counts,
         scale if scale is not None else 1.0 / math.sqrt(d), num_kv_heads,
         has_row_map=not identity, has_pool_lens=pool_lens is not None,
-        new_k_rows=new_k_rows, new_v_rows=new_v_rows, sliced=sliced,
+        new_k_rows=new_k_rows, new_v_rows=new_v_rows, sliced=sliced, softcap=scoring.softcap, slopes=slopes,
+        has_first_keys=masked_first, has_prefix_lens=masked_prefix,
     )

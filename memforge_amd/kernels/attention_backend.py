@@ -113,8 +113,10 @@ class _VarlenBinding:
         b.write_slots = write_slots
         return b
 
-    def meta(self, num_q_heads: int, head_dim: int, dtype: torch.dtype, device) -> dict:
-        if self._meta is not None:
+    def meta(self, num_q_heads: int, head_dim: int, dtype: torch.dtype, device, scored: bool = False) -> dict:
+        """``scored``: the layer caps its scores, which slice plans do not serve (a
+        pass whose earlier layers did not is planned again)."""
+        if self._meta is not None and not (scored and getattr(self._meta["plan"], "sliced", False)):
             return self._meta
         tables = [as_table_list(t) for t in self.block_tables]
         groups, order = {}, []
@@ -139,7 +141,7 @@ class _VarlenBinding:
                 )
         identity = row_map == list(range(len(row_map)))
         # a large decode step on 16-token blocks runs as one round of slices
-        sliceable = identity and self.pool_lens is None and self.pool.block_size == 16
+        sliceable = identity and self.pool_lens is None and self.pool.block_size == 16 and not scored
         items, merges, counts, sliced = nat.plan_host(cu, kvl, num_q_heads, self.pool.spec.num_kv_heads,
                                                       head_dim, dtype, device, decode_slices=sliceable)
         # everything the launch reads crosses to the device in one copy
@@ -216,7 +218,8 @@ def _mask_is_permissive(attention_mask: Optional[torch.Tensor]) -> bool:
     return bool(torch.all(attention_mask == 0))
 
 
-def _varlen_forward(module, query, key, value, scaling, binding: _VarlenBinding) -> torch.Tensor:
+def _varlen_forward(module, query, key, value, scaling, binding: _VarlenBinding,
+                    softcap: Optional[float] = None) -> torch.Tensor:
     if query.shape[0] != 1 or query.shape[2] != binding.num_rows:
         raise ValueError(
             f"varlen pass expected one packed row of {binding.num_rows} tokens, got {tuple(query.shape)}"
@@ -224,7 +227,8 @@ def _varlen_forward(module, query, key, value, scaling, binding: _VarlenBinding)
     _, hq, total, d = query.shape
     pool = binding.pool
     dtype = pool.key_pool.dtype
-    meta = binding.meta(hq, d, dtype, query.device)
+    scoring = nat.Scoring(softcap) if softcap else None
+    meta = binding.meta(hq, d, dtype, query.device, scored=scoring is not None)
     q_rows = query[0].to(dtype).permute(1, 0, 2)
     out = torch.empty((1, total, hq, d), dtype=dtype, device=query.device)
     layer = module.layer_idx
@@ -243,7 +247,7 @@ def _varlen_forward(module, query, key, value, scaling, binding: _VarlenBinding)
             q_rows, out[0], pool.layer_view(layer), meta["block_tables"], meta["cu_seqlens"],
             meta["kv_lens"], meta["positions"], meta["plan"],
             scaling if scaling is not None else 1.0 / math.sqrt(d), pool.spec.num_kv_heads, wk, wv,
-            binding.write_slots,
+            binding.write_slots, scoring=scoring,
         )
         if timer is not None:
             timer.stop("attention_kv_write", began)
@@ -252,7 +256,7 @@ def _varlen_forward(module, query, key, value, scaling, binding: _VarlenBinding)
         q_rows, out[0], pool.layer_view(layer), meta["block_tables"], meta["cu_seqlens"],
         meta["kv_lens"], meta["positions"], meta["plan"],
         scaling if scaling is not None else 1.0 / math.sqrt(d), pool.spec.num_kv_heads,
-        row_map=meta["row_map"], pool_lens=binding.pool_lens, new_k_rows=nk, new_v_rows=nv,
+        row_map=meta["row_map"], pool_lens=binding.pool_lens, new_k_rows=nk, new_v_rows=nv, scoring=scoring,
     )
     if timer is not None:
         timer.stop("attention", began)
@@ -263,11 +267,13 @@ def paged_attention_forward(module: Any, query: torch.Tensor, key: torch.Tensor,
                             attention_mask: Optional[torch.Tensor] = None, scaling: Optional[float] = None,
                             dropout: float = 0.0, **kwargs: Any) -> Tuple[torch.Tensor, None]:
     """The function registered as ``memforge_paged`` (attention_backend.py:195-272).
-    Returns ``(batch, q_len, heads, head_dim)`` as transformers expects."""
+    Returns ``(batch, q_len, heads, head_dim)`` as transformers expects. A model
+    that caps its attention scores passes ``softcap``, which every route applies."""
+    softcap = kwargs.get("softcap")
     varlen = _current_varlen()
     if varlen is not None:
         varlen.used += 1
-        return _varlen_forward(module, query, key, value, scaling, varlen), None
+        return _varlen_forward(module, query, key, value, scaling, varlen, softcap), None
 
     binding = _current()
     single_query = query.shape[0] == 1 and query.shape[2] == 1
@@ -275,12 +281,12 @@ def paged_attention_forward(module: Any, query: torch.Tensor, key: torch.Tensor,
         binding.used += 1
         out = paged_attention_blockwise(query, binding.pool.key_pool, binding.pool.value_pool,
                                         module.layer_idx, binding.block_table, binding.context_length,
-                                        binding.pool.block_size, scale=scaling)
+                                        binding.pool.block_size, scale=scaling, softcap=softcap)
         return _to_attention_output_layout(out), None
 
     if binding is not None:
         binding.fallbacks += 1
-    return _eager_attention(module, query, key, value, attention_mask, scaling), None
+    return _eager_attention(module, query, key, value, attention_mask, scaling, softcap), None
 
 
 def _to_attention_output_layout(attn_output: torch.Tensor) -> torch.Tensor:
@@ -288,7 +294,8 @@ def _to_attention_output_layout(attn_output: torch.Tensor) -> torch.Tensor:
     return attn_output.transpose(1, 2).contiguous()
 
 
-def _eager_attention(module, query, key, value, attention_mask, scaling) -> torch.Tensor:
+def _eager_attention(module, query, key, value, attention_mask, scaling,
+                     softcap: Optional[float] = None) -> torch.Tensor:
     """Plain attention with grouped-query expansion for unbound calls
     (attention_backend.py:295-328); softmax in fp32."""
     num_heads, head_dim = query.shape[1], query.shape[3]
@@ -299,6 +306,8 @@ def _eager_attention(module, query, key, value, attention_mask, scaling) -> torc
         k = k.repeat_interleave(group, dim=1)
         v = v.repeat_interleave(group, dim=1)
     scores = torch.matmul(query, k.transpose(2, 3).contiguous()) * scaling
+    if softcap:
+        scores = torch.tanh(scores / softcap) * softcap
     if attention_mask is not None:
         scores = scores + attention_mask[:, :, :, : k.shape[-2]]
     else:

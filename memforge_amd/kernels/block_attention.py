@@ -4,7 +4,8 @@ The contract of the reference's ``paged_attention_blockwise``
 (memforge_ml/kernels/block_attention.py:51-145): one query position
 ``(1, H, 1, D)`` against the first ``context_length`` tokens of one sequence,
 grouped-query heads sharing KV heads, fp32 accumulation, output in the query
-dtype. It is the varlen kernel with one row.
+dtype. It is the varlen kernel with one row. ``softcap`` caps the scores with a
+tanh (past the reference).
 """
 
 from __future__ import annotations
@@ -20,7 +21,8 @@ from memforge_amd.kernels._varlen import as_table_list, run_varlen
 
 def paged_attention_blockwise(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor,
                               layer_idx: int, block_table: torch.Tensor, context_length: int,
-                              block_size: int, scale: Optional[float] = None) -> torch.Tensor:
+                              block_size: int, scale: Optional[float] = None,
+                              softcap: Optional[float] = None) -> torch.Tensor:
     if query.shape[0] != 1 or query.shape[2] != 1:
         raise ValueError(f"expected a single query position (1, H, 1, D), got {tuple(query.shape)}")
     if context_length <= 0:
@@ -39,7 +41,7 @@ def paged_attention_blockwise(query: torch.Tensor, key_pool: torch.Tensor, value
     q = query[0].to(dtype).permute(1, 0, 2)  # (1, H, D)
     out = torch.empty((1, num_heads, 1, head_dim), dtype=dtype, device=query.device)
     run_varlen(q, out[0].permute(1, 0, 2), nat.PoolView.from_bshd(key_pool[layer_idx], value_pool[layer_idx]),
-               [table], [0], [context_length - 1], scale, num_kv_heads)
+               [table], [0], [context_length - 1], scale, num_kv_heads, softcap=softcap)
     return out.to(query.dtype)
 
 

@@ -64,28 +64,37 @@ def _validate(query: torch.Tensor, num_kv_heads: int, seq_ids, positions, block_
     return tables
 
 
-def _run(query, key_pool_layer, value_pool_layer, tables, seq_ids, positions, scale):
+def _run(query, key_pool_layer, value_pool_layer, tables, seq_ids, positions, scale, **scoring):
     num_kv_heads = key_pool_layer.shape[2]
     dtype = key_pool_layer.dtype
     q = query[0].to(dtype).permute(1, 0, 2)  # (T, H, D)
     total, heads, dim = q.shape
     out = torch.empty((1, heads, total, dim), dtype=dtype, device=query.device)
     run_varlen(q, out[0].permute(1, 0, 2), nat.PoolView.from_bshd(key_pool_layer, value_pool_layer),
-               tables, list(seq_ids), list(positions), scale, num_kv_heads)
+               tables, list(seq_ids), list(positions), scale, num_kv_heads, **scoring)
     return out.to(query.dtype)
 
 
 def paged_attention_varlen(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor,
                            layer_idx: int, block_tables: Sequence[torch.Tensor], seq_ids: Sequence[int],
                            positions: Sequence[int], block_size: int,
-                           scale: Optional[float] = None) -> torch.Tensor:
+                           scale: Optional[float] = None, softcap: Optional[float] = None,
+                           slopes: Optional[torch.Tensor] = None, doc_starts: Optional[Sequence[int]] = None,
+                           prefix_lens: Optional[Sequence[int]] = None) -> torch.Tensor:
     """Attention for a packed run of query tokens from several sequences
-    (varlen_attention.py:78-235). Pools are ``(layers, blocks, slots, kv_heads, head_dim)``."""
+    (varlen_attention.py:78-235). Pools are ``(layers, blocks, slots, kv_heads, head_dim)``.
+
+    Past the reference, the scores may be changed (``nat.Scoring``): ``softcap``
+    caps them with a tanh, ``slopes`` (fp32 per query head) subtracts
+    ``slopes[h] * |position - key|``, ``doc_starts`` (per query token) hides the
+    keys before the token's document, and keys before ``prefix_lens`` (per
+    sequence) are seen by all of its tokens. A token that sees no key gets zeros."""
     nat.require_device(query, key_pool)
     if key_pool.shape[2] != block_size:
         raise ValueError(f"pool block size {key_pool.shape[2]} does not match {block_size}")
     tables = _validate(query, key_pool.shape[3], seq_ids, positions, block_tables, block_size, False)
-    return _run(query, key_pool[layer_idx], value_pool[layer_idx], tables, seq_ids, positions, scale)
+    return _run(query, key_pool[layer_idx], value_pool[layer_idx], tables, seq_ids, positions, scale,
+                softcap=softcap, slopes=slopes, doc_starts=doc_starts, prefix_lens=prefix_lens)
 
 
 def paged_attention_varlen_materialised(query: torch.Tensor, pool, layer_idx: int,
