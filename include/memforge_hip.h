@@ -323,6 +323,53 @@ int mf_paged_attention_scored(const mf_scoring* scoring, const void* q, int64_t 
                               int64_t num_merges, const int32_t* device_counts, float* partials,
                               int64_t partials_floats, mf_stream_t stream);
 
+/* ------------------------------------------------------------- 4-bit pool
+ * A pool layer that holds K and V in 4 bits: e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4,
+ * 6 and their negatives), eight to a 32-bit word, the first element in the low
+ * bits, and one e8m0 scale byte (2^(byte - 127); 255: NaN) for 32 consecutive
+ * elements of a token's head. All four arrays are contiguous:
+ *   key_codes    (blocks, heads, slots, head_dim / 8) words
+ *   key_scales   (blocks, heads, slots, head_dim / 32) bytes
+ *   value_codes  (blocks, heads, head_dim / 8, slots) words
+ *   value_scales (blocks, heads, head_dim / 32, slots) bytes
+ * (a token's value words lie apart: the product with V wants several tokens of a
+ * few elements in a lane). block_size is a multiple of 16 up to 512, head_dim 32,
+ * 64, 128 or 256, the codes 16-byte aligned, the scales 4-byte. dtype is the type
+ * attention over the pool runs in; scales are bounded so that every value is
+ * finite in it: 2^-23 to 2^13 for fp16, 2^-125 to 2^125 for the others.
+ *
+ * mf_kv4_write rounds rows into it: a group's scale is the smallest permitted
+ * power of two whose sevenfold reaches the group's largest magnitude, a code the
+ * nearest one, ties to the even code; a group with a NaN or an infinity reads as
+ * NaN. Rows whose slot lies outside the pool are skipped; slots must be distinct.
+ * Any source type and strides (head_dim contiguous). mf_kv4_gather writes the values back
+ * as dst_dtype, leaving rows with such slots unwritten.
+ * No counterpart in the reference, whose pools hold the model's type. */
+typedef struct mf_pool4 {
+    uint32_t* key_codes;
+    uint8_t* key_scales;
+    uint32_t* value_codes;
+    uint8_t* value_scales;
+    int64_t num_blocks;
+    int block_size, num_heads, head_dim, dtype;
+} mf_pool4;
+int mf_kv4_write(const void* k_src, const void* v_src, int src_dtype, int64_t src_stride_t, int64_t src_stride_h,
+                 const int64_t* slot_mapping, int64_t num_tokens, const mf_pool4* pool, mf_stream_t stream);
+int mf_kv4_gather(const mf_pool4* pool, const int64_t* slot_mapping, int64_t num_tokens, void* k_dst, void* v_dst,
+                  int dst_dtype, int64_t dst_stride_t, int64_t dst_stride_h, mf_stream_t stream);
+
+/* mf_paged_attention (or, with scoring, mf_paged_attention_scored) over a 4-bit
+ * pool: every key is read from the pool, as the value its codes stand for. dtype
+ * (q and out) is the pool's, fp16 or bf16, and plans are made for it.
+ * device_counts as in mf_paged_attention_counted. */
+int mf_paged_attention4(const mf_scoring* scoring, const void* q, int64_t q_stride_row, int64_t q_stride_head,
+                        void* out, int64_t out_stride_row, int64_t out_stride_head, int dtype, const mf_pool4* pool,
+                        const int32_t* block_tables, int64_t block_table_stride, const int32_t* cu_seqlens,
+                        const int32_t* kv_lens, const int64_t* positions, const int32_t* row_map, int num_q_heads,
+                        float scale, const int32_t* plan_items, int64_t num_items_narrow, int64_t num_items_wide,
+                        const int32_t* plan_merges, int64_t num_merges, const int32_t* device_counts,
+                        float* partials, int64_t partials_floats, mf_stream_t stream);
+
 /* mf_paged_attention without a partials buffer or merge counters, so that
  * the call allocates nothing. No counterpart in the reference: it is for
  * callers that cannot allocate device memory (code under HIP graph capture,

@@ -74,6 +74,11 @@ _SIGNATURES = {
         _vp, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_int, _vp, _vp, _c_i64, _c_i64, _c_i64,
         _c_int, _vp, _c_i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64,
         _c_int, _c_int, _c_int, _c_f32, _vp, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp, _c_i64, _vp]),
+    "mf_kv4_write": (_c_int, [_vp, _vp, _c_int, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp]),
+    "mf_kv4_gather": (_c_int, [_vp, _vp, _c_i64, _vp, _vp, _c_int, _c_i64, _c_i64, _vp]),
+    "mf_paged_attention4": (_c_int, [
+        _vp, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_int, _vp, _vp, _c_i64, _vp, _vp, _vp, _vp, _c_int,
+        _c_f32, _vp, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp, _c_i64, _vp]),
     "mf_paged_attention_noalloc": (_c_int, [
         _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_int, _vp, _vp, _c_i64, _c_i64, _c_i64,
         _c_int, _vp, _c_i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_int, _c_int,
@@ -207,6 +212,52 @@ class PoolView:
         return PoolView(k, v, k.stride(0), k.stride(2), k.stride(1), bs, h, d)
 
 
+class _Pool4Struct(ctypes.Structure):
+    _fields_ = [("key_codes", _vp), ("key_scales", _vp), ("value_codes", _vp), ("value_scales", _vp),
+                ("num_blocks", _c_i64), ("block_size", _c_int), ("num_heads", _c_int), ("head_dim", _c_int),
+                ("dtype", _c_int)]
+
+
+GROUP4 = 32  # elements of a 4-bit pool that share a scale
+HEAD_DIMS4 = (32, 64, 128, 256)
+
+
+class Pool4View:
+    """One layer of a pool held in 4 bits (mf_pool4): int32 ``key_codes`` (blocks,
+    heads, slots, head_dim / 8) and ``value_codes`` (blocks, heads, head_dim / 8,
+    slots), uint8 ``key_scales`` (blocks, heads, slots, head_dim / 32) and
+    ``value_scales`` (blocks, heads, head_dim / 32, slots), all contiguous.
+    ``dtype`` is the type attention over it runs in."""
+
+    def __init__(self, key_codes: torch.Tensor, key_scales: torch.Tensor, value_codes: torch.Tensor,
+                 value_scales: torch.Tensor, dtype: torch.dtype):
+        n, h, bs, words = key_codes.shape
+        want = ((key_codes, torch.int32, (n, h, bs, words)), (key_scales, torch.uint8, (n, h, bs, words // 4)),
+                (value_codes, torch.int32, (n, h, words, bs)), (value_scales, torch.uint8, (n, h, words // 4, bs)))
+        for x, dt, shape in want:
+            if x.dtype != dt or tuple(x.shape) != shape or not x.is_contiguous() or x.device != key_codes.device:
+                raise ValueError(f"a 4-bit pool layer needs a contiguous {dt} tensor of {shape} on one device, got "
+                                 f"{x.dtype} {tuple(x.shape)} on {x.device}")
+        if 8 * words not in HEAD_DIMS4:
+            raise ValueError(f"a 4-bit pool holds head_dims {HEAD_DIMS4}, got {8 * words}")
+        if bs % 16 or bs > 512:
+            raise ValueError(f"a 4-bit pool's block_size is a multiple of 16 up to 512, got {bs}")
+        self.key_codes, self.key_scales = key_codes, key_scales
+        self.value_codes, self.value_scales = value_codes, value_scales
+        self.dtype = dtype
+        self.num_blocks, self.num_heads, self.block_size, self.head_dim = n, h, bs, 8 * words
+        self.struct = _Pool4Struct(_ptr(key_codes), _ptr(key_scales), _ptr(value_codes), _ptr(value_scales), n, bs, h,
+                                   8 * words, dtype_code(dtype))
+
+    @property
+    def num_slots(self) -> int:
+        return self.num_blocks * self.block_size
+
+    @property
+    def device(self) -> torch.device:
+        return self.key_codes.device
+
+
 def same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Same shape and the same strides on every axis longer than one (the
     stride of a length-one axis is never used to address an element)."""
@@ -261,6 +312,44 @@ def kv_gather(pool: PoolView, slots: torch.Tensor, k_rows: torch.Tensor, v_rows:
         pool.stride_head, pool.block_size, pool.num_slots, _ptr(slots), T, _ptr(k_rows), _ptr(v_rows),
         dtype_code(k_rows.dtype), k_rows.stride(0), k_rows.stride(1), H, D, _stream(k_rows.device),
     ), "mf_kv_gather")
+
+
+def _rows4(k_rows, v_rows, slots, pool: Pool4View):
+    _rows_ok(k_rows, "k_rows")
+    _rows_ok(v_rows, "v_rows")
+    require_device(k_rows, v_rows, slots, pool.key_codes)
+    if not k_rows.device == v_rows.device == slots.device == pool.device:
+        raise ValueError("rows, slots and pool must be on one device")
+    if slots.dtype != torch.int64 or not slots.is_contiguous():
+        slots = slots.to(torch.int64).contiguous()
+    if k_rows.shape != v_rows.shape or k_rows.dtype != v_rows.dtype \
+            or tuple(k_rows.shape) != (slots.numel(), pool.num_heads, pool.head_dim):
+        raise ValueError(f"rows {tuple(k_rows.shape)} / {tuple(v_rows.shape)} and {slots.numel()} slots do not match a "
+                         f"pool of {pool.num_heads} heads x {pool.head_dim}")
+    return slots
+
+
+def kv4_write(k_rows: torch.Tensor, v_rows: torch.Tensor, slots: torch.Tensor, pool: Pool4View) -> None:
+    """Round (T, H, D) rows to 4 bits into the pool slots ``slots`` (int64, device,
+    distinct; a slot outside the pool skips its row)."""
+    slots = _rows4(k_rows, v_rows, slots, pool)
+    if not same_layout(k_rows, v_rows):
+        k_rows, v_rows = k_rows.contiguous(), v_rows.contiguous()
+    with _on(pool.device):
+        _check(lib().mf_kv4_write(
+            _ptr(k_rows), _ptr(v_rows), dtype_code(k_rows.dtype), k_rows.stride(0), k_rows.stride(1), _ptr(slots),
+            slots.numel(), ctypes.addressof(pool.struct), _stream(pool.device)), "mf_kv4_write")
+
+
+def kv4_gather(pool: Pool4View, slots: torch.Tensor, k_rows: torch.Tensor, v_rows: torch.Tensor) -> None:
+    """The values that pool slots ``slots`` stand for, into preallocated (T, H, D) rows."""
+    slots = _rows4(k_rows, v_rows, slots, pool)
+    if not same_layout(k_rows, v_rows):
+        raise ValueError("k_rows and v_rows must share strides")
+    with _on(pool.device):
+        _check(lib().mf_kv4_gather(
+            ctypes.addressof(pool.struct), _ptr(slots), slots.numel(), _ptr(k_rows), _ptr(v_rows),
+            dtype_code(k_rows.dtype), k_rows.stride(0), k_rows.stride(1), _stream(pool.device)), "mf_kv4_gather")
 
 
 def kv_copy_blocks(key_pool: torch.Tensor, value_pool: torch.Tensor,
@@ -760,7 +849,9 @@ def paged_attention(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: PoolView
                     scoring: Optional[Scoring] = None) -> None:
     """Varlen paged attention into ``out_rows`` ((rows, Hq, D) views, device).
     ``scoring``: capped, biased or masked scores (mf_paged_attention_scored;
-    per-range plans, no fused merge).
+    per-range plans, no fused merge). ``pool``: a layer of a 16- or 32-bit pool, or
+    of one held in 4 bits (``Pool4View``; mf_paged_attention4, 16-bit queries,
+    per-range plans made with ``kv_bits=4``, every key in the pool).
 
     Split-K partitions are merged by a separate merge kernel; with
     ``fused_merge`` the attention kernel merges them itself (the last partition
@@ -769,6 +860,11 @@ def paged_attention(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: PoolView
     must release its partials with an agent-scope fence."""
     _rows_ok(q_rows, "q_rows")
     _rows_ok(out_rows, "out_rows")
+    if isinstance(pool, Pool4View):
+        if pool_lens is not None or fused_merge:
+            raise ValueError("a 4-bit pool takes no in-flight keys or fused merge")
+        return _paged_attention4(scoring, q_rows, out_rows, pool, block_tables, cu_seqlens, kv_lens, positions, plan,
+                                 scale, num_kv_heads, row_map, partials)
     require_device(q_rows, out_rows, pool.k, block_tables, cu_seqlens, kv_lens, positions)
     if q_rows.dtype != pool.k.dtype or out_rows.dtype != pool.k.dtype:
         raise TypeError("query, output and pool must share a dtype")
@@ -881,6 +977,44 @@ def _paged_attention_scored(scoring: Scoring, q_rows, out_rows, pool, block_tabl
             _ptr(plan.items), p.narrow, p.wide, _ptr(plan.merges), p.merges, _ptr(p.counts),
             _ptr(p.partials), p.partials.numel() if p.partials is not None else 0, _stream(dev),
         ), "mf_paged_attention_scored")
+
+
+def _check4(q_rows, out_rows, pool: Pool4View, num_kv_heads: int) -> None:
+    require_device(q_rows, out_rows, pool.key_codes)
+    if not q_rows.device == out_rows.device == pool.device:
+        raise ValueError("query, output and pool must be on one device")
+    if pool.dtype == torch.float32:
+        raise TypeError("attention over a 4-bit pool runs in float16 or bfloat16; this pool's dtype is float32")
+    if q_rows.dtype != pool.dtype or out_rows.dtype != pool.dtype:
+        raise TypeError(f"query and output must be of the pool's dtype {pool.dtype}")
+    if num_kv_heads != pool.num_heads or q_rows.shape[2] != pool.head_dim or out_rows.shape != q_rows.shape:
+        raise ValueError(f"query {tuple(q_rows.shape)}, output {tuple(out_rows.shape)} and {num_kv_heads} kv heads do "
+                         f"not match a pool of {pool.num_heads} heads x {pool.head_dim}")
+
+
+def _paged_attention4(scoring, q_rows, out_rows, pool: Pool4View, block_tables, cu_seqlens, kv_lens, positions, plan,
+                      scale, num_kv_heads, row_map=None, partials=None) -> None:
+    _check4(q_rows, out_rows, pool, num_kv_heads)
+    dev = q_rows.device
+    for name, t, dt in (("block_tables", block_tables, torch.int32), ("cu_seqlens", cu_seqlens, torch.int32),
+                        ("kv_lens", kv_lens, torch.int32), ("positions", positions, torch.int64)):
+        if t.dtype != dt or not t.is_contiguous():
+            raise TypeError(f"{name} must be a contiguous {dt} tensor")
+        if t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, the query on {dev}")
+    p = _Plan(plan, dev, partials)
+    scoring = _scored(scoring)
+    mods = scoring.struct(q_rows.shape[1], kv_lens.numel(), dev) if scoring is not None else None
+    bt_stride = block_tables.shape[1] if block_tables.dim() == 2 else 0
+    with _on(dev):
+        _check(lib().mf_paged_attention4(
+            ctypes.addressof(mods) if mods is not None else None,
+            _ptr(q_rows), q_rows.stride(0), q_rows.stride(1), _ptr(out_rows), out_rows.stride(0), out_rows.stride(1),
+            dtype_code(q_rows.dtype), ctypes.addressof(pool.struct), _ptr(block_tables), bt_stride,
+            _ptr(cu_seqlens), _ptr(kv_lens), _ptr(positions), _ptr(row_map), q_rows.shape[1], float(scale),
+            _ptr(plan.items), p.narrow, p.wide, _ptr(plan.merges), p.merges, _ptr(p.counts),
+            _ptr(p.partials), p.partials.numel() if p.partials is not None else 0, _stream(dev),
+        ), "mf_paged_attention4")
 
 
 def paged_attention_kv_write(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: PoolView,
@@ -1037,9 +1171,15 @@ def paged_attention_packed(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: P
     is a slice plan (mf_paged_attention_slices; no row map or pool lengths)."""
     _rows_ok(q_rows, "q_rows")
     _rows_ok(out_rows, "out_rows")
-    require_device(q_rows, out_rows, pool.k, buf)
-    if q_rows.dtype != pool.k.dtype or out_rows.dtype != pool.k.dtype:
-        raise TypeError("query, output and pool must share a dtype")
+    four = isinstance(pool, Pool4View)
+    if four:
+        _check4(q_rows, out_rows, pool, num_kv_heads)
+        if has_pool_lens or sliced:
+            raise ValueError("a 4-bit pool takes no in-flight keys or slice plans")
+    else:
+        require_device(q_rows, out_rows, pool.k, buf)
+        if q_rows.dtype != pool.k.dtype or out_rows.dtype != pool.k.dtype:
+            raise TypeError("query, output and pool must share a dtype")
     if buf.dtype != torch.int32 or not buf.is_contiguous():
         raise TypeError("buf must be a contiguous int32 tensor")
     nk, nv = new_k_rows, new_v_rows
@@ -1069,11 +1209,25 @@ def paged_attention_packed(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: P
         return
     row_map = addr[5] if has_row_map else None
     pool_lens = addr[5 + int(has_row_map)] if has_pool_lens else None
+    mods = None
     if softcap or slopes is not None or has_first_keys or has_prefix_lens:
         at = 5 + int(has_row_map) + int(has_pool_lens)
         mods = Scoring(softcap, slopes).struct(q_rows.shape[1], num_seqs, dev)
         mods.first_keys = addr[at] if has_first_keys else None
         mods.prefix_lens = addr[at + int(has_first_keys)] if has_prefix_lens else None
+    if four:
+        with _on(dev):
+            _check(lib().mf_paged_attention4(
+                ctypes.addressof(mods) if mods is not None else None,
+                _ptr(q_rows), q_rows.stride(0), q_rows.stride(1),
+                _ptr(out_rows), out_rows.stride(0), out_rows.stride(1),
+                dtype_code(q_rows.dtype), ctypes.addressof(pool.struct), addr[0], bt_stride,
+                addr[3], addr[3] + 4 * (num_seqs + 1), addr[4], row_map, q_rows.shape[1], float(scale),
+                addr[1], n_narrow, n_wide, addr[2], n_merges, None,
+                _ptr(partials), partials.numel() if partials is not None else 0, _stream(dev),
+            ), "mf_paged_attention4")
+        return
+    if mods is not None:
         with _on(dev):
             _check(lib().mf_paged_attention_scored(
                 ctypes.addressof(mods), _ptr(q_rows), q_rows.stride(0), q_rows.stride(1),

@@ -26,6 +26,7 @@
 
 #include <algorithm>
 #include <array>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -2278,6 +2279,19 @@ int launch_slices(AttnArgs a, const int32_t* slices, int64_t n_slices, int hkv, 
     if (n_merges > 0) {
         if (int st = launch_merge<DT, DP>(a, merges, n_merges, stream)) return st;
     }
+    return MF_OK;
+}
+
+// A scored launch's fields; a.scale_log2 is set. A cap so small or so large against
+// the scale that their quotient leaves fp32's normal numbers is refused.
+inline int set_scoring(ScoredArgs& a, const mf_scoring& s) {
+    if (!(s.softcap >= 0.f) || !(s.softcap < INFINITY)) return MF_ERR_ARG;
+    a.slopes = s.slopes;
+    a.first_keys = s.first_keys;
+    a.prefix_lens = s.prefix_lens;
+    a.cap_in = s.softcap > 0.f ? 2.f * a.scale_log2 / s.softcap : 0.f;
+    a.cap_log2 = s.softcap * 1.4426950408889634f;
+    if (s.softcap > 0.f && !(a.cap_in >= FLT_MIN && a.cap_in < INFINITY && a.cap_log2 < INFINITY)) return MF_ERR_ARG;
     return MF_OK;
 }
 

@@ -1,0 +1,752 @@
+// Varlen paged attention over a 4-bit pool (mf_pool4), with or without capped,
+// biased and masked scores, on the plans of the 16-bit kernels (attn_kernels.h).
+//
+// The mathematics is theirs: columns are (row, query head) pairs of one kv head,
+// S^T = K Q^T, an online softmax in log2 units with a lazy running maximum,
+// O^T += V^T P^T. What differs is where K and V come from: codes go through
+// gfx950's scaled conversions (two elements an instruction, the group's scale
+// applied, exact in fp16 and bf16) on their way into the MFMA operands, so the
+// products run on the 16-bit matrix rate with q and p unchanged.
+//
+// Decode items (attn4_narrow): a wave takes 32 keys at a time of 16 columns. Of the
+// contraction over head_dim, lane (g, j) holds elements [g D/4, (g + 1) D/4) of key j
+// -- for K one load of D/8 bytes, contiguous over the wave, whose scale is (D 128)
+// the lane's own byte -- and Q's fragments are read in the same order. V lies
+// token-minor in the pool, so a lane's 16 bytes are four keys of eight head_dim
+// elements, which four conversions a key and a byte permute a pair turn into the
+// operand of the 32-key product.
+//
+// Prefill items (attn4_wide): the four waves of a workgroup share a key range; each
+// stage's codes are converted once, while they pass from registers to LDS, and the
+// loop over the stage is the 16-bit kernels'.
+#include "attn_kernels.h"
+#include "kv4.h"
+
+namespace mf {
+namespace {
+
+struct Attn4Args : ScoredArgs {
+    const uint32_t* kc;
+    const uint8_t* ks;
+    const uint32_t* vc;
+    const uint8_t* vs;
+    int H;               // kv heads
+    int tpb;             // 16-key tiles of a block
+    uint32_t tpb_magic;  // ceil(2^32 / tpb), unused for 1
+};
+
+// Block index of tile t in its sequence's table.
+__device__ __forceinline__ int block_of(const Attn4Args& a, int t) {
+    return a.tpb == 1 ? t : (int)__umulhi((uint32_t)t, a.tpb_magic);
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+    if constexpr (DT == MF_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){x, y}, bf16x2));
+    else return f32_to_bits<DT>(x) | (f32_to_bits<DT>(y) << 16);
+}
+
+constexpr int kDepth4 = 3;  // register buffers of the decode loop, 32 keys each
+
+// One wave, one 16-column tile (c0 + ct of its item), the item's keys.
+template <int DT, int DP, bool SC>
+__device__ __forceinline__ void attn4_narrow(const Attn4Args& a, const int32_t* it, const int wave, const int ct,
+                                             const bool coop) {
+    constexpr int KW = DP / 32;                // words of a lane's K per 16 keys
+    constexpr int VCH = DP / 16;               // head_dim elements of a lane's V per key
+    constexpr int VW = DP == 256 ? 8 : 4;      // words of its V per 16 keys
+    constexpr int XW = VCH / 2;                // 16-bit pairs of a lane's V per key
+    constexpr float kNegInf = -__builtin_huge_valf();
+    const int lane = threadIdx.x & 63;
+    const int g = lane >> 4, j = lane & 15;
+    const int s = it[0], h = it[1], c0 = it[2] + ct, kt0 = it[4], kt1 = it[5];
+    const int pslot = it[6] < 0 ? -1 : it[6] + ct;
+    const int row0 = it[8], ncols = it[9] * a.G, kv_len = it[10];
+    int first = 0, prefix = 0;
+    if constexpr (SC) {
+        if (a.first_keys) first = a.first_keys[s];
+        if (a.prefix_lens) prefix = a.prefix_lens[s];
+    }
+    // ---- the item's blocks: entry of tile kt0 + lane and kt0 + 64 + lane
+    const int32_t* trow = a.block_tables + (int64_t)s * a.bt_stride;
+    const int last_tile = max(kt1 - 1, 0);
+    const int tbl = trow[block_of(a, min(kt0 + lane, last_tile))];
+    const int tbl_hi = trow[block_of(a, min(kt0 + 64 + lane, last_tile))];
+
+    // ---- this lane's column
+    const int cidx = c0 * 16 + j;
+    const bool valid = cidx < ncols && ct < it[3];
+    const int r = valid ? cidx / a.G : 0;
+    int prow = row0 + r;
+    if (a.row_map) prow = a.row_map[prow];
+    const int qhead = h * a.G + (valid ? cidx - r * a.G : 0);
+    const int pos = reinterpret_cast<const int32_t*>(a.positions)[2 * (int64_t)prow];
+    float slope = 0.f;
+    if constexpr (SC) {
+        if (a.slopes) slope = a.slopes[qhead] * 1.4426950408889634f;
+    }
+    uint4 qf[KW];
+#pragma unroll
+    for (int c = 0; c < KW; ++c) {
+        const uint4 v = *(const uint4*)(a.q + ((int64_t)prow * a.q_sr + (int64_t)qhead * a.q_sh + g * (DP / 4) + c * 8) * 2);
+        qf[c] = make_uint4(v.x ^ a.q_sign, v.y ^ a.q_sign, v.z ^ a.q_sign, v.w ^ a.q_sign);
+    }
+    const int reach = valid ? (SC ? max(pos, prefix - 1) : pos) : -1;
+    const int lim = reach >= 0 ? min(min(reach, kv_len - 1), kt1 * 16 - 1) : -1;  // last key of the item the column sees
+
+    // ---- the stream
+    struct Tile {
+        uint32_t kw[KW], ks, vw[VW], vs;
+    };
+    const int bs = a.tpb * 16;
+    const uint32_t k_lane = (uint32_t)(j * (DP / 8) + g * KW);
+    constexpr int VSH = DP == 64 ? 1 : DP == 32 ? 2 : 0;  // lanes that share a word's eight elements: 2^VSH
+    const int vchunk = DP == 256 ? 2 * j : j >> VSH;
+    const uint32_t v_lane = (uint32_t)(vchunk * bs + 4 * g);
+    const uint32_t ks_lane = (uint32_t)(j * (DP / 32) + (DP == 256 ? 2 * g : DP == 128 ? g : DP == 64 ? g >> 1 : 0));
+    const uint32_t vs_lane = (uint32_t)((vchunk >> 2) * bs + 4 * g);
+    auto load = [&](int t, Tile& x) __attribute__((always_inline)) {
+        const int i = t - kt0;
+        const int e0 = __builtin_amdgcn_readlane(tbl, i & 63), e1 = __builtin_amdgcn_readlane(tbl_hi, i & 63);
+        const int blk = i < 64 ? e0 : e1;
+        const int off = (t - block_of(a, t) * a.tpb) * 16;
+        const int64_t row = (int64_t)blk * a.H + h;
+        const uint32_t* kc = a.kc + (row * bs + off) * (DP / 8);
+        const uint8_t* ks = a.ks + (row * bs + off) * (DP / 32);
+        const uint32_t* vc = a.vc + row * (DP / 8) * bs + off;
+        const uint8_t* vs = a.vs + row * (DP / 32) * bs + off;
+        ld_words<KW * 4>((const char*)(kc + k_lane), x.kw);
+        if constexpr (DP == 256) x.ks = *(const uint16_t*)(ks + ks_lane);
+        else x.ks = ks[ks_lane];
+        ld_words<16>((const char*)(vc + v_lane), x.vw);
+        if constexpr (DP == 256) ld_words<16>((const char*)(vc + v_lane + bs), x.vw + 4);
+        x.vs = *(const uint32_t*)(vs + vs_lane);
+    };
+
+    float m = kMinM, l = 0.f;
+    float thr = SC ? kMinM + kLazyLog2 : (kMinM + kLazyLog2) * a.inv_scale_log2;
+    f32x4 acc[VCH];
+#pragma unroll
+    for (int c = 0; c < VCH; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    if (kt1 > kt0) {
+        int maxlim = lim, minlim = valid ? lim : INT_MAX;
+#pragma unroll
+        for (int o = 8; o >= 1; o >>= 1) {  // the four lane groups hold the same columns
+            maxlim = max(maxlim, __shfl_xor(maxlim, o, 64));
+            minlim = min(minlim, __shfl_xor(minlim, o, 64));
+        }
+        maxlim = __builtin_amdgcn_readfirstlane(maxlim);
+        minlim = __builtin_amdgcn_readfirstlane(minlim);
+        const int tb = min(max(kt0, first >> 4), kt1);
+        const int te = maxlim < 0 ? tb : max(tb, min(kt1, (maxlim >> 4) + 1));
+
+        auto process = [&](int t, Tile& x, Tile& y) __attribute__((always_inline)) {
+            const int key0 = t * 16 + 4 * g;  // this lane's keys: key0 + r, key0 + 16 + r
+            // keys no column sees may hold anything: their V is cleared, and with
+            // it a scale that makes zeros NaN
+            float vscale[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                vscale[k] = scale4((x.vs >> (8 * k)) & 255u);
+                vscale[4 + k] = scale4((y.vs >> (8 * k)) & 255u);
+            }
+            if (t * 16 + 31 > maxlim || t * 16 < first) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int key = key0 + (k & 3) + 16 * (k >> 2);
+                    const bool live = key >= first && key <= maxlim;
+                    vscale[k] = live ? vscale[k] : 1.f;
+#pragma unroll
+                    for (int u = 0; u < VW / 4; ++u) {
+                        uint32_t& w = (k < 4 ? x : y).vw[4 * u + (k & 3)];
+                        w = live ? w : 0u;
+                    }
+                }
+            }
+            f32x4 st[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const Tile& z = u ? y : x;
+                st[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < KW; ++c) {
+                    const float ks = scale4(DP == 256 ? (c < 4 ? z.ks & 255u : z.ks >> 8) : z.ks);
+                    st[u] = mfma_qk<DT>(octet4<DT>(z.kw[c], ks), qf[c], st[u]);
+                }
+            }
+            float sv[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                sv[k] = st[k >> 2][k & 3];
+                if constexpr (SC)
+                    sv[k] = scored<DT>(sv[k], a.scale_log2, a.cap_in, a.cap_log2, slope,
+                                       (float)(key0 + (k & 3) + 16 * (k >> 2) - pos));
+            }
+            if (t * 16 + 31 > minlim || t * 16 < first) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int key = key0 + (k & 3) + 16 * (k >> 2);
+                    sv[k] = key <= lim && key >= first ? sv[k] : kNegInf;
+                }
+            }
+            float lmax = sv[0];
+#pragma unroll
+            for (int k = 1; k < 8; ++k) lmax = fmax_prop(lmax, sv[k]);
+            if (__builtin_amdgcn_ballot_w64(lmax > thr) != 0) {
+                const float cm = group_max4(lmax);
+                const float mn = fmaxf(m, SC ? cm : cm * a.scale_log2);
+                const float alpha = __builtin_amdgcn_exp2f(m - mn);
+                l *= alpha;
+#pragma unroll
+                for (int c = 0; c < VCH; ++c) acc[c] *= alpha;
+                m = mn;
+                thr = SC ? mn + kLazyLog2 : (mn + kLazyLog2) * a.inv_scale_log2;
+            }
+            float p[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                p[k] = __builtin_amdgcn_exp2f(SC ? sv[k] - m : __builtin_fmaf(sv[k], a.scale_log2, -m));
+            l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            const uint4 pf = make_uint4(pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]), pack2<DT>(p[4], p[5]),
+                                        pack2<DT>(p[6], p[7]));
+            // V: XW pairs of the lane's elements for each of its eight keys, then
+            // pairs of keys per element
+            uint32_t v[8][XW];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t* w = (k < 4 ? x : y).vw + (k & 3);
+                if constexpr (VCH >= 8) {
+#pragma unroll
+                    for (int u = 0; u < VW / 4; ++u) {
+                        const uint4 o = octet4<DT>(w[4 * u], vscale[k]);
+                        v[k][4 * u] = o.x; v[k][4 * u + 1] = o.y; v[k][4 * u + 2] = o.z; v[k][4 * u + 3] = o.w;
+                    }
+                } else if constexpr (VCH == 4) {
+                    const uint32_t half = w[0] >> (16 * (j & 1));
+                    v[k][0] = pair4<DT, 0>(half, vscale[k]);
+                    v[k][1] = pair4<DT, 1>(half, vscale[k]);
+                } else {
+                    v[k][0] = pair4<DT, 0>(w[0] >> (8 * (j & 3)), vscale[k]);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < XW; ++u) {
+                uint32_t lo[4], hi[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    lo[k] = __builtin_amdgcn_perm(v[2 * k + 1][u], v[2 * k][u], 0x05040100u);
+                    hi[k] = __builtin_amdgcn_perm(v[2 * k + 1][u], v[2 * k][u], 0x07060302u);
+                }
+                acc[2 * u] = mfma_qk<DT>(make_uint4(lo[0], lo[1], lo[2], lo[3]), pf, acc[2 * u]);
+                acc[2 * u + 1] = mfma_qk<DT>(make_uint4(hi[0], hi[1], hi[2], hi[3]), pf, acc[2 * u + 1]);
+            }
+        };
+        if (tb < te) {
+            // a ring of kDepth4 buffers of two tiles; loads past the range's end
+            // read its last tile again, masked
+            Tile ring[kDepth4][2];
+            const int last = te - 1;
+            auto fetch = [&](int t, Tile (&x)[2]) __attribute__((always_inline)) {
+                load(min(t, last), x[0]);
+                load(min(t + 1, last), x[1]);
+            };
+            int t = tb;
+#pragma unroll
+            for (int i = 0; i < kDepth4 - 1; ++i) fetch(t + 2 * i, ring[i]);
+            for (int n = (te - tb + 1) / 2 / kDepth4; n > 0; --n) {
+#pragma unroll
+                for (int u = 0; u < kDepth4; ++u) {
+                    fetch(t + 2 * (kDepth4 - 1), ring[(u + kDepth4 - 1) % kDepth4]);
+                    process(t, ring[u][0], ring[u][1]);
+                    t += 2;
+                }
+            }
+            auto tail = [&](auto self, auto U) {
+                constexpr int u = decltype(U)::value;
+                if constexpr (u < kDepth4 - 1) {
+                    if (t <= last) {
+                        process(t, ring[u][0], ring[u][1]);
+                        t += 2;
+                        self(self, std::integral_constant<int, u + 1>{});
+                    }
+                }
+            };
+            tail(tail, std::integral_constant<int, 0>{});
+        }
+    }
+
+    // ---- finish: lane (g, j) holds column j's elements (4g + r) VCH + c in acc[c][r]
+    l = group_sum4(l);
+    float M = m, L = l;
+    if (coop) {
+        // the four waves took quarters of one range: each combines the elements of
+        // its own r over the waves' states, left in LDS
+        auto s_acc = reinterpret_cast<float (*)[4 * VCH][64]>(attn_lds);
+        auto s_m = reinterpret_cast<float (*)[16]>(attn_lds + kWaves * 4 * VCH * 64 * 4);
+        auto s_l = s_m + kWaves;
+#pragma unroll
+        for (int rr = 0; rr < 4; ++rr)
+#pragma unroll
+            for (int c = 0; c < VCH; ++c) s_acc[wave][rr * VCH + c][lane] = acc[c][rr];
+        if (g == 0) {
+            s_m[wave][j] = m;
+            s_l[wave][j] = l;
+        }
+        __syncthreads();
+        float o[VCH];
+        M = kMinM;
+        L = 0.f;
+#pragma unroll
+        for (int u = 0; u < kWaves; ++u) M = fmaxf(M, s_m[u][j]);
+#pragma unroll
+        for (int c = 0; c < VCH; ++c) o[c] = 0.f;
+#pragma unroll
+        for (int u = 0; u < kWaves; ++u) {
+            const float w = __builtin_amdgcn_exp2f(s_m[u][j] - M);
+            L += s_l[u][j] * w;
+#pragma unroll
+            for (int c = 0; c < VCH; ++c) o[c] += w * s_acc[u][wave * VCH + c][lane];
+        }
+        if (!valid) return;
+        const float inv = L > 0.f ? 1.f / L : 0.f;
+#pragma unroll
+        for (int c = 0; c < VCH; ++c) o[c] *= inv;
+        const int d0 = (4 * g + wave) * VCH;
+        if (pslot < 0) {
+            store_elems<DT, VCH>(a.out + ((int64_t)prow * a.o_sr + (int64_t)qhead * a.o_sh + d0) * 2, o);
+        } else {
+            bool fp32 = false;
+            if constexpr (has_fp32_partials<DT, DP>()) fp32 = (it[7] & MF_PLAN_FP32_PARTIALS) != 0;
+            if (fp32) store_elems<MF_F32, VCH>(partial_out<MF_F32>(a, pslot, j, d0), o);
+            else store_elems<DT, VCH>(partial_out<DT>(a, pslot, j, d0), o);
+            if (g == 0 && wave == 0) {
+                partial_ml(a, pslot)[j] = M;
+                partial_ml(a, pslot)[16 + j] = L;
+            }
+        }
+        return;
+    }
+    if (!valid) return;
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    float o[4 * VCH];
+#pragma unroll
+    for (int rr = 0; rr < 4; ++rr)
+#pragma unroll
+        for (int c = 0; c < VCH; ++c) o[rr * VCH + c] = acc[c][rr] * inv;
+    if (pslot < 0) {
+        store_out_chunk<DT, VCH>(a.out + ((int64_t)prow * a.o_sr + (int64_t)qhead * a.o_sh + 4 * g * VCH) * 2, o);
+    } else {
+        store_out_chunk<DT, VCH>(partial_out<DT>(a, pslot, j, 4 * g * VCH), o);
+        if (g == 0) {
+            partial_ml(a, pslot)[j] = M;
+            partial_ml(a, pslot)[16 + j] = L;
+        }
+    }
+}
+
+// ------------------------------------------------------- workgroup-shared items
+// Keys of a stage: two 8 KB (K and V of 32 keys at D 128, of 64 below) buffers.
+constexpr int wide_keys4(int dp) { return dp >= 128 ? 32 : 64; }
+template <int DP>
+constexpr int wide_lds4() { return 2 * 2 * wide_keys4(DP) * DP * 2; }
+
+// cols: first column tile and tiles of the workgroup's four items.
+template <int DT, int DP, bool SC>
+__device__ __forceinline__ void attn4_wide(const Attn4Args& a, const int32_t* it, const int wave,
+                                           const int (&cols)[kWaves][2]) {
+    constexpr int RB = DP * 2;       // bytes of a key's row in LDS
+    constexpr int NCH = RB / 16;     // 16-byte chunks of a row: the eight elements of a word
+    constexpr int KEYS = wide_keys4(DP), TS = KEYS / 16;
+    constexpr int RPB = 256 / RB;    // rows in 256 bytes
+    constexpr int NQ = DP / 16, ND = DP / 32;
+    constexpr int HALF = KEYS * RB, STG = 2 * HALF;
+    constexpr int NW = KEYS * (DP / 8) / 256;  // words of a thread's K (and V) per stage
+    static_assert(NW == 1 || NW == 2, "stage layout");
+    constexpr float kNegInf = -__builtin_huge_valf();
+    const int lane = threadIdx.x & 63;
+    const int hf = lane >> 5;
+    const int s = it[0], h = it[1], c0 = it[2], nct = it[3], kt0 = it[4], kt1 = it[5], pslot = it[6];
+    const int row0 = it[8], nrows = it[9], kv_len = it[10];
+    int first = 0, prefix = 0;
+    if constexpr (SC) {
+        if (a.first_keys) first = a.first_keys[s];
+        if (a.prefix_lens) prefix = a.prefix_lens[s];
+    }
+    const int32_t* trow = a.block_tables + (int64_t)s * a.bt_stride;
+
+    // ---- this lane's column, and two of the workgroup's other columns, whose
+    // positions say how far the stages run
+    const int ct = (lane & 31) >> 4, j = lane & 15;
+    const int cidx = c0 * 16 + (lane & 31);
+    const bool valid = ct < nct && cidx < nrows * a.G;
+    const int col = valid ? cidx : 0;
+    const int crow = (int)((unsigned)col / (unsigned)a.G);
+    const int qhead = h * a.G + col - crow * a.G;
+    int rows[3] = {row0 + crow, row0, row0};
+    bool other[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int c = (hf ? cols[2 * k + 1][0] : cols[2 * k][0]) * 16 + (lane & 31);
+        other[k] = ct < (hf ? cols[2 * k + 1][1] : cols[2 * k][1]) && c < nrows * a.G;
+        rows[1 + k] = row0 + (int)((unsigned)(other[k] ? c : 0) / (unsigned)a.G);
+    }
+    if (a.row_map) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) rows[k] = a.row_map[rows[k]];
+    }
+    int rpos[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) rpos[k] = reinterpret_cast<const int32_t*>(a.positions)[2 * (int64_t)rows[k]];
+    const int prow = rows[0];
+    float slope = 0.f;
+    if constexpr (SC) {
+        if (a.slopes) slope = a.slopes[qhead] * 1.4426950408889634f;
+    }
+    auto reach = [&](int pos) { return SC ? max(pos, prefix - 1) : pos; };
+    const int qpos = valid ? reach(rpos[0]) : -1;
+    const int wpos = max(other[0] ? reach(rpos[1]) : -1, other[1] ? reach(rpos[2]) : -1);
+    uint4 qf[NQ];
+#pragma unroll
+    for (int c = 0; c < NQ; ++c) {
+        const uint4 v = *(const uint4*)(a.q + ((int64_t)prow * a.q_sr + (int64_t)qhead * a.q_sh + c * 16 + hf * 8) * 2);
+        qf[c] = make_uint4(v.x ^ a.q_sign, v.y ^ a.q_sign, v.z ^ a.q_sign, v.w ^ a.q_sign);
+    }
+    const int end_key = min(kv_len, kt1 * 16);
+    const int lim = qpos >= 0 ? min(qpos, end_key - 1) : -1;
+    int maxlim = lim, minlim = valid ? lim : INT_MAX, wglim = min(wpos, end_key - 1);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        maxlim = max(maxlim, __shfl_xor(maxlim, o, 64));
+        minlim = min(minlim, __shfl_xor(minlim, o, 64));
+        wglim = max(wglim, __shfl_xor(wglim, o, 64));
+    }
+    maxlim = __builtin_amdgcn_readfirstlane(maxlim);
+    minlim = __builtin_amdgcn_readfirstlane(minlim);
+    wglim = __builtin_amdgcn_readfirstlane(wglim);
+    const int te = wglim < kt0 * 16 ? kt0 : (wglim >> 4) + 1;
+    const int nst = (te - kt0 + TS - 1) / TS;
+
+    // ---- staging: this thread's words of a stage. K: NW words of one key; V: NW
+    // tokens of one word's elements. A 16-key tile belongs to whole waves.
+    const int x = (int)threadIdx.x;
+    const int tt = x / (256 / TS);       // tile of the stage
+    const int xi = x % (256 / TS);       // thread of the tile
+    constexpr int KT = (DP / 8) / NW;    // threads of a key
+    const int kkey = xi / KT, kword = (xi % KT) * NW;
+    const int vword = xi % (DP / 8), vtok = xi / (DP / 8) * NW;
+    const int bs = a.tpb * 16;
+    struct Codes {
+        uint32_t kw[NW], vw[NW], ks, vs;
+    };
+    auto entry = [&](int u) { return trow[block_of(a, min(kt0 + TS * u + tt, te - 1))]; };
+    auto fetch = [&](int u, int blk, Codes& c) __attribute__((always_inline)) {
+        const int t = min(kt0 + TS * u + tt, te - 1);
+        const int off = (t - block_of(a, t) * a.tpb) * 16;
+        const int64_t row = (int64_t)blk * a.H + h;
+        ld_words<NW * 4>((const char*)(a.kc + (row * bs + off + kkey) * (DP / 8) + kword), c.kw);
+        c.ks = a.ks[(row * bs + off + kkey) * (DP / 32) + (kword >> 2)];
+        ld_words<NW * 4>((const char*)(a.vc + (row * (DP / 8) + vword) * bs + off + vtok), c.vw);
+        const uint8_t* vs = a.vs + (row * (DP / 32) + (vword >> 2)) * bs + off + vtok;
+        if constexpr (NW == 2) c.vs = *(const uint16_t*)vs;
+        else c.vs = *vs;
+    };
+    auto stage = [&](int u, char* stg, const Codes& c) __attribute__((always_inline)) {
+        const float ks = scale4(c.ks);
+        const int krow = tt * 16 + kkey;
+#pragma unroll
+        for (int k = 0; k < NW; ++k)
+            *(uint4*)(stg + krow * RB + (((kword + k) ^ ((kkey / RPB) & (NCH - 1))) << 4)) = octet4<DT>(c.kw[k], ks);
+#pragma unroll
+        for (int k = 0; k < NW; ++k) {
+            const int tok = vtok + k, key = (kt0 + TS * u + tt) * 16 + tok;
+            const bool live = key <= wglim && (!SC || key >= first);
+            const float vs = live ? scale4((c.vs >> (8 * k)) & 255u) : 1.f;
+            *(uint4*)(stg + HALF + (tt * 16 + tok) * RB + ((vword ^ (((tok & 3) / RPB) << 2)) << 4)) =
+                octet4<DT>(live ? c.vw[k] : 0u, vs);
+        }
+    };
+    auto sync = [&]() {
+        __builtin_amdgcn_s_waitcnt((15) | (3 << 14) | (7 << 4) | (0 << 8));  // lgkmcnt(0)
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+
+    float m = kMinM, l = 0.f;
+    float thr = SC ? kMinM + kLazyLog2 : (kMinM + kLazyLog2) * a.inv_scale_log2;
+    f32x16 acc[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+    uint32_t kaddr[NQ], vaddr[ND];
+#pragma unroll
+    for (int c = 0; c < NQ; ++c)
+        kaddr[c] = (uint32_t)((lane & 31) * RB + (((2 * c + hf) ^ ((j / RPB) & (NCH - 1))) << 4));
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+        vaddr[d] = (uint32_t)(HALF + (4 * hf + (j >> 2)) * RB +
+                              (((4 * d + 2 * ct + ((j & 3) >> 1)) ^ (((j >> 2) / RPB) << 2)) << 4) + 8 * (j & 1));
+
+    auto tile = [&](const char* stg, int key0) __attribute__((always_inline)) {
+        f32x16 st;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st[i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NQ; ++c) st = mfma32<DT>(*(const uint4*)(stg + kaddr[c]), qf[c], st);
+        if constexpr (SC) {
+            const float dist = (float)(key0 + 4 * hf - rpos[0]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                st[i] = scored<DT>(st[i], a.scale_log2, a.cap_in, a.cap_log2, slope, dist + (8 * (i >> 2) + (i & 3)));
+        }
+        if (key0 + 31 > minlim || (SC && key0 < first)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = key0 + 8 * (i >> 2) + 4 * hf + (i & 3);
+                st[i] = key <= lim && (!SC || key >= first) ? st[i] : kNegInf;
+            }
+        }
+        float lmax = st[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) lmax = fmax_prop(lmax, st[i]);
+        if (__builtin_amdgcn_ballot_w64(lmax > thr) != 0) {
+            auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(lmax), __float_as_uint(lmax), false, false);
+            const float cm = fmax_prop(__uint_as_float(r[0]), __uint_as_float(r[1]));
+            const float mn = fmaxf(m, SC ? cm : cm * a.scale_log2);
+            const float alpha = __builtin_amdgcn_exp2f(m - mn);
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
+            m = mn;
+            thr = SC ? mn + kLazyLog2 : (mn + kLazyLog2) * a.inv_scale_log2;
+        }
+        uint32_t pw[8];
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float p0 = __builtin_amdgcn_exp2f(SC ? st[2 * i] - m : __builtin_fmaf(st[2 * i], a.scale_log2, -m));
+            const float p1 =
+                __builtin_amdgcn_exp2f(SC ? st[2 * i + 1] - m : __builtin_fmaf(st[2 * i + 1], a.scale_log2, -m));
+            sum += p0 + p1;
+            pw[i] = pack2<DT>(p0, p1);
+        }
+        l += sum;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const uint4 pf = make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                const uint2 v0 = ld_tr16(stg + vaddr[d] + (16 * k) * RB);
+                const uint2 v1 = ld_tr16(stg + vaddr[d] + (16 * k + 8) * RB);
+                acc[d] = mfma32<DT>(make_uint4(v0.x, v0.y, v1.x, v1.y), pf, acc[d]);
+            }
+        }
+    };
+
+    if (nst > 0) {
+        Codes c;
+        fetch(0, entry(0), c);
+        int blk = entry(1);
+        stage(0, attn_lds, c);
+        fetch(1, blk, c);
+        blk = entry(2);
+        sync();
+        for (int u = 0; u < nst; ++u) {
+            // the buffer being written was read in the round before, which every
+            // wave has left; the codes in flight meanwhile are two stages ahead
+            if (u + 1 < nst) {
+                stage(u + 1, attn_lds + ((u + 1) & 1) * STG, c);
+                fetch(u + 2, blk, c);
+                blk = entry(u + 3);
+            }
+            const char* stg = attn_lds + (u & 1) * STG;
+            const int key0 = (kt0 + TS * u) * 16;
+#pragma unroll
+            for (int v = 0; v < KEYS / 32; ++v)
+                if (key0 + 32 * v <= maxlim) tile(stg + v * 32 * RB, key0 + 32 * v);
+            sync();
+        }
+    }
+
+    // ---- finish: lane (hf, column) holds elements 32d + 8b + 4hf .. + 3
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+    const float lt = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    const float inv = lt > 0.f ? 1.f / lt : 0.f;
+    char* dst = nullptr;
+    if (valid)
+        dst = pslot < 0 ? a.out + ((int64_t)prow * a.o_sr + (int64_t)qhead * a.o_sh) * 2
+                        : partial_out<DT>(a, pslot + ct, j, 0);
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int b = 0; b < 4; b += 2) {
+            uint32_t w[2][2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    w[e][k] = f32_to_bits<DT>(acc[d][4 * (b + e) + 2 * k] * inv) |
+                              (f32_to_bits<DT>(acc[d][4 * (b + e) + 2 * k + 1] * inv) << 16);
+            auto y = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+            auto z = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+            if (valid) *(uint4*)(dst + (32 * d + 8 * (b + hf)) * 2) = make_uint4(y[0], z[0], y[1], z[1]);
+        }
+    if (pslot >= 0 && valid && hf == 0) {
+        partial_ml(a, pslot + ct)[j] = m;
+        partial_ml(a, pslot + ct)[16 + j] = lt;
+    }
+}
+
+template <int DP>
+constexpr int lds4(bool wide) {
+    if constexpr (DP == 256) return coop_lds_bytes<DP>();
+    else return wide && wide_lds4<DP>() > coop_lds_bytes<DP>() ? wide_lds4<DP>() : coop_lds_bytes<DP>();
+}
+
+// WIDE: the launch also has wide items, in the workgroups after the narrow ones.
+template <int DT, int DP, bool SC, bool WIDE>
+__global__ __launch_bounds__(256) void attn4_kernel(const int32_t* items, Attn4Args a, int narrow_blocks,
+                                                    const int32_t* wide_items, int wide_num, const int32_t* wide_count) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int b = blockIdx.x;
+    if (!WIDE || b < narrow_blocks) {
+        const int item = b * kWaves + wave;
+        const int32_t* it = items + (int64_t)item * MF_PLAN_ITEM_INTS;
+        if (item >= (a.dev_count ? *a.dev_count : a.num_items)) return;
+        const bool coop = it[11] != 0;  // of the whole workgroup
+        if (!coop && it[3] == 0) return;  // padding
+        attn4_narrow<DT, DP, SC>(a, it, wave, 0, coop);
+        return;
+    }
+    if constexpr (WIDE && DP < 256) {
+        const int block = b - narrow_blocks;
+        const int num = wide_count ? *wide_count : wide_num;
+        if (block * kWaves >= num) return;
+        const int32_t* i0 = wide_items + (int64_t)block * kWaves * MF_PLAN_ITEM_INTS;
+        int cols[kWaves][2];
+        bool same = true;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const int32_t* iw = i0 + w * MF_PLAN_ITEM_INTS;
+            cols[w][0] = iw[2];
+            cols[w][1] = iw[3];
+            same = same & (iw[0] == i0[0]) & (iw[1] == i0[1]) & (iw[4] == i0[4]) & (iw[5] == i0[5]);
+        }
+        const int32_t* it = i0 + wave * MF_PLAN_ITEM_INTS;
+        if (same) {
+            attn4_wide<DT, DP, SC>(a, it, wave, cols);
+        } else {
+            // a workgroup of unrelated short items: each wave its own, a column
+            // tile at a time
+#pragma unroll 1
+            for (int ct = 0; ct < it[3]; ++ct) attn4_narrow<DT, DP, SC>(a, it, wave, ct, false);
+        }
+    }
+}
+
+template <int DT, int DP, bool SC>
+int launch4(Attn4Args a, const int32_t* items, int64_t n_narrow, int64_t n_wide, const int32_t* merges,
+            int64_t n_merges, const int32_t* dev_counts, hipStream_t stream) {
+    if (DP == 256 && n_wide > 0) return MF_ERR_ARG;  // the plan was made for another head_dim
+    if (n_narrow + n_wide > 0) {
+        a.num_items = (int)n_narrow;
+        a.dev_count = dev_counts;
+        const int32_t* wide = items + n_narrow * MF_PLAN_ITEM_INTS;
+        const int nb = (int)(n_narrow / kWaves);
+        const dim3 grid((unsigned)((n_narrow + n_wide) / kWaves));
+        if (n_wide > 0)
+            hipLaunchKernelGGL((attn4_kernel<DT, DP, SC, true>), grid, dim3(256), lds4<DP>(true), stream, items, a, nb,
+                               wide, (int)n_wide, dev_counts ? dev_counts + 1 : nullptr);
+        else
+            hipLaunchKernelGGL((attn4_kernel<DT, DP, SC, false>), grid, dim3(256), lds4<DP>(false), stream, items, a, nb,
+                               wide, 0, (const int32_t*)nullptr);
+        if (int st = check_launch()) return st;
+    }
+    if (n_merges > 0) {
+        a.dev_count = dev_counts ? dev_counts + 2 : nullptr;
+        return launch_merge<DT, DP>(a, merges, n_merges, stream);
+    }
+    return MF_OK;
+}
+
+}  // namespace
+}  // namespace mf
+
+extern "C" int mf_paged_attention4(const mf_scoring* scoring, const void* q, int64_t q_stride_row,
+                                   int64_t q_stride_head, void* out, int64_t out_stride_row, int64_t out_stride_head,
+                                   int dtype, const mf_pool4* pool, const int32_t* block_tables,
+                                   int64_t block_table_stride, const int32_t* cu_seqlens, const int32_t* kv_lens,
+                                   const int64_t* positions, const int32_t* row_map, int num_q_heads, float scale,
+                                   const int32_t* plan_items, int64_t num_items_narrow, int64_t num_items_wide,
+                                   const int32_t* plan_merges, int64_t num_merges, const int32_t* device_counts,
+                                   float* partials, int64_t partials_floats, mf_stream_t stream) {
+    using namespace mf;
+    if (int st = check_pool4(pool)) return st;
+    if (!dtype_ok(dtype) || dtype == MF_F32) return MF_ERR_UNSUPPORTED;
+    if (dtype != pool->dtype) return MF_ERR_ARG;
+    if (!(std::fabs(scale) < INFINITY) || num_q_heads <= 0 || num_q_heads % pool->num_heads) return MF_ERR_ARG;
+    if (num_items_narrow < 0 || num_items_wide < 0 || num_merges < 0 || num_items_narrow % kWaves ||
+        num_items_wide % kWaves)
+        return MF_ERR_ARG;
+    if (num_items_narrow + num_items_wide == 0 && num_merges == 0) return MF_OK;
+    if (!q || !out || !block_tables || !cu_seqlens || !kv_lens || !positions) return MF_ERR_ARG;
+    if (num_items_narrow + num_items_wide > 0 && !plan_items) return MF_ERR_ARG;
+    if (num_merges > 0 && (!plan_merges || !partials || partials_floats <= 0)) return MF_ERR_WORKSPACE;
+    if ((q_stride_row | q_stride_head) % 8 || (uintptr_t)q % 16) return MF_ERR_ARG;
+    const int out_align = std::min(16, 4 * (pool->head_dim / 16) * 2);
+    if ((out_stride_row * 2) % out_align || (out_stride_head * 2) % out_align || (uintptr_t)out % out_align)
+        return MF_ERR_ARG;
+    Attn4Args a{};
+    a.q = (const char*)q;
+    a.q_sr = q_stride_row;
+    a.q_sh = q_stride_head;
+    a.out = (char*)out;
+    a.o_sr = out_stride_row;
+    a.o_sh = out_stride_head;
+    a.block_size = pool->block_size;
+    a.block_tables = block_tables;
+    a.bt_stride = block_table_stride;
+    a.positions = positions;
+    a.row_map = row_map;
+    a.H = a.num_kv_heads = pool->num_heads;
+    a.G = num_q_heads / pool->num_heads;
+    a.head_dim = pool->head_dim;
+    a.kc = pool->key_codes;
+    a.ks = pool->key_scales;
+    a.vc = pool->value_codes;
+    a.vs = pool->value_scales;
+    a.tpb = pool->block_size / 16;
+    a.tpb_magic = a.tpb > 1 ? (uint32_t)(((1ull << 32) + a.tpb - 1) / a.tpb) : 0u;
+    // as in mf_paged_attention: a negative scale turns q's signs, a zero one becomes
+    // 2^-100
+    a.q_sign = scale < 0.f ? 0x80008000u : 0u;
+    a.scale_log2 = scale == 0.f ? 0x1p-100f : std::fabs(scale) * 1.4426950408889634f;
+    a.inv_scale_log2 = 1.f / a.scale_log2;
+    a.partials = partials;
+    a.part_dstride = part_dstride_for(pool->head_dim);
+    a.merges = plan_merges;
+    if (scoring) {
+        if (int st = set_scoring(a, *scoring)) return st;
+    }
+    hipStream_t st = (hipStream_t)stream;
+#define MF_ATTN4_CASE(DT, DPV)                                                                                       \
+    if (dtype == DT && pool->head_dim == DPV)                                                                        \
+        return scoring ? launch4<DT, DPV, true>(a, plan_items, num_items_narrow, num_items_wide, plan_merges,        \
+                                                num_merges, device_counts, st)                                       \
+                       : launch4<DT, DPV, false>(a, plan_items, num_items_narrow, num_items_wide, plan_merges,       \
+                                                 num_merges, device_counts, st);
+    MF_ATTN4_CASE(MF_BF16, 32)
+    MF_ATTN4_CASE(MF_BF16, 64)
+    MF_ATTN4_CASE(MF_BF16, 128)
+    MF_ATTN4_CASE(MF_BF16, 256)
+    MF_ATTN4_CASE(MF_F16, 32)
+    MF_ATTN4_CASE(MF_F16, 64)
+    MF_ATTN4_CASE(MF_F16, 128)
+    MF_ATTN4_CASE(MF_F16, 256)
+#undef MF_ATTN4_CASE
+    return MF_ERR_UNSUPPORTED;
+}

@@ -1,7 +1,6 @@
 // Planners and C entry points of the varlen paged attention (the kernels are in
 // attn_kernels.h).
 #include <atomic>
-#include <cfloat>
 #include <mutex>
 #include <vector>
 
@@ -1056,16 +1055,7 @@ int paged_attention_impl(
         return MF_ERR_UNSUPPORTED;
     if (scoring) {
         if (sliced || merge_counters) return MF_ERR_UNSUPPORTED;
-        if (!(scoring->softcap >= 0.f) || !(scoring->softcap < INFINITY)) return MF_ERR_ARG;
-        a.slopes = scoring->slopes;
-        a.first_keys = scoring->first_keys;
-        a.prefix_lens = scoring->prefix_lens;
-        a.cap_in = scoring->softcap > 0.f ? 2.f * a.scale_log2 / scoring->softcap : 0.f;
-        a.cap_log2 = scoring->softcap * 1.4426950408889634f;
-        // a cap so small or so large against the scale that the quotient leaves
-        // fp32's normal numbers
-        if (scoring->softcap > 0.f && !(a.cap_in >= FLT_MIN && a.cap_in < INFINITY && a.cap_log2 < INFINITY))
-            return MF_ERR_ARG;
+        if (int se = set_scoring(a, *scoring)) return se;
         return launch_scored(dtype, DP, tail_inflight, a, plan_items, num_items_narrow, num_items_wide, plan_merges,
                              num_merges, fast, device_counts, st);
     }

@@ -108,13 +108,15 @@ def run_varlen(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: nat.PoolView,
     # the whole array is not in range)
     if int(tables64.min()) < 0 or int(tables64.max()) >= nblocks:
         _check_ids(tables, order, need, nblocks)
-    nat.require_device(q_rows, out_rows, pool.k)
+    four = isinstance(pool, nat.Pool4View)
+    nat.require_device(q_rows, out_rows, pool.key_codes if four else pool.k)
     # a large decode step on 16-token blocks runs as one round of slices
-    sliceable = identity and pool_lens is None and pool.block_size == 16 and not scoring.active
+    sliceable = identity and pool_lens is None and pool.block_size == 16 and not scoring.active and not four
     items, merges, counts, sliced = nat.plan_host(cu, kvl, hq, num_kv_heads, d, q_rows.dtype, dev,
                                                   decode_slices=sliceable,
                                                   first_keys=firsts if masked_first else None,
-                                                  prefix_lens=prefixes if masked_prefix else None)
+                                                  prefix_lens=prefixes if masked_prefix else None,
+                                                  kv_bits=4 if four else 16)
     # tables, plan, cu/kv lengths, positions, row map and pool lengths cross
     # to the device in one copy (none when the same bytes crossed before on
     # this stream), and the launch addresses them inside that one buffer

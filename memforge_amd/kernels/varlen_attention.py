@@ -108,6 +108,27 @@ def paged_attention_varlen_materialised(query: torch.Tensor, pool, layer_idx: in
     return _run(query, pool.key_pool[layer_idx], pool.value_pool[layer_idx], tables, seq_ids, positions, scale)
 
 
+def paged_attention_varlen_pool(query: torch.Tensor, pool, layer_idx: int, block_tables: Sequence[torch.Tensor],
+                                seq_ids: Sequence[int], positions: Sequence[int], scale: Optional[float] = None,
+                                softcap: Optional[float] = None, slopes: Optional[torch.Tensor] = None,
+                                doc_starts: Optional[Sequence[int]] = None,
+                                prefix_lens: Optional[Sequence[int]] = None) -> torch.Tensor:
+    """``paged_attention_varlen`` over a pool object of either kind: ``PagedKVPool``, or
+    ``PagedKVPool4``, whose keys and values are held in 4 bits (fp16 or bf16 pools;
+    the query is taken to the pool's dtype)."""
+    view = pool.layer_view(layer_idx)
+    nat.require_device(query)
+    tables = _validate(query, view.num_heads, seq_ids, positions, block_tables, pool.block_size, False)
+    q = query[0].to(pool.spec.dtype).permute(1, 0, 2)  # (T, H, D)
+    if q.stride(-1) != 1:
+        q = q.contiguous()
+    total, heads, dim = q.shape
+    out = torch.empty((1, heads, total, dim), dtype=q.dtype, device=query.device)
+    run_varlen(q, out[0].permute(1, 0, 2), view, tables, list(seq_ids), list(positions), scale, view.num_heads,
+               softcap=softcap, slopes=slopes, doc_starts=doc_starts, prefix_lens=prefix_lens)
+    return out.to(query.dtype)
+
+
 def reference_varlen_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor,
                                layer_idx: int, block_tables: Sequence[torch.Tensor], seq_ids: Sequence[int],
                                positions: Sequence[int], block_size: int,

@@ -2,7 +2,7 @@
 sampling, the engine and speculative verification (the reference package
 memforge_ml/runtime/__init__.py exports the same names)."""
 
-from memforge_amd.runtime.kv_pool import ModelKVSpec, PagedKVPool
+from memforge_amd.runtime.kv_pool import ModelKVSpec, PagedKVPool, PagedKVPool4
 from memforge_amd.runtime.paged_cache import PagedCache, PagedCacheLayer
 from memforge_amd.runtime.sampling import SamplingParams, sample_logits
 from memforge_amd.runtime.continuous_engine import (
@@ -16,6 +16,7 @@ from memforge_amd.runtime.continuous_engine import (
 __all__ = [
     "ModelKVSpec",
     "PagedKVPool",
+    "PagedKVPool4",
     "PagedCache",
     "PagedCacheLayer",
     "SamplingParams",

@@ -157,3 +157,147 @@ class PagedKVPool:
             "block_table_dtype": "int32",
             "slot_mapping_dtype": "int64",
         }
+
+
+class PagedKVPool4:
+    """A physical block pool that holds K and V in 4 bits: ``PagedKVPool``'s
+    interface over a quarter of its bytes (and a sixteenth for the scales).
+
+    The format is the OCP microscaling one: e2m1 codes and one power-of-two scale
+    for 32 consecutive elements of a token's head, which gfx950 converts in
+    hardware. Rows are rounded when they are written; reads give the values they
+    stand for, in ``spec.dtype``. Attention runs over it in place
+    (``_native.paged_attention``, ``paged_attention_varlen_pool``) where
+    ``spec.dtype`` is float16 or bfloat16. head_dim is 32, 64, 128 or 256,
+    block_size a multiple of 16 up to 512. A group with a NaN or an infinity reads
+    as NaN.
+
+    ``key_codes`` (int32) is (layers, blocks, heads, slots, head_dim / 8) and
+    ``value_codes`` (layers, blocks, heads, head_dim / 8, slots), eight codes to a
+    word; ``key_scales`` and ``value_scales`` (uint8) hold the exponents."""
+
+    kv_bits = 4
+
+    def __init__(self, spec: ModelKVSpec, num_blocks: int, block_size: int = 16):
+        _require_gpu_device(spec.device)
+        self._check_format(spec, block_size)
+        self.spec = spec
+        self.num_blocks = num_blocks
+        self.block_size = block_size
+        words, groups = spec.head_dim // 8, spec.head_dim // nat.GROUP4
+        lead = (spec.num_layers, num_blocks, spec.num_kv_heads)
+
+        def zeros(tail, dtype):
+            return torch.zeros(lead + tail, dtype=dtype, device=spec.device)
+
+        self.key_codes = zeros((block_size, words), torch.int32)
+        self.key_scales = zeros((block_size, groups), torch.uint8)
+        self.value_codes = zeros((words, block_size), torch.int32)
+        self.value_scales = zeros((groups, block_size), torch.uint8)
+        self._views = {}
+
+    @staticmethod
+    def _check_format(spec: ModelKVSpec, block_size: int) -> None:
+        if spec.head_dim not in nat.HEAD_DIMS4:
+            raise ValueError(f"a 4-bit pool holds head_dims {nat.HEAD_DIMS4}, got {spec.head_dim}")
+        if block_size <= 0 or block_size % 16 or block_size > 512:
+            raise ValueError(f"a 4-bit pool's block_size is a multiple of 16 up to 512, got {block_size}")
+        nat.dtype_code(spec.dtype)
+
+    # ---------------------------------------------------------------- sizing
+
+    @staticmethod
+    def _bytes_per_token(spec: ModelKVSpec) -> int:
+        return 2 * spec.num_layers * spec.num_kv_heads * (spec.head_dim // 2 + spec.head_dim // nat.GROUP4)
+
+    @property
+    def bytes_per_token(self) -> int:
+        """KV bytes of one token across all layers, scales included."""
+        return self._bytes_per_token(self.spec)
+
+    @property
+    def bytes_per_block(self) -> int:
+        return self.bytes_per_token * self.block_size
+
+    @property
+    def total_bytes(self) -> int:
+        return self.bytes_per_block * self.num_blocks
+
+    @property
+    def capacity_tokens(self) -> int:
+        return self.num_blocks * self.block_size
+
+    @staticmethod
+    def blocks_for_budget(spec: ModelKVSpec, block_size: int, budget_mb: float) -> int:
+        """Largest number of physical blocks inside a memory budget."""
+        return max(1, int((budget_mb * 1024 * 1024) // (PagedKVPool4._bytes_per_token(spec) * block_size)))
+
+    # -------------------------------------------------------------- indexing
+
+    slot_indices = PagedKVPool.slot_indices
+    flat_indices = PagedKVPool.flat_indices
+    block_table_tensor = staticmethod(PagedKVPool.block_table_tensor)
+
+    # ----------------------------------------------------------------- I / O
+
+    def layer_view(self, layer_idx: int) -> nat.Pool4View:
+        arrays = (self.key_codes, self.key_scales, self.value_codes, self.value_scales)
+        held, view = self._views.get(layer_idx, ((), None))
+        if view is None or any(x is not y for x, y in zip(held, arrays)):
+            view = nat.Pool4View(*(x[layer_idx] for x in arrays), self.spec.dtype)
+            self._views[layer_idx] = (arrays, view)
+        return view
+
+    def write(self, layer_idx: int, physical: torch.Tensor, slots: torch.Tensor, keys: torch.Tensor,
+              values: torch.Tensor) -> None:
+        """Round ``(1, num_kv_heads, T, head_dim)`` K/V into (physical, slot)."""
+        self.write_flat(layer_idx, paged_gather.flat_slot_index(physical, slots, self.block_size), keys, values)
+
+    def write_flat(self, layer_idx: int, flat_index: torch.Tensor, keys: torch.Tensor, values: torch.Tensor) -> None:
+        nat.kv4_write(keys[0].permute(1, 0, 2), values[0].permute(1, 0, 2), flat_index.reshape(-1),
+                      self.layer_view(layer_idx))
+
+    def gather(self, layer_idx: int, physical: torch.Tensor, slots: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The values of (physical, slot) as contiguous ``(1, num_kv_heads, T, head_dim)`` K/V."""
+        return self.gather_flat(layer_idx, paged_gather.flat_slot_index(physical, slots, self.block_size))
+
+    def gather_flat(self, layer_idx: int, flat_index: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        spec = self.spec
+        k = torch.empty((1, spec.num_kv_heads, flat_index.numel(), spec.head_dim), dtype=spec.dtype,
+                        device=self.key_codes.device)
+        v = torch.empty_like(k)
+        nat.kv4_gather(self.layer_view(layer_idx), flat_index.reshape(-1), k[0].permute(1, 0, 2),
+                       v[0].permute(1, 0, 2))
+        return k, v
+
+    def copy_blocks(self, pairs) -> None:
+        """Copy block ``src`` to ``dst`` for every pair, in every layer
+        (``prefix_sharing.copy_blocks``): codes and scales move as they are."""
+        for k, v in ((self.key_codes, self.value_codes), (self.key_scales, self.value_scales)):
+            # a block of a layer as one run of 4-byte words
+            k, v = (x.reshape(x.shape[0], x.shape[1], 1, 1, -1).view(torch.float32) for x in (k, v))
+            nat.kv_copy_blocks(k, v, pairs)
+
+    def zero_(self) -> None:
+        for x in (self.key_codes, self.key_scales, self.value_codes, self.value_scales):
+            x.zero_()
+
+    def describe(self) -> dict:
+        return {
+            "num_blocks": self.num_blocks,
+            "block_size": self.block_size,
+            "capacity_tokens": self.capacity_tokens,
+            "bytes_per_token": self.bytes_per_token,
+            "bytes_per_block": self.bytes_per_block,
+            "total_mb": round(self.total_bytes / (1024 * 1024), 2),
+            "num_layers": self.spec.num_layers,
+            "num_kv_heads": self.spec.num_kv_heads,
+            "head_dim": self.spec.head_dim,
+            "dtype": str(self.spec.dtype),
+            "device": self.spec.device,
+            "layout": "codes (layers, blocks, kv_heads, block_size, head_dim / 8) words of eight e2m1 elements, "
+                      "values (layers, blocks, kv_heads, head_dim / 8, block_size); one e8m0 byte for 32 elements",
+            "element_bits": 4,
+            "block_table_dtype": "int32",
+            "slot_mapping_dtype": "int64",
+        }

@@ -10,7 +10,7 @@ import itertools
 from typing import Any, Dict, Iterable, List, Optional, Sequence, Tuple
 
 from memforge_amd import _native
-from memforge_amd.runtime.kv_pool import PagedKVPool
+from memforge_amd.runtime.kv_pool import PagedKVPool, PagedKVPool4
 
 
 def copy_block(pool: PagedKVPool, src: int, dst: int) -> None:
@@ -29,7 +29,10 @@ def copy_blocks(pool: PagedKVPool, pairs: Sequence[Tuple[int, int]]) -> None:
     pairs = [(int(s), int(d)) for s, d in pairs]
     if not pairs:
         return
-    _native.kv_copy_blocks(pool.key_pool, pool.value_pool, pairs)
+    if isinstance(pool, PagedKVPool4):
+        pool.copy_blocks(pairs)
+    else:
+        _native.kv_copy_blocks(pool.key_pool, pool.value_pool, pairs)
 
 
 def block_owners(runtimes: Iterable[Tuple[int, List[int]]], total_blocks: int) -> Dict[str, List[int]]:

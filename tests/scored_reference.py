@@ -67,3 +67,29 @@ def check(got, out, weight, size, dtype, d, keys, softcap=0.0, what=""):
     over = (got - out).abs() / bound(out, weight, size, dtype, d, keys, softcap).clamp_min(1e-30)
     worst = float(over.max()) if over.numel() else 0.0
     assert worst <= 1.0, f"{what}: {worst:.2f} of the bound at {np.unravel_index(int(over.argmax()), over.shape)}"
+
+
+LEVELS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def round4(x, dtype):
+    """The values rows stand for in a 4-bit pool whose attention runs in ``dtype``: per 32 elements the smallest permitted
+    power of two whose sevenfold reaches the largest magnitude, then the nearest level (the even one on a tie); a
+    group with a NaN or an infinity is NaN. Float64."""
+    g = x.detach().cpu().double().unflatten(-1, (-1, 32)).numpy()
+    lo, hi = (-23, 13) if dtype == torch.float16 else (-125, 125)
+    top = np.abs(g).max(-1, keepdims=True)
+    bad = ~np.isfinite(g).all(-1, keepdims=True)
+    top = np.where(bad | (top == 0), 1.0, top)
+    e = np.frexp(top)[1] - 3  # top < 2^(e + 3), so 7 * 2^(e - 1) < top
+    e = np.where(7.0 * np.exp2(e.astype(np.float64)) < top, e + 1, e)
+    e = np.where((np.abs(g).max(-1, keepdims=True) == 0) & ~bad, lo, e)
+    step = np.exp2(np.clip(e, lo, hi).astype(np.float64))
+    # past 8 the nearest level is 6 in any case (and past 2^53 a difference to a level is rounded away)
+    r = np.minimum(np.abs(np.where(bad, 0.0, g)) / step, 8.0)
+    gap = np.abs(r[..., None] - np.array(LEVELS))
+    near = gap == gap.min(-1, keepdims=True)
+    even = np.array([i % 2 == 0 for i in range(8)])
+    code = np.where((near & even).any(-1), (near & even).argmax(-1), near.argmax(-1))
+    out = np.where(bad, np.nan, np.sign(np.where(bad, 0.0, g)) * np.array(LEVELS)[code] * step)
+    return torch.from_numpy(out).flatten(-2)

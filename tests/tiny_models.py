@@ -62,3 +62,18 @@ def hf_greedy(model, prompt_ids: List[int], max_new_tokens: int, eos_ids=(1,), s
             return generated
         out = model(input_ids=torch.tensor([[tok]], dtype=torch.long, device=device), past_key_values=cache,
                     use_cache=True)
+
+
+def tiny_capped(seed: int = 0, device="cuda:0", dtype=torch.float32, softcap: float = 2.0):
+    """A Gemma2 model of the same size: its attention scores are capped by a tanh."""
+    from transformers import Gemma2Config, Gemma2ForCausalLM
+
+    torch.manual_seed(seed)
+    config = Gemma2Config(vocab_size=VOCAB_SIZE, hidden_size=64, intermediate_size=128, num_hidden_layers=2,
+                          num_attention_heads=4, num_key_value_heads=2, head_dim=32, max_position_embeddings=1024,
+                          sliding_window=1024, attn_logit_softcapping=softcap, query_pre_attn_scalar=2,
+                          initializer_range=0.3, tie_word_embeddings=False, eos_token_id=1, bos_token_id=0, pad_token_id=0)
+    config._attn_implementation = "eager"  # the oracle's: transformers' other kernels drop the cap
+    model = Gemma2ForCausalLM(config).to(device=device, dtype=dtype)
+    model.eval()
+    return model
