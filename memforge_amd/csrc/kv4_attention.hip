@@ -48,10 +48,9 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
 
 constexpr int kDepth4 = 3;  // register buffers of the decode loop, 32 keys each
 
-// One wave, one 16-column tile (c0 + ct of its item), the item's keys.
+// One wave: the 16-column tile and the keys of its item.
 template <int DT, int DP, bool SC>
-__device__ __forceinline__ void attn4_narrow(const Attn4Args& a, const int32_t* it, const int wave, const int ct,
-                                             const bool coop) {
+__device__ __forceinline__ void attn4_narrow(const Attn4Args& a, const int32_t* it, const int wave, const bool coop) {
     constexpr int KW = DP / 32;                // words of a lane's K per 16 keys
     constexpr int VCH = DP / 16;               // head_dim elements of a lane's V per key
     constexpr int VW = DP == 256 ? 8 : 4;      // words of its V per 16 keys
@@ -59,8 +58,7 @@ __device__ __forceinline__ void attn4_narrow(const Attn4Args& a, const int32_t* 
     constexpr float kNegInf = -__builtin_huge_valf();
     const int lane = threadIdx.x & 63;
     const int g = lane >> 4, j = lane & 15;
-    const int s = it[0], h = it[1], c0 = it[2] + ct, kt0 = it[4], kt1 = it[5];
-    const int pslot = it[6] < 0 ? -1 : it[6] + ct;
+    const int s = it[0], h = it[1], c0 = it[2], kt0 = it[4], kt1 = it[5], pslot = it[6];
     const int row0 = it[8], ncols = it[9] * a.G, kv_len = it[10];
     int first = 0, prefix = 0;
     if constexpr (SC) {
@@ -75,7 +73,7 @@ __device__ __forceinline__ void attn4_narrow(const Attn4Args& a, const int32_t* 
 
     // ---- this lane's column
     const int cidx = c0 * 16 + j;
-    const bool valid = cidx < ncols && ct < it[3];
+    const bool valid = cidx < ncols && it[3] > 0;
     const int r = valid ? cidx / a.G : 0;
     int prow = row0 + r;
     if (a.row_map) prow = a.row_map[prow];
@@ -346,27 +344,32 @@ __device__ __forceinline__ void attn4_narrow(const Attn4Args& a, const int32_t* 
 }
 
 // ------------------------------------------------------- workgroup-shared items
-// Keys of a stage: two 8 KB (K and V of 32 keys at D 128, of 64 below) buffers.
-constexpr int wide_keys4(int dp) { return dp >= 128 ? 32 : 64; }
+// Keys of a stage (two buffers of K and V rows, 64 KB of LDS at D 128) and of one
+// softmax step. Two chunks of 2048 rows after up to 6144 keys, 40/8 heads x 128 (450
+// GFLOP): 541 us with stages and steps of 32 keys at three waves per SIMD, 487 with
+// stages of 64 at two, 472 with steps of 64 as well (952 TFLOP/s): two score chains at
+// once, one test of the maximum for both, half the barriers.
+constexpr int kWideKeys4 = 64;
 template <int DP>
-constexpr int wide_lds4() { return 2 * 2 * wide_keys4(DP) * DP * 2; }
+constexpr int wide_lds4() { return 2 * 2 * kWideKeys4 * DP * 2; }
 
-// cols: first column tile and tiles of the workgroup's four items.
+// `it` is this wave's item, nct the column tiles it takes of it; cols holds the first
+// column tile and the tiles of all four.
 template <int DT, int DP, bool SC>
-__device__ __forceinline__ void attn4_wide(const Attn4Args& a, const int32_t* it, const int wave,
+__device__ __forceinline__ void attn4_wide(const Attn4Args& a, const int32_t* it, const int nct,
                                            const int (&cols)[kWaves][2]) {
     constexpr int RB = DP * 2;       // bytes of a key's row in LDS
     constexpr int NCH = RB / 16;     // 16-byte chunks of a row: the eight elements of a word
-    constexpr int KEYS = wide_keys4(DP), TS = KEYS / 16;
+    constexpr int KEYS = kWideKeys4, TS = KEYS / 16;
     constexpr int RPB = 256 / RB;    // rows in 256 bytes
     constexpr int NQ = DP / 16, ND = DP / 32;
     constexpr int HALF = KEYS * RB, STG = 2 * HALF;
     constexpr int NW = KEYS * (DP / 8) / 256;  // words of a thread's K (and V) per stage
-    static_assert(NW == 1 || NW == 2, "stage layout");
+    static_assert(NW == 1 || NW == 2 || NW == 4, "stage layout");
     constexpr float kNegInf = -__builtin_huge_valf();
     const int lane = threadIdx.x & 63;
     const int hf = lane >> 5;
-    const int s = it[0], h = it[1], c0 = it[2], nct = it[3], kt0 = it[4], kt1 = it[5], pslot = it[6];
+    const int s = it[0], h = it[1], c0 = it[2], kt0 = it[4], kt1 = it[5], pslot = it[6];
     const int row0 = it[8], nrows = it[9], kv_len = it[10];
     int first = 0, prefix = 0;
     if constexpr (SC) {
@@ -428,43 +431,60 @@ __device__ __forceinline__ void attn4_wide(const Attn4Args& a, const int32_t* it
     const int nst = (te - kt0 + TS - 1) / TS;
 
     // ---- staging: this thread's words of a stage. K: NW words of one key; V: NW
-    // tokens of one word's elements. A 16-key tile belongs to whole waves.
+    // tokens of one word's elements. A 16-key tile belongs to whole waves, so a
+    // stage's addresses are scalar bases and lane offsets that never change.
     const int x = (int)threadIdx.x;
-    const int tt = x / (256 / TS);       // tile of the stage
-    const int xi = x % (256 / TS);       // thread of the tile
-    constexpr int KT = (DP / 8) / NW;    // threads of a key
+    const int tt = __builtin_amdgcn_readfirstlane(x / (256 / TS));  // tile of the stage
+    const int xi = x % (256 / TS);                                  // thread of the tile
+    constexpr int KT = (DP / 8) / NW;                               // threads of a key
     const int kkey = xi / KT, kword = (xi % KT) * NW;
     const int vword = xi % (DP / 8), vtok = xi / (DP / 8) * NW;
     const int bs = a.tpb * 16;
+    const uint32_t kc_lane = (uint32_t)(kkey * (DP / 8) + kword) * 4, ks_lane = (uint32_t)(kkey * (DP / 32) + (kword >> 2));
+    const uint32_t vc_lane = (uint32_t)(vword * bs + vtok) * 4, vs_lane = (uint32_t)((vword >> 2) * bs + vtok);
+    uint32_t k_dst[NW], v_dst[NW];  // bytes inside a stage
+#pragma unroll
+    for (int k = 0; k < NW; ++k) {
+        k_dst[k] = (uint32_t)((tt * 16 + kkey) * RB + (((kword + k) ^ ((kkey / RPB) & (NCH - 1))) << 4));
+        v_dst[k] = (uint32_t)(HALF + (tt * 16 + vtok + k) * RB + ((vword ^ ((((vtok + k) & 3) / RPB) << 2)) << 4));
+    }
     struct Codes {
         uint32_t kw[NW], vw[NW], ks, vs;
     };
     auto entry = [&](int u) { return trow[block_of(a, min(kt0 + TS * u + tt, te - 1))]; };
-    auto fetch = [&](int u, int blk, Codes& c) __attribute__((always_inline)) {
+    auto fetch = [&](int u, int entry_, Codes& c) __attribute__((always_inline)) {
         const int t = min(kt0 + TS * u + tt, te - 1);
         const int off = (t - block_of(a, t) * a.tpb) * 16;
-        const int64_t row = (int64_t)blk * a.H + h;
-        ld_words<NW * 4>((const char*)(a.kc + (row * bs + off + kkey) * (DP / 8) + kword), c.kw);
-        c.ks = a.ks[(row * bs + off + kkey) * (DP / 32) + (kword >> 2)];
-        ld_words<NW * 4>((const char*)(a.vc + (row * (DP / 8) + vword) * bs + off + vtok), c.vw);
-        const uint8_t* vs = a.vs + (row * (DP / 32) + (vword >> 2)) * bs + off + vtok;
-        if constexpr (NW == 2) c.vs = *(const uint16_t*)vs;
-        else c.vs = *vs;
+        const int64_t row = (int64_t)__builtin_amdgcn_readfirstlane(entry_) * a.H + h;
+        ld_words<NW * 4>((const char*)(a.kc + (row * bs + off) * (DP / 8)) + kc_lane, c.kw);
+        c.ks = (a.ks + (row * bs + off) * (DP / 32))[ks_lane];
+        ld_words<NW * 4>((const char*)(a.vc + row * (DP / 8) * bs + off) + vc_lane, c.vw);
+        const uint8_t* vs = a.vs + row * (DP / 32) * bs + off;
+        if constexpr (NW == 4) c.vs = *(const uint32_t*)(vs + vs_lane);
+        else if constexpr (NW == 2) c.vs = *(const uint16_t*)(vs + vs_lane);
+        else c.vs = vs[vs_lane];
     };
-    auto stage = [&](int u, char* stg, const Codes& c) __attribute__((always_inline)) {
+    auto stage = [&](int u, char* stg, Codes& c) __attribute__((always_inline)) {
         const float ks = scale4(c.ks);
-        const int krow = tt * 16 + kkey;
 #pragma unroll
-        for (int k = 0; k < NW; ++k)
-            *(uint4*)(stg + krow * RB + (((kword + k) ^ ((kkey / RPB) & (NCH - 1))) << 4)) = octet4<DT>(c.kw[k], ks);
+        for (int k = 0; k < NW; ++k) *(uint4*)(stg + k_dst[k]) = octet4<DT>(c.kw[k], ks);
+        uint32_t vs[NW];
 #pragma unroll
-        for (int k = 0; k < NW; ++k) {
-            const int tok = vtok + k, key = (kt0 + TS * u + tt) * 16 + tok;
-            const bool live = key <= wglim && (!SC || key >= first);
-            const float vs = live ? scale4((c.vs >> (8 * k)) & 255u) : 1.f;
-            *(uint4*)(stg + HALF + (tt * 16 + tok) * RB + ((vword ^ (((tok & 3) / RPB) << 2)) << 4)) =
-                octet4<DT>(live ? c.vw[k] : 0u, vs);
+        for (int k = 0; k < NW; ++k) vs[k] = ((c.vs >> (8 * k)) << 23) & 0x7f800000u;
+        const int key0 = (kt0 + TS * u + tt) * 16;
+        if (key0 + 15 > wglim || (SC && key0 < first)) {
+            // keys no row sees may hold anything: cleared, and a scale that makes
+            // zeros NaN with them
+#pragma unroll
+            for (int k = 0; k < NW; ++k) {
+                const int key = key0 + vtok + k;
+                const bool live = key <= wglim && (!SC || key >= first);
+                vs[k] = live ? vs[k] : 0x3f800000u;
+                c.vw[k] = live ? c.vw[k] : 0u;
+            }
         }
+#pragma unroll
+        for (int k = 0; k < NW; ++k) *(uint4*)(stg + v_dst[k]) = octet4<DT>(c.vw[k], __uint_as_float(vs[k]));
     };
     auto sync = [&]() {
         __builtin_amdgcn_s_waitcnt((15) | (3 << 14) | (7 << 4) | (0 << 8));  // lgkmcnt(0)
@@ -489,28 +509,41 @@ __device__ __forceinline__ void attn4_wide(const Attn4Args& a, const int32_t* it
         vaddr[d] = (uint32_t)(HALF + (4 * hf + (j >> 2)) * RB +
                               (((4 * d + 2 * ct + ((j & 3) >> 1)) ^ (((j >> 2) / RPB) << 2)) << 4) + 8 * (j & 1));
 
+    // NS blocks of 32 keys, one softmax step
+    constexpr int NS = KEYS / 32;
     auto tile = [&](const char* stg, int key0) __attribute__((always_inline)) {
-        f32x16 st;
+        f32x16 st[NS];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) st[i] = 0.f;
+        for (int n = 0; n < NS; ++n)
 #pragma unroll
-        for (int c = 0; c < NQ; ++c) st = mfma32<DT>(*(const uint4*)(stg + kaddr[c]), qf[c], st);
+            for (int i = 0; i < 16; ++i) st[n][i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NQ; ++c)
+#pragma unroll
+            for (int n = 0; n < NS; ++n) st[n] = mfma32<DT>(*(const uint4*)(stg + n * 32 * RB + kaddr[c]), qf[c], st[n]);
         if constexpr (SC) {
             const float dist = (float)(key0 + 4 * hf - rpos[0]);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                st[i] = scored<DT>(st[i], a.scale_log2, a.cap_in, a.cap_log2, slope, dist + (8 * (i >> 2) + (i & 3)));
-        }
-        if (key0 + 31 > minlim || (SC && key0 < first)) {
+            for (int n = 0; n < NS; ++n)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int key = key0 + 8 * (i >> 2) + 4 * hf + (i & 3);
-                st[i] = key <= lim && (!SC || key >= first) ? st[i] : kNegInf;
-            }
+                for (int i = 0; i < 16; ++i)
+                    st[n][i] = scored<DT>(st[n][i], a.scale_log2, a.cap_in, a.cap_log2, slope,
+                                          dist + (32 * n + 8 * (i >> 2) + (i & 3)));
         }
-        float lmax = st[0];
+        if (key0 + KEYS - 1 > minlim || (SC && key0 < first)) {
 #pragma unroll
-        for (int i = 1; i < 16; ++i) lmax = fmax_prop(lmax, st[i]);
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int key = key0 + 32 * n + 8 * (i >> 2) + 4 * hf + (i & 3);
+                    st[n][i] = key <= lim && (!SC || key >= first) ? st[n][i] : kNegInf;
+                }
+        }
+        float lmax = st[0][0];
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) lmax = fmax_prop(lmax, st[n][i]);
         if (__builtin_amdgcn_ballot_w64(lmax > thr) != 0) {
             auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(lmax), __float_as_uint(lmax), false, false);
             const float cm = fmax_prop(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -524,25 +557,29 @@ __device__ __forceinline__ void attn4_wide(const Attn4Args& a, const int32_t* it
             m = mn;
             thr = SC ? mn + kLazyLog2 : (mn + kLazyLog2) * a.inv_scale_log2;
         }
-        uint32_t pw[8];
-        float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float p0 = __builtin_amdgcn_exp2f(SC ? st[2 * i] - m : __builtin_fmaf(st[2 * i], a.scale_log2, -m));
-            const float p1 =
-                __builtin_amdgcn_exp2f(SC ? st[2 * i + 1] - m : __builtin_fmaf(st[2 * i + 1], a.scale_log2, -m));
-            sum += p0 + p1;
-            pw[i] = pack2<DT>(p0, p1);
-        }
-        l += sum;
+        for (int n = 0; n < NS; ++n) {
+            uint32_t pw[8];
+            float sum = 0.f;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const uint4 pf = make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]);
+            for (int i = 0; i < 8; ++i) {
+                const float p0 =
+                    __builtin_amdgcn_exp2f(SC ? st[n][2 * i] - m : __builtin_fmaf(st[n][2 * i], a.scale_log2, -m));
+                const float p1 =
+                    __builtin_amdgcn_exp2f(SC ? st[n][2 * i + 1] - m : __builtin_fmaf(st[n][2 * i + 1], a.scale_log2, -m));
+                sum += p0 + p1;
+                pw[i] = pack2<DT>(p0, p1);
+            }
+            l += sum;
 #pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                const uint2 v0 = ld_tr16(stg + vaddr[d] + (16 * k) * RB);
-                const uint2 v1 = ld_tr16(stg + vaddr[d] + (16 * k + 8) * RB);
-                acc[d] = mfma32<DT>(make_uint4(v0.x, v0.y, v1.x, v1.y), pf, acc[d]);
+            for (int k = 0; k < 2; ++k) {
+                const uint4 pf = make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    const uint2 v0 = ld_tr16(stg + vaddr[d] + (32 * n + 16 * k) * RB);
+                    const uint2 v1 = ld_tr16(stg + vaddr[d] + (32 * n + 16 * k + 8) * RB);
+                    acc[d] = mfma32<DT>(make_uint4(v0.x, v0.y, v1.x, v1.y), pf, acc[d]);
+                }
             }
         }
     };
@@ -555,20 +592,22 @@ __device__ __forceinline__ void attn4_wide(const Attn4Args& a, const int32_t* it
         fetch(1, blk, c);
         blk = entry(2);
         sync();
-        for (int u = 0; u < nst; ++u) {
-            // the buffer being written was read in the round before, which every
-            // wave has left; the codes in flight meanwhile are two stages ahead
+        // the buffer being written was read in the round before, which every wave
+        // has left; the codes in flight meanwhile are two stages ahead
+        auto round = [&](int u, auto odd) __attribute__((always_inline)) {
+            constexpr int B = decltype(odd)::value;
             if (u + 1 < nst) {
-                stage(u + 1, attn_lds + ((u + 1) & 1) * STG, c);
+                stage(u + 1, attn_lds + (1 - B) * STG, c);
                 fetch(u + 2, blk, c);
                 blk = entry(u + 3);
             }
-            const char* stg = attn_lds + (u & 1) * STG;
             const int key0 = (kt0 + TS * u) * 16;
-#pragma unroll
-            for (int v = 0; v < KEYS / 32; ++v)
-                if (key0 + 32 * v <= maxlim) tile(stg + v * 32 * RB, key0 + 32 * v);
+            if (key0 <= maxlim) tile(attn_lds + B * STG, key0);
             sync();
+        };
+        for (int u = 0; u < nst; u += 2) {
+            round(u, std::integral_constant<int, 0>{});
+            if (u + 1 < nst) round(u + 1, std::integral_constant<int, 1>{});
         }
     }
 
@@ -607,43 +646,57 @@ constexpr int lds4(bool wide) {
     else return wide && wide_lds4<DP>() > coop_lds_bytes<DP>() ? wide_lds4<DP>() : coop_lds_bytes<DP>();
 }
 
-// WIDE: the launch also has wide items, in the workgroups after the narrow ones.
-template <int DT, int DP, bool SC, bool WIDE>
-__global__ __launch_bounds__(256) void attn4_kernel(const int32_t* items, Attn4Args a, int narrow_blocks,
-                                                    const int32_t* wide_items, int wide_num, const int32_t* wide_count) {
+// What a launch holds: narrow items, wide ones, or both (the narrow ones' workgroups
+// first).
+enum { kNarrow4, kWide4, kBoth4 };
+
+// Waves per SIMD the register allocator leaves room for. A wide workgroup at D 128
+// takes 245 registers; held to the 168 of three waves it spills.
+template <int DP, int KIND>
+constexpr int waves4() {
+    return DP == 256 ? 1 : KIND == kNarrow4 || DP == 128 ? 2 : 3;
+}
+
+template <int DT, int DP, bool SC, int KIND>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(waves4<DP, KIND>())))
+void attn4_kernel(const int32_t* items, Attn4Args a, int narrow_blocks, const int32_t* wide_items, int wide_num,
+                  const int32_t* wide_count) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int b = blockIdx.x;
-    if (!WIDE || b < narrow_blocks) {
+    if (KIND == kNarrow4 || (KIND == kBoth4 && b < narrow_blocks)) {
         const int item = b * kWaves + wave;
         const int32_t* it = items + (int64_t)item * MF_PLAN_ITEM_INTS;
         if (item >= (a.dev_count ? *a.dev_count : a.num_items)) return;
         const bool coop = it[11] != 0;  // of the whole workgroup
         if (!coop && it[3] == 0) return;  // padding
-        attn4_narrow<DT, DP, SC>(a, it, wave, 0, coop);
+        attn4_narrow<DT, DP, SC>(a, it, wave, coop);
         return;
     }
-    if constexpr (WIDE && DP < 256) {
-        const int block = b - narrow_blocks;
+    if constexpr (KIND != kNarrow4 && DP < 256) {
+        const int block = KIND == kBoth4 ? b - narrow_blocks : b;
         const int num = wide_count ? *wide_count : wide_num;
         if (block * kWaves >= num) return;
         const int32_t* i0 = wide_items + (int64_t)block * kWaves * MF_PLAN_ITEM_INTS;
-        int cols[kWaves][2];
         bool same = true;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 1; w < kWaves; ++w) {
             const int32_t* iw = i0 + w * MF_PLAN_ITEM_INTS;
-            cols[w][0] = iw[2];
-            cols[w][1] = iw[3];
             same = same & (iw[0] == i0[0]) & (iw[1] == i0[1]) & (iw[4] == i0[4]) & (iw[5] == i0[5]);
         }
-        const int32_t* it = i0 + wave * MF_PLAN_ITEM_INTS;
-        if (same) {
-            attn4_wide<DT, DP, SC>(a, it, wave, cols);
-        } else {
-            // a workgroup of unrelated short items: each wave its own, a column
-            // tile at a time
+        // A workgroup of unrelated items (plans that are not made for a device pool
+        // short ones) runs them one after the other, each the columns of one wave.
 #pragma unroll 1
-            for (int ct = 0; ct < it[3]; ++ct) attn4_narrow<DT, DP, SC>(a, it, wave, ct, false);
+        for (int k = 0; k < (same ? 1 : kWaves); ++k) {
+            int cols[kWaves][2];
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const int32_t* iw = i0 + (same ? w : k) * MF_PLAN_ITEM_INTS;
+                const int2 tiles = *(const int2*)(iw + 2);
+                cols[w][0] = tiles.x;
+                cols[w][1] = same | (w == k) ? tiles.y : 0;
+            }
+            const int32_t* it = i0 + (same ? wave : k) * MF_PLAN_ITEM_INTS;
+            attn4_wide<DT, DP, SC>(a, it, same | (wave == k) ? it[3] : 0, cols);
         }
     }
 }
@@ -658,12 +711,18 @@ int launch4(Attn4Args a, const int32_t* items, int64_t n_narrow, int64_t n_wide,
         const int32_t* wide = items + n_narrow * MF_PLAN_ITEM_INTS;
         const int nb = (int)(n_narrow / kWaves);
         const dim3 grid((unsigned)((n_narrow + n_wide) / kWaves));
-        if (n_wide > 0)
-            hipLaunchKernelGGL((attn4_kernel<DT, DP, SC, true>), grid, dim3(256), lds4<DP>(true), stream, items, a, nb,
-                               wide, (int)n_wide, dev_counts ? dev_counts + 1 : nullptr);
-        else
-            hipLaunchKernelGGL((attn4_kernel<DT, DP, SC, false>), grid, dim3(256), lds4<DP>(false), stream, items, a, nb,
+        const int32_t* wide_count = dev_counts ? dev_counts + 1 : nullptr;
+        if (n_wide == 0)
+            hipLaunchKernelGGL((attn4_kernel<DT, DP, SC, kNarrow4>), grid, dim3(256), lds4<DP>(false), stream, items, a, nb,
                                wide, 0, (const int32_t*)nullptr);
+        else if constexpr (DP < 256) {
+            if (n_narrow == 0)
+                hipLaunchKernelGGL((attn4_kernel<DT, DP, SC, kWide4>), grid, dim3(256), wide_lds4<DP>(), stream, items, a,
+                                   0, wide, (int)n_wide, wide_count);
+            else
+                hipLaunchKernelGGL((attn4_kernel<DT, DP, SC, kBoth4>), grid, dim3(256), lds4<DP>(true), stream, items, a,
+                                   nb, wide, (int)n_wide, wide_count);
+        }
         if (int st = check_launch()) return st;
     }
     if (n_merges > 0) {
