@@ -90,6 +90,8 @@ struct ScoredArgs : AttnArgs {
     const int32_t* prefix_lens;   // per sequence, or null
     float cap_in;    // 2 * log2(e) * |scale| / softcap, 0: scores are not capped
     float cap_log2;  // softcap * log2(e)
+    float cap_x;     // |scale| / softcap
+    float cap_c[4];  // cap_log2 times the coefficients of tanh(x) / x in x^2 (score_all)
 };
 
 // The launches of scored_attention.hip, as launch_attention's: padded head_dim
@@ -162,33 +164,60 @@ __host__ __device__ constexpr int wide_tiles(int dt, int dp) {
 template <bool SC>
 using ArgsOf = std::conditional_t<SC, ScoredArgs, AttnArgs>;
 
-// A raw score q.k (log2 units are what the exponent takes) after the scored
-// launch's scale, cap and distance bias. tanh(x) = 1 - 2 / (e^2x + 1): one
-// exponential and one reciprocal, exact at both infinities, and NaN for NaN. Its
-// error is absolute, about 1e-7 of the cap: for 16-bit types far below the
-// rounding of p, while fp32 takes the odd series below |x| = 0.35 (to x^11; the
-// next term is 2e-8 of x there), where most scores lie.
-template <int DT>
-__device__ __forceinline__ float scored(float raw, float scale_log2, float cap_in, float cap_log2, float slope_log2,
-                                        float dist) {
-    float x;
-    if (cap_in != 0.f) {  // wave-uniform
-        const float y = raw * cap_in;
-        float th = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y) + 1.f);
-        if constexpr (DT == MF_F32) {
-            const float h = y * 0.34657359028f;  // y = 2 h log2(e)
-            const float z = h * h;
-            float c = __builtin_fmaf(z, -1382.f / 155925.f, 62.f / 2835.f);
-            c = __builtin_fmaf(z, c, -17.f / 315.f);
-            c = __builtin_fmaf(z, c, 2.f / 15.f);
-            c = __builtin_fmaf(z, c, -1.f / 3.f);
-            th = z < 0.1225f ? __builtin_fmaf(h * z, c, h) : th;
+// Raw scores q.k brought to log2 units (what the exponent takes): the scored launch's
+// scale, cap and distance bias; dist(i) is position - key of score i, either sign.
+//
+// tanh(x) = 1 - 2 / (e^2x + 1): one exponential and one reciprocal, exact at both
+// infinities, NaN for NaN, its error about 1e-7 of the cap. Both instructions run at a
+// quarter of the rate, and prefill is bound by the VALU, so where every score of the
+// wave's block lies below half the cap (most do) 16-bit types take an odd polynomial
+// instead: x (c0 + c1 z + c2 z^2 + c3 z^3), z = x^2, fitted to tanh(x) / x over
+// |x| <= 0.5 for the least relative error, 5.4e-7. One test of the block's largest
+// magnitude decides. fp32 takes the series to x^11 below 0.35 (the next term is 2e-8 of
+// x there) score by score: its launches are not bound by this.
+template <int DT, int N, class Dist>
+__device__ __forceinline__ void score_all(float (&s)[N], const ScoredArgs& a, float slope_log2, Dist dist) {
+    if (a.cap_in != 0.f) {
+        bool small = false;
+        if constexpr (DT != MF_F32) {
+            float top = __builtin_fabsf(s[0]);
+#pragma unroll
+            for (int i = 1; i < N; ++i) top = fmax_prop(top, __builtin_fabsf(s[i]));
+            small = __builtin_amdgcn_ballot_w64(!(top * a.cap_x <= 0.5f)) == 0;
         }
-        x = th * cap_log2;
+        if (small) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float x = s[i] * a.cap_x, z = x * x;
+                float c = __builtin_fmaf(z, a.cap_c[3], a.cap_c[2]);
+                c = __builtin_fmaf(z, c, a.cap_c[1]);
+                c = __builtin_fmaf(z, c, a.cap_c[0]);
+                s[i] = x * c;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float y = s[i] * a.cap_in;
+                float th = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y) + 1.f);
+                if constexpr (DT == MF_F32) {
+                    const float h = s[i] * a.cap_x, z = h * h;
+                    float c = __builtin_fmaf(z, -1382.f / 155925.f, 62.f / 2835.f);
+                    c = __builtin_fmaf(z, c, -17.f / 315.f);
+                    c = __builtin_fmaf(z, c, 2.f / 15.f);
+                    c = __builtin_fmaf(z, c, -1.f / 3.f);
+                    th = z < 0.1225f ? __builtin_fmaf(h * z, c, h) : th;
+                }
+                s[i] = th * a.cap_log2;
+            }
+        }
     } else {
-        x = raw * scale_log2;
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] *= a.scale_log2;
     }
-    return __builtin_fmaf(-slope_log2, __builtin_fabsf(dist), x);
+    if (a.slopes) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] = __builtin_fmaf(-slope_log2, __builtin_fabsf(dist(i)), s[i]);
+    }
 }
 
 // The copy of a written-in-flight launch: workgroup `wblock` of the leading
@@ -504,10 +533,18 @@ __device__ __forceinline__ void arrive_and_merge(const AttnArgs& a, int m0, int 
 #ifndef MF_WIDE_WAVES
 #define MF_WIDE_WAVES(dp) ((dp) == 128 ? 3 : 4)
 #endif
-template <int DT, int DP, int NT>
+// Scored wide launches at 256-byte rows run two waves of 64-key stages and softmax steps
+// (two score chains at once, one test of the maximum for both): the transforms' registers
+// spill at three. Two chunks of 2048 rows after up to 6144 keys, 40/8 heads x 128, capped
+// scores (475 GFLOP): 836 us at three waves and 32 keys, 778 at two, 698 with stages of
+// 64, 689 with steps of 64. At 128-byte rows four waves and 32-key steps stay the faster
+// (8 packed prompts of documents 49 us, 57 at three waves with steps of 64).
+constexpr int scored_waves(int dp) { return dp == 128 ? 2 : 4; }
+constexpr int scored_step(int dp) { return dp == 128 ? 2 : 1; }  // 32-key blocks
+template <int DT, int DP, int NT, bool SC = false>
 constexpr int attn_waves_per_eu() {
     constexpr int row_bytes = DP * (DT == MF_F32 ? 4 : 2);
-    if (DT != MF_F32 && NT > 1) return MF_WIDE_WAVES(DP);
+    if (DT != MF_F32 && NT > 1) return SC ? scored_waves(DP) : MF_WIDE_WAVES(DP);
     return (row_bytes <= 128 || (row_bytes <= 256 && NT == 1)) ? 2 : 1;
 }
 
@@ -549,20 +586,20 @@ extern __shared__ __attribute__((aligned(16))) char attn_lds[];
 #ifndef MF_WIDE_KEYS
 #define MF_WIDE_KEYS(dp) ((dp) == 128 ? 32 : 64)
 #endif
-constexpr int wide_keys(int dp) { return MF_WIDE_KEYS(dp); }
-template <int DT, int DP>
+constexpr int wide_keys(int dp, bool sc) { return sc ? 64 : MF_WIDE_KEYS(dp); }
+template <int DT, int DP, bool SC>
 constexpr int wide_lds_bytes() {
     if constexpr (DT == MF_F32) return 0;  // the workgroup-shared loop is 16-bit only
-    else return 2 * 2 * wide_keys(DP) * DP * 2;
+    else return 2 * 2 * wide_keys(DP, SC) * DP * 2;
 }
 template <int DP>
 constexpr int coop_lds_bytes() {
     return (kWaves * 4 * (DP / 16) * 64 + 2 * kWaves * 16) * 4;
 }
-template <int DT, int DP, int NT, bool FAST>
+template <int DT, int DP, int NT, bool FAST, bool SC = false>
 constexpr int attn_lds_bytes() {
     if constexpr (NT == 1) return coop_lds_bytes<DP>();
-    else return wide_lds_bytes<DT, DP>();
+    else return wide_lds_bytes<DT, DP, SC>();
 }
 
 // The body of one workgroup of the attention kernel: `block` is its index
@@ -927,12 +964,14 @@ __device__ __forceinline__ void attn_body(const ArgsOf<SC>& a, const int block) 
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                sv[nt][r] = st[nt][r];
-                if constexpr (SC)
-                    sv[nt][r] = scored<DT>(st[nt][r], a.scale_log2, a.cap_in, a.cap_log2, slope[nt],
-                                           (float)(kt * 16 + 4 * g + r - at_pos[nt]));
+            for (int r = 0; r < 4; ++r) sv[nt][r] = st[nt][r];
+        if constexpr (SC) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float dist = (float)(kt * 16 + 4 * g - at_pos[nt]);
+                score_all<DT>(sv[nt], a, slope[nt], [&](int i) { return dist + i; });
             }
+        }
         // Every key of a tile wholly inside the context and at or before every
         // column's position is visible to all columns: no mask to apply.
         if (!(kt * 16 + 15 <= minpos && (kt + 1) * 16 <= kv_len && (!SC || kt * 16 >= first))) {
@@ -1331,7 +1370,8 @@ __device__ __forceinline__ void attn_wide_body(const ArgsOf<SC>& a, const int bl
                                                const int (&cols)[kWaves][2]) {
     constexpr int RB = DP * 2;       // bytes of one key row
     constexpr int NCH = RB / 16;     // 16-byte chunks per row
-    constexpr int KEYS = wide_keys(DP), TS = KEYS / 16;  // keys and 16-key blocks per stage
+    constexpr int KEYS = wide_keys(DP, SC), TS = KEYS / 16;  // keys and 16-key blocks per stage
+    constexpr int NS = SC ? scored_step(DP) : 1;
     constexpr int RPB = 256 / RB;    // rows per 256 bytes (all LDS banks once)
     constexpr int NQ = DP / 16;      // MFMA steps of S^T
     constexpr int ND = DP / 32;      // 32-row blocks of O^T
@@ -1340,7 +1380,7 @@ __device__ __forceinline__ void attn_wide_body(const ArgsOf<SC>& a, const int bl
     constexpr int NOFF = DP == 128 ? 2 : 1;  // a wave's distinct pieces of a block
     constexpr int HALF = KEYS * RB;     // K rows of a stage, then its V rows
     constexpr int STG = 2 * HALF;
-    static_assert(DT != MF_F32 && RPB >= 1 && wide_lds_bytes<DT, DP>() == 2 * STG, "stage layout");
+    static_assert(DT != MF_F32 && RPB >= 1 && wide_lds_bytes<DT, DP, SC>() == 2 * STG, "stage layout");
     constexpr float kNegInf = -__builtin_huge_valf();
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1581,29 +1621,41 @@ __device__ __forceinline__ void attn_wide_body(const ArgsOf<SC>& a, const int bl
         vaddr[d] = (uint32_t)(HALF + (4 * hf + (j >> 2)) * RB +
                               (((4 * d + 2 * ct + ((j & 3) >> 1)) ^ (((j >> 2) / RPB) << 2)) << 4) + 8 * (j & 1));
 
+    // NS blocks of 32 keys, one softmax step
     auto tile = [&](const char* stg, int key0) __attribute__((always_inline)) {
-        f32x16 st;
+        f32x16 st[NS];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) st[i] = 0.f;
+        for (int n = 0; n < NS; ++n)
 #pragma unroll
-        for (int c = 0; c < NQ; ++c) st = mfma32<DT>(*(const uint4*)(stg + kaddr[c]), qf[c], st);
+            for (int i = 0; i < 16; ++i) st[n][i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NQ; ++c)
+#pragma unroll
+            for (int n = 0; n < NS; ++n) st[n] = mfma32<DT>(*(const uint4*)(stg + n * 32 * RB + kaddr[c]), qf[c], st[n]);
         if constexpr (SC) {
             const float dist = (float)(key0 + 4 * hf - rpos[0]);
+            float x[16 * NS];
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                st[i] = scored<DT>(st[i], a.scale_log2, a.cap_in, a.cap_log2, slope, dist + (8 * (i >> 2) + (i & 3)));
+            for (int i = 0; i < 16 * NS; ++i) x[i] = st[i >> 4][i & 15];
+            score_all<DT>(x, a, slope, [&](int i) { return dist + (32 * (i >> 4) + 8 * ((i & 15) >> 2) + (i & 3)); });
+#pragma unroll
+            for (int i = 0; i < 16 * NS; ++i) st[i >> 4][i & 15] = x[i];
         }
-        if (key0 + 31 > minlim || (SC && key0 < first_key)) {
+        if (key0 + 32 * NS - 1 > minlim || (SC && key0 < first_key)) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int key = key0 + 8 * (i >> 2) + 4 * hf + (i & 3);
-                st[i] = key <= lim && (!SC || key >= first_key) ? st[i] : kNegInf;
-            }
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int key = key0 + 32 * n + 8 * (i >> 2) + 4 * hf + (i & 3);
+                    st[n][i] = key <= lim && (!SC || key >= first_key) ? st[n][i] : kNegInf;
+                }
         }
         // lazy rescale, as in attn_body; a column's keys lie in two lanes
-        float lmax = st[0];
+        float lmax = st[0][0];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) lmax = fmax_prop(lmax, st[i]);
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int i = n ? 0 : 1; i < 16; ++i) lmax = fmax_prop(lmax, st[n][i]);
         if (__builtin_amdgcn_ballot_w64(lmax > thr) != 0) {
             auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(lmax), __float_as_uint(lmax), false, false);
             const float cm = fmax_prop(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -1617,28 +1669,31 @@ __device__ __forceinline__ void attn_wide_body(const ArgsOf<SC>& a, const int bl
             m = mn;
             thr = SC ? mn + kLazyLog2 : (mn + kLazyLog2) * a.inv_scale_log2;
         }
-        uint32_t pw[8];
-        float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float p0 = __builtin_amdgcn_exp2f(SC ? st[2 * i] - m : __builtin_fmaf(st[2 * i], a.scale_log2, -m));
-            const float p1 =
-                __builtin_amdgcn_exp2f(SC ? st[2 * i + 1] - m : __builtin_fmaf(st[2 * i + 1], a.scale_log2, -m));
-            sum += p0 + p1;
-            if constexpr (DT == MF_BF16)
-                pw[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){p0, p1}, bf16x2));
-            else
-                pw[i] = f32_to_bits<DT>(p0) | (f32_to_bits<DT>(p1) << 16);
-        }
-        l += sum;
+        for (int n = 0; n < NS; ++n) {
+            uint32_t pw[8];
+            float sum = 0.f;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const uint4 pf = make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]);
+            for (int i = 0; i < 8; ++i) {
+                const float s0 = st[n][2 * i], s1 = st[n][2 * i + 1];
+                const float p0 = __builtin_amdgcn_exp2f(SC ? s0 - m : __builtin_fmaf(s0, a.scale_log2, -m));
+                const float p1 = __builtin_amdgcn_exp2f(SC ? s1 - m : __builtin_fmaf(s1, a.scale_log2, -m));
+                sum += p0 + p1;
+                if constexpr (DT == MF_BF16)
+                    pw[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){p0, p1}, bf16x2));
+                else
+                    pw[i] = f32_to_bits<DT>(p0) | (f32_to_bits<DT>(p1) << 16);
+            }
+            l += sum;
 #pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                const uint2 v0 = ld_tr16(stg + vaddr[d] + (16 * k) * RB);
-                const uint2 v1 = ld_tr16(stg + vaddr[d] + (16 * k + 8) * RB);
-                acc[d] = mfma32<DT>(make_uint4(v0.x, v0.y, v1.x, v1.y), pf, acc[d]);
+            for (int k = 0; k < 2; ++k) {
+                const uint4 pf = make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    const uint2 v0 = ld_tr16(stg + vaddr[d] + (32 * n + 16 * k) * RB);
+                    const uint2 v1 = ld_tr16(stg + vaddr[d] + (32 * n + 16 * k + 8) * RB);
+                    acc[d] = mfma32<DT>(make_uint4(v0.x, v0.y, v1.x, v1.y), pf, acc[d]);
+                }
             }
         }
     };
@@ -1666,8 +1721,8 @@ __device__ __forceinline__ void attn_wide_body(const ArgsOf<SC>& a, const int bl
                 sync();
             }
 #pragma unroll
-            for (int v = 0; v < KEYS / 32; ++v)
-                if (key0 + 32 * v <= maxlim) tile(stg + v * 32 * RB, key0 + 32 * v);
+            for (int v = 0; v < KEYS / (32 * NS); ++v)
+                if (key0 + 32 * NS * v <= maxlim) tile(stg + v * 32 * NS * RB, key0 + 32 * NS * v);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             sync();
             if (u + 2 < nst) {
@@ -1754,7 +1809,7 @@ __device__ __forceinline__ void attn_block(const ArgsOf<SC>& a, const int block)
 // hardware preload into scalar registers: a wave's first item load then
 // needs no load of the argument block (see attn_body).
 template <int DT, int DP, int NT, bool FAST, bool TAIL = false, bool SC = false>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(attn_waves_per_eu<DT, DP, NT>())))
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(attn_waves_per_eu<DT, DP, NT, SC>())))
 void attn_kernel(const int32_t* items, ArgsOf<SC> a) {
     a.items = items;
     if constexpr (TAIL) {
@@ -1805,14 +1860,15 @@ __device__ __forceinline__ void narrow_start_delay() {
 // single-tile body's own need (140 registers), left the C2 step's 1,104
 // workgroups in more than one round of three per CU. Measured on the C2
 // engine layer as graph replays: 55.1-56.3 us at four, 56.0-57.3 at three.
-template <int DT, int DP, int NTW>
+template <int DT, int DP, int NTW, bool SC = false>
 constexpr int mixed_waves_per_eu() {
-    if constexpr (DT != MF_F32 && DP == 64) return 4;
+    if constexpr (SC && DT != MF_F32) return scored_waves(DP);
+    else if constexpr (DT != MF_F32 && DP == 64) return 4;
     else return attn_waves_per_eu<DT, DP, NTW>() < attn_waves_per_eu<DT, DP, 1>() ? attn_waves_per_eu<DT, DP, NTW>()
                                                                                  : attn_waves_per_eu<DT, DP, 1>();
 }
 template <int DT, int DP, int NTW, bool SC = false>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(mixed_waves_per_eu<DT, DP, NTW>())))
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(mixed_waves_per_eu<DT, DP, NTW, SC>())))
 void attn_mixed_kernel(ArgsOf<SC> narrow, ArgsOf<SC> wide, int wide_blocks) {
     const int b = blockIdx.x;
     const int narrow_blocks = (int)gridDim.x - wide_blocks;
@@ -1828,7 +1884,7 @@ void attn_mixed_kernel(ArgsOf<SC> narrow, ArgsOf<SC> wide, int wide_blocks) {
 // wide ones. One argument block (the wide items differ only in their list):
 // the larger body needs the scalar registers a second block would take.
 template <int DT, int DP, int NTW, bool SC = false>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(mixed_waves_per_eu<DT, DP, NTW>())))
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(mixed_waves_per_eu<DT, DP, NTW, SC>())))
 void attn_mixed_tail_kernel(ArgsOf<SC> a, const int32_t* wide_items, int wide_num_items,
                             const int32_t* wide_dev_count, int wide_blocks) {
     const int b = blockIdx.x - a.w_blocks;
@@ -2212,8 +2268,8 @@ int launch_attention(ArgsOf<SC> a, const int32_t* items, int64_t n_narrow, int64
             aw.dev_count = dev_counts ? dev_counts + 1 : nullptr;
             const int64_t wide_blocks = (n_wide + kWaves - 1) / kWaves;
             const dim3 grid((unsigned)(a.w_blocks + wide_blocks + (n_narrow + kWaves - 1) / kWaves));
-            constexpr int lds = attn_lds_bytes<DT, DP, 1, true>() > attn_lds_bytes<DT, DP, NTW, true>()
-                                    ? attn_lds_bytes<DT, DP, 1, true>() : attn_lds_bytes<DT, DP, NTW, true>();
+            constexpr int lds = attn_lds_bytes<DT, DP, 1, true>() > attn_lds_bytes<DT, DP, NTW, true, SC>()
+                                    ? attn_lds_bytes<DT, DP, 1, true>() : attn_lds_bytes<DT, DP, NTW, true, SC>();
             if constexpr (TAIL)
                 hipLaunchKernelGGL((attn_mixed_tail_kernel<DT, DP, NTW, SC>), grid, dim3(256), lds, stream, an,
                                    aw.items, aw.num_items, aw.dev_count, (int)wide_blocks);
@@ -2248,10 +2304,10 @@ int launch_attention(ArgsOf<SC> a, const int32_t* items, int64_t n_narrow, int64
             const dim3 grid((unsigned)(a.w_blocks + (n_wide + kWaves - 1) / kWaves));
             if (fast)
                 hipLaunchKernelGGL((attn_kernel<DT, DP, NTW, true, TAIL, SC>), grid, dim3(256),
-                                   (attn_lds_bytes<DT, DP, NTW, true>()), stream, a.items, a);
+                                   (attn_lds_bytes<DT, DP, NTW, true, SC>()), stream, a.items, a);
             else if constexpr (!TAIL)
                 hipLaunchKernelGGL((attn_kernel<DT, DP, NTW, false, false, SC>), grid, dim3(256),
-                                   (attn_lds_bytes<DT, DP, NTW, false>()), stream, a.items, a);
+                                   (attn_lds_bytes<DT, DP, NTW, false, SC>()), stream, a.items, a);
             if (int st = check_launch()) return st;
         }
     } else {
@@ -2291,6 +2347,9 @@ inline int set_scoring(ScoredArgs& a, const mf_scoring& s) {
     a.prefix_lens = s.prefix_lens;
     a.cap_in = s.softcap > 0.f ? 2.f * a.scale_log2 / s.softcap : 0.f;
     a.cap_log2 = s.softcap * 1.4426950408889634f;
+    a.cap_x = s.softcap > 0.f ? a.scale_log2 / a.cap_log2 : 0.f;
+    const float tanh_c[4] = {0.99999946f, -0.33326317f, 0.13190283f, -0.04440178f};
+    for (int i = 0; i < 4; ++i) a.cap_c[i] = a.cap_log2 * tanh_c[i];
     if (s.softcap > 0.f && !(a.cap_in >= FLT_MIN && a.cap_in < INFINITY && a.cap_log2 < INFINITY)) return MF_ERR_ARG;
     return MF_OK;
 }

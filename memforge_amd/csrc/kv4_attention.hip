@@ -175,11 +175,10 @@ __device__ __forceinline__ void attn4_narrow(const Attn4Args& a, const int32_t* 
             }
             float sv[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                sv[k] = st[k >> 2][k & 3];
-                if constexpr (SC)
-                    sv[k] = scored<DT>(sv[k], a.scale_log2, a.cap_in, a.cap_log2, slope,
-                                       (float)(key0 + (k & 3) + 16 * (k >> 2) - pos));
+            for (int k = 0; k < 8; ++k) sv[k] = st[k >> 2][k & 3];
+            if constexpr (SC) {
+                const float dist = (float)(key0 - pos);
+                score_all<DT>(sv, a, slope, [&](int k) { return dist + ((k & 3) + 16 * (k >> 2)); });
             }
             if (t * 16 + 31 > minlim || t * 16 < first) {
 #pragma unroll
@@ -523,12 +522,12 @@ __device__ __forceinline__ void attn4_wide(const Attn4Args& a, const int32_t* it
             for (int n = 0; n < NS; ++n) st[n] = mfma32<DT>(*(const uint4*)(stg + n * 32 * RB + kaddr[c]), qf[c], st[n]);
         if constexpr (SC) {
             const float dist = (float)(key0 + 4 * hf - rpos[0]);
+            float x[16 * NS];
 #pragma unroll
-            for (int n = 0; n < NS; ++n)
+            for (int i = 0; i < 16 * NS; ++i) x[i] = st[i >> 4][i & 15];
+            score_all<DT>(x, a, slope, [&](int i) { return dist + (32 * (i >> 4) + 8 * ((i & 15) >> 2) + (i & 3)); });
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    st[n][i] = scored<DT>(st[n][i], a.scale_log2, a.cap_in, a.cap_log2, slope,
-                                          dist + (32 * n + 8 * (i >> 2) + (i & 3)));
+            for (int i = 0; i < 16 * NS; ++i) st[i >> 4][i & 15] = x[i];
         }
         if (key0 + KEYS - 1 > minlim || (SC && key0 < first)) {
 #pragma unroll
