@@ -360,7 +360,8 @@ int mf_kv4_gather(const mf_pool4* pool, const int64_t* slot_mapping, int64_t num
 
 /* mf_paged_attention (or, with scoring, mf_paged_attention_scored) over a 4-bit
  * pool: every key is read from the pool, as the value its codes stand for. dtype
- * (q and out) is the pool's, fp16 or bf16, and plans are made for it.
+ * (q and out) is the pool's, fp16 or bf16, and plans are made for it, by
+ * mf_attention_plan4 or any other per-range planner.
  * device_counts as in mf_paged_attention_counted. */
 int mf_paged_attention4(const mf_scoring* scoring, const void* q, int64_t q_stride_row, int64_t q_stride_head,
                         void* out, int64_t out_stride_row, int64_t out_stride_head, int dtype, const mf_pool4* pool,
@@ -470,6 +471,13 @@ int mf_attention_plan_merge_free(int num_seqs, const int32_t* cu_seqlens, const 
                                  int num_q_heads, int num_kv_heads, int head_dim, int dtype, int num_cus,
                                  int32_t* items, int64_t items_capacity, int32_t* merges,
                                  int64_t merges_capacity, int64_t* counts);
+
+/* mf_attention_plan_device for mf_paged_attention4: the same records, ranges cut
+ * for the bytes and the pace of a 4-bit pool. */
+int mf_attention_plan4(int num_seqs, const int32_t* cu_seqlens, const int32_t* kv_lens,
+                       int num_q_heads, int num_kv_heads, int head_dim, int dtype, int num_cus,
+                       int32_t* items, int64_t items_capacity, int32_t* merges,
+                       int64_t merges_capacity, int64_t* counts);
 
 /* ------------------------------------------------- decode slice plans
  * A second plan form for large decode launches, with the same results as

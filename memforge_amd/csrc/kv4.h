@@ -15,8 +15,9 @@ inline int min_scale4(int dtype) { return dtype == MF_F16 ? 127 - 23 : 127 - 125
 inline int max_scale4(int dtype) { return dtype == MF_F16 ? 127 + 13 : 127 + 125; }
 constexpr int kNaNScale4 = 255;
 
-// The scale a byte stands for, as the operand of the conversions (they read its
-// exponent; 255 makes every code NaN).
+// The scale a byte stands for, as the operand of the conversions (255 makes every code
+// NaN). They read bits 30 to 23 alone, whatever stands in the others (checked over
+// random words).
 __device__ __forceinline__ float scale4(uint32_t byte) { return __uint_as_float(byte << 23); }
 
 // Byte B of w, two codes, as two elements of the 16-bit type: one instruction, the

@@ -33,6 +33,7 @@ struct Attn4Args : ScoredArgs {
     int H;               // kv heads
     int tpb;             // 16-key tiles of a block
     uint32_t tpb_magic;  // ceil(2^32 / tpb), unused for 1
+    uint32_t blk_bytes;  // codes of one block, K or V, all heads; its scales take a sixteenth
 };
 
 // Block index of tile t in its sequence's table.
@@ -46,10 +47,12 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
     else return f32_to_bits<DT>(x) | (f32_to_bits<DT>(y) << 16);
 }
 
-constexpr int kDepth4 = 3;  // register buffers of the decode loop, 32 keys each
+constexpr int kDepth4 = 2;  // register buffers of the decode loop, 32 keys each
 
-// One wave: the 16-column tile and the keys of its item.
-template <int DT, int DP, bool SC>
+// One wave: the 16-column tile and the keys of its item. BLK16: 16-token blocks, where
+// a tile is a block and the addresses of its slots fall away (of a pair of tiles, 81
+// scalar instructions with them).
+template <int DT, int DP, bool SC, bool BLK16>
 __device__ __forceinline__ void attn4_narrow(const Attn4Args& a, const int32_t* it, const int wave, const bool coop) {
     constexpr int KW = DP / 32;                // words of a lane's K per 16 keys
     constexpr int VCH = DP / 16;               // head_dim elements of a lane's V per key
@@ -65,11 +68,11 @@ __device__ __forceinline__ void attn4_narrow(const Attn4Args& a, const int32_t* 
         if (a.first_keys) first = a.first_keys[s];
         if (a.prefix_lens) prefix = a.prefix_lens[s];
     }
-    // ---- the item's blocks: entry of tile kt0 + lane and kt0 + 64 + lane
+    // ---- the item's blocks (at most as many as its 128 tiles), two a lane
     const int32_t* trow = a.block_tables + (int64_t)s * a.bt_stride;
-    const int last_tile = max(kt1 - 1, 0);
-    const int tbl = trow[block_of(a, min(kt0 + lane, last_tile))];
-    const int tbl_hi = trow[block_of(a, min(kt0 + 64 + lane, last_tile))];
+    const int last_block = block_of(a, max(kt1 - 1, 0)), block0 = min(block_of(a, kt0), last_block);
+    const int tbl = trow[min(block0 + lane, last_block)];
+    const int tbl_hi = trow[min(block0 + 64 + lane, last_block)];
 
     // ---- this lane's column
     const int cidx = c0 * 16 + j;
@@ -92,32 +95,38 @@ __device__ __forceinline__ void attn4_narrow(const Attn4Args& a, const int32_t* 
     const int reach = valid ? (SC ? max(pos, prefix - 1) : pos) : -1;
     const int lim = reach >= 0 ? min(min(reach, kv_len - 1), kt1 * 16 - 1) : -1;  // last key of the item the column sees
 
-    // ---- the stream
+    // ---- the stream. A tile's addresses are scalar: the head's bases, the block and
+    // the 16 slots of it; a lane's byte offsets never change.
     struct Tile {
         uint32_t kw[KW], ks, vw[VW], vs;
     };
-    const int bs = a.tpb * 16;
-    const uint32_t k_lane = (uint32_t)(j * (DP / 8) + g * KW);
+    const int bs = BLK16 ? 16 : a.tpb * 16;
     constexpr int VSH = DP == 64 ? 1 : DP == 32 ? 2 : 0;  // lanes that share a word's eight elements: 2^VSH
     const int vchunk = DP == 256 ? 2 * j : j >> VSH;
-    const uint32_t v_lane = (uint32_t)(vchunk * bs + 4 * g);
+    const uint32_t k_lane = (uint32_t)(j * (DP / 8) + g * KW) * 4;
+    const uint32_t v_lane = (uint32_t)(vchunk * bs + 4 * g) * 4;
     const uint32_t ks_lane = (uint32_t)(j * (DP / 32) + (DP == 256 ? 2 * g : DP == 128 ? g : DP == 64 ? g >> 1 : 0));
     const uint32_t vs_lane = (uint32_t)((vchunk >> 2) * bs + 4 * g);
-    auto load = [&](int t, Tile& x) __attribute__((always_inline)) {
-        const int i = t - kt0;
-        const int e0 = __builtin_amdgcn_readlane(tbl, i & 63), e1 = __builtin_amdgcn_readlane(tbl_hi, i & 63);
-        const int blk = i < 64 ? e0 : e1;
-        const int off = (t - block_of(a, t) * a.tpb) * 16;
-        const int64_t row = (int64_t)blk * a.H + h;
-        const uint32_t* kc = a.kc + (row * bs + off) * (DP / 8);
-        const uint8_t* ks = a.ks + (row * bs + off) * (DP / 32);
-        const uint32_t* vc = a.vc + row * (DP / 8) * bs + off;
-        const uint8_t* vs = a.vs + row * (DP / 32) * bs + off;
-        ld_words<KW * 4>((const char*)(kc + k_lane), x.kw);
+    const char* kc_h = (const char*)a.kc + (int64_t)h * bs * (DP / 2);
+    const char* ks_h = (const char*)a.ks + (int64_t)h * bs * (DP / 32);
+    const char* vc_h = (const char*)a.vc + (int64_t)h * bs * (DP / 2);
+    const char* vs_h = (const char*)a.vs + (int64_t)h * bs * (DP / 32);
+    int at_block = 0, at_off = 0;  // of the next tile to load: table entry, first slot
+    auto load = [&](Tile& x) __attribute__((always_inline)) {
+        const int e0 = __builtin_amdgcn_readlane(tbl, at_block & 63), e1 = __builtin_amdgcn_readlane(tbl_hi, at_block & 63);
+        const uint64_t o = (uint64_t)(uint32_t)(at_block < 64 ? e0 : e1) * a.blk_bytes;
+        const char *kc = kc_h + o, *ks = ks_h + (o >> 4), *vc = vc_h + o, *vs = vs_h + (o >> 4);
+        if constexpr (!BLK16) {
+            kc += (uint32_t)(at_off * (DP / 2));
+            ks += (uint32_t)(at_off * (DP / 32));
+            vc += (uint32_t)(at_off * 4);
+            vs += (uint32_t)at_off;
+        }
+        ld_words<KW * 4>(kc + k_lane, x.kw);
         if constexpr (DP == 256) x.ks = *(const uint16_t*)(ks + ks_lane);
-        else x.ks = ks[ks_lane];
-        ld_words<16>((const char*)(vc + v_lane), x.vw);
-        if constexpr (DP == 256) ld_words<16>((const char*)(vc + v_lane + bs), x.vw + 4);
+        else x.ks = *(const uint8_t*)(ks + ks_lane);
+        ld_words<16>(vc + v_lane, x.vw);
+        if constexpr (DP == 256) ld_words<16>(vc + (v_lane + 4 * (uint32_t)bs), x.vw + 4);
         x.vs = *(const uint32_t*)(vs + vs_lane);
     };
 
@@ -136,25 +145,28 @@ __device__ __forceinline__ void attn4_narrow(const Attn4Args& a, const int32_t* 
         }
         maxlim = __builtin_amdgcn_readfirstlane(maxlim);
         minlim = __builtin_amdgcn_readfirstlane(minlim);
-        const int tb = min(max(kt0, first >> 4), kt1);
+        const int tb = SC ? min(max(kt0, first >> 4), kt1) : kt0;
         const int te = maxlim < 0 ? tb : max(tb, min(kt1, (maxlim >> 4) + 1));
 
         auto process = [&](int t, Tile& x, Tile& y) __attribute__((always_inline)) {
             const int key0 = t * 16 + 4 * g;  // this lane's keys: key0 + r, key0 + 16 + r
-            // keys no column sees may hold anything: their V is cleared, and with
-            // it a scale that makes zeros NaN
-            float vscale[8];
+            // a key's V scale: its byte among the bits the conversion reads
+            uint32_t vscale[8];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                vscale[k] = scale4((x.vs >> (8 * k)) & 255u);
-                vscale[4 + k] = scale4((y.vs >> (8 * k)) & 255u);
+                vscale[k] = k < 3 ? x.vs << (23 - 8 * k) : x.vs >> 1;
+                vscale[4 + k] = k < 3 ? y.vs << (23 - 8 * k) : y.vs >> 1;
             }
-            if (t * 16 + 31 > maxlim || t * 16 < first) {
+            // keys no column sees may hold anything: their V is cleared, and with it
+            // a scale that makes zeros NaN
+            if (t * 16 + 31 > maxlim || (SC && t * 16 < first)) {
+                asm volatile("");  // a branch: one tile in a range takes it, as selects all would
+                const int end = maxlim - key0, begin = first - key0;
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    const int key = key0 + (k & 3) + 16 * (k >> 2);
-                    const bool live = key >= first && key <= maxlim;
-                    vscale[k] = live ? vscale[k] : 1.f;
+                    const int key = (k & 3) + 16 * (k >> 2);
+                    const bool live = key <= end && (!SC || key >= begin);
+                    vscale[k] = live ? vscale[k] : 0x3f800000u;
 #pragma unroll
                     for (int u = 0; u < VW / 4; ++u) {
                         uint32_t& w = (k < 4 ? x : y).vw[4 * u + (k & 3)];
@@ -180,11 +192,13 @@ __device__ __forceinline__ void attn4_narrow(const Attn4Args& a, const int32_t* 
                 const float dist = (float)(key0 - pos);
                 score_all<DT>(sv, a, slope, [&](int k) { return dist + ((k & 3) + 16 * (k >> 2)); });
             }
-            if (t * 16 + 31 > minlim || t * 16 < first) {
+            if (t * 16 + 31 > minlim || (SC && t * 16 < first)) {
+                asm volatile("");
+                const int end = lim - key0, begin = first - key0;
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    const int key = key0 + (k & 3) + 16 * (k >> 2);
-                    sv[k] = key <= lim && key >= first ? sv[k] : kNegInf;
+                    const int key = (k & 3) + 16 * (k >> 2);
+                    sv[k] = key <= end && (!SC || key >= begin) ? sv[k] : kNegInf;
                 }
             }
             float lmax = sv[0];
@@ -216,15 +230,15 @@ __device__ __forceinline__ void attn4_narrow(const Attn4Args& a, const int32_t* 
                 if constexpr (VCH >= 8) {
 #pragma unroll
                     for (int u = 0; u < VW / 4; ++u) {
-                        const uint4 o = octet4<DT>(w[4 * u], vscale[k]);
+                        const uint4 o = octet4<DT>(w[4 * u], __uint_as_float(vscale[k]));
                         v[k][4 * u] = o.x; v[k][4 * u + 1] = o.y; v[k][4 * u + 2] = o.z; v[k][4 * u + 3] = o.w;
                     }
                 } else if constexpr (VCH == 4) {
                     const uint32_t half = w[0] >> (16 * (j & 1));
-                    v[k][0] = pair4<DT, 0>(half, vscale[k]);
-                    v[k][1] = pair4<DT, 1>(half, vscale[k]);
+                    v[k][0] = pair4<DT, 0>(half, __uint_as_float(vscale[k]));
+                    v[k][1] = pair4<DT, 1>(half, __uint_as_float(vscale[k]));
                 } else {
-                    v[k][0] = pair4<DT, 0>(w[0] >> (8 * (j & 3)), vscale[k]);
+                    v[k][0] = pair4<DT, 0>(w[0] >> (8 * (j & 3)), __uint_as_float(vscale[k]));
                 }
             }
 #pragma unroll
@@ -244,17 +258,32 @@ __device__ __forceinline__ void attn4_narrow(const Attn4Args& a, const int32_t* 
             // read its last tile again, masked
             Tile ring[kDepth4][2];
             const int last = te - 1;
-            auto fetch = [&](int t, Tile (&x)[2]) __attribute__((always_inline)) {
-                load(min(t, last), x[0]);
-                load(min(t + 1, last), x[1]);
+            int next = tb;
+            at_block = block_of(a, tb) - block0;
+            at_off = (tb - block_of(a, tb) * a.tpb) * 16;
+            auto step = [&]() __attribute__((always_inline)) {
+                if constexpr (BLK16) {
+                    at_block = min(at_block + 1, last - block0);
+                } else {
+                    const bool more = next < last, wrap = more && at_off + 16 == bs;
+                    at_off = wrap ? 0 : more ? at_off + 16 : at_off;
+                    at_block += wrap ? 1 : 0;
+                    ++next;
+                }
+            };
+            auto fetch = [&](Tile (&x)[2]) __attribute__((always_inline)) {
+                load(x[0]);
+                step();
+                load(x[1]);
+                step();
             };
             int t = tb;
 #pragma unroll
-            for (int i = 0; i < kDepth4 - 1; ++i) fetch(t + 2 * i, ring[i]);
+            for (int i = 0; i < kDepth4 - 1; ++i) fetch(ring[i]);
             for (int n = (te - tb + 1) / 2 / kDepth4; n > 0; --n) {
 #pragma unroll
                 for (int u = 0; u < kDepth4; ++u) {
-                    fetch(t + 2 * (kDepth4 - 1), ring[(u + kDepth4 - 1) % kDepth4]);
+                    fetch(ring[(u + kDepth4 - 1) % kDepth4]);
                     process(t, ring[u][0], ring[u][1]);
                     t += 2;
                 }
@@ -656,7 +685,7 @@ constexpr int waves4() {
     return DP == 256 ? 1 : KIND == kNarrow4 || DP == 128 ? 2 : 3;
 }
 
-template <int DT, int DP, bool SC, int KIND>
+template <int DT, int DP, bool SC, int KIND, bool BLK16>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(waves4<DP, KIND>())))
 void attn4_kernel(const int32_t* items, Attn4Args a, int narrow_blocks, const int32_t* wide_items, int wide_num,
                   const int32_t* wide_count) {
@@ -668,7 +697,7 @@ void attn4_kernel(const int32_t* items, Attn4Args a, int narrow_blocks, const in
         if (item >= (a.dev_count ? *a.dev_count : a.num_items)) return;
         const bool coop = it[11] != 0;  // of the whole workgroup
         if (!coop && it[3] == 0) return;  // padding
-        attn4_narrow<DT, DP, SC>(a, it, wave, coop);
+        attn4_narrow<DT, DP, SC, BLK16>(a, it, wave, coop);
         return;
     }
     if constexpr (KIND != kNarrow4 && DP < 256) {
@@ -700,6 +729,63 @@ void attn4_kernel(const int32_t* items, Attn4Args a, int narrow_blocks, const in
     }
 }
 
+// ------------------------------------------------------------------- merge
+// One workgroup per record, its partitions dealt to the four waves, whose results
+// are combined through LDS as the cooperative units' states are. Ranges here are cut
+// into more partitions than the 16-bit plans make (a tile's bytes are a quarter), and a
+// single wave reads them four at a time: 4 sequences of 16384 to 65536 keys, 32
+// records of up to 36 partitions, 19 us that way.
+template <int DT, int DP>
+__global__ __launch_bounds__(256) void merge4_kernel(const int32_t* merges, int num_merges, Attn4Args a) {
+    constexpr int VCH = DP / 16;
+    const int mi = blockIdx.x;
+    int32_t mg[MF_PLAN_MERGE_INTS];
+    load_merge_record(a, merges, mi, num_merges, mg);
+    if (mi >= (a.dev_count ? *a.dev_count : num_merges)) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
+    int prow = 0, qhead = 0;
+    const bool valid = merge_column(a, mg, j, prow, qhead);
+    float mx = kMinM, L = 0.f, o[4 * VCH];
+#pragma unroll
+    for (int e = 0; e < 4 * VCH; ++e) o[e] = 0.f;
+    if (valid && wave < mg[3]) {
+        bool fp32 = false;
+        if constexpr (has_fp32_partials<DT, DP>()) fp32 = (mg[7] & MF_PLAN_FP32_PARTIALS) != 0;
+        if (fp32) merge_range<DT, DP, MF_F32, (DP > 128 ? 2 : 4)>(a, mg, wave, kWaves, j, 4 * g * VCH, mx, L, o);
+        else merge_range<DT, DP, DT, (DP > 128 ? 4 : 8)>(a, mg, wave, kWaves, j, 4 * g * VCH, mx, L, o);
+    }
+    auto s_o = reinterpret_cast<float (*)[4 * VCH][64]>(attn_lds);
+    auto s_m = reinterpret_cast<float (*)[64]>(attn_lds + kWaves * 4 * VCH * 64 * 4);
+    auto s_l = s_m + kWaves;
+#pragma unroll
+    for (int e = 0; e < 4 * VCH; ++e) s_o[wave][e][lane] = o[e];
+    s_m[wave][lane] = mx;
+    s_l[wave][lane] = L;
+    __syncthreads();
+    if (!valid) return;
+    float M = kMinM;
+#pragma unroll
+    for (int u = 0; u < kWaves; ++u) M = fmaxf(M, s_m[u][lane]);
+    L = 0.f;
+    float r[VCH];
+#pragma unroll
+    for (int c = 0; c < VCH; ++c) r[c] = 0.f;
+#pragma unroll
+    for (int u = 0; u < kWaves; ++u) {
+        const float w = __builtin_amdgcn_exp2f(s_m[u][lane] - M);
+        L += s_l[u][lane] * w;
+#pragma unroll
+        for (int c = 0; c < VCH; ++c) r[c] += w * s_o[u][wave * VCH + c][lane];
+    }
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+#pragma unroll
+    for (int c = 0; c < VCH; ++c) r[c] *= inv;
+    store_elems<DT, VCH>(a.out + ((int64_t)prow * a.o_sr + (int64_t)qhead * a.o_sh + (4 * g + wave) * VCH) * 2, r);
+}
+template <int DP>
+constexpr int merge4_lds() { return (kWaves * 4 * (DP / 16) * 64 + 2 * kWaves * 64) * 4; }
+
 template <int DT, int DP, bool SC>
 int launch4(Attn4Args a, const int32_t* items, int64_t n_narrow, int64_t n_wide, const int32_t* merges,
             int64_t n_merges, const int32_t* dev_counts, hipStream_t stream) {
@@ -711,22 +797,26 @@ int launch4(Attn4Args a, const int32_t* items, int64_t n_narrow, int64_t n_wide,
         const int nb = (int)(n_narrow / kWaves);
         const dim3 grid((unsigned)((n_narrow + n_wide) / kWaves));
         const int32_t* wide_count = dev_counts ? dev_counts + 1 : nullptr;
-        if (n_wide == 0)
-            hipLaunchKernelGGL((attn4_kernel<DT, DP, SC, kNarrow4>), grid, dim3(256), lds4<DP>(false), stream, items, a, nb,
-                               wide, 0, (const int32_t*)nullptr);
-        else if constexpr (DP < 256) {
-            if (n_narrow == 0)
-                hipLaunchKernelGGL((attn4_kernel<DT, DP, SC, kWide4>), grid, dim3(256), wide_lds4<DP>(), stream, items, a,
-                                   0, wide, (int)n_wide, wide_count);
-            else
-                hipLaunchKernelGGL((attn4_kernel<DT, DP, SC, kBoth4>), grid, dim3(256), lds4<DP>(true), stream, items, a,
-                                   nb, wide, (int)n_wide, wide_count);
+        const bool blk16 = a.tpb == 1;
+#define MF_LAUNCH4(KIND, B16, LDS)                                                                                   \
+    hipLaunchKernelGGL((attn4_kernel<DT, DP, SC, KIND, B16>), grid, dim3(256), LDS, stream, items, a, nb, wide,      \
+                       (int)n_wide, wide_count)
+        if (n_wide == 0) {
+            if (blk16) MF_LAUNCH4(kNarrow4, true, lds4<DP>(false));
+            else MF_LAUNCH4(kNarrow4, false, lds4<DP>(false));
+        } else if constexpr (DP < 256) {
+            if (n_narrow == 0) MF_LAUNCH4(kWide4, false, wide_lds4<DP>());
+            else if (blk16) MF_LAUNCH4(kBoth4, true, lds4<DP>(true));
+            else MF_LAUNCH4(kBoth4, false, lds4<DP>(true));
         }
+#undef MF_LAUNCH4
         if (int st = check_launch()) return st;
     }
     if (n_merges > 0) {
         a.dev_count = dev_counts ? dev_counts + 2 : nullptr;
-        return launch_merge<DT, DP>(a, merges, n_merges, stream);
+        hipLaunchKernelGGL((merge4_kernel<DT, DP>), dim3((unsigned)n_merges), dim3(256), merge4_lds<DP>(), stream, merges,
+                           (int)n_merges, a);
+        return check_launch();
     }
     return MF_OK;
 }
@@ -778,6 +868,9 @@ extern "C" int mf_paged_attention4(const mf_scoring* scoring, const void* q, int
     a.vc = pool->value_codes;
     a.vs = pool->value_scales;
     a.tpb = pool->block_size / 16;
+    const int64_t blk_bytes = (int64_t)pool->num_heads * pool->block_size * (pool->head_dim / 2);
+    if (blk_bytes > INT_MAX) return MF_ERR_ARG;
+    a.blk_bytes = (uint32_t)blk_bytes;
     a.tpb_magic = a.tpb > 1 ? (uint32_t)(((1ull << 32) + a.tpb - 1) / a.tpb) : 0u;
     // as in mf_paged_attention: a negative scale turns q's signs, a zero one becomes
     // 2^-100

@@ -7,11 +7,12 @@
 #include "attn_kernels.h"
 
 namespace {
-// The planner of mf_attention_plan (num_cus 0), mf_attention_plan_device and
-// mf_attention_plan_merge_free (cut false).
+// The planner of mf_attention_plan (num_cus 0), mf_attention_plan_device,
+// mf_attention_plan_merge_free (cut false) and mf_attention_plan4 (four).
 int attention_plan(int num_seqs, const int32_t* cu_seqlens, const int32_t* kv_lens, int num_q_heads,
                    int num_kv_heads, int head_dim, int dtype, int partition_tiles, int num_cus, bool cut, int32_t* items,
-                   int64_t items_capacity, int32_t* merges, int64_t merges_capacity, int64_t* counts) {
+                   int64_t items_capacity, int32_t* merges, int64_t merges_capacity, int64_t* counts,
+                   bool four = false) {
     if (num_seqs < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || !counts)
         return MF_ERR_ARG;
     if (num_q_heads % num_kv_heads) return MF_ERR_ARG;
@@ -196,7 +197,46 @@ int attention_plan(int num_seqs, const int32_t* cu_seqlens, const int32_t* kv_le
         const int n = std::max(1, (int)std::lround(tiles / per_unit));
         return std::max(n, (tiles + mf::kWaves * mf::kMaxItemTiles - 1) / (mf::kWaves * mf::kMaxItemTiles));
     };
-    if (num_cus > 0 && partition_tiles <= 0 && !mixed) {
+    if (four && partition_tiles <= 0 && !mixed) {
+        // A 4-bit pool's tile is a quarter of the bytes and about a third of the chain
+        // (0.3 us a wave at head_dim 128). Ranges are cut into units for two workgroups
+        // a compute unit in all, three below head_dim 128, of at least 64 tiles and at
+        // least a 32nd of the longest range (a merge reads its partitions four by four,
+        // dealt to four waves), at most 512. Measured, us, at units of 64 / 96 / 160 /
+        // 256 / 512 tiles: 4 sequences of 16384 to 65536 keys at 40/8 heads x 128
+        // (rule 164) 48 / 46 / 41 / 48 / 54, with the 16-bit rule 56; one of 65536
+        // (128) 24.6 / 26 / 21.8 / 25 / 41; 64 of 200 to 3000 (100) 29 / 32 / 27 / 28 /
+        // 42; 256 of a median of 2048 (512) 214 / 200 / 190 / 184.5 / 183.4; at 15/5 x
+        // 64 32 of 1000 to 8000 (64) 18.5 / 19.4 / 21.8 / 26 / 40.
+        int64_t pairs = 0, tiles_all = 0;
+        int longest = 0;
+        for (int s = 0; s < num_seqs; ++s) {
+            const int nct = col_tiles(s);
+            if (!nct || !(nct == 1 || WT == 1)) continue;
+            const int T = (kv_lens[s] + 15) / 16;
+            pairs += (int64_t)Hkv * nct;
+            tiles_all += (int64_t)Hkv * nct * T;
+            longest = std::max(longest, T);
+        }
+        const double wgs = (head_dim >= 128 ? 2.0 : 3.0) * num_cus;
+        single_max = std::min(P, pairs <= num_cus ? 4 : pairs <= 2 * (int64_t)num_cus ? 16
+                                 : pairs <= 4 * (int64_t)num_cus ? 32 : mf::kMaxItemTiles);
+        // a few workgroups over a whole round would run alone after it, so the units
+        // grow until they fit (32 of 1000 to 8000 at 40/8 x 128: 552 workgroups 42 us,
+        // 480 37)
+        auto workgroups = [&]() {
+            double n = 0;
+            for (int s = 0; s < num_seqs; ++s) {
+                const int nct = col_tiles(s), T = (kv_lens[s] + 15) / 16;
+                if (!nct || !(nct == 1 || WT == 1)) continue;
+                n += (double)Hkv * nct * (T <= single_max ? 0.25 : decode_units(T, unit_tiles));
+            }
+            return n;
+        };
+        unit_tiles = std::max({64.0, longest / 32.0, tiles_all / wgs});
+        while (unit_tiles < 512 && workgroups() > wgs) unit_tiles *= 1.04;
+        unit_tiles = std::min(unit_tiles, 512.0);
+    } else if (num_cus > 0 && partition_tiles <= 0 && !mixed) {
         int64_t pairs = 0, tiles_all = 0, singles = 0, units = 0;
         int longest = 0;
         bool decode = true;
@@ -309,7 +349,7 @@ int attention_plan(int num_seqs, const int32_t* cu_seqlens, const int32_t* kv_le
     // 28.6 and 16 prompts of up to 1024 (64) 30 / 32. At 256-byte rows it always
     // does: 2 chunks of 2048 after 6144 keys 370 against 428 (10,240 merges).
     const bool device = num_cus > 0 && partition_tiles <= 0 && WT > 1 && dtype != MF_F32 && head_dim == DP &&
-                        (mixed || DP >= 128 || PW < 32);
+                        (mixed || DP >= 128 || PW < 32 || four);
     auto quads = [&](int s) -> int {  // column quads of s, 0 if s is not a shared wide sequence
         const int nct = col_tiles(s);
         if (!(mixed || device) || !nct || nct == 1 || WT == 1) return 0;
@@ -563,7 +603,7 @@ int attention_plan(int num_seqs, const int32_t* cu_seqlens, const int32_t* kv_le
                 // mod 8, its XCD's number, and an XCD that reads one head of
                 // every row uses one channel in eight of its L2 (67 against 75
                 // us, the 4 long sequences at 64-tile units).
-                const int h = narrow && unit_tiles > 0 ? (hi + p + s) % Hkv : hi;
+                const int h = narrow && unit_tiles > 0 && !four ? (hi + p + s) % Hkv : hi;
                 if (narrow) {
                     for (int gi = 0; gi < ngroups; ++gi) {
                         if (!coop) {
@@ -787,6 +827,14 @@ extern "C" int mf_attention_plan_merge_free(int num_seqs, const int32_t* cu_seql
 // multiple of the kernel's ring depth; a workload whose even share would
 // exceed that gets more slices (a second round). A sequence cut across
 // slices leaves one partial per piece and kv head, merged afterwards.
+extern "C" int mf_attention_plan4(int num_seqs, const int32_t* cu_seqlens, const int32_t* kv_lens, int num_q_heads,
+                                  int num_kv_heads, int head_dim, int dtype, int num_cus, int32_t* items,
+                                  int64_t items_capacity, int32_t* merges, int64_t merges_capacity, int64_t* counts) {
+    if (num_cus <= 0) return MF_ERR_ARG;
+    return attention_plan(num_seqs, cu_seqlens, kv_lens, num_q_heads, num_kv_heads, head_dim, dtype, 0, num_cus, true,
+                          items, items_capacity, merges, merges_capacity, counts, /*four=*/true);
+}
+
 extern "C" int mf_attention_plan_slices(int num_seqs, const int32_t* cu_seqlens, const int32_t* kv_lens,
                                         int num_q_heads, int num_kv_heads, int head_dim, int dtype,
                                         int num_cus, int min_tiles_per_wave, int32_t* slices,

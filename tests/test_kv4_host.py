@@ -139,3 +139,40 @@ def test_list_operator_checks_before_the_device():
     from memforge_amd.kernels.varlen_attention import paged_attention_varlen_pool
     with pytest.raises(ValueError):
         paged_attention_varlen_pool(torch.zeros(1, 3, 1, 64), Pool(), 0, [[0]], [0], [3])
+
+
+def test_plans_for_a_4_bit_pool():
+    """Every tile of every (sequence, kv head, column tile) in one item, ranges that a wave's registers hold, whole
+    workgroups of wide items, merge records that name their partitions."""
+    import numpy as np
+
+    rng = np.random.default_rng(1)
+    for _ in range(40):
+        n = int(rng.integers(1, 40))
+        rows = np.ones(n, dtype=int) if rng.random() < 0.5 else rng.integers(1, 60, n)
+        kv = rows + (10 ** rng.uniform(0, 4.7, n)).astype(int)
+        hq, hkv, d = ((40, 8, 128), (15, 5, 64), (8, 8, 32), (16, 2, 256))[rng.integers(4)]
+        cu = np.concatenate([[0], np.cumsum(rows)])
+        items, merges, counts = nat.plan_attention_host(cu, kv, hq, hkv, d, torch.bfloat16, num_cus=256, kv_bits=4)
+        narrow = int(counts[0])
+        seen, parts = {}, {}
+        for i, it in enumerate(items):
+            if i < narrow:
+                assert it[5] - it[4] <= 128
+            if it[9] == 0 or it[3] == 0:
+                continue
+            for c in range(it[2], it[2] + it[3]):
+                seen.setdefault((it[0], it[1], c), set()).update(range(it[4], it[5]))
+                if it[6] >= 0:
+                    parts.setdefault((it[0], it[1], c), set()).add(it[6] + c - it[2])
+        for s in range(n):
+            for h in range(hkv):
+                for c in range(-(-rows[s] * (hq // hkv) // 16)):
+                    got = seen[(s, h, c)]
+                    last = kv[s] - rows[s] + min((c * 16 + 15) // (hq // hkv), rows[s] - 1)  # the tile's last position
+                    assert got >= set(range(last // 16 + 1))
+        for m in merges:
+            want = {m[4] + p * m[5] for p in range(m[3])}
+            assert parts[(m[0], m[1], m[2])] == want
+        wide = items[narrow:].reshape(-1, 4, 12)
+        assert (wide[:, :, [0, 1, 4, 5]] == wide[:, :1, [0, 1, 4, 5]]).all()
