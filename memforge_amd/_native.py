@@ -10,7 +10,6 @@ runs on the MI355X or not at all.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from collections import OrderedDict
 from dataclasses import dataclass
@@ -248,16 +247,14 @@ class Pool4View:
         self.value_codes, self.value_scales = value_codes, value_scales
         self.dtype = dtype
         self.num_blocks, self.num_heads, self.block_size, self.head_dim = n, h, bs, 8 * words
+        self.device = key_codes.device
         self.struct = _Pool4Struct(_ptr(key_codes), _ptr(key_scales), _ptr(value_codes), _ptr(value_scales), n, bs, h,
                                    8 * words, dtype_code(dtype))
+        self.address = ctypes.addressof(self.struct)
 
     @property
     def num_slots(self) -> int:
         return self.num_blocks * self.block_size
-
-    @property
-    def device(self) -> torch.device:
-        return self.key_codes.device
 
 
 def same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -316,42 +313,74 @@ def kv_gather(pool: PoolView, slots: torch.Tensor, k_rows: torch.Tensor, v_rows:
     ), "mf_kv_gather")
 
 
-def _rows4(k_rows, v_rows, slots, pool: Pool4View):
-    _rows_ok(k_rows, "k_rows")
-    _rows_ok(v_rows, "v_rows")
-    require_device(k_rows, v_rows, slots, pool.key_codes)
-    if not k_rows.device == v_rows.device == slots.device == pool.device:
-        raise ValueError("rows, slots and pool must be on one device")
+def _slots4(slots: torch.Tensor, pool: Pool4View) -> torch.Tensor:
     if slots.dtype != torch.int64 or not slots.is_contiguous():
         slots = slots.to(torch.int64).contiguous()
-    if k_rows.shape != v_rows.shape or k_rows.dtype != v_rows.dtype \
-            or tuple(k_rows.shape) != (slots.numel(), pool.num_heads, pool.head_dim):
-        raise ValueError(f"rows {tuple(k_rows.shape)} / {tuple(v_rows.shape)} and {slots.numel()} slots do not match a "
-                         f"pool of {pool.num_heads} heads x {pool.head_dim}")
+    if slots.get_device() != pool.device.index:
+        raise ValueError(f"slots are on {slots.device}, the pool on {pool.device}")
     return slots
+
+
+def _check_rows4(k: torch.Tensor, v: torch.Tensor, tokens: int, heads: int, dim: int, num_slots: int,
+                 pool: Pool4View) -> None:
+    if k.get_device() != pool.device.index or v.get_device() != pool.device.index:
+        raise ValueError(f"rows are on {k.device} / {v.device}, the pool on {pool.device}")
+    if k.shape != v.shape or k.dtype != v.dtype or tokens != num_slots or heads != pool.num_heads \
+            or dim != pool.head_dim:
+        raise ValueError(f"rows {tuple(k.shape)} / {tuple(v.shape)} of {k.dtype} / {v.dtype} and {num_slots} slots do "
+                         f"not match a pool of {pool.num_heads} heads x {pool.head_dim}")
 
 
 def kv4_write(k_rows: torch.Tensor, v_rows: torch.Tensor, slots: torch.Tensor, pool: Pool4View) -> None:
     """Round (T, H, D) rows to 4 bits into the pool slots ``slots`` (int64, device,
     distinct; a slot outside the pool skips its row)."""
-    slots = _rows4(k_rows, v_rows, slots, pool)
+    _rows_ok(k_rows, "k_rows")
+    _rows_ok(v_rows, "v_rows")
+    slots = _slots4(slots, pool)
+    n = slots.numel()
+    _check_rows4(k_rows, v_rows, *k_rows.shape, n, pool)
     if not same_layout(k_rows, v_rows):
         k_rows, v_rows = k_rows.contiguous(), v_rows.contiguous()
-    with _on(pool.device):
-        _check(lib().mf_kv4_write(
-            _ptr(k_rows), _ptr(v_rows), dtype_code(k_rows.dtype), k_rows.stride(0), k_rows.stride(1), _ptr(slots),
-            slots.numel(), ctypes.addressof(pool.struct), _stream(pool.device)), "mf_kv4_write")
+    _launch(pool.device, "mf_kv4_write", lib().mf_kv4_write, k_rows.data_ptr(), v_rows.data_ptr(),
+            dtype_code(k_rows.dtype), k_rows.stride(0), k_rows.stride(1), slots.data_ptr(), n, pool.address)
+
+
+def kv4_write_states(keys: torch.Tensor, values: torch.Tensor, slots: torch.Tensor, pool: Pool4View) -> None:
+    """``kv4_write`` of a layer's ``(1, H, T, D)`` key and value states, as they are laid out."""
+    if keys.dim() != 4 or keys.shape[0] != 1:
+        raise ValueError(f"expected (1, heads, tokens, head_dim) states, got {tuple(keys.shape)}")
+    if keys.stride() != values.stride() or keys.stride(3) != 1:
+        return kv4_write(keys[0].permute(1, 0, 2).contiguous(), values[0].permute(1, 0, 2).contiguous(), slots, pool)
+    slots = _slots4(slots, pool)
+    n = slots.numel()
+    _, h, tokens, d = keys.shape
+    _check_rows4(keys, values, tokens, h, d, n, pool)
+    _launch(pool.device, "mf_kv4_write", lib().mf_kv4_write, keys.data_ptr(), values.data_ptr(),
+            dtype_code(keys.dtype), keys.stride(2), keys.stride(1), slots.data_ptr(), n, pool.address)
 
 
 def kv4_gather(pool: Pool4View, slots: torch.Tensor, k_rows: torch.Tensor, v_rows: torch.Tensor) -> None:
     """The values that pool slots ``slots`` stand for, into preallocated (T, H, D) rows."""
-    slots = _rows4(k_rows, v_rows, slots, pool)
+    _rows_ok(k_rows, "k_rows")
+    _rows_ok(v_rows, "v_rows")
+    slots = _slots4(slots, pool)
+    n = slots.numel()
+    _check_rows4(k_rows, v_rows, *k_rows.shape, n, pool)
     if not same_layout(k_rows, v_rows):
         raise ValueError("k_rows and v_rows must share strides")
-    with _on(pool.device):
-        _check(lib().mf_kv4_gather(
-            ctypes.addressof(pool.struct), _ptr(slots), slots.numel(), _ptr(k_rows), _ptr(v_rows),
-            dtype_code(k_rows.dtype), k_rows.stride(0), k_rows.stride(1), _stream(pool.device)), "mf_kv4_gather")
+    _launch(pool.device, "mf_kv4_gather", lib().mf_kv4_gather, pool.address, slots.data_ptr(), n, k_rows.data_ptr(),
+            v_rows.data_ptr(), dtype_code(k_rows.dtype), k_rows.stride(0), k_rows.stride(1))
+
+
+def kv4_gather_states(pool: Pool4View, slots: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The values of ``slots`` as new contiguous ``(1, H, T, D)`` keys and values in the pool's dtype."""
+    slots = _slots4(slots, pool)
+    n, h, d = slots.numel(), pool.num_heads, pool.head_dim
+    k = torch.empty((1, h, n, d), dtype=pool.dtype, device=pool.device)
+    v = torch.empty((1, h, n, d), dtype=pool.dtype, device=pool.device)
+    _launch(pool.device, "mf_kv4_gather", lib().mf_kv4_gather, pool.address, slots.data_ptr(), n, k.data_ptr(),
+            v.data_ptr(), dtype_code(pool.dtype), d, n * d)
+    return k, v
 
 
 def kv_copy_blocks(key_pool: torch.Tensor, value_pool: torch.Tensor,
@@ -949,9 +978,25 @@ class _Plan:
             raise ValueError(f"the plan needs {plan.partials_floats} partial floats, got {self.partials.numel()}")
 
 
-def _on(device: torch.device):
-    """The device's context, entered only when another device is current."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _launch(device: torch.device, what: str, fn, *args) -> None:
+    """``fn(*args, stream)`` on the device's current stream, with the device current."""
+    if device.index == torch.cuda.current_device():
+        status = fn(*args, _stream(device))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, _stream(device))
+    if status:
+        _check(status, what)
+
+
+def _index_tensors(device: torch.device, block_tables, cu_seqlens, kv_lens, positions) -> None:
+    index = device.index
+    for name, t, dt in (("block_tables", block_tables, torch.int32), ("cu_seqlens", cu_seqlens, torch.int32),
+                        ("kv_lens", kv_lens, torch.int32), ("positions", positions, torch.int64)):
+        if t.dtype != dt or not t.is_contiguous():
+            raise TypeError(f"{name} must be a contiguous {dt} tensor")
+        if t.get_device() != index:
+            raise ValueError(f"{name} is on {t.device}, the query on {device}")
 
 
 def _paged_attention_scored(scoring: Scoring, q_rows, out_rows, pool, block_tables, cu_seqlens, kv_lens, positions,
@@ -967,25 +1012,24 @@ def _paged_attention_scored(scoring: Scoring, q_rows, out_rows, pool, block_tabl
     p = _Plan(plan, dev, partials)
     mods = scoring.struct(q_rows.shape[1], kv_lens.numel(), dev)
     bt_stride = block_tables.shape[1] if block_tables.dim() == 2 else 0
-    with _on(dev):
-        _check(lib().mf_paged_attention_scored(
-            ctypes.addressof(mods), _ptr(q_rows), q_rows.stride(0), q_rows.stride(1),
-            _ptr(out_rows), out_rows.stride(0), out_rows.stride(1),
-            dtype_code(q_rows.dtype), _ptr(pool.k), _ptr(pool.v),
-            pool.stride_block, pool.stride_slot, pool.stride_head, pool.block_size,
-            _ptr(block_tables), bt_stride, _ptr(cu_seqlens), _ptr(kv_lens), _ptr(positions),
-            _ptr(row_map), _ptr(pool_lens), _ptr(nk), _ptr(nv),
-            nk.stride(0) if nk is not None else 0, nk.stride(1) if nk is not None else 0,
-            _ptr(slot_mapping), slot_mapping.numel() if slot_mapping is not None else 0, pool.num_slots,
-            q_rows.shape[1], num_kv_heads, q_rows.shape[2], float(scale),
-            _ptr(plan.items), p.narrow, p.wide, _ptr(plan.merges), p.merges, _ptr(p.counts),
-            _ptr(p.partials), p.partials.numel() if p.partials is not None else 0, _stream(dev),
-        ), "mf_paged_attention_scored")
+    _launch(
+        dev, "mf_paged_attention_scored", lib().mf_paged_attention_scored,
+        ctypes.addressof(mods), _ptr(q_rows), q_rows.stride(0), q_rows.stride(1),
+        _ptr(out_rows), out_rows.stride(0), out_rows.stride(1),
+        dtype_code(q_rows.dtype), _ptr(pool.k), _ptr(pool.v),
+        pool.stride_block, pool.stride_slot, pool.stride_head, pool.block_size,
+        _ptr(block_tables), bt_stride, _ptr(cu_seqlens), _ptr(kv_lens), _ptr(positions),
+        _ptr(row_map), _ptr(pool_lens), _ptr(nk), _ptr(nv),
+        nk.stride(0) if nk is not None else 0, nk.stride(1) if nk is not None else 0,
+        _ptr(slot_mapping), slot_mapping.numel() if slot_mapping is not None else 0, pool.num_slots,
+        q_rows.shape[1], num_kv_heads, q_rows.shape[2], float(scale),
+        _ptr(plan.items), p.narrow, p.wide, _ptr(plan.merges), p.merges, _ptr(p.counts),
+        _ptr(p.partials), p.partials.numel() if p.partials is not None else 0)
 
 
 def _check4(q_rows, out_rows, pool: Pool4View, num_kv_heads: int) -> None:
     require_device(q_rows, out_rows, pool.key_codes)
-    if not q_rows.device == out_rows.device == pool.device:
+    if not q_rows.get_device() == out_rows.get_device() == pool.device.index:
         raise ValueError("query, output and pool must be on one device")
     if pool.dtype == torch.float32:
         raise TypeError("attention over a 4-bit pool runs in float16 or bfloat16; this pool's dtype is float32")
@@ -1000,25 +1044,20 @@ def _paged_attention4(scoring, q_rows, out_rows, pool: Pool4View, block_tables, 
                       scale, num_kv_heads, row_map=None, partials=None) -> None:
     _check4(q_rows, out_rows, pool, num_kv_heads)
     dev = q_rows.device
-    for name, t, dt in (("block_tables", block_tables, torch.int32), ("cu_seqlens", cu_seqlens, torch.int32),
-                        ("kv_lens", kv_lens, torch.int32), ("positions", positions, torch.int64)):
-        if t.dtype != dt or not t.is_contiguous():
-            raise TypeError(f"{name} must be a contiguous {dt} tensor")
-        if t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, the query on {dev}")
+    _index_tensors(dev, block_tables, cu_seqlens, kv_lens, positions)
     p = _Plan(plan, dev, partials)
     scoring = _scored(scoring)
     mods = scoring.struct(q_rows.shape[1], kv_lens.numel(), dev) if scoring is not None else None
-    bt_stride = block_tables.shape[1] if block_tables.dim() == 2 else 0
-    with _on(dev):
-        _check(lib().mf_paged_attention4(
-            ctypes.addressof(mods) if mods is not None else None,
-            _ptr(q_rows), q_rows.stride(0), q_rows.stride(1), _ptr(out_rows), out_rows.stride(0), out_rows.stride(1),
-            dtype_code(q_rows.dtype), ctypes.addressof(pool.struct), _ptr(block_tables), bt_stride,
-            _ptr(cu_seqlens), _ptr(kv_lens), _ptr(positions), _ptr(row_map), q_rows.shape[1], float(scale),
-            _ptr(plan.items), p.narrow, p.wide, _ptr(plan.merges), p.merges, _ptr(p.counts),
-            _ptr(p.partials), p.partials.numel() if p.partials is not None else 0, _stream(dev),
-        ), "mf_paged_attention4")
+    _launch(
+        dev, "mf_paged_attention4", lib().mf_paged_attention4,
+        ctypes.addressof(mods) if mods is not None else None,
+        q_rows.data_ptr(), q_rows.stride(0), q_rows.stride(1),
+        out_rows.data_ptr(), out_rows.stride(0), out_rows.stride(1),
+        dtype_code(q_rows.dtype), pool.address, block_tables.data_ptr(),
+        block_tables.shape[1] if block_tables.dim() == 2 else 0,
+        cu_seqlens.data_ptr(), kv_lens.data_ptr(), positions.data_ptr(), _ptr(row_map), q_rows.shape[1], float(scale),
+        plan.items.data_ptr(), p.narrow, p.wide, plan.merges.data_ptr(), p.merges, _ptr(p.counts),
+        _ptr(p.partials), p.partials.numel() if p.partials is not None else 0)
 
 
 def paged_attention_kv_write(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: PoolView,
@@ -1219,32 +1258,30 @@ def paged_attention_packed(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: P
         mods = Scoring(softcap, slopes).struct(q_rows.shape[1], num_seqs, dev)
         mods.first_keys = addr[at] if has_first_keys else None
         mods.prefix_lens = addr[at + int(has_first_keys)] if has_prefix_lens else None
+    scored_at = ctypes.addressof(mods) if mods is not None else None
     if four:
-        with _on(dev):
-            _check(lib().mf_paged_attention4(
-                ctypes.addressof(mods) if mods is not None else None,
-                _ptr(q_rows), q_rows.stride(0), q_rows.stride(1),
-                _ptr(out_rows), out_rows.stride(0), out_rows.stride(1),
-                dtype_code(q_rows.dtype), ctypes.addressof(pool.struct), addr[0], bt_stride,
-                addr[3], addr[3] + 4 * (num_seqs + 1), addr[4], row_map, q_rows.shape[1], float(scale),
-                addr[1], n_narrow, n_wide, addr[2], n_merges, None,
-                _ptr(partials), partials.numel() if partials is not None else 0, _stream(dev),
-            ), "mf_paged_attention4")
+        _launch(
+            dev, "mf_paged_attention4", lib().mf_paged_attention4, scored_at,
+            _ptr(q_rows), q_rows.stride(0), q_rows.stride(1),
+            _ptr(out_rows), out_rows.stride(0), out_rows.stride(1),
+            dtype_code(q_rows.dtype), pool.address, addr[0], bt_stride,
+            addr[3], addr[3] + 4 * (num_seqs + 1), addr[4], row_map, q_rows.shape[1], float(scale),
+            addr[1], n_narrow, n_wide, addr[2], n_merges, None,
+            _ptr(partials), partials.numel() if partials is not None else 0)
         return
     if mods is not None:
-        with _on(dev):
-            _check(lib().mf_paged_attention_scored(
-                ctypes.addressof(mods), _ptr(q_rows), q_rows.stride(0), q_rows.stride(1),
-                _ptr(out_rows), out_rows.stride(0), out_rows.stride(1),
-                dtype_code(q_rows.dtype), _ptr(pool.k), _ptr(pool.v),
-                pool.stride_block, pool.stride_slot, pool.stride_head, pool.block_size,
-                addr[0], bt_stride, addr[3], addr[3] + 4 * (num_seqs + 1), addr[4],
-                row_map, pool_lens, _ptr(nk), _ptr(nv),
-                nk.stride(0) if nk is not None else 0, nk.stride(1) if nk is not None else 0, None, 0, 0,
-                q_rows.shape[1], num_kv_heads, q_rows.shape[2], float(scale),
-                addr[1], n_narrow, n_wide, addr[2], n_merges, None,
-                _ptr(partials), partials.numel() if partials is not None else 0, _stream(dev),
-            ), "mf_paged_attention_scored")
+        _launch(
+            dev, "mf_paged_attention_scored", lib().mf_paged_attention_scored, scored_at,
+            _ptr(q_rows), q_rows.stride(0), q_rows.stride(1),
+            _ptr(out_rows), out_rows.stride(0), out_rows.stride(1),
+            dtype_code(q_rows.dtype), _ptr(pool.k), _ptr(pool.v),
+            pool.stride_block, pool.stride_slot, pool.stride_head, pool.block_size,
+            addr[0], bt_stride, addr[3], addr[3] + 4 * (num_seqs + 1), addr[4],
+            row_map, pool_lens, _ptr(nk), _ptr(nv),
+            nk.stride(0) if nk is not None else 0, nk.stride(1) if nk is not None else 0, None, 0, 0,
+            q_rows.shape[1], num_kv_heads, q_rows.shape[2], float(scale),
+            addr[1], n_narrow, n_wide, addr[2], n_merges, None,
+            _ptr(partials), partials.numel() if partials is not None else 0)
         return
     _check(lib().mf_paged_attention(
         _ptr(q_rows), q_rows.stride(0), q_rows.stride(1),

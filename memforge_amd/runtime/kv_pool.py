@@ -254,21 +254,14 @@ class PagedKVPool4:
         self.write_flat(layer_idx, paged_gather.flat_slot_index(physical, slots, self.block_size), keys, values)
 
     def write_flat(self, layer_idx: int, flat_index: torch.Tensor, keys: torch.Tensor, values: torch.Tensor) -> None:
-        nat.kv4_write(keys[0].permute(1, 0, 2), values[0].permute(1, 0, 2), flat_index.reshape(-1),
-                      self.layer_view(layer_idx))
+        nat.kv4_write_states(keys, values, flat_index.reshape(-1), self.layer_view(layer_idx))
 
     def gather(self, layer_idx: int, physical: torch.Tensor, slots: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         """The values of (physical, slot) as contiguous ``(1, num_kv_heads, T, head_dim)`` K/V."""
         return self.gather_flat(layer_idx, paged_gather.flat_slot_index(physical, slots, self.block_size))
 
     def gather_flat(self, layer_idx: int, flat_index: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
-        spec = self.spec
-        k = torch.empty((1, spec.num_kv_heads, flat_index.numel(), spec.head_dim), dtype=spec.dtype,
-                        device=self.key_codes.device)
-        v = torch.empty_like(k)
-        nat.kv4_gather(self.layer_view(layer_idx), flat_index.reshape(-1), k[0].permute(1, 0, 2),
-                       v[0].permute(1, 0, 2))
-        return k, v
+        return nat.kv4_gather_states(self.layer_view(layer_idx), flat_index.reshape(-1))
 
     def copy_blocks(self, pairs) -> None:
         """Copy block ``src`` to ``dst`` for every pair, in every layer
