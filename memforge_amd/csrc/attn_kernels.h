@@ -389,7 +389,8 @@ __device__ __forceinline__ void store_out_chunk(char* p, const float* vals) {
 // instead (the slot has the room): a device's decode plan cuts ranges that the
 // general plan runs as one cooperative unit, whose waves combine in fp32, and the
 // cut must not round what the whole unit does not. 16-bit launches of 256-byte
-// rows and more only, as that rule.
+// rows and more only, as that rule. Scored launches and those over a 4-bit pool keep
+// every partial in fp32.
 template <int DT, int DP>
 constexpr bool has_fp32_partials() { return DT != MF_F32 && DP >= 128; }
 template <int DT>
@@ -478,8 +479,9 @@ __device__ __forceinline__ bool merge_column(const AttnArgs& a, const int32_t* m
 }
 
 // Single-wave merge of one record. FP32B: partitions per batch of a record of
-// fp32 partials, 0 where the caller's records have none (prefill items).
-template <int DT, int DP, int FP32B = 0>
+// fp32 partials, 0 where the caller's records have none (prefill items). ALL32: every
+// record's are.
+template <int DT, int DP, int FP32B = 0, bool ALL32 = false>
 __device__ __forceinline__ void merge_tile(const AttnArgs& a, const int32_t* mg, int g, int j) {
     constexpr int VCH = DP / 16;
     constexpr int ES = DT == MF_F32 ? 4 : 2;
@@ -488,7 +490,10 @@ __device__ __forceinline__ void merge_tile(const AttnArgs& a, const int32_t* mg,
     if (!merge_column(a, mg, j, prow, qhead) || dbase >= a.head_dim) return;
     float mx, L, o[4 * VCH];
     bool merged = false;
-    if constexpr (has_fp32_partials<DT, DP>() && FP32B > 0) {
+    if constexpr (ALL32) {
+        merge_range<DT, DP, MF_F32, FP32B>(a, mg, 0, 1, j, dbase, mx, L, o);
+        merged = true;
+    } else if constexpr (has_fp32_partials<DT, DP>() && FP32B > 0) {
         if (mg[7] & MF_PLAN_FP32_PARTIALS) {
             merge_range<DT, DP, MF_F32, FP32B>(a, mg, 0, 1, j, dbase, mx, L, o);
             merged = true;
@@ -1207,8 +1212,8 @@ __device__ __forceinline__ void attn_body(const ArgsOf<SC>& a, const int block) 
                     const float inv = L > 0.f ? 1.f / L : 0.f;
 #pragma unroll
                     for (int c = 0; c < VCH; ++c) o[c] *= inv;
-                    bool fp32 = false;
-                    if constexpr (has_fp32_partials<DT, DP>()) fp32 = (iv1.w & MF_PLAN_FP32_PARTIALS) != 0;
+                    bool fp32 = SC;
+                    if constexpr (!SC && has_fp32_partials<DT, DP>()) fp32 = (iv1.w & MF_PLAN_FP32_PARTIALS) != 0;
                     if (fp32) store_elems<MF_F32, VCH>(partial_out<MF_F32>(a, pslot, j, d0), o);
                     else store_elems<DT, VCH>(partial_out<DT>(a, pslot, j, d0), o);
                     if (g == 0 && wave == 0) {
@@ -1265,7 +1270,8 @@ __device__ __forceinline__ void attn_body(const ArgsOf<SC>& a, const int block) 
             for (int r = 0; r < 4; ++r)
 #pragma unroll
                 for (int c = 0; c < VCH; ++c) vals[r * VCH + c] = acc[nt][c][r] * inv;
-            store_out_chunk<DT, VCH>(partial_out<DT>(a, pslot + nt, j, dbase), vals);
+            constexpr int PT = SC ? MF_F32 : DT;
+            store_out_chunk<PT, VCH>(partial_out<PT>(a, pslot + nt, j, dbase), vals);
             if (g == 0) {
                 float* ml = partial_ml(a, pslot + nt);
                 ml[j] = m[nt];
@@ -1739,6 +1745,28 @@ __device__ __forceinline__ void attn_wide_body(const ArgsOf<SC>& a, const int bl
     auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
     const float lt = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     const float inv = lt > 0.f ? 1.f / lt : 0.f;
+    if (SC && pslot >= 0) {
+        if (qpos >= 0) {
+            char* part = partial_out<MF_F32>(a, pslot + ct, j, 0);
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    float4 o;
+                    o.x = acc[d][4 * b] * inv;
+                    o.y = acc[d][4 * b + 1] * inv;
+                    o.z = acc[d][4 * b + 2] * inv;
+                    o.w = acc[d][4 * b + 3] * inv;
+                    *(float4*)(part + (32 * d + 8 * b + 4 * hf) * 4) = o;
+                }
+            if (hf == 0) {
+                float* ml = partial_ml(a, pslot + ct);
+                ml[j] = m;
+                ml[16 + j] = lt;
+            }
+        }
+        return;
+    }
     char* dst = nullptr;
     if (qpos >= 0)
         dst = pslot < 0 ? a.out + ((int64_t)prow * a.o_sr + (int64_t)qhead * a.o_sh) * 2
@@ -2213,14 +2241,66 @@ __device__ __forceinline__ void load_merge_record(const AttnArgs& a, const int32
 // combining them in LDS below 128 records, four records per workgroup above):
 // C3's verify layer (75 records) 11.36-11.38 us against 12.29-12.40, the C2
 // layer (1,955 records) 37.9-38.1 against 38.2-38.3, C5 (824) the same.
-template <int DT, int DP>
+template <int DT, int DP, bool ALL32 = false>
 __global__ __launch_bounds__(64) void merge_kernel(const int32_t* merges, int num_merges, AttnArgs a) {
     const int mi = blockIdx.x;
     int32_t mg[MF_PLAN_MERGE_INTS];
     load_merge_record(a, merges, mi, num_merges, mg);
     if (mi >= (a.dev_count ? *a.dev_count : num_merges)) return;
     const int lane = threadIdx.x & 63;
-    merge_tile<DT, DP, (DP > 128 ? 2 : 4)>(a, mg, lane >> 4, lane & 15);
+    merge_tile<DT, DP, (DP > 128 ? 2 : 4), ALL32>(a, mg, lane >> 4, lane & 15);
+}
+
+// Fp32 partials of decode ranges: one workgroup per record, its partitions dealt to the
+// four waves, whose results are combined through LDS as the cooperative units' states
+// are. A long range is cut into some thirty, which one wave reads four at a time: 32
+// records of up to 36 partitions, 19 us that way, 8 this way.
+constexpr int merge_quad_lds(int dp) { return (kWaves * (dp / 4) * 64 + 2 * kWaves * 64) * 4; }
+template <int DT, int DP>
+__global__ __launch_bounds__(256) void merge_quad_kernel(const int32_t* merges, int num_merges, AttnArgs a) {
+    constexpr int VCH = DP / 16;
+    const int mi = blockIdx.x;
+    int32_t mg[MF_PLAN_MERGE_INTS];
+    load_merge_record(a, merges, mi, num_merges, mg);
+    if (mi >= (a.dev_count ? *a.dev_count : num_merges)) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
+    int prow = 0, qhead = 0;
+    const bool valid = merge_column(a, mg, j, prow, qhead) && 4 * g * VCH < a.head_dim;
+    float mx = kMinM, L = 0.f, o[4 * VCH];
+#pragma unroll
+    for (int e = 0; e < 4 * VCH; ++e) o[e] = 0.f;
+    if (valid && wave < mg[3])
+        merge_range<DT, DP, MF_F32, (DP > 128 ? 2 : 4)>(a, mg, wave, kWaves, j, 4 * g * VCH, mx, L, o);
+    auto s_o = reinterpret_cast<float (*)[4 * VCH][64]>(attn_lds);
+    auto s_m = reinterpret_cast<float (*)[64]>(attn_lds + kWaves * 4 * VCH * 64 * 4);
+    auto s_l = s_m + kWaves;
+#pragma unroll
+    for (int e = 0; e < 4 * VCH; ++e) s_o[wave][e][lane] = o[e];
+    s_m[wave][lane] = mx;
+    s_l[wave][lane] = L;
+    __syncthreads();
+    const int d0 = (4 * g + wave) * VCH;
+    if (!valid || d0 >= a.head_dim) return;
+    float M = kMinM;
+#pragma unroll
+    for (int u = 0; u < kWaves; ++u) M = fmaxf(M, s_m[u][lane]);
+    L = 0.f;
+    float r[VCH];
+#pragma unroll
+    for (int c = 0; c < VCH; ++c) r[c] = 0.f;
+#pragma unroll
+    for (int u = 0; u < kWaves; ++u) {
+        const float w = __builtin_amdgcn_exp2f(s_m[u][lane] - M);
+        L += s_l[u][lane] * w;
+#pragma unroll
+        for (int c = 0; c < VCH; ++c) r[c] += w * s_o[u][wave * VCH + c][lane];
+    }
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+#pragma unroll
+    for (int c = 0; c < VCH; ++c) r[c] *= inv;
+    constexpr int ES = DT == MF_F32 ? 4 : 2;
+    store_elems<DT, VCH>(a.out + ((int64_t)prow * a.o_sr + (int64_t)qhead * a.o_sh + d0) * ES, r);
 }
 
 // The split-K merge launch: one single-wave workgroup per record.
@@ -2228,6 +2308,20 @@ template <int DT, int DP>
 int launch_merge(const AttnArgs& a, const int32_t* merges, int64_t n_merges, hipStream_t stream) {
     hipLaunchKernelGGL((merge_kernel<DT, DP>), dim3((unsigned)n_merges), dim3(64), 0, stream, merges, (int)n_merges,
                        a);
+    return check_launch();
+}
+
+// The merge of a launch whose partials are all fp32: four waves a record where all its
+// items are decode ranges, one where prefill items leave many records of two or three
+// partitions.
+template <int DT, int DP>
+int launch_merge32(const AttnArgs& a, const int32_t* merges, int64_t n_merges, bool decode, hipStream_t stream) {
+    if (decode)
+        hipLaunchKernelGGL((merge_quad_kernel<DT, DP>), dim3((unsigned)n_merges), dim3(256), merge_quad_lds(DP), stream,
+                           merges, (int)n_merges, a);
+    else
+        hipLaunchKernelGGL((merge_kernel<DT, DP, true>), dim3((unsigned)n_merges), dim3(64), 0, stream, merges,
+                           (int)n_merges, a);
     return check_launch();
 }
 
@@ -2241,6 +2335,7 @@ int launch_attention(ArgsOf<SC> a, const int32_t* items, int64_t n_narrow, int64
     // With arrival counters the attention kernel merges its own partitions;
     // a merges-only call (no items) still runs the separate merge kernel.
     const bool fused = a.counters != nullptr && (n_narrow + n_wide) > 0;
+    const bool decode = n_wide == 0;
     constexpr int NTW = wide_tiles(DT, DP);
     if constexpr (TAIL) {
         if (!fast) return MF_ERR_UNSUPPORTED;
@@ -2315,7 +2410,8 @@ int launch_attention(ArgsOf<SC> a, const int32_t* items, int64_t n_narrow, int64
     }
     if (n_merges > 0 && !fused) {
         a.dev_count = dev_counts ? dev_counts + 2 : nullptr;
-        if (int st = launch_merge<DT, DP>(a, merges, n_merges, stream)) return st;
+        if constexpr (SC) return launch_merge32<DT, DP>(a, merges, n_merges, decode, stream);
+        else if (int st = launch_merge<DT, DP>(a, merges, n_merges, stream)) return st;
     }
     return MF_OK;
 }

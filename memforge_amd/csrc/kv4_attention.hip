@@ -342,10 +342,7 @@ __device__ __forceinline__ void attn4_narrow(const Attn4Args& a, const int32_t* 
         if (pslot < 0) {
             store_elems<DT, VCH>(a.out + ((int64_t)prow * a.o_sr + (int64_t)qhead * a.o_sh + d0) * 2, o);
         } else {
-            bool fp32 = false;
-            if constexpr (has_fp32_partials<DT, DP>()) fp32 = (it[7] & MF_PLAN_FP32_PARTIALS) != 0;
-            if (fp32) store_elems<MF_F32, VCH>(partial_out<MF_F32>(a, pslot, j, d0), o);
-            else store_elems<DT, VCH>(partial_out<DT>(a, pslot, j, d0), o);
+            store_elems<MF_F32, VCH>(partial_out<MF_F32>(a, pslot, j, d0), o);
             if (g == 0 && wave == 0) {
                 partial_ml(a, pslot)[j] = M;
                 partial_ml(a, pslot)[16 + j] = L;
@@ -363,7 +360,7 @@ __device__ __forceinline__ void attn4_narrow(const Attn4Args& a, const int32_t* 
     if (pslot < 0) {
         store_out_chunk<DT, VCH>(a.out + ((int64_t)prow * a.o_sr + (int64_t)qhead * a.o_sh + 4 * g * VCH) * 2, o);
     } else {
-        store_out_chunk<DT, VCH>(partial_out<DT>(a, pslot, j, 4 * g * VCH), o);
+        store_out_chunk<MF_F32, VCH>(partial_out<MF_F32>(a, pslot, j, 4 * g * VCH), o);
         if (g == 0) {
             partial_ml(a, pslot)[j] = M;
             partial_ml(a, pslot)[16 + j] = L;
@@ -643,14 +640,33 @@ __device__ __forceinline__ void attn4_wide(const Attn4Args& a, const int32_t* it
     auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
     const float lt = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     const float inv = lt > 0.f ? 1.f / lt : 0.f;
-    char* dst = nullptr;
-    if (valid)
-        dst = pslot < 0 ? a.out + ((int64_t)prow * a.o_sr + (int64_t)qhead * a.o_sh) * 2
-                        : partial_out<DT>(a, pslot + ct, j, 0);
+    if (!valid) return;
+    if (pslot >= 0) {
+        char* part = partial_out<MF_F32>(a, pslot + ct, j, 0);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                float4 o;
+                o.x = acc[d][4 * b] * inv;
+                o.y = acc[d][4 * b + 1] * inv;
+                o.z = acc[d][4 * b + 2] * inv;
+                o.w = acc[d][4 * b + 3] * inv;
+                *(float4*)(part + (32 * d + 8 * b + 4 * hf) * 4) = o;
+            }
+        if (hf == 0) {
+            partial_ml(a, pslot + ct)[j] = m;
+            partial_ml(a, pslot + ct)[16 + j] = lt;
+        }
+        return;
+    }
+    char* dst = a.out + ((int64_t)prow * a.o_sr + (int64_t)qhead * a.o_sh) * 2;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int b = 0; b < 4; b += 2) {
+            // the column's two lanes trade blocks, so that each stores 16 bytes (both
+            // are valid or neither)
             uint32_t w[2][2];
 #pragma unroll
             for (int e = 0; e < 2; ++e)
@@ -660,12 +676,8 @@ __device__ __forceinline__ void attn4_wide(const Attn4Args& a, const int32_t* it
                               (f32_to_bits<DT>(acc[d][4 * (b + e) + 2 * k + 1] * inv) << 16);
             auto y = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
             auto z = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
-            if (valid) *(uint4*)(dst + (32 * d + 8 * (b + hf)) * 2) = make_uint4(y[0], z[0], y[1], z[1]);
+            *(uint4*)(dst + (32 * d + 8 * (b + hf)) * 2) = make_uint4(y[0], z[0], y[1], z[1]);
         }
-    if (pslot >= 0 && valid && hf == 0) {
-        partial_ml(a, pslot + ct)[j] = m;
-        partial_ml(a, pslot + ct)[16 + j] = lt;
-    }
 }
 
 template <int DP>
@@ -729,63 +741,6 @@ void attn4_kernel(const int32_t* items, Attn4Args a, int narrow_blocks, const in
     }
 }
 
-// ------------------------------------------------------------------- merge
-// One workgroup per record, its partitions dealt to the four waves, whose results
-// are combined through LDS as the cooperative units' states are. Ranges here are cut
-// into more partitions than the 16-bit plans make (a tile's bytes are a quarter), and a
-// single wave reads them four at a time: 4 sequences of 16384 to 65536 keys, 32
-// records of up to 36 partitions, 19 us that way.
-template <int DT, int DP>
-__global__ __launch_bounds__(256) void merge4_kernel(const int32_t* merges, int num_merges, Attn4Args a) {
-    constexpr int VCH = DP / 16;
-    const int mi = blockIdx.x;
-    int32_t mg[MF_PLAN_MERGE_INTS];
-    load_merge_record(a, merges, mi, num_merges, mg);
-    if (mi >= (a.dev_count ? *a.dev_count : num_merges)) return;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
-    int prow = 0, qhead = 0;
-    const bool valid = merge_column(a, mg, j, prow, qhead);
-    float mx = kMinM, L = 0.f, o[4 * VCH];
-#pragma unroll
-    for (int e = 0; e < 4 * VCH; ++e) o[e] = 0.f;
-    if (valid && wave < mg[3]) {
-        bool fp32 = false;
-        if constexpr (has_fp32_partials<DT, DP>()) fp32 = (mg[7] & MF_PLAN_FP32_PARTIALS) != 0;
-        if (fp32) merge_range<DT, DP, MF_F32, (DP > 128 ? 2 : 4)>(a, mg, wave, kWaves, j, 4 * g * VCH, mx, L, o);
-        else merge_range<DT, DP, DT, (DP > 128 ? 4 : 8)>(a, mg, wave, kWaves, j, 4 * g * VCH, mx, L, o);
-    }
-    auto s_o = reinterpret_cast<float (*)[4 * VCH][64]>(attn_lds);
-    auto s_m = reinterpret_cast<float (*)[64]>(attn_lds + kWaves * 4 * VCH * 64 * 4);
-    auto s_l = s_m + kWaves;
-#pragma unroll
-    for (int e = 0; e < 4 * VCH; ++e) s_o[wave][e][lane] = o[e];
-    s_m[wave][lane] = mx;
-    s_l[wave][lane] = L;
-    __syncthreads();
-    if (!valid) return;
-    float M = kMinM;
-#pragma unroll
-    for (int u = 0; u < kWaves; ++u) M = fmaxf(M, s_m[u][lane]);
-    L = 0.f;
-    float r[VCH];
-#pragma unroll
-    for (int c = 0; c < VCH; ++c) r[c] = 0.f;
-#pragma unroll
-    for (int u = 0; u < kWaves; ++u) {
-        const float w = __builtin_amdgcn_exp2f(s_m[u][lane] - M);
-        L += s_l[u][lane] * w;
-#pragma unroll
-        for (int c = 0; c < VCH; ++c) r[c] += w * s_o[u][wave * VCH + c][lane];
-    }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
-#pragma unroll
-    for (int c = 0; c < VCH; ++c) r[c] *= inv;
-    store_elems<DT, VCH>(a.out + ((int64_t)prow * a.o_sr + (int64_t)qhead * a.o_sh + (4 * g + wave) * VCH) * 2, r);
-}
-template <int DP>
-constexpr int merge4_lds() { return (kWaves * 4 * (DP / 16) * 64 + 2 * kWaves * 64) * 4; }
-
 template <int DT, int DP, bool SC>
 int launch4(Attn4Args a, const int32_t* items, int64_t n_narrow, int64_t n_wide, const int32_t* merges,
             int64_t n_merges, const int32_t* dev_counts, hipStream_t stream) {
@@ -814,9 +769,7 @@ int launch4(Attn4Args a, const int32_t* items, int64_t n_narrow, int64_t n_wide,
     }
     if (n_merges > 0) {
         a.dev_count = dev_counts ? dev_counts + 2 : nullptr;
-        hipLaunchKernelGGL((merge4_kernel<DT, DP>), dim3((unsigned)n_merges), dim3(256), merge4_lds<DP>(), stream, merges,
-                           (int)n_merges, a);
-        return check_launch();
+        return launch_merge32<DT, DP>(a, merges, n_merges, n_wide == 0, stream);
     }
     return MF_OK;
 }
