@@ -34,6 +34,7 @@ import torch
 from memforge_amd import _native as nat
 from memforge_amd.kernels._varlen import as_table_list, padded_tables_host, run_varlen
 from memforge_amd.kernels.block_attention import paged_attention_blockwise
+from memforge_amd.kernels.varlen_attention import paged_attention_varlen_pool
 
 BACKEND_NAME = "memforge_paged"
 
@@ -141,9 +142,11 @@ class _VarlenBinding:
                 )
         identity = row_map == list(range(len(row_map)))
         # a large decode step on 16-token blocks runs as one round of slices
-        sliceable = identity and self.pool_lens is None and self.pool.block_size == 16 and not scored
+        sliceable = identity and self.pool_lens is None and self.pool.block_size == 16 and not scored \
+            and self.pool.kv_bits != 4
         items, merges, counts, sliced = nat.plan_host(cu, kvl, num_q_heads, self.pool.spec.num_kv_heads,
-                                                      head_dim, dtype, device, decode_slices=sliceable)
+                                                      head_dim, dtype, device, decode_slices=sliceable,
+                                                      kv_bits=self.pool.kv_bits)
         # everything the launch reads crosses to the device in one copy
         parts = [padded_tables_host([tables[s] for s in order]), *nat.plan_upload_parts(items, merges),
                  np.asarray(cu + kvl, dtype=np.int32), np.asarray(list(self.positions), dtype=np.int64)]
@@ -226,13 +229,15 @@ def _varlen_forward(module, query, key, value, scaling, binding: _VarlenBinding,
         )
     _, hq, total, d = query.shape
     pool = binding.pool
-    dtype = pool.key_pool.dtype
+    dtype = pool.spec.dtype
     scoring = nat.Scoring(softcap) if softcap else None
     meta = binding.meta(hq, d, dtype, query.device, scored=scoring is not None)
     q_rows = query[0].to(dtype).permute(1, 0, 2)
     out = torch.empty((1, total, hq, d), dtype=dtype, device=query.device)
     layer = module.layer_idx
     nk = nv = None
+    if binding.pool_lens is not None and pool.kv_bits == 4:
+        raise ValueError("a pass that attends to unwritten keys (a speculative verify) needs a 16- or 32-bit pool")
     if binding.pool_lens is not None:
         nk = key[0].to(dtype).permute(1, 0, 2)
         nv = value[0].to(dtype).permute(1, 0, 2)
@@ -279,9 +284,13 @@ def paged_attention_forward(module: Any, query: torch.Tensor, key: torch.Tensor,
     single_query = query.shape[0] == 1 and query.shape[2] == 1
     if binding is not None and single_query and _mask_is_permissive(attention_mask) and binding.context_length > 0:
         binding.used += 1
-        out = paged_attention_blockwise(query, binding.pool.key_pool, binding.pool.value_pool,
-                                        module.layer_idx, binding.block_table, binding.context_length,
-                                        binding.pool.block_size, scale=scaling, softcap=softcap)
+        if binding.pool.kv_bits == 4:
+            out = paged_attention_varlen_pool(query, binding.pool, module.layer_idx, [binding.block_table], [0],
+                                              [binding.context_length - 1], scale=scaling, softcap=softcap)
+        else:
+            out = paged_attention_blockwise(query, binding.pool.key_pool, binding.pool.value_pool,
+                                            module.layer_idx, binding.block_table, binding.context_length,
+                                            binding.pool.block_size, scale=scaling, softcap=softcap)
         return _to_attention_output_layout(out), None
 
     if binding is not None:

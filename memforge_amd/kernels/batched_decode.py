@@ -67,16 +67,17 @@ def assemble_batch(pool, buffers: BatchedDecodeBuffers, block_tables: Sequence[t
         raise ValueError(f"{len(block_tables)} block tables for {batch} sequences")
     max_len = max(context_lengths)
     heads, dim = pool.spec.num_kv_heads, pool.spec.head_dim
-    keys, values, padded = buffers.acquire(batch, max_len, heads, dim, pool.key_pool.dtype, pool.spec.device)
+    keys, values, padded = buffers.acquire(batch, max_len, heads, dim, pool.spec.dtype, pool.spec.device)
     flat = [pool.flat_indices(t, 0, c) for t, c in zip(block_tables, context_lengths)]
+    gather = nat.kv4_gather if pool.kv_bits == 4 else nat.kv_gather
     for layer in range(pool.spec.num_layers):
         view = pool.layer_view(layer)
         for row, (index, ctx) in enumerate(zip(flat, context_lengths)):
             if ctx == 0:
                 continue
             start = padded - ctx
-            nat.kv_gather(view, index, keys[layer, row, :, start:padded, :].permute(1, 0, 2),
-                          values[layer, row, :, start:padded, :].permute(1, 0, 2))
+            gather(view, index, keys[layer, row, :, start:padded, :].permute(1, 0, 2),
+                   values[layer, row, :, start:padded, :].permute(1, 0, 2))
     mask = torch.zeros((batch, padded), dtype=torch.long, device=pool.spec.device)
     for row, ctx in enumerate(context_lengths):
         mask[row, padded - ctx:] = 1
@@ -89,6 +90,7 @@ def scatter_new_tokens(pool, block_tables: Sequence[torch.Tensor], context_lengt
     ``context_lengths[row]`` (batched_decode.py:194-219): one KV-write launch
     per layer for the whole batch."""
     slots = torch.cat([pool.flat_indices(t, c, c + 1) for t, c in zip(block_tables, context_lengths)])
+    write = nat.kv4_write if pool.kv_bits == 4 else nat.kv_write
     for layer in range(pool.spec.num_layers):
         k, v = new_keys[layer], new_values[layer]  # (batch, heads, 1, dim)
-        nat.kv_write(k[:, :, 0, :], v[:, :, 0, :], slots, pool.layer_view(layer))
+        write(k[:, :, 0, :], v[:, :, 0, :], slots, pool.layer_view(layer))

@@ -64,7 +64,7 @@ from memforge_amd.runtime.batched_speculative import (
 )
 from memforge_amd.runtime.engine_telemetry import DataPathMeter, device_figures
 from memforge_amd.runtime.graphed_paged_decode import GraphedPagedDecoder
-from memforge_amd.runtime.kv_pool import ModelKVSpec, PagedKVPool
+from memforge_amd.runtime.kv_pool import ModelKVSpec, PagedKVPool, PagedKVPool4
 from memforge_amd.runtime.packed_pass import packed_forward
 from memforge_amd.runtime.prefix_sharing import block_owners, copy_block, sharing_telemetry
 from memforge_amd.runtime.sampling import SamplingParams, sample_logits
@@ -238,7 +238,7 @@ class ContinuousBatchingEngine:
                  block_attention: bool = False, max_prefill_tokens_per_step: int = 0,
                  draft_model=None, lookahead_k: int = 0, fused_prefill: bool = False,
                  paged_attn_kernel: str = "gather", draft_cuda_graph=False, paged_cuda_graph=False,
-                 telemetry_sample_every: int = 16, fused_kv_write: bool = True):
+                 telemetry_sample_every: int = 16, fused_kv_write: bool = True, kv_cache_bits: int = 16):
         if not HAS_CPP_ENGINE:
             raise RuntimeError("The native memforge_c extension is required; build it with "
                                "`python -m memforge_amd._build`")
@@ -265,9 +265,20 @@ class ContinuousBatchingEngine:
         self.decode_view_cache = False
 
         self.spec = ModelKVSpec.from_config(model.config, self.dtype, self.device)
+        # 4: the pool holds keys and values in 4 bits (PagedKVPool4), 3.8 times the
+        # tokens of a 16-bit pool in the same memory
+        if kv_cache_bits not in (4, 16):
+            raise ValueError(f"kv_cache_bits must be 16 (the model's type) or 4, got {kv_cache_bits}")
+        if kv_cache_bits == 4:
+            if self.dtype not in (torch.float16, torch.bfloat16):
+                raise ValueError(f"attention over a 4-bit pool runs in float16 or bfloat16, not {self.dtype}")
+            if draft_model is not None and lookahead_k > 0:
+                raise ValueError("speculative decoding attends to unwritten candidates, which a 4-bit pool does not serve")
+            self._fused_kv_write = fused_kv_write = False
+        pool_class = PagedKVPool4 if kv_cache_bits == 4 else PagedKVPool
         if num_blocks is None:
-            num_blocks = PagedKVPool.blocks_for_budget(self.spec, block_size, kv_budget_mb)
-        self.pool = PagedKVPool(self.spec, num_blocks=num_blocks, block_size=block_size)
+            num_blocks = pool_class.blocks_for_budget(self.spec, block_size, kv_budget_mb)
+        self.pool = pool_class(self.spec, num_blocks=num_blocks, block_size=block_size)
 
         self.allocator = memforge_c.BlockAllocator(num_blocks, block_size)
         self.prefix_cache = memforge_c.PrefixCache(self.allocator, block_size) if enable_prefix_sharing else None
@@ -333,7 +344,7 @@ class ContinuousBatchingEngine:
         self._throughput = _ThroughputWindow(5.0)
         weight_bytes = sum(p.numel() * p.element_size() for p in model.parameters())
         self._meter = DataPathMeter(self.spec, model.config.num_attention_heads, block_size, weight_bytes,
-                                    every=telemetry_sample_every)
+                                    every=telemetry_sample_every, kv_bits=self.pool.kv_bits)
 
     @property
     def throughput_window_s(self) -> float:

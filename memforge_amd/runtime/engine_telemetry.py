@@ -104,11 +104,14 @@ class _PassRecord:
 class DataPathMeter:
     """Sampled HIP-event timing of the attention and KV-write kernels."""
 
-    def __init__(self, spec, num_q_heads: int, block_size: int, weight_bytes: int, every: int = 16):
+    def __init__(self, spec, num_q_heads: int, block_size: int, weight_bytes: int, every: int = 16,
+                 kv_bits: int = 16):
         self.every = max(0, int(every))
         self.weight_bytes = int(weight_bytes)
         self.elt = torch.tensor([], dtype=spec.dtype).element_size()
         self.kv_row = spec.num_kv_heads * spec.head_dim * self.elt  # one token's K (or V) in one layer
+        # the same in the pool: codes and scale bytes where it is held in 4 bits
+        self.pool_row = spec.num_kv_heads * (spec.head_dim // 2 + spec.head_dim // 32) if kv_bits == 4 else self.kv_row
         self.q_row = num_q_heads * spec.head_dim * self.elt
         self.block_size = block_size
         self.num_layers = spec.num_layers
@@ -128,8 +131,8 @@ class DataPathMeter:
         """Algorithmic bytes of one layer's attention and KV write."""
         kv = sum(int(n) for n in kv_lens)
         tables = sum((int(n) + self.block_size - 1) // self.block_size for n in kv_lens) * 4
-        attention = 2 * kv * self.kv_row + tables + 2 * rows * self.q_row
-        kv_write = 2 * 2 * rows * self.kv_row + 8 * rows
+        attention = 2 * kv * self.pool_row + tables + 2 * rows * self.q_row
+        kv_write = 2 * rows * (self.kv_row + self.pool_row) + 8 * rows
         return {"attention": attention, "kv_write": kv_write, "attention_kv_write": attention + kv_write}
 
     def step_bytes(self, kv_lens: List[int], rows: int) -> int:

@@ -55,6 +55,8 @@ class ModelKVSpec:
 class PagedKVPool:
     """Fixed-size physical block pool backing the paged KV cache."""
 
+    kv_bits = 16  # of an element, or 32: what spec.dtype takes
+
     def __init__(self, spec: ModelKVSpec, num_blocks: int, block_size: int = 16):
         _require_gpu_device(spec.device)
         self.spec = spec

@@ -46,7 +46,8 @@ def packed_forward(model, pool, tokens: Sequence[Sequence[int]], starts: Sequenc
     ``timer`` (a sampled pass's event record) every layer's KV write and
     attention launch is bracketed by HIP events. With ``fuse_kv_write`` each
     layer's KV write rides in its attention launch (mf_paged_attention_kv_write)
-    instead of running as a launch of its own."""
+    instead of running as a launch of its own (never over a 4-bit pool, whose
+    keys are all read from it)."""
     bs = pool.block_size
     spec = pool.spec
     B = len(tokens)
@@ -73,8 +74,8 @@ def packed_forward(model, pool, tokens: Sequence[Sequence[int]], starts: Sequenc
     flat_tokens = np.fromiter((tok for run in tokens for tok in run), dtype=np.int32)
     nat.check_pack_entries(ent, flat_tables, len(flat_tokens), T, pool.num_blocks)
     items, merges, counts = nat.plan_attention_host(cu.tolist(), kv_lens, model.config.num_attention_heads,
-                                                    spec.num_kv_heads, spec.head_dim, pool.key_pool.dtype,
-                                                    num_cus=nat.device_cus(spec.device))
+                                                    spec.num_kv_heads, spec.head_dim, spec.dtype,
+                                                    num_cus=nat.device_cus(spec.device), kv_bits=pool.kv_bits)
     keep_np = np.asarray(list(keep_rows), dtype=np.int64)
     # descriptors, tables, tokens, the attention plan and the kept rows cross
     # to the device in one copy
@@ -85,7 +86,8 @@ def packed_forward(model, pool, tokens: Sequence[Sequence[int]], starts: Sequenc
     meta = {"block_tables": packed.block_tables, "cu_seqlens": packed.cu_seqlens,
             "kv_lens": packed.kv_lens, "positions": packed.positions, "row_map": None,
             "plan": attn_plan}
-    fuse = fuse_kv_write and pool.key_pool.dtype == model.dtype
+    # rows are rounded into a 4-bit pool before anything attends to them
+    fuse = fuse_kv_write and spec.dtype == model.dtype and pool.kv_bits != 4
     binding = attention_backend._VarlenBinding.from_packed(pool, meta, T,
                                                            write_slots=packed.slot_mapping if fuse else None)
     cache = VarlenPackedCache.from_slot_mapping(pool, spec.num_layers, packed.slot_mapping, write_in_attention=fuse)

@@ -11,6 +11,7 @@ import torch
 from memforge_amd import _native as nat
 from memforge_amd.kernels.varlen_attention import paged_attention_varlen_pool
 from memforge_amd.runtime import ModelKVSpec, PagedKVPool4
+from memforge_amd.runtime.graphed_paged_decode import split_plan_capacity
 from memforge_amd.runtime.prefix_sharing import copy_blocks
 from tests.gpu_helpers import pad_tables, random_tables
 from tests.scored_reference import attend, check, round4
@@ -232,6 +233,19 @@ def test_nan_where_no_row_looks(device, dtype, d, bs, planned):
     out = st.run(st.scoring(25.0), plan)
     st.k, st.v = keep
     st.verify(out, 25.0, what="nan")
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(64, 15, 5), (128, 8, 8)])
+def test_plans_of_a_captured_decode(device, d, hq, hkv):
+    """The plans that a captured decode step takes: without merges, with fixed capacities, with split ranges."""
+    lens = [4000, 1, 333, 2017]
+    st = Step4(device, torch.float16, hq, hkv, d, 16, [(0, n - 1, 1, 0) for n in lens], seed=d)
+    args = (st.cu, st.kv, hq, hkv, d, torch.float16)
+    for made in (nat.plan_attention_host(*args, num_cus=256, merge_free=True, kv_bits=4),
+                 nat.plan_attention_host(*args, partition_tiles=64), nat.plan_attention_host(*args, num_cus=256, kv_bits=4)):
+        plan = nat.CountedPlan(*split_plan_capacity(len(lens), hkv, 252, 16, d), device)
+        plan.update(*made)
+        st.verify(st.run(None, plan), what=f"{made[2].tolist()}")
 
 
 def test_replays_of_a_captured_step(device):
