@@ -290,7 +290,8 @@ int mf_paged_attention_kv_write(const void* q, int64_t q_stride_row, int64_t q_s
  * and with key k visible to row r when k < kv_lens[s], k >= first_keys[s]
  * (NULL: 0), and k <= positions[r] or k < prefix_lens[s] (NULL: 0). A row that
  * sees no key gets zeros. Keys below first_keys[s] and from kv_lens[s] on may
- * hold anything, NaN included. A document mask runs each document's rows as a
+ * hold anything, NaN included; between them a value that is not finite reaches
+ * rows of s that do not see it too (zero times it), as in a plain call. A document mask runs each document's rows as a
  * sequence of their own over the same block table, first_keys the document's
  * first position; rows before the prefix's end see the whole prefix.
  * softcap: finite, 0 for none; so small or large against the scale that their

@@ -535,7 +535,10 @@ class Scoring:
       row, those after the row's position too (from ``first_keys`` on).
 
     A row that sees no key gets zeros. Plans for masked calls are made with the
-    same ``first_keys`` and ``prefix_lens`` as host lists (``plan_attention``)."""
+    same ``first_keys`` and ``prefix_lens`` as host lists (``plan_attention``).
+    Keys that no row of a sequence sees may hold anything; a value that is not
+    finite reaches the rows of its sequence that do not see it too, as zero times
+    it does in a product (a plain call's rows the same)."""
 
     softcap: float = 0.0
     slopes: Optional[torch.Tensor] = None
@@ -735,6 +738,9 @@ def plan_host(cu_seqlens: Sequence[int], kv_lens: Sequence[int], num_q_heads: in
     for name, x in (("first_keys", first_keys), ("prefix_lens", prefix_lens)):
         if x is not None and len(x) != len(kv_lens):
             raise ValueError(f"{len(x)} {name} for {len(kv_lens)} sequences")
+    if prefix_lens is not None and not on_gpu and partition_tiles <= 0:
+        raise ValueError("a plan for prefix_lens is made for a GPU device (or with partition_tiles): other plans leave "
+                         "out tiles that only a prefix makes visible")
     slices = decode_slices and on_gpu and not masked and kv_bits == 16
     cus = device_cus(device) if on_gpu else 0
     firsts = None if first_keys is None else tuple(int(x) for x in first_keys)
@@ -836,6 +842,10 @@ class Workspace:
     def partials(self, floats: int, device) -> Optional[torch.Tensor]:
         if floats <= 0:
             return None
+        if torch.cuda.is_current_stream_capturing():
+            # the graph's own: a shared buffer would be freed under it when a later call
+            # grows it, and shared with every other graph captured on this stream
+            return torch.empty(floats, dtype=torch.float32, device=device)
         dev = torch.device(device)
         key = (dev.index, _stream(dev))
         buf = self._partials.get(key)
@@ -974,8 +984,10 @@ class _Plan:
         self.narrow, self.wide, self.merges = plan.n_narrow, plan.n_wide, plan.n_merges
         self.counts = None
         self.partials = partials if partials is not None else _WORKSPACE.partials(plan.partials_floats, device)
-        if self.partials is not None and self.partials.numel() < plan.partials_floats:
-            raise ValueError(f"the plan needs {plan.partials_floats} partial floats, got {self.partials.numel()}")
+        if partials is not None and (partials.dtype != torch.float32 or not partials.is_contiguous()
+                                     or partials.device != device or partials.numel() < plan.partials_floats):
+            raise ValueError(f"the plan needs {plan.partials_floats} contiguous fp32 partials on {device}, got "
+                             f"{partials.numel()} of {partials.dtype} on {partials.device}")
 
 
 def _launch(device: torch.device, what: str, fn, *args) -> None:
@@ -1009,6 +1021,12 @@ def _paged_attention_scored(scoring: Scoring, q_rows, out_rows, pool, block_tabl
         if not same_layout(nk, nv):
             raise ValueError("in-flight K and V rows must share strides")
     dev = q_rows.device
+    if out_rows.shape != q_rows.shape or q_rows.shape[1:] != (q_rows.shape[1], pool.head_dim) \
+            or num_kv_heads != pool.num_heads:
+        raise ValueError(f"query {tuple(q_rows.shape)}, output {tuple(out_rows.shape)} and {num_kv_heads} kv heads do "
+                         f"not match a pool of {pool.num_heads} heads x {pool.head_dim}")
+    if not dev == out_rows.device == pool.k.device == block_tables.device == positions.device:
+        raise ValueError(f"query, output, pool and index tensors must be on one device, the query is on {dev}")
     p = _Plan(plan, dev, partials)
     mods = scoring.struct(q_rows.shape[1], kv_lens.numel(), dev)
     bt_stride = block_tables.shape[1] if block_tables.dim() == 2 else 0

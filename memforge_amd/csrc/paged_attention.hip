@@ -1,6 +1,7 @@
 // Planners and C entry points of the varlen paged attention (the kernels are in
 // attn_kernels.h).
 #include <atomic>
+#include <exception>
 #include <mutex>
 #include <vector>
 
@@ -819,6 +820,18 @@ extern "C" int mf_attention_plan_merge_free(int num_seqs, const int32_t* cu_seql
                           items, items_capacity, merges, merges_capacity, counts);
 }
 
+extern "C" int mf_attention_plan4(int num_seqs, const int32_t* cu_seqlens, const int32_t* kv_lens, int num_q_heads,
+                                  int num_kv_heads, int head_dim, int dtype, int num_cus, int32_t* items,
+                                  int64_t items_capacity, int32_t* merges, int64_t merges_capacity, int64_t* counts) {
+    if (num_cus <= 0) return MF_ERR_ARG;
+    try {
+        return attention_plan(num_seqs, cu_seqlens, kv_lens, num_q_heads, num_kv_heads, head_dim, dtype, 0, num_cus,
+                              true, items, items_capacity, merges, merges_capacity, counts, /*four=*/true);
+    } catch (const std::exception&) {  // no memory for a plan of this size
+        return MF_ERR_ARG;
+    }
+}
+
 // Slice plan for a large decode launch (attn_slice_kernel). The sequences'
 // 16-key tiles, in sequence order, are cut into slices of about
 // total / (num_cus * MF_SLICE_WAVES_PER_CU / Hkv) tiles, so one wave per
@@ -827,14 +840,6 @@ extern "C" int mf_attention_plan_merge_free(int num_seqs, const int32_t* cu_seql
 // multiple of the kernel's ring depth; a workload whose even share would
 // exceed that gets more slices (a second round). A sequence cut across
 // slices leaves one partial per piece and kv head, merged afterwards.
-extern "C" int mf_attention_plan4(int num_seqs, const int32_t* cu_seqlens, const int32_t* kv_lens, int num_q_heads,
-                                  int num_kv_heads, int head_dim, int dtype, int num_cus, int32_t* items,
-                                  int64_t items_capacity, int32_t* merges, int64_t merges_capacity, int64_t* counts) {
-    if (num_cus <= 0) return MF_ERR_ARG;
-    return attention_plan(num_seqs, cu_seqlens, kv_lens, num_q_heads, num_kv_heads, head_dim, dtype, 0, num_cus, true,
-                          items, items_capacity, merges, merges_capacity, counts, /*four=*/true);
-}
-
 extern "C" int mf_attention_plan_slices(int num_seqs, const int32_t* cu_seqlens, const int32_t* kv_lens,
                                         int num_q_heads, int num_kv_heads, int head_dim, int dtype,
                                         int num_cus, int min_tiles_per_wave, int32_t* slices,

@@ -272,3 +272,47 @@ def test_eager_and_block_routes_of_the_backend_cap_scores(device):
     check(out[:, :, 0], *ref, torch.float32, 64, 41, 6.0)
     eager = _eager_attention(None, q, k.transpose(0, 1)[None], v.transpose(0, 1)[None], None, None, 6.0)
     assert float((eager[:, 0].cpu().double() - ref[0]).abs().max()) < 1e-4
+
+
+def test_captured_calls_have_partials_of_their_own(device, monkeypatch):
+    """Calls that split ranges, captured into two graphs with ordinary plans: no graph's partials are another's or an
+    eager call's, and replays stay right after a larger call has grown the eager workspace."""
+    steps = [Step(device, torch.bfloat16, 8, 2, 64, 16, [(0, n - 1, 1, 0)] * 2, seed=n) for n in (3000, 5000, 9000)]
+    plans = [st.plan() for st in steps]
+    assert all(p.partials_floats > 0 for p in plans)
+    at, real = [], nat.Workspace.partials
+
+    def spy(self, floats, dev):
+        at.append(real(self, floats, dev))
+        return at[-1]
+
+    monkeypatch.setattr(nat.Workspace, "partials", spy)
+    graphs, outs = [], []
+    for st, plan in zip(steps[:2], plans):
+        st.run(st.scoring(20.0), plan)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(st.run(st.scoring(20.0), plan))
+        graphs.append(graph)
+    spans = [(x.data_ptr(), x.data_ptr() + 4 * x.numel()) for x in (at[2], at[1], at[3])]
+    assert all(a[1] <= b[0] or b[1] <= a[0] for i, a in enumerate(spans) for b in spans[:i])
+    for _ in range(3):
+        for graph in graphs:
+            graph.replay()
+        steps[2].verify(steps[2].run(steps[2].scoring(20.0), plans[2]), 20.0)
+        for st, out in zip(steps, outs):
+            st.verify(out, 20.0, what="replay")
+            out.zero_()
+
+
+def test_shapes_are_checked(device):
+    st = Step(device, torch.bfloat16, 8, 2, 64, 16, [(0, 40, 1, 0)])
+    args = (st.bt, st.cu_t, st.kv_t, st.pos_t, st.plan(), st.scale)
+    pool, mods = nat.PoolView.from_bshd(st.kp, st.vp), st.scoring(20.0)
+    with pytest.raises(ValueError):
+        nat.paged_attention(st.q, torch.empty_like(st.q[:, :4]), pool, *args, 2, scoring=mods)
+    with pytest.raises(ValueError):
+        nat.paged_attention(st.q, torch.empty_like(st.q), pool, *args, 1, scoring=mods)
+    with pytest.raises(ValueError):
+        nat.paged_attention(st.q, torch.empty_like(st.q), pool, *args, 2, scoring=mods,
+                            partials=torch.empty(1 << 20, dtype=torch.bfloat16, device=device))

@@ -123,3 +123,13 @@ def _varlen(**kw):
 def test_list_operator_refuses(kw, err):
     with pytest.raises(err):
         _varlen(**kw)
+
+
+def test_prefix_plans_need_a_device():
+    """A plan made for no device may leave out tiles that only a prefix makes visible."""
+    with pytest.raises(ValueError):
+        nat.plan_host([0, 300, 301], [600, 900], 8, 2, 64, torch.bfloat16, prefix_lens=[600, 0])
+    items = nat.plan_host([0, 300, 301], [600, 900], 8, 2, 64, torch.bfloat16, prefix_lens=[600, 0], partition_tiles=8)[0]
+    for head in range(2):
+        for group in {int(i[2]) for i in items if i[0] == 0 and i[9] > 0}:
+            assert max(i[5] for i in items if i[0] == 0 and i[1] == head and i[2] == group) == 38
