@@ -6,6 +6,7 @@ uses its own pre-packed path instead of this one."""
 from __future__ import annotations
 
 import math
+from itertools import accumulate
 from typing import List, Optional, Sequence
 
 import numpy as np
@@ -72,34 +73,32 @@ def run_varlen(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: nat.PoolView,
         raise ValueError(f"doc_starts must be {T} positions, none negative")
     if prefix_lens is not None and (len(prefix_lens) != len(tables) or any(x < 0 for x in prefix_lens)):
         raise ValueError(f"prefix_lens must be {len(tables)} lengths, none negative")
-    groups = {}
-    order: List[int] = []
-    firsts: List[int] = []
-    for r, s in enumerate(seq_ids):
-        key = s if doc_starts is None else (s, int(doc_starts[r]))
-        if key not in groups:
-            groups[key] = []
-            order.append(s)
-            firsts.append(0 if doc_starts is None else key[1])
-        groups[key].append(r)
-    row_map: List[int] = []
-    cu = [0]
-    kvl: List[int] = []
-    prefixes: List[int] = []
-    for s, members in zip(order, groups.values()):
-        rows = sorted(members, key=lambda r: positions[r])
-        row_map.extend(rows)
-        cu.append(len(row_map))
-        prefixes.append(int(prefix_lens[s]) if prefix_lens is not None else 0)
-        kvl.append(kv_lens[s] if kv_lens is not None else max(max(positions[r] for r in rows) + 1, prefixes[-1]))
+    keys = seq_ids if doc_starts is None else list(zip(seq_ids, map(int, doc_starts)))
+    prefix_of = [0] * len(tables) if prefix_lens is None else [int(x) for x in prefix_lens]
+    if len(set(keys)) == T:  # a decode step: every row is a sequence's only one
+        order, members = list(seq_ids), [[r] for r in range(T)]
+        row_map, cu = list(range(T)), list(range(T + 1))
+        last = list(positions)
+    else:
+        groups = {}
+        for r, key in enumerate(keys):
+            groups.setdefault(key, []).append(r)
+        members = [sorted(rows, key=lambda r: positions[r]) for rows in groups.values()]
+        order = [seq_ids[rows[0]] for rows in members]
+        row_map = [r for rows in members for r in rows]
+        cu = [0, *accumulate(map(len, members))]
+        last = [positions[rows[-1]] for rows in members]
+    firsts = [0] * len(order) if doc_starts is None else [int(doc_starts[rows[0]]) for rows in members]
+    prefixes = [prefix_of[s] for s in order]
+    kvl = [max(n + 1, p) for n, p in zip(last, prefixes)] if kv_lens is None else [kv_lens[s] for s in order]
     masked_first, masked_prefix = any(firsts), any(prefixes)
     identity = row_map == list(range(T))
     # every block id the kernel will read must address the pool
     bs, nblocks = pool.block_size, pool.num_blocks
     need: List[int] = []
     for i, s in enumerate(order):
-        keys = kvl[i] if pool_lens is None else min(kvl[i], pool_lens[s])
-        need.append((keys + bs - 1) // bs)
+        held = kvl[i] if pool_lens is None else min(kvl[i], pool_lens[s])
+        need.append((held + bs - 1) // bs)
         if need[i] > len(tables[s]):
             _check_ids(tables, order[:i], need, nblocks)  # an earlier sequence's bad id is reported first
             raise IndexError(f"sequence {s} needs {need[i]} blocks but its block table has {len(tables[s])}")
