@@ -91,7 +91,8 @@ struct ScoredArgs : AttnArgs {
     float cap_in;    // 2 * log2(e) * |scale| / softcap, 0: scores are not capped
     float cap_log2;  // softcap * log2(e)
     float cap_x;     // |scale| / softcap
-    float cap_c[4];  // cap_log2 times the coefficients of tanh(x) / x in x^2 (score_all)
+    float cap_top, cap_top4;     // largest raw scores of score_all's polynomials of three and four terms
+    float cap_p3[3], cap_p4[4];  // their coefficients, raw scores to capped log2 units
 };
 
 // The launches of scored_attention.hip, as launch_attention's: padded head_dim
@@ -171,28 +172,36 @@ using ArgsOf = std::conditional_t<SC, ScoredArgs, AttnArgs>;
 // infinities, NaN for NaN, its error about 1e-7 of the cap. Both instructions run at a
 // quarter of the rate, and prefill is bound by the VALU, so where every score of the
 // wave's block lies below half the cap (most do) 16-bit types take an odd polynomial
-// instead: x (c0 + c1 z + c2 z^2 + c3 z^3), z = x^2, fitted to tanh(x) / x over
-// |x| <= 0.5 for the least relative error, 5.4e-7. One test of the block's largest
-// magnitude decides. fp32 takes the series to x^11 below 0.35 (the next term is 2e-8 of
-// x there) score by score: its launches are not bound by this.
+// instead, in the raw score: s (p0 + p1 z + p2 z^2 [+ p3 z^3]), z = s^2, fitted to
+// tanh(x) / x for the least relative error: three terms over |x| <= 0.25 (4.0e-7), four
+// over |x| <= 0.5 (5.4e-7). One test of the block's largest magnitude picks. With four
+// terms alone and x formed first, two chunks of 2048 rows after up to 6144 keys took 707
+// us at a cap that no score comes near (40/8 heads x 128, 475 GFLOP), 665 with both; at
+// one whose quarter many pass 746 and 752. fp32 takes the series to x^11 below 0.35 (the
+// next term is 2e-8 of x there) score by score: its launches are not bound by this.
 template <int DT, int N, class Dist>
 __device__ __forceinline__ void score_all(float (&s)[N], const ScoredArgs& a, float slope_log2, Dist dist) {
     if (a.cap_in != 0.f) {
-        bool small = false;
+        float top = __builtin_huge_valf();
         if constexpr (DT != MF_F32) {
-            float top = __builtin_fabsf(s[0]);
+            top = __builtin_fabsf(s[0]);
 #pragma unroll
             for (int i = 1; i < N; ++i) top = fmax_prop(top, __builtin_fabsf(s[i]));
-            small = __builtin_amdgcn_ballot_w64(!(top * a.cap_x <= 0.5f)) == 0;
         }
-        if (small) {
+        if (DT != MF_F32 && __builtin_amdgcn_ballot_w64(!(top <= a.cap_top)) == 0) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float x = s[i] * a.cap_x, z = x * x;
-                float c = __builtin_fmaf(z, a.cap_c[3], a.cap_c[2]);
-                c = __builtin_fmaf(z, c, a.cap_c[1]);
-                c = __builtin_fmaf(z, c, a.cap_c[0]);
-                s[i] = x * c;
+                const float z = s[i] * s[i];
+                const float c = __builtin_fmaf(z, a.cap_p3[2], a.cap_p3[1]);
+                s[i] *= __builtin_fmaf(z, c, a.cap_p3[0]);
+            }
+        } else if (DT != MF_F32 && __builtin_amdgcn_ballot_w64(!(top <= a.cap_top4)) == 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float z = s[i] * s[i];
+                float c = __builtin_fmaf(z, a.cap_p4[3], a.cap_p4[2]);
+                c = __builtin_fmaf(z, c, a.cap_p4[1]);
+                s[i] *= __builtin_fmaf(z, c, a.cap_p4[0]);
             }
         } else {
 #pragma unroll
@@ -542,7 +551,7 @@ __device__ __forceinline__ void arrive_and_merge(const AttnArgs& a, int m0, int 
 // (two score chains at once, one test of the maximum for both): the transforms' registers
 // spill at three. Two chunks of 2048 rows after up to 6144 keys, 40/8 heads x 128, capped
 // scores (475 GFLOP): 836 us at three waves and 32 keys, 778 at two, 698 with stages of
-// 64, 689 with steps of 64. At 128-byte rows four waves and 32-key steps stay the faster
+// 64, 689 with steps of 64 (659 since, by the cap's polynomials and the stages' addresses). At 128-byte rows four waves and 32-key steps stay the faster
 // (8 packed prompts of documents 49 us, 57 at three waves with steps of 64).
 constexpr int scored_waves(int dp) { return dp == 128 ? 2 : 4; }
 constexpr int scored_step(int dp) { return dp == 128 ? 2 : 1; }  // 32-key blocks
@@ -1497,6 +1506,28 @@ __device__ __forceinline__ void attn_wide_body(const ArgsOf<SC>& a, const int bl
     const char* nk_h = new_k + ((int64_t)(row0 - pool_len) * a.n_sr + (int64_t)h * a.n_sh) * 2;
     const int64_t v_delta = v_pool - k_pool, nv_delta = new_v - new_k;
     const int64_t tile_bytes = 16 * a.n_sr * 2;
+    // Where this kv head's K rows of tile t begin. Scored launches, whose loop has few
+    // scalar registers left, keep the 64 tiles' addresses in lanes rather than form each
+    // from its entry: a stage's fetch is 60 scalar instructions shorter (the two chunks
+    // above 667 -> 659 us).
+    uint32_t base_lo = 0, base_hi = 0;
+    auto set_bases = [&]() {
+        if constexpr (SC && BLK16) {
+            const uint64_t b = (uint64_t)kp_h + (uint64_t)((int64_t)tbl * blk_bytes);
+            base_lo = (uint32_t)b;
+            base_hi = (uint32_t)(b >> 32);
+        }
+    };
+    set_bases();
+    auto rows_at = [&](int t) -> const char* {
+        if constexpr (SC && BLK16) {
+            const uint32_t lo = __builtin_amdgcn_readlane(base_lo, t - tbl_base);
+            const uint32_t hi = __builtin_amdgcn_readlane(base_hi, t - tbl_base);
+            return (const char*)((uint64_t)hi << 32 | lo);
+        } else {
+            return kp_h + (int64_t)tbl_at(t) * blk_bytes;
+        }
+    };
     // tiles the fetches clamp to: the item's range for the first stage, the
     // workgroup's last read tile once the positions are in
     int fetch_end = kt1;
@@ -1529,6 +1560,7 @@ __device__ __forceinline__ void attn_wide_body(const ArgsOf<SC>& a, const int bl
             tbl_base += 64;
             tbl = tbl_next;
             tbl_next = trow[min(tbl_base + 64 + lane, tbl_last)];
+            set_bases();
         }
         const uint32_t dst0 = lds_base + (uint32_t)(buf * STG);
         const int key1 = (t0 + TS) * 16;
@@ -1547,7 +1579,7 @@ __device__ __forceinline__ void attn_wide_body(const ArgsOf<SC>& a, const int bl
         if (in_pool) {
 #pragma unroll
             for (int i = 0; i < NLD; ++i)
-                piece(i, kp_h + (int64_t)tbl_at(t0 + (wave + 4 * i) / (2 * PK)) * blk_bytes, v_delta, off[i % NOFF]);
+                piece(i, rows_at(t0 + (wave + 4 * i) / (2 * PK)), v_delta, off[i % NOFF]);
         } else if (in_new) {
 #pragma unroll
             for (int i = 0; i < NLD; ++i)
@@ -1569,8 +1601,12 @@ __device__ __forceinline__ void attn_wide_body(const ArgsOf<SC>& a, const int bl
                 const int key = inflight ? min(t * 16 + k16, kv_len - 1) : t * 16 + k16;
                 const char* src;
                 if (!inflight || key < pool_len) {
-                    const int64_t blk = tbl_at(t);
-                    src = k_pool + (isv ? v_delta : 0) + (blk * a.p_sb + (int64_t)k16 * a.p_ss + (int64_t)h * a.p_sh) * 2;
+                    if constexpr (SC) {
+                        src = rows_at(t) + (isv ? v_delta : 0) + (int64_t)k16 * a.p_ss * 2;
+                    } else {
+                        const int64_t blk = tbl_at(t);
+                        src = k_pool + (isv ? v_delta : 0) + (blk * a.p_sb + (int64_t)k16 * a.p_ss + (int64_t)h * a.p_sh) * 2;
+                    }
                 } else {
                     int nr = row0 + key - pool_len;
                     if (a.row_map) nr = a.row_map[nr];
@@ -2444,8 +2480,26 @@ inline int set_scoring(ScoredArgs& a, const mf_scoring& s) {
     a.cap_in = s.softcap > 0.f ? 2.f * a.scale_log2 / s.softcap : 0.f;
     a.cap_log2 = s.softcap * 1.4426950408889634f;
     a.cap_x = s.softcap > 0.f ? a.scale_log2 / a.cap_log2 : 0.f;
-    const float tanh_c[4] = {0.99999946f, -0.33326317f, 0.13190283f, -0.04440178f};
-    for (int i = 0; i < 4; ++i) a.cap_c[i] = a.cap_log2 * tanh_c[i];
+    // The polynomials' coefficients by powers of cap_x, so that they take raw scores. Where
+    // one leaves fp32's normal numbers: four terms are not used; three lose those that have
+    // no weight (relative to the score) below 3e-4 of the cap, and are used below that; a cap
+    // so small that they overflow is left to the exponential (1e-7 of it is nothing).
+    const double p3[3] = {0.9999996, -0.33321908, 0.12841609};
+    const double p4[4] = {0.99999946, -0.33326318, 0.13190299, -0.04440228};
+    double power = (double)a.cap_log2 * a.cap_x;
+    bool low = false, high = false;
+    for (int i = 0; i < 4; ++i, power *= (double)a.cap_x * a.cap_x) {
+        const double c = power * (i < 3 ? p3[i] : p4[i]);
+        high |= std::abs(c) > 1e37;
+        if (i < 3) {
+            low |= std::abs(c) < FLT_MIN;
+            a.cap_p3[i] = std::abs(c) < FLT_MIN ? 0.f : (float)c;
+        }
+        a.cap_p4[i] = (float)(power * p4[i]);
+    }
+    // z = s^2 stays finite
+    a.cap_top = high ? -1.f : std::fmin((low ? 3e-4f : 0.25f) / a.cap_x, 1e18f);
+    a.cap_top4 = high || std::abs(a.cap_p4[3]) < FLT_MIN ? -1.f : 0.5f / a.cap_x;
     if (s.softcap > 0.f && !(a.cap_in >= FLT_MIN && a.cap_in < INFINITY && a.cap_log2 < INFINITY)) return MF_ERR_ARG;
     return MF_OK;
 }

@@ -316,3 +316,17 @@ def test_shapes_are_checked(device):
     with pytest.raises(ValueError):
         nat.paged_attention(st.q, torch.empty_like(st.q), pool, *args, 2, scoring=mods,
                             partials=torch.empty(1 << 20, dtype=torch.bfloat16, device=device))
+
+
+@pytest.mark.parametrize("cap", [1e-9, 1e-6, 1e-2, 300.0, 1e5, 1e8, 1e12, 1e20])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_caps_of_any_size(device, dtype, cap):
+    """A cap no score comes near leaves the scores to a relative 5.5e-7 (the bound takes 2e-7 of a cap of 4 |t|); one
+    far below them keeps 2e-7 of itself."""
+    st = Step(device, dtype, 6, 2, 64, 16, DECODES + PREFILLS, seed=11)
+    out = st.run(st.scoring(cap))
+    flat_k, flat_v = (x.view(-1, 2, 64).cpu() for x in (st.kp, st.vp))
+    for i, (_, start, n, _) in enumerate(st.runs):
+        at, rows = st.slots(i, 0, st.kv[i]), slice(st.cu[i], st.cu[i + 1])
+        ref = attend(st.q[rows], flat_k[at], flat_v[at], range(start, start + n), st.scale, cap)
+        check(out[rows], *ref, dtype, 64, st.kv[i], min(cap, 4 * float(ref[2][..., 1].max())), f"cap {cap} run {i}")
