@@ -177,7 +177,7 @@ using ArgsOf = std::conditional_t<SC, ScoredArgs, AttnArgs>;
 // over |x| <= 0.5 (5.4e-7). One test of the block's largest magnitude picks. With four
 // terms alone and x formed first, two chunks of 2048 rows after up to 6144 keys took 707
 // us at a cap that no score comes near (40/8 heads x 128, 475 GFLOP), 665 with both; at
-// one whose quarter many pass 746 and 752. fp32 takes the series to x^11 below 0.35 (the
+// one whose quarter many pass 746 and 752 us. fp32 takes the series to x^11 below 0.35 (the
 // next term is 2e-8 of x there) score by score: its launches are not bound by this.
 template <int DT, int N, class Dist>
 __device__ __forceinline__ void score_all(float (&s)[N], const ScoredArgs& a, float slope_log2, Dist dist) {
@@ -551,7 +551,7 @@ __device__ __forceinline__ void arrive_and_merge(const AttnArgs& a, int m0, int 
 // (two score chains at once, one test of the maximum for both): the transforms' registers
 // spill at three. Two chunks of 2048 rows after up to 6144 keys, 40/8 heads x 128, capped
 // scores (475 GFLOP): 836 us at three waves and 32 keys, 778 at two, 698 with stages of
-// 64, 689 with steps of 64 (659 since, by the cap's polynomials and the stages' addresses). At 128-byte rows four waves and 32-key steps stay the faster
+// 64, 689 with steps of 64 (648 since, by the cap's polynomials and the stages' addresses). At 128-byte rows four waves and 32-key steps stay the faster
 // (8 packed prompts of documents 49 us, 57 at three waves with steps of 64).
 constexpr int scored_waves(int dp) { return dp == 128 ? 2 : 4; }
 constexpr int scored_step(int dp) { return dp == 128 ? 2 : 1; }  // 32-key blocks
