@@ -51,10 +51,13 @@ def _validate(query: torch.Tensor, num_kv_heads: int, seq_ids, positions, block_
     if num_heads % num_kv_heads != 0:
         raise ValueError(f"{num_heads} query heads is not a multiple of {num_kv_heads} kv heads")
     tables = [as_table_list(t) for t in block_tables]
-    for seq_id, rows in group_by_sequence(seq_ids):
+    last = {}
+    for seq_id, pos in zip(seq_ids, positions):
+        if pos > last.get(seq_id, -1):
+            last[seq_id] = pos
+    for seq_id, last_key in last.items():
         if seq_id < 0 or seq_id >= len(tables):
             raise IndexError(f"seq_id {seq_id} has no block table (got {len(tables)})")
-        last_key = max(positions[r] for r in rows)
         needed = (last_key + 1 + block_size - 1) // block_size
         if needed > len(tables[seq_id]):
             raise IndexError(
