@@ -72,11 +72,12 @@ class _VarlenBinding:
     ``pool_lens`` turns the pass into a verify pass: keys at or above
     pool_lens[s] are the layer's in-flight key/value rows, not pool slots. A
     host sequence is uploaded with the rest of the metadata; a device tensor
-    must already be in the grouped sequence order.
+    must already be in the grouped sequence order. ``longest`` is the pass's
+    longest context, ``window`` the shortest sliding window its layers named.
     """
 
     __slots__ = ("pool", "block_tables", "seq_ids", "positions", "block_wise", "used", "_meta",
-                 "pool_lens", "num_rows", "timer", "write_slots")
+                 "pool_lens", "num_rows", "timer", "write_slots", "longest", "window")
 
     def __init__(self, pool, block_tables, seq_ids, positions, block_wise=False, pool_lens=None):
         self.pool = pool
@@ -90,11 +91,14 @@ class _VarlenBinding:
         self.num_rows = len(self.seq_ids)
         self.timer = None  # a sampled pass's event record (engine telemetry)
         self.write_slots = None
+        self.longest = max((int(p) for p in self.positions), default=-1) + 1
+        self.window = None
 
     @classmethod
     def from_packed(cls, pool, meta: dict, num_rows: int, pool_lens: Optional[torch.Tensor] = None,
-                    write_slots: Optional[torch.Tensor] = None):
-        """A prepared binding. ``write_slots`` (the step's slot_mapping, with a
+                    write_slots: Optional[torch.Tensor] = None, longest: Optional[int] = None):
+        """A prepared binding (``longest`` None: read from the device if a layer
+        has a sliding window). ``write_slots`` (the step's slot_mapping, with a
         cache made by ``VarlenPackedCache.from_slot_mapping(...,
         write_in_attention=True)``): every layer's attention launch also writes
         the new K/V rows it is handed into the pool and reads each sequence's
@@ -112,7 +116,17 @@ class _VarlenBinding:
         b.num_rows = num_rows
         b.timer = None
         b.write_slots = write_slots
+        b.longest = longest
+        b.window = None
         return b
+
+    def check_window(self, window: Optional[int]) -> None:
+        """A layer of this pass names a sliding window: refused where a context is longer."""
+        if not window:
+            return
+        self.window = min(int(window), self.window or int(window))
+        longest = self.longest if self.longest is not None else int(self._meta["kv_lens"].max())
+        _check_window(window, longest)
 
     def meta(self, num_q_heads: int, head_dim: int, dtype: torch.dtype, device, scored: bool = False) -> dict:
         """``scored``: the layer caps its scores, which slice plans do not serve (a
@@ -168,6 +182,23 @@ class _VarlenBinding:
             "plan": plan,
         }
         return self._meta
+
+
+def _check_window(window: Optional[int], context: int) -> None:
+    """The paged kernels attend to a row's whole context, which is what a layer with
+    a sliding window does only while the context is no longer than the window."""
+    if window and context > window:
+        raise ValueError(f"a layer attends within a sliding window of {window} keys, which the paged kernels do not "
+                         f"serve past it: the context has {context}")
+
+
+def attention_window(config) -> Optional[int]:
+    """The sliding window that some layer of a model with this config attends within, None for none."""
+    window = getattr(config, "sliding_window", None)
+    kinds = getattr(config, "layer_types", None)
+    if not window or (kinds is not None and "sliding_attention" not in kinds):
+        return None
+    return int(window)
 
 
 def _current() -> Optional[_Binding]:
@@ -273,16 +304,23 @@ def paged_attention_forward(module: Any, query: torch.Tensor, key: torch.Tensor,
                             dropout: float = 0.0, **kwargs: Any) -> Tuple[torch.Tensor, None]:
     """The function registered as ``memforge_paged`` (attention_backend.py:195-272).
     Returns ``(batch, q_len, heads, head_dim)`` as transformers expects. A model
-    that caps its attention scores passes ``softcap``, which every route applies."""
-    softcap = kwargs.get("softcap")
+    that caps its attention scores passes ``softcap``, which every route applies; a
+    layer with a sliding window passes ``sliding_window``, and the paged routes
+    refuse a context longer than it (the eager one masks it)."""
+    softcap, window = kwargs.get("softcap"), kwargs.get("sliding_window")
     varlen = _current_varlen()
     if varlen is not None:
+        varlen.check_window(window)
         varlen.used += 1
         return _varlen_forward(module, query, key, value, scaling, varlen, softcap), None
 
     binding = _current()
     single_query = query.shape[0] == 1 and query.shape[2] == 1
-    if binding is not None and single_query and _mask_is_permissive(attention_mask) and binding.context_length > 0:
+    past_window = bool(window) and binding is not None and binding.context_length > window
+    if past_window and key.shape[2] < binding.context_length:  # a lazy cache hands on the new key alone
+        _check_window(window, binding.context_length)
+    if binding is not None and single_query and _mask_is_permissive(attention_mask) and binding.context_length > 0 \
+            and not past_window:
         binding.used += 1
         if binding.pool.kv_bits == 4:
             out = paged_attention_varlen_pool(query, binding.pool, module.layer_idx, [binding.block_table], [0],
@@ -295,7 +333,7 @@ def paged_attention_forward(module: Any, query: torch.Tensor, key: torch.Tensor,
 
     if binding is not None:
         binding.fallbacks += 1
-    return _eager_attention(module, query, key, value, attention_mask, scaling, softcap), None
+    return _eager_attention(module, query, key, value, attention_mask, scaling, softcap, window), None
 
 
 def _to_attention_output_layout(attn_output: torch.Tensor) -> torch.Tensor:
@@ -304,7 +342,7 @@ def _to_attention_output_layout(attn_output: torch.Tensor) -> torch.Tensor:
 
 
 def _eager_attention(module, query, key, value, attention_mask, scaling,
-                     softcap: Optional[float] = None) -> torch.Tensor:
+                     softcap: Optional[float] = None, window: Optional[int] = None) -> torch.Tensor:
     """Plain attention with grouped-query expansion for unbound calls
     (attention_backend.py:295-328); softmax in fp32."""
     num_heads, head_dim = query.shape[1], query.shape[3]
@@ -320,18 +358,21 @@ def _eager_attention(module, query, key, value, attention_mask, scaling,
     if attention_mask is not None:
         scores = scores + attention_mask[:, :, :, : k.shape[-2]]
     else:
-        scores = _apply_implicit_causal_mask(scores)
+        scores = _apply_implicit_causal_mask(scores, window)
     weights = torch.softmax(scores, dim=-1, dtype=torch.float32).to(query.dtype)
     return _to_attention_output_layout(torch.matmul(weights, v))
 
 
-def _apply_implicit_causal_mask(scores: torch.Tensor) -> torch.Tensor:
+def _apply_implicit_causal_mask(scores: torch.Tensor, window: Optional[int] = None) -> torch.Tensor:
     """Right-aligned causality when transformers passes no mask
-    (attention_backend.py:331-357)."""
+    (attention_backend.py:331-357); with ``window`` a row's last ``window`` keys."""
     q_len, kv_len = scores.shape[-2], scores.shape[-1]
-    if q_len <= 1:
+    windowed = bool(window) and kv_len > window
+    if q_len <= 1 and not windowed:
         return scores
     causal = torch.ones(q_len, kv_len, dtype=torch.bool, device=scores.device).tril(diagonal=kv_len - q_len)
+    if windowed:
+        causal = causal.triu(diagonal=kv_len - q_len - window + 1)
     return scores.masked_fill(~causal, torch.finfo(scores.dtype).min)
 
 

@@ -255,6 +255,13 @@ class ContinuousBatchingEngine:
         self.dtype = dtype or next(model.parameters()).dtype
         self.block_size = block_size
         self.max_num_seqs = max_num_seqs
+        # the paged kernels attend to whole contexts, so a model with sliding
+        # windows is served as far as its shortest window
+        window = attention_backend.attention_window(model.config)
+        if window is not None and window < max_model_len:
+            warnings.warn(f"the model's layers attend within sliding windows of {window} tokens: max_model_len is "
+                          f"{window} instead of {max_model_len}", stacklevel=2)
+            max_model_len = window
         self.max_model_len = max_model_len
         # Accepted for API compatibility: every step is one packed varlen pass,
         # which is what the reference's batched_decode / block_attention /
@@ -307,6 +314,7 @@ class ContinuousBatchingEngine:
         # "batched" whenever the draft's head grouping allows it. True, the
         # reference's superseded per-sequence graphs, runs as "batched".
         self._draft_pool = None
+        self._draft_limit = max_model_len  # the longest context a draft round may reach
         if draft_cuda_graph == "auto":
             draft_cuda_graph = "batched" if (draft_model is not None
                                              and self._graph_heads_ok(draft_model)) else False
@@ -323,6 +331,9 @@ class ContinuousBatchingEngine:
             self._draft_pool = BatchedGraphedDraftPool(
                 draft_model, max_len=max_model_len, num_slots=max_num_seqs, device=self.device,
                 unroll=draft_cuda_graph == "batched-unrolled")
+            # graphed drafts run the paged kernels too
+            self._draft_limit = min(max_model_len, attention_backend.attention_window(draft_model.config)
+                                    or max_model_len)
         # every speculative step resolves its rows with one kernel launch; the
         # one-row-at-a-time form stays selectable for differential tests
         self._batched_resolve = True
@@ -662,7 +673,7 @@ class ContinuousBatchingEngine:
 
     def _speculation_headroom(self, rt: SequenceRuntime) -> bool:
         span = self.lookahead_k + 1
-        if rt.cache.position + span > self.max_model_len:
+        if rt.cache.position + span > self._draft_limit:
             return False
         return len(rt.generated) + span <= rt.params.max_new_tokens
 

@@ -89,7 +89,8 @@ def packed_forward(model, pool, tokens: Sequence[Sequence[int]], starts: Sequenc
     # rows are rounded into a 4-bit pool before anything attends to them
     fuse = fuse_kv_write and spec.dtype == model.dtype and pool.kv_bits != 4
     binding = attention_backend._VarlenBinding.from_packed(pool, meta, T,
-                                                           write_slots=packed.slot_mapping if fuse else None)
+                                                           write_slots=packed.slot_mapping if fuse else None,
+                                                           longest=max(kv_lens))
     cache = VarlenPackedCache.from_slot_mapping(pool, spec.num_layers, packed.slot_mapping, write_in_attention=fuse)
     binding.timer = cache.timer = timer
     with attention_backend.backend_enabled_on(model) as routed:
