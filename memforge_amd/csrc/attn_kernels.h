@@ -177,7 +177,9 @@ using ArgsOf = std::conditional_t<SC, ScoredArgs, AttnArgs>;
 // over |x| <= 0.5 (5.4e-7). One test of the block's largest magnitude picks. With four
 // terms alone and x formed first, two chunks of 2048 rows after up to 6144 keys took 707
 // us at a cap that no score comes near (40/8 heads x 128, 475 GFLOP), 665 with both; at
-// one whose quarter many pass 746 and 752 us. fp32 takes the series to x^11 below 0.35 (the
+// one whose quarter many pass 746 and 752 us. Slots that no row sees are cleared and pick
+// nothing; where another row's score of the block passes half the cap, a row's scores are
+// off by 1e-7 of the cap, 2e-7 of that score. fp32 takes the series to x^11 below 0.35 (the
 // next term is 2e-8 of x there) score by score: its launches are not bound by this.
 template <int DT, int N, class Dist>
 __device__ __forceinline__ void score_all(float (&s)[N], const ScoredArgs& a, float slope_log2, Dist dist) {
@@ -979,16 +981,26 @@ __device__ __forceinline__ void attn_body(const ArgsOf<SC>& a, const int block) 
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int r = 0; r < 4; ++r) sv[nt][r] = st[nt][r];
+        // Every key of a tile wholly inside the context and at or before every
+        // column's position is visible to all columns: no mask to apply.
+        const bool edge = !(kt * 16 + 15 <= minpos && (kt + 1) * 16 <= kv_len && (!SC || kt * 16 >= first));
         if constexpr (SC) {
+            // a block's largest score picks how it is capped (score_all): no hidden one does
+            if (edge) {
+                asm volatile("");
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        sv[nt][r] = kt * 16 + 4 * g + r <= lim[nt] && kt * 16 + 4 * g + r >= first ? sv[nt][r] : 0.f;
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const float dist = (float)(kt * 16 + 4 * g - at_pos[nt]);
                 score_all<DT>(sv[nt], a, slope[nt], [&](int i) { return dist + i; });
             }
         }
-        // Every key of a tile wholly inside the context and at or before every
-        // column's position is visible to all columns: no mask to apply.
-        if (!(kt * 16 + 15 <= minpos && (kt + 1) * 16 <= kv_len && (!SC || kt * 16 >= first))) {
+        if (edge) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -1752,14 +1764,19 @@ __device__ __forceinline__ void attn_wide_body(const ArgsOf<SC>& a, const int bl
             const int key0 = (kt0 + TS * u) * 16;
             if (key0 + KEYS > live_end) {
                 // the last stage: p is 0 for its rows past the context, and 0 * NaN is NaN
+                // (SC: nor may their scores pick how the rest is capped)
                 const int first = live_end - key0;
-                for (int x = first * NCH + (int)threadIdx.x; x < KEYS * NCH; x += 256)
+                for (int x = first * NCH + (int)threadIdx.x; x < KEYS * NCH; x += 256) {
                     *(uint4*)(stg + HALF + x * 16) = make_uint4(0, 0, 0, 0);
+                    if constexpr (SC) *(uint4*)(stg + x * 16) = make_uint4(0, 0, 0, 0);
+                }
                 sync();
             }
             if (SC && key0 < first_key) {  // likewise the keys no row of the sequence sees
-                for (int x = (int)threadIdx.x; x < min(first_key - key0, KEYS) * NCH; x += 256)
+                for (int x = (int)threadIdx.x; x < min(first_key - key0, KEYS) * NCH; x += 256) {
                     *(uint4*)(stg + HALF + x * 16) = make_uint4(0, 0, 0, 0);
+                    *(uint4*)(stg + x * 16) = make_uint4(0, 0, 0, 0);
+                }
                 sync();
             }
 #pragma unroll
@@ -2481,24 +2498,26 @@ inline int set_scoring(ScoredArgs& a, const mf_scoring& s) {
     a.cap_log2 = s.softcap * 1.4426950408889634f;
     a.cap_x = s.softcap > 0.f ? a.scale_log2 / a.cap_log2 : 0.f;
     // The polynomials' coefficients by powers of cap_x, so that they take raw scores. Where
-    // one leaves fp32's normal numbers: four terms are not used; three lose those that have
-    // no weight (relative to the score) below 3e-4 of the cap, and are used below that; a cap
-    // so small that they overflow is left to the exponential (1e-7 of it is nothing).
+    // one leaves fp32's normal numbers: four terms are not used; three lose the last (2e-8 of
+    // the score at a fiftieth of the cap) or the last two (1.2e-5 at 6e-3 of it, for caps past
+    // 1e17), and are used below that; a cap so small that they overflow is left to the
+    // exponential (1e-7 of it is nothing).
     const double p3[3] = {0.9999996, -0.33321908, 0.12841609};
     const double p4[4] = {0.99999946, -0.33326318, 0.13190299, -0.04440228};
     double power = (double)a.cap_log2 * a.cap_x;
-    bool low = false, high = false;
+    float reach = 0.25f;
+    bool high = false;
     for (int i = 0; i < 4; ++i, power *= (double)a.cap_x * a.cap_x) {
         const double c = power * (i < 3 ? p3[i] : p4[i]);
         high |= std::abs(c) > 1e37;
         if (i < 3) {
-            low |= std::abs(c) < FLT_MIN;
+            if (std::abs(c) < FLT_MIN) reach = std::fmin(reach, i == 2 ? 0.02f : 6e-3f);
             a.cap_p3[i] = std::abs(c) < FLT_MIN ? 0.f : (float)c;
         }
         a.cap_p4[i] = (float)(power * p4[i]);
     }
     // z = s^2 stays finite
-    a.cap_top = high ? -1.f : std::fmin((low ? 3e-4f : 0.25f) / a.cap_x, 1e18f);
+    a.cap_top = high ? -1.f : std::fmin(reach / a.cap_x, 1e18f);
     a.cap_top4 = high || std::abs(a.cap_p4[3]) < FLT_MIN ? -1.f : 0.5f / a.cap_x;
     if (s.softcap > 0.f && !(a.cap_in >= FLT_MIN && a.cap_in < INFINITY && a.cap_log2 < INFINITY)) return MF_ERR_ARG;
     return MF_OK;

@@ -173,6 +173,19 @@ __device__ __forceinline__ void attn4_narrow(const Attn4Args& a, const int32_t* 
                         w = live ? w : 0u;
                     }
                 }
+                // K likewise in a scored launch: a block's largest score picks how it is
+                // capped (score_all)
+                if constexpr (SC) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        Tile& z = u ? y : x;
+                        const int key = t * 16 + 16 * u + j;
+                        const bool live = key <= maxlim && key >= first;
+                        z.ks = live ? z.ks : 0x7f7fu;
+#pragma unroll
+                        for (int c = 0; c < KW; ++c) z.kw[c] = live ? z.kw[c] : 0u;
+                    }
+                }
             }
             f32x4 st[2];
 #pragma unroll
@@ -490,9 +503,6 @@ __device__ __forceinline__ void attn4_wide(const Attn4Args& a, const int32_t* it
         else c.vs = vs[vs_lane];
     };
     auto stage = [&](int u, char* stg, Codes& c) __attribute__((always_inline)) {
-        const float ks = scale4(c.ks);
-#pragma unroll
-        for (int k = 0; k < NW; ++k) *(uint4*)(stg + k_dst[k]) = octet4<DT>(c.kw[k], ks);
         uint32_t vs[NW];
 #pragma unroll
         for (int k = 0; k < NW; ++k) vs[k] = ((c.vs >> (8 * k)) << 23) & 0x7f800000u;
@@ -507,7 +517,16 @@ __device__ __forceinline__ void attn4_wide(const Attn4Args& a, const int32_t* it
                 vs[k] = live ? vs[k] : 0x3f800000u;
                 c.vw[k] = live ? c.vw[k] : 0u;
             }
+            if constexpr (SC) {  // K too, as in attn4_narrow
+                const bool live = key0 + kkey <= wglim && key0 + kkey >= first;
+                c.ks = live ? c.ks : 127u;
+#pragma unroll
+                for (int k = 0; k < NW; ++k) c.kw[k] = live ? c.kw[k] : 0u;
+            }
         }
+        const float ks = scale4(c.ks);
+#pragma unroll
+        for (int k = 0; k < NW; ++k) *(uint4*)(stg + k_dst[k]) = octet4<DT>(c.kw[k], ks);
 #pragma unroll
         for (int k = 0; k < NW; ++k) *(uint4*)(stg + v_dst[k]) = octet4<DT>(c.vw[k], __uint_as_float(vs[k]));
     };

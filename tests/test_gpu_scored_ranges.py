@@ -8,7 +8,6 @@ import pytest
 import torch
 
 from memforge_amd import _native as nat
-from tests.scored_reference import attend, check
 from tests.test_gpu_kv4 import Step4
 from tests.test_gpu_scored import Step, slopes_of
 
