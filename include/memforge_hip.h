@@ -289,11 +289,13 @@ int mf_paged_attention_kv_write(const void* q, int64_t q_stride_row, int64_t q_s
  *     t = t - slopes[h] * |positions[r] - k|             slopes non-NULL
  * and with key k visible to row r when k < kv_lens[s], k >= first_keys[s]
  * (NULL: 0), and k <= positions[r] or k < prefix_lens[s] (NULL: 0). A row that
- * sees no key gets zeros. Keys below first_keys[s] and from kv_lens[s] on may
- * hold anything, NaN included; between them a value that is not finite reaches
- * rows of s that do not see it too (zero times it), as in a plain call. A document mask runs each document's rows as a
- * sequence of their own over the same block table, first_keys the document's
- * first position; rows before the prefix's end see the whole prefix.
+ * sees no key gets zeros, one at a negative position too; a sequence with
+ * kv_lens[s] = 0 has no items in a plan, and its rows stay as they were. Keys
+ * below first_keys[s] and from kv_lens[s] on may hold anything, NaN included;
+ * between them a value that is not finite reaches rows of s that do not see it
+ * too (zero times it), as in a plain call. A document mask runs each document's
+ * rows as a sequence of their own over the same block table, first_keys the
+ * document's first position; rows before the prefix's end see the whole prefix.
  * softcap: finite, 0 for none; so small or large against the scale that their
  * quotient leaves fp32's normal numbers is MF_ERR_ARG. slopes: fp32[num_q_heads],
  * first_keys / prefix_lens: int32 per sequence, all on the device.

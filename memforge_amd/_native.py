@@ -534,7 +534,8 @@ class Scoring:
     * ``prefix_lens`` (int32, one per sequence): keys before it are seen by every
       row, those after the row's position too (from ``first_keys`` on).
 
-    A row that sees no key gets zeros. Plans for masked calls are made with the
+    A row that sees no key gets zeros, except in a sequence whose ``kv_lens`` entry is
+    0: those rows are not in the plan and stay as they were. Plans for masked calls are made with the
     same ``first_keys`` and ``prefix_lens`` as host lists (``plan_attention``).
     Keys that no row of a sequence sees may hold anything; a value that is not
     finite reaches the rows of its sequence that do not see it too, as zero times

@@ -1221,7 +1221,7 @@ __device__ __forceinline__ void attn_body(const ArgsOf<SC>& a, const int block) 
                 for (int c = 0; c < VCH; ++c) o[c] += w * s_acc[u][wave * VCH + c][lane];
             }
             const int d0 = (4 * g + wave) * VCH;
-            if (nct > 0 && qpos[0] >= 0) {
+            if (nct > 0 && (SC ? qvalid[0] : qpos[0] >= 0)) {
                 if (pslot < 0) {
                     if (d0 < D) {
                         const float inv = L > 0.f ? 1.f / L : 0.f;
@@ -1272,7 +1272,7 @@ __device__ __forceinline__ void attn_body(const ArgsOf<SC>& a, const int block) 
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const float lt = group_sum4(l[nt]);
-        if (nt >= nct || qpos[nt] < 0) continue;
+        if (nt >= nct || (SC ? !qvalid[nt] : qpos[nt] < 0)) continue;
         if (pslot < 0) {
             if (dbase < D) {
                 const float inv = lt > 0.f ? 1.f / lt : 0.f;
@@ -1798,8 +1798,9 @@ __device__ __forceinline__ void attn_wide_body(const ArgsOf<SC>& a, const int bl
     auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
     const float lt = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     const float inv = lt > 0.f ? 1.f / lt : 0.f;
+    const bool live = SC ? valid : qpos >= 0;  // scored rows that see no key get zeros
     if (SC && pslot >= 0) {
-        if (qpos >= 0) {
+        if (live) {
             char* part = partial_out<MF_F32>(a, pslot + ct, j, 0);
 #pragma unroll
             for (int d = 0; d < ND; ++d)
@@ -1821,7 +1822,7 @@ __device__ __forceinline__ void attn_wide_body(const ArgsOf<SC>& a, const int bl
         return;
     }
     char* dst = nullptr;
-    if (qpos >= 0)
+    if (live)
         dst = pslot < 0 ? a.out + ((int64_t)prow * a.o_sr + (int64_t)qhead * a.o_sh) * 2
                         : partial_out<DT>(a, pslot + ct, j, 0);
 #pragma unroll
@@ -1837,10 +1838,10 @@ __device__ __forceinline__ void attn_wide_body(const ArgsOf<SC>& a, const int bl
                               (f32_to_bits<DT>(acc[d][4 * (b + e) + 2 * k + 1] * inv) << 16);
             auto x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
             auto y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
-            if (qpos >= 0) *(uint4*)(dst + (32 * d + 8 * (b + hf)) * 2) = make_uint4(x[0], y[0], x[1], y[1]);
+            if (live) *(uint4*)(dst + (32 * d + 8 * (b + hf)) * 2) = make_uint4(x[0], y[0], x[1], y[1]);
         }
     if (pslot >= 0) {
-        if (qpos >= 0 && hf == 0) {
+        if (live && hf == 0) {
             float* ml = partial_ml(a, pslot + ct);
             ml[j] = m;
             ml[16 + j] = lt;

@@ -1,10 +1,11 @@
-"""Calls at the edges of scored attention: caps of any size beside slots that no row sees."""
+"""Calls at the edges of scored attention: caps of any size beside slots that no row sees, rows at negative positions."""
 
 from __future__ import annotations
 
 import pytest
 import torch
 
+from memforge_amd import _native as nat
 from tests.scored_reference import attend, check
 from tests.test_gpu_kv4 import Step4
 from tests.test_gpu_scored import DECODES, PREFILLS, Step, slopes_of
@@ -54,3 +55,38 @@ def test_hidden_slots_change_no_bit(device, bits, dtype, d, bs, hidden):
         outs.append([st.run(st.scoring(cap, slopes_of(6, device))) for cap in (30.0, 1e6)])
     for a, b in zip(*outs):
         assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+NEGATIVE_RUNS = [(0, 200, 1, 0), (0, 0, 40, 0), (0, 2000, 1, 0), (0, 900, 60, 0), (0, 2100, 3, 0)]
+
+
+def _at_negative_positions(st, device):
+    """Every third row of each run, and all of the first one's, lie at position -1."""
+    for i in range(len(st.runs)):
+        for r in range(st.cu[i], st.cu[i + 1]):
+            if i == 0 or (r - st.cu[i]) % 3 == 1:
+                st.positions[r] = -1
+    st.pos_t = torch.tensor(st.positions, dtype=torch.int64, device=device)
+
+
+@pytest.mark.parametrize("dtype,d,bits", [(torch.bfloat16, 64, 16), (torch.float16, 128, 16), (torch.float32, 64, 16),
+                                          (torch.bfloat16, 256, 16), (torch.bfloat16, 64, 4), (torch.float16, 256, 4)])
+@pytest.mark.parametrize("tiles", [0, 8])
+def test_rows_at_negative_positions_get_zeros(device, dtype, d, bits, tiles):
+    st = (Step4 if bits == 4 else Step)(device, dtype, 6, 2, d, 16, NEGATIVE_RUNS, seed=13)
+    _at_negative_positions(st, device)
+    plan = st.plan(partition_tiles=tiles)
+    if tiles:
+        assert plan.n_merges > 0
+    # partials of an earlier call must not be taken for this one's
+    nat._WORKSPACE.partials(max(plan.partials_floats, 1), device).fill_(float("nan"))
+    out = st.run(st.scoring(30.0), plan).cpu().double()
+    seen = torch.tensor(st.positions) >= 0
+    assert (out[~seen] == 0).all()
+    assert torch.isfinite(out[seen]).all()
+    if bits == 16:
+        for i in range(len(st.runs)):
+            rows = slice(st.cu[i], st.cu[i + 1])
+            at = st.slots(i, 0, st.kv[i])
+            k, v = (x.view(-1, 2, d).cpu()[at] for x in (st.kp, st.vp))
+            check(out[rows], *attend(st.q[rows], k, v, st.positions[rows], st.scale, 30.0), dtype, d, st.kv[i], 30.0, f"run {i}")
