@@ -549,7 +549,7 @@ class Scoring:
     def __post_init__(self):
         cap = 0.0 if self.softcap is None else float(self.softcap)
         held = ctypes.c_float(cap).value  # what the launch takes: a cap that vanishes there would be none
-        if not 0.0 <= held < float("inf") or (cap > 0.0) != (held > 0.0):
+        if not 0.0 <= cap or not held < float("inf") or (cap > 0.0 and held == 0.0):
             raise ValueError(f"softcap must be finite and not negative in 32 bits, got {self.softcap}")
         object.__setattr__(self, "softcap", cap)
 
