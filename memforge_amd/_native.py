@@ -257,6 +257,22 @@ class Pool4View:
         return self.num_blocks * self.block_size
 
 
+def kv_bits(pool) -> int:
+    """4 for a pool object that holds its keys and values in 4 bits, 16 for any other
+    (a caller's own class need not say)."""
+    return getattr(pool, "kv_bits", 16)
+
+
+def kv_dtype(pool) -> torch.dtype:
+    """The type attention over a pool object runs in: its elements', or what a 4-bit one names."""
+    return pool.spec.dtype if kv_bits(pool) == 4 else pool.key_pool.dtype
+
+
+def kv_device(pool) -> torch.device:
+    """Where a pool object's memory lies (its spec may name a kind of device alone)."""
+    return (pool.key_codes if kv_bits(pool) == 4 else pool.key_pool).device
+
+
 def same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Same shape and the same strides on every axis longer than one (the
     stride of a length-one axis is never used to address an element)."""

@@ -157,10 +157,10 @@ class _VarlenBinding:
         identity = row_map == list(range(len(row_map)))
         # a large decode step on 16-token blocks runs as one round of slices
         sliceable = identity and self.pool_lens is None and self.pool.block_size == 16 and not scored \
-            and self.pool.kv_bits != 4
+            and nat.kv_bits(self.pool) != 4
         items, merges, counts, sliced = nat.plan_host(cu, kvl, num_q_heads, self.pool.spec.num_kv_heads,
                                                       head_dim, dtype, device, decode_slices=sliceable,
-                                                      kv_bits=self.pool.kv_bits)
+                                                      kv_bits=nat.kv_bits(self.pool))
         # everything the launch reads crosses to the device in one copy
         parts = [padded_tables_host([tables[s] for s in order]), *nat.plan_upload_parts(items, merges),
                  np.asarray(cu + kvl, dtype=np.int32), np.asarray(list(self.positions), dtype=np.int64)]
@@ -260,14 +260,14 @@ def _varlen_forward(module, query, key, value, scaling, binding: _VarlenBinding,
         )
     _, hq, total, d = query.shape
     pool = binding.pool
-    dtype = pool.spec.dtype
+    dtype = nat.kv_dtype(pool)
     scoring = nat.Scoring(softcap) if softcap else None
     meta = binding.meta(hq, d, dtype, query.device, scored=scoring is not None)
     q_rows = query[0].to(dtype).permute(1, 0, 2)
     out = torch.empty((1, total, hq, d), dtype=dtype, device=query.device)
     layer = module.layer_idx
     nk = nv = None
-    if binding.pool_lens is not None and pool.kv_bits == 4:
+    if binding.pool_lens is not None and nat.kv_bits(pool) == 4:
         raise ValueError("a pass that attends to unwritten keys (a speculative verify) needs a 16- or 32-bit pool")
     if binding.pool_lens is not None:
         nk = key[0].to(dtype).permute(1, 0, 2)
@@ -322,7 +322,7 @@ def paged_attention_forward(module: Any, query: torch.Tensor, key: torch.Tensor,
     if binding is not None and single_query and _mask_is_permissive(attention_mask) and binding.context_length > 0 \
             and not past_window:
         binding.used += 1
-        if binding.pool.kv_bits == 4:
+        if nat.kv_bits(binding.pool) == 4:
             out = paged_attention_varlen_pool(query, binding.pool, module.layer_idx, [binding.block_table], [0],
                                               [binding.context_length - 1], scale=scaling, softcap=softcap)
         else:

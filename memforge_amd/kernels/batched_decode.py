@@ -67,9 +67,9 @@ def assemble_batch(pool, buffers: BatchedDecodeBuffers, block_tables: Sequence[t
         raise ValueError(f"{len(block_tables)} block tables for {batch} sequences")
     max_len = max(context_lengths)
     heads, dim = pool.spec.num_kv_heads, pool.spec.head_dim
-    keys, values, padded = buffers.acquire(batch, max_len, heads, dim, pool.spec.dtype, pool.spec.device)
+    keys, values, padded = buffers.acquire(batch, max_len, heads, dim, nat.kv_dtype(pool), pool.spec.device)
     flat = [pool.flat_indices(t, 0, c) for t, c in zip(block_tables, context_lengths)]
-    gather = nat.kv4_gather if pool.kv_bits == 4 else nat.kv_gather
+    gather = nat.kv4_gather if nat.kv_bits(pool) == 4 else nat.kv_gather
     for layer in range(pool.spec.num_layers):
         view = pool.layer_view(layer)
         for row, (index, ctx) in enumerate(zip(flat, context_lengths)):
@@ -90,7 +90,7 @@ def scatter_new_tokens(pool, block_tables: Sequence[torch.Tensor], context_lengt
     ``context_lengths[row]`` (batched_decode.py:194-219): one KV-write launch
     per layer for the whole batch."""
     slots = torch.cat([pool.flat_indices(t, c, c + 1) for t, c in zip(block_tables, context_lengths)])
-    write = nat.kv4_write if pool.kv_bits == 4 else nat.kv_write
+    write = nat.kv4_write if nat.kv_bits(pool) == 4 else nat.kv_write
     for layer in range(pool.spec.num_layers):
         k, v = new_keys[layer], new_values[layer]  # (batch, heads, 1, dim)
         write(k[:, :, 0, :], v[:, :, 0, :], slots, pool.layer_view(layer))

@@ -122,7 +122,7 @@ def paged_attention_varlen_pool(query: torch.Tensor, pool, layer_idx: int, block
     view = pool.layer_view(layer_idx)
     nat.require_device(query)
     tables = _validate(query, view.num_heads, seq_ids, positions, block_tables, pool.block_size, False)
-    q = query[0].to(pool.spec.dtype).permute(1, 0, 2)  # (T, H, D)
+    q = query[0].to(nat.kv_dtype(pool)).permute(1, 0, 2)  # (T, H, D)
     if q.stride(-1) != 1:
         q = q.contiguous()
     total, heads, dim = q.shape

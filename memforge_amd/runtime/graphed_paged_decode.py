@@ -109,7 +109,7 @@ class GraphedPagedDecoder:
         if not attention_backend.register():
             raise RuntimeError("the transformers attention registry is required")
         self.model, self.pool = model, pool
-        self.fuse_kv_write = bool(fuse_kv_write) and pool.spec.dtype == model.dtype and pool.kv_bits != 4
+        self.fuse_kv_write = bool(fuse_kv_write) and nat.kv_dtype(pool) == model.dtype and nat.kv_bits(pool) != 4
         self.device = pool.spec.device
         self.bs = pool.block_size
         self.max_batch = max(1, int(max_batch))
@@ -196,9 +196,9 @@ class GraphedPagedDecoder:
         bk.copied.record()
         kv = [int(c) + 1 for c in ctx_lens] + [0] * (b - n)
         plan_args = (list(range(b + 1)), kv, self.num_q_heads, self.pool.spec.num_kv_heads,
-                     self.pool.spec.head_dim, self.pool.spec.dtype)
+                     self.pool.spec.head_dim, nat.kv_dtype(self.pool))
         items, merges, counts = nat.plan_attention_host(*plan_args, num_cus=nat.device_cus(self.device),
-                                                        merge_free=self.merge_free, kv_bits=self.pool.kv_bits)
+                                                        merge_free=self.merge_free, kv_bits=nat.kv_bits(self.pool))
         if self.merge_free and counts[2] > 0:
             # the planner's pick splits a range: take the smallest partition
             # whose units hold the longest context whole instead

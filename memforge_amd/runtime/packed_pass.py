@@ -74,8 +74,8 @@ def packed_forward(model, pool, tokens: Sequence[Sequence[int]], starts: Sequenc
     flat_tokens = np.fromiter((tok for run in tokens for tok in run), dtype=np.int32)
     nat.check_pack_entries(ent, flat_tables, len(flat_tokens), T, pool.num_blocks)
     items, merges, counts = nat.plan_attention_host(cu.tolist(), kv_lens, model.config.num_attention_heads,
-                                                    spec.num_kv_heads, spec.head_dim, spec.dtype,
-                                                    num_cus=nat.device_cus(spec.device), kv_bits=pool.kv_bits)
+                                                    spec.num_kv_heads, spec.head_dim, nat.kv_dtype(pool),
+                                                    num_cus=nat.device_cus(spec.device), kv_bits=nat.kv_bits(pool))
     keep_np = np.asarray(list(keep_rows), dtype=np.int64)
     # descriptors, tables, tokens, the attention plan and the kept rows cross
     # to the device in one copy
@@ -87,7 +87,7 @@ def packed_forward(model, pool, tokens: Sequence[Sequence[int]], starts: Sequenc
             "kv_lens": packed.kv_lens, "positions": packed.positions, "row_map": None,
             "plan": attn_plan}
     # rows are rounded into a 4-bit pool before anything attends to them
-    fuse = fuse_kv_write and spec.dtype == model.dtype and pool.kv_bits != 4
+    fuse = fuse_kv_write and nat.kv_dtype(pool) == model.dtype and nat.kv_bits(pool) != 4
     binding = attention_backend._VarlenBinding.from_packed(pool, meta, T,
                                                            write_slots=packed.slot_mapping if fuse else None,
                                                            longest=max(kv_lens))

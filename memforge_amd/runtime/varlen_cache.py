@@ -98,7 +98,7 @@ def _slot_bitmap(pool) -> torch.Tensor:
     bm = getattr(pool, "_mf_slot_bitmap", None)
     words = (pool.capacity_tokens + 31) // 32
     if bm is None or bm.numel() < words:
-        bm = torch.zeros(words, dtype=torch.int32, device=pool.spec.device)
+        bm = torch.zeros(words, dtype=torch.int32, device=nat.kv_device(pool))
         pool._mf_slot_bitmap = bm
     return bm
 
@@ -125,7 +125,7 @@ def build_write_index(pool, block_tables: Sequence, seq_ids: Sequence[int],
     for s, start, n in runs:
         entries.append([n, start, start + n, len(flat_tables), len(tables[s]), 0])
         flat_tables.extend(tables[s])
-    dev = pool.spec.device
+    dev = nat.kv_device(pool)
     ints = torch.tensor([x for e in entries for x in e] + flat_tables, dtype=torch.int32).to(dev)
     ne = len(entries) * nat.ENTRY_INTS
     # the pass only needs slots: every entry reads dummy token ids from one zero run
