@@ -850,7 +850,14 @@ class CountedPlan:
 class Workspace:
     """Grow-only scratch for split-K partials (fp32), merge arrival counters
     (int32, kept all-zero between calls by the kernels) and the rejection
-    verify, one per (device, stream) so concurrent streams never share it."""
+    verify, one per (device, stream) so concurrent streams never share it.
+
+    A call recorded into a graph gets memory of its own, which the graph's private
+    pool holds: a shared buffer would be freed under the graph when a later call
+    grows it, and shared with every other graph captured on the stream; one first
+    made under capture would, kept here, be handed to eager calls though nothing
+    has run yet. Captures that torch does not allocate a private pool for (begun
+    by other means than torch.cuda.CUDAGraph) must hand in buffers of their own."""
 
     def __init__(self) -> None:
         self._partials = {}
@@ -861,8 +868,6 @@ class Workspace:
         if floats <= 0:
             return None
         if torch.cuda.is_current_stream_capturing():
-            # the graph's own: a shared buffer would be freed under it when a later call
-            # grows it, and shared with every other graph captured on this stream
             return torch.empty(floats, dtype=torch.float32, device=device)
         dev = torch.device(device)
         key = (dev.index, _stream(dev))
@@ -875,6 +880,8 @@ class Workspace:
     def verify(self, nbytes: int, device, stream: Optional[int] = None) -> torch.Tensor:
         """mf_spec_verify's scratch, kept between calls (``stream``: the raw
         handle of the device's current stream, when the caller has it)."""
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(nbytes, dtype=torch.uint8, device=device)
         dev = device if isinstance(device, torch.device) else torch.device(device)
         key = (dev.index, _stream(dev) if stream is None else stream)
         buf = self._verify.get(key)
@@ -886,6 +893,8 @@ class Workspace:
     def counters(self, n: int, device) -> Optional[torch.Tensor]:
         if n <= 0:
             return None
+        if torch.cuda.is_current_stream_capturing():  # zeroed by a kernel that the graph replays
+            return torch.zeros(n, dtype=torch.int32, device=device)
         dev = torch.device(device)
         key = (dev.index, _stream(dev))
         buf = self._counters.get(key)
