@@ -1008,6 +1008,8 @@ class _Plan:
             return
         if plan.sliced:
             raise ValueError("scored attention takes per-range plans (mf_attention_plan)")
+        if plan.items.device != device:
+            raise ValueError(f"the plan is on {plan.items.device}, the query on {device}")
         self.narrow, self.wide, self.merges = plan.n_narrow, plan.n_wide, plan.n_merges
         self.counts = None
         self.partials = partials if partials is not None else _WORKSPACE.partials(plan.partials_floats, device)
@@ -1028,32 +1030,43 @@ def _launch(device: torch.device, what: str, fn, *args) -> None:
         _check(status, what)
 
 
-def _index_tensors(device: torch.device, block_tables, cu_seqlens, kv_lens, positions) -> None:
-    index = device.index
+def _index_tensors(q_rows: torch.Tensor, block_tables, cu_seqlens, kv_lens, positions, row_map=None,
+                   pool_lens=None) -> None:
+    index = q_rows.get_device()
     for name, t, dt in (("block_tables", block_tables, torch.int32), ("cu_seqlens", cu_seqlens, torch.int32),
-                        ("kv_lens", kv_lens, torch.int32), ("positions", positions, torch.int64)):
+                        ("kv_lens", kv_lens, torch.int32), ("positions", positions, torch.int64),
+                        ("row_map", row_map, torch.int32), ("pool_lens", pool_lens, torch.int32)):
+        if t is None:
+            continue
         if t.dtype != dt or not t.is_contiguous():
             raise TypeError(f"{name} must be a contiguous {dt} tensor")
         if t.get_device() != index:
-            raise ValueError(f"{name} is on {t.device}, the query on {device}")
+            raise ValueError(f"{name} is on {t.device}, the query on {q_rows.device}")
 
 
 def _paged_attention_scored(scoring: Scoring, q_rows, out_rows, pool, block_tables, cu_seqlens, kv_lens, positions,
                             plan, scale, num_kv_heads, row_map=None, pool_lens=None, nk=None, nv=None,
                             slot_mapping=None, partials=None) -> None:
+    dev = q_rows.device
     if pool_lens is not None:
         if nk is None or nv is None:
             raise ValueError("pool_lens needs the in-flight new_k_rows/new_v_rows")
-        require_device(pool_lens, nk, nv)
+        if pool_lens.numel() != kv_lens.numel():
+            raise ValueError(f"{pool_lens.numel()} pool_lens for {kv_lens.numel()} sequences")
+        for name, x in (("new_k_rows", nk), ("new_v_rows", nv)):
+            _rows_ok(x, name)
+            if x.dtype != pool.k.dtype or x.shape[1:] != (pool.num_heads, pool.head_dim) or x.device != dev:
+                raise ValueError(f"{name} must be rows of {pool.num_heads} heads x {pool.head_dim} in {pool.k.dtype} on "
+                                 f"{dev}, got {tuple(x.shape)} in {x.dtype} on {x.device}")
         if not same_layout(nk, nv):
             raise ValueError("in-flight K and V rows must share strides")
-    dev = q_rows.device
     if out_rows.shape != q_rows.shape or q_rows.shape[1:] != (q_rows.shape[1], pool.head_dim) \
             or num_kv_heads != pool.num_heads:
         raise ValueError(f"query {tuple(q_rows.shape)}, output {tuple(out_rows.shape)} and {num_kv_heads} kv heads do "
                          f"not match a pool of {pool.num_heads} heads x {pool.head_dim}")
-    if not dev == out_rows.device == pool.k.device == block_tables.device == positions.device:
-        raise ValueError(f"query, output, pool and index tensors must be on one device, the query is on {dev}")
+    if not dev == out_rows.device == pool.k.device:
+        raise ValueError(f"query, output and pool must be on one device, the query is on {dev}")
+    _index_tensors(q_rows, block_tables, cu_seqlens, kv_lens, positions, row_map, pool_lens)
     p = _Plan(plan, dev, partials)
     mods = scoring.struct(q_rows.shape[1], kv_lens.numel(), dev)
     bt_stride = block_tables.shape[1] if block_tables.dim() == 2 else 0
@@ -1089,7 +1102,7 @@ def _paged_attention4(scoring, q_rows, out_rows, pool: Pool4View, block_tables, 
                       scale, num_kv_heads, row_map=None, partials=None) -> None:
     _check4(q_rows, out_rows, pool, num_kv_heads)
     dev = q_rows.device
-    _index_tensors(dev, block_tables, cu_seqlens, kv_lens, positions)
+    _index_tensors(q_rows, block_tables, cu_seqlens, kv_lens, positions, row_map)
     p = _Plan(plan, dev, partials)
     scoring = _scored(scoring)
     mods = scoring.struct(q_rows.shape[1], kv_lens.numel(), dev) if scoring is not None else None
@@ -1118,7 +1131,10 @@ def paged_attention_kv_write(q_rows: torch.Tensor, out_rows: torch.Tensor, pool:
     pool. Row cu_seqlens[s] + i must be sequence s's new token at position
     kv_lens[s] - q_len[s] + i. ``plan`` is an AttentionPlan or a CountedPlan
     (graph capture). Same pool contents and output as ``kv_write`` followed by
-    ``paged_attention`` (with the same ``scoring``)."""
+    ``paged_attention`` (with the same ``scoring``). Not for a pool held in 4 bits,
+    whose rows are rounded before anything attends to them (``kv4_write``)."""
+    if isinstance(pool, Pool4View):
+        raise ValueError("a 4-bit pool takes no write in the attention launch: kv4_write, then paged_attention")
     _rows_ok(q_rows, "q_rows")
     _rows_ok(out_rows, "out_rows")
     _rows_ok(new_k_rows, "new_k_rows")
