@@ -41,6 +41,11 @@ __device__ __forceinline__ int block_of(const Attn4Args& a, int t) {
     return a.tpb == 1 ? t : (int)__umulhi((uint32_t)t, a.tpb_magic);
 }
 
+// Two softmax weights for the product with V, in the launch's 16-bit type, which the matrix
+// instructions take both operands in. Rounding them (at most 2^-8 of a weight in bf16, 2^-11
+// in fp16) is what the output's error has over one whose weights stay in 32 bits: 0.0022 of
+// its norm against 0.0017 in bf16, 0.00025 against 0.00021 in fp16. The sums of weights and
+// outputs are fp32.
 template <int DT>
 __device__ __forceinline__ uint32_t pack2(float x, float y) {
     if constexpr (DT == MF_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){x, y}, bf16x2));
