@@ -73,7 +73,8 @@ class _VarlenBinding:
     pool_lens[s] are the layer's in-flight key/value rows, not pool slots. A
     host sequence is uploaded with the rest of the metadata; a device tensor
     must already be in the grouped sequence order. ``longest`` is the pass's
-    longest context, ``window`` the shortest sliding window its layers named.
+    longest context where known (else found when a layer has a sliding window),
+    ``window`` the shortest sliding window its layers named.
     """
 
     __slots__ = ("pool", "block_tables", "seq_ids", "positions", "block_wise", "used", "_meta",
@@ -91,14 +92,13 @@ class _VarlenBinding:
         self.num_rows = len(self.seq_ids)
         self.timer = None  # a sampled pass's event record (engine telemetry)
         self.write_slots = None
-        self.longest = max((int(p) for p in self.positions), default=-1) + 1
+        self.longest = None
         self.window = None
 
     @classmethod
     def from_packed(cls, pool, meta: dict, num_rows: int, pool_lens: Optional[torch.Tensor] = None,
                     write_slots: Optional[torch.Tensor] = None, longest: Optional[int] = None):
-        """A prepared binding (``longest`` None: read from the device if a layer
-        has a sliding window). ``write_slots`` (the step's slot_mapping, with a
+        """A prepared binding. ``write_slots`` (the step's slot_mapping, with a
         cache made by ``VarlenPackedCache.from_slot_mapping(...,
         write_in_attention=True)``): every layer's attention launch also writes
         the new K/V rows it is handed into the pool and reads each sequence's
@@ -122,11 +122,12 @@ class _VarlenBinding:
 
     def check_window(self, window: Optional[int]) -> None:
         """A layer of this pass names a sliding window: refused where a context is longer."""
-        if not window:
+        if not window or window < 0:
             return
         self.window = min(int(window), self.window or int(window))
-        longest = self.longest if self.longest is not None else int(self._meta["kv_lens"].max())
-        _check_window(window, longest)
+        if self.longest is None:
+            self.longest = int(max(self.positions)) + 1 if self.positions else int(self._meta["kv_lens"].max())
+        _check_window(window, self.longest)
 
     def meta(self, num_q_heads: int, head_dim: int, dtype: torch.dtype, device, scored: bool = False) -> dict:
         """``scored``: the layer caps its scores, which slice plans do not serve (a
@@ -187,7 +188,7 @@ class _VarlenBinding:
 def _check_window(window: Optional[int], context: int) -> None:
     """The paged kernels attend to a row's whole context, which is what a layer with
     a sliding window does only while the context is no longer than the window."""
-    if window and context > window:
+    if window and 0 < window < context:
         raise ValueError(f"a layer attends within a sliding window of {window} keys, which the paged kernels do not "
                          f"serve past it: the context has {context}")
 
@@ -196,7 +197,7 @@ def attention_window(config) -> Optional[int]:
     """The sliding window that some layer of a model with this config attends within, None for none."""
     window = getattr(config, "sliding_window", None)
     kinds = getattr(config, "layer_types", None)
-    if not window or (kinds is not None and "sliding_attention" not in kinds):
+    if not window or window < 0 or (kinds is not None and "sliding_attention" not in kinds):
         return None
     return int(window)
 
@@ -308,6 +309,8 @@ def paged_attention_forward(module: Any, query: torch.Tensor, key: torch.Tensor,
     layer with a sliding window passes ``sliding_window``, and the paged routes
     refuse a context longer than it (the eager one masks it)."""
     softcap, window = kwargs.get("softcap"), kwargs.get("sliding_window")
+    if window is not None and window < 0:  # some configs' way to say none
+        window = None
     varlen = _current_varlen()
     if varlen is not None:
         varlen.check_window(window)

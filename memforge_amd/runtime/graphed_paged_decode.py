@@ -163,9 +163,9 @@ class GraphedPagedDecoder:
 
     def _stage(self, bk: _Bucket, tokens, ctx_lens, tables) -> None:
         n, b, mb = len(tokens), bk.b, self.max_blocks
-        # the layers' check for their sliding windows, which a replay does not run
-        bk.binding.longest = max(int(c) for c in ctx_lens) + 1
-        bk.binding.check_window(bk.binding.window)
+        if bk.graph is None or bk.binding.window:  # the layers' check of their windows, which a replay does not run
+            bk.binding.longest = max(int(c) for c in ctx_lens) + 1
+            bk.binding.check_window(bk.binding.window)
         if bk.copied is not None:
             bk.copied.synchronize()  # the previous step's copy has left the pinned buffer
         h = bk.host.numpy()

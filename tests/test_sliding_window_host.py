@@ -36,6 +36,7 @@ def test_a_window_no_context_reaches_is_not_refused():
     binding = backend._VarlenBinding(None, [], [0, 0], [62, 63])
     binding.check_window(64)
     binding.check_window(None)
+    binding.check_window(-1)
     binding.check_window(200)
     assert binding.window == 64  # the shortest named: what a captured step's later contexts are checked against
     with pytest.raises(ValueError):
@@ -67,6 +68,7 @@ def test_windows_of_a_config():
 
     assert backend.attention_window(config()) is None
     assert backend.attention_window(config(sliding_window=None)) is None
+    assert backend.attention_window(config(sliding_window=-1)) is None
     assert backend.attention_window(config(sliding_window=128)) == 128
     assert backend.attention_window(config(sliding_window=128, layer_types=["full_attention"] * 2)) is None
     assert backend.attention_window(config(sliding_window=128, layer_types=["full_attention", "sliding_attention"])) == 128
