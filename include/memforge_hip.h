@@ -578,6 +578,92 @@ int mf_spec_verify(int num_rows, int num_draft, int vocab,
                    int32_t* out_num_accepted, void* workspace, int64_t workspace_bytes,
                    mf_stream_t stream);
 
+/* ------------------------------------------------- block tables on the device
+ * A batch's block tables kept on the device. Request s owns row s of `tables`
+ * (int32, `max_blocks` entries, row stride `table_stride`), of which the first
+ * held[s] are its blocks, and lens[s] tokens (all int32, device). Unused blocks
+ * are the first *free_count entries of `free_blocks` (capacity `free_capacity`),
+ * a stack whose top is the last.
+ *
+ * mf_tables_extend grows request s by new_tokens[s] (int32; negative: none). In
+ * request order each takes the blocks it lacks from the stack's top. A request
+ * is refused, and keeps what it has, when its table row is too short, its rows
+ * end past max_rows, or the blocks asked for up to and including it (those of
+ * requests that are refused for the first two reasons not counted) are more than
+ * the stack holds and it lacks any. Outputs: cu_seqlens (num_requests + 1) sums of
+ * new_tokens, kv_lens the new lengths, *refused their number, and for every row
+ * r < max_rows slot_mapping / positions (int64): row cu_seqlens[s] + i is the
+ * i-th new token of request s, at position lens[s] + i and in slot
+ * tables[s][pos / block_size] * block_size + pos % block_size, or -1 if s is
+ * refused; rows past the last have slot -1 and position 0. With `rows` (int32,
+ * row stride rows_stride, rows_width entries) token i of request s is row
+ * rows[s][i] instead (negative or past max_rows: none; no row twice), every other
+ * row has slot -1, and a request of more than rows_width new tokens is refused.
+ *
+ * mf_tables_truncate cuts request s back to min(lens[s], lengths[s]) tokens
+ * (negative: 0) and gives back the blocks it then does not need, in an order
+ * that makes the stack after an extend what it was before; their table entries
+ * become 0.
+ *
+ * arrivals: one uint32 that is 0 before the call and after it. Both are one
+ * launch (extend with `rows`: two), at most 4096 requests.
+ * Beyond PagedKVPool.slot_indices (memforge_ml/runtime/kv_pool.py:92-110) and the
+ * host's BlockAllocator (engine/include/memforge/block_allocator.hpp:19-161).
+ */
+int mf_tables_extend(int32_t* tables, int64_t table_stride, int max_blocks, int32_t* lens,
+                     int32_t* held, int32_t* free_blocks, int64_t free_capacity,
+                     int32_t* free_count, const int32_t* new_tokens, int num_requests,
+                     int block_size, int64_t max_rows, const int32_t* rows,
+                     int64_t rows_stride, int rows_width, int64_t* slot_mapping,
+                     int64_t* positions, int32_t* cu_seqlens, int32_t* kv_lens,
+                     int32_t* refused, uint32_t* arrivals, mf_stream_t stream);
+int mf_tables_truncate(int32_t* tables, int64_t table_stride, int max_blocks, int32_t* lens,
+                       int32_t* held, int32_t* free_blocks, int64_t free_capacity,
+                       int32_t* free_count, const int32_t* lengths, int num_requests,
+                       int block_size, uint32_t* arrivals, mf_stream_t stream);
+
+/* ------------------------------------------------------- accepted path of trees
+ * Rows cu_nodes[s] .. cu_nodes[s+1] - 1 (int32, at most max_nodes <=
+ * MF_TREE_MAX_NODES of them count) are the nodes of sequence s's tree: node i's
+ * parent is node parents[row] < i of the same tree (anything else: none), its
+ * token tokens[row], and targets[row] the token that the target drew from the
+ * logits at it. The accepted path starts at node 0 and goes on from each node to
+ * its first child whose token is the node's target. Outputs, max_nodes to a
+ * sequence: path (int32 rows, -1 past the path's end), out_tokens (int64, the
+ * targets along it: the tokens the round emits; -1 past its end), and count.
+ * A sequence without nodes, or whose rows are not within num_rows, has count 0.
+ * The tree form of RejectionSampler.verify_tokens
+ * (memforge_ml/speculative/rejection_sampler.py:28-83) for targets drawn beforehand.
+ */
+#define MF_TREE_MAX_NODES 1024
+int mf_tree_accept(const int64_t* tokens, const int64_t* targets, const int32_t* parents,
+                   const int32_t* cu_nodes, int num_seqs, int64_t num_rows, int max_nodes,
+                   int32_t* path, int64_t* out_tokens, int32_t* count, mf_stream_t stream);
+
+/* ------------------------------------------------------------------- sampling
+ * One token for each of `num_rows` rows of `vocab` logits (row r at logits + r *
+ * stride_row, any stride and alignment of the type) from uniforms[r] in [0, 1)
+ * (fp32; clamped to it). Tokens are ranked by (logit descending, index ascending)
+ * and weighted by w = exp((logit - largest) / T), the largest logit's being 1 also
+ * where it is infinite; a NaN logit counts as -infinity. Kept are the first top_k
+ * of the ranking (<= 0: all), of those the ones with at most top_p of their mass
+ * before them (>= 1: all), and w >= min_p (<= 0: all); the first token always is.
+ * tokens[r] (int64) is the first kept token whose inclusive mass, in rank order,
+ * exceeds uniforms[r] times the kept mass, and probs[r] (fp32, or NULL) its share
+ * of that mass. T <= 0 or NaN: the first largest logit, share 1. The four settings
+ * are fp32 / int32 arrays of num_rows, or NULL for the scalar behind each.
+ * Weights below e^-32 of the largest count as 0; sums are exact to 2^-30 of a
+ * weight or better, so tokens are those of 64-bit arithmetic but where the draw
+ * falls that close to a border.
+ * Beyond sampling.sample_logits (memforge_ml/runtime/sampling.py:33-75).
+ */
+#define MF_SAMPLE_MAX_VOCAB (1 << 20)
+int mf_sample(const void* logits, int dtype, int64_t stride_row, int num_rows, int vocab,
+              const float* uniforms, const float* temperature, float temperature0,
+              const int32_t* top_k, int top_k0, const float* top_p, float top_p0,
+              const float* min_p, float min_p0, int64_t* tokens, float* probs,
+              mf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

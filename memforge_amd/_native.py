@@ -100,6 +100,12 @@ _SIGNATURES = {
     "mf_spec_verify": (_c_int, [_c_int, _c_int, _c_int, _vp, _vp, _c_i64, _c_i64, _vp, _c_int,
                                 _c_i64, _c_i64, _c_f32, _c_int, _vp, _vp, _c_i64, _vp, _vp, _vp,
                                 _vp, _vp, _c_i64, _vp]),
+    "mf_tables_extend": (_c_int, [_vp, _c_i64, _c_int, _vp, _vp, _vp, _c_i64, _vp, _vp, _c_int, _c_int, _c_i64,
+                                  _vp, _c_i64, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "mf_tables_truncate": (_c_int, [_vp, _c_i64, _c_int, _vp, _vp, _vp, _c_i64, _vp, _vp, _c_int, _c_int, _vp, _vp]),
+    "mf_tree_accept": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_i64, _c_int, _vp, _vp, _vp, _vp]),
+    "mf_sample": (_c_int, [_vp, _c_int, _c_i64, _c_int, _c_int, _vp, _vp, _c_f32, _vp, _c_int, _vp, _c_f32, _vp,
+                           _c_f32, _vp, _vp, _vp]),
 }
 
 _LIB: Optional[ctypes.CDLL] = None
@@ -1537,3 +1543,77 @@ def spec_verify(draft_tokens: torch.Tensor, draft_probs: torch.Tensor, target_lo
         base + 4 * (n + B), ws.data_ptr(), ws_bytes, stream,
     ), "mf_spec_verify")
     return VerifyResult.split(out, B, K)
+
+
+def check_index(name: str, x: torch.Tensor, dtype: torch.dtype, device: torch.device, shape: Optional[tuple] = None) -> None:
+    """An index tensor of a call: its type, its device, contiguous, and its shape when given."""
+    if x.dtype != dtype or not x.is_contiguous():
+        raise TypeError(f"{name} must be a contiguous {dtype} tensor, got {x.dtype} with strides {x.stride()}")
+    if shape is not None and tuple(x.shape) != shape:
+        raise ValueError(f"{name} must be of shape {shape}, got {tuple(x.shape)}")
+    if x.device != device:
+        raise ValueError(f"{name} is on {x.device}, the call's other tensors on {device}")
+
+
+# ---------------------------------------------------------------- sampling
+
+SAMPLE_MAX_VOCAB = 1 << 20
+
+
+def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
+           min_p=0.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """mf_sample: (tokens int64, probs fp32), one per row of ``logits`` ((rows, vocab),
+    the last axis contiguous). Settings are numbers, or tensors with one per row
+    (fp32; top_k int32)."""
+    require_device(logits, uniforms)
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError(f"logits must be (rows, vocab) with a contiguous vocabulary axis, got {tuple(logits.shape)} "
+                         f"with strides {logits.stride()}")
+    rows, vocab = logits.shape
+    if not 1 <= vocab <= SAMPLE_MAX_VOCAB:
+        raise ValueError(f"a vocabulary holds 1 to {SAMPLE_MAX_VOCAB} tokens, got {vocab}")
+    dev = logits.device
+    check_index("uniforms", uniforms, torch.float32, dev, (rows,))
+    settings = []
+    for name, x, dt in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                        ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if isinstance(x, torch.Tensor):
+            require_device(x)
+            check_index(name, x, dt, dev, (rows,))
+            settings += [x.data_ptr(), 0]
+        elif dt == torch.int32:
+            settings += [None, min(int(x), SAMPLE_MAX_VOCAB) if x > 0 else 0]
+        else:
+            if x != x:
+                raise ValueError(f"{name} must be a number, got {x}")
+            settings += [None, float(x)]
+    tokens = torch.empty(rows, dtype=torch.int64, device=dev)
+    probs = torch.empty(rows, dtype=torch.float32, device=dev)
+    _launch(dev, "mf_sample", lib().mf_sample, logits.data_ptr(), dtype_code(logits.dtype), logits.stride(0), rows,
+            vocab, uniforms.data_ptr(), *settings, tokens.data_ptr(), probs.data_ptr())
+    return tokens, probs
+
+
+# ---------------------------------------------------- trees of drafted tokens
+
+TREE_MAX_NODES = 1024
+
+
+def tree_accept(tokens: torch.Tensor, targets: torch.Tensor, parents: torch.Tensor, cu_nodes: torch.Tensor,
+                max_nodes: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """mf_tree_accept: (path int32 (B, max_nodes), tokens int64 (B, max_nodes), count int32 (B))."""
+    require_device(tokens, targets, parents, cu_nodes)
+    dev, rows, seqs = parents.device, parents.numel(), cu_nodes.numel() - 1
+    for name, x, dt, n in (("tokens", tokens, torch.int64, rows), ("targets", targets, torch.int64, rows),
+                           ("parents", parents, torch.int32, rows), ("cu_nodes", cu_nodes, torch.int32, seqs + 1)):
+        check_index(name, x, dt, dev, (n,))
+    if seqs < 0:
+        raise ValueError("cu_nodes must have one more entry than sequences")
+    if not 1 <= max_nodes <= TREE_MAX_NODES:
+        raise ValueError(f"max_nodes must be 1 to {TREE_MAX_NODES}, got {max_nodes}")
+    path = torch.empty((seqs, max_nodes), dtype=torch.int32, device=dev)
+    out = torch.empty((seqs, max_nodes), dtype=torch.int64, device=dev)
+    count = torch.empty(seqs, dtype=torch.int32, device=dev)
+    _launch(dev, "mf_tree_accept", lib().mf_tree_accept, tokens.data_ptr(), targets.data_ptr(), parents.data_ptr(),
+            cu_nodes.data_ptr(), seqs, rows, max_nodes, path.data_ptr(), out.data_ptr(), count.data_ptr())
+    return path, out, count

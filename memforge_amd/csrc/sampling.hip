@@ -1,0 +1,836 @@
+// One token per row of logits from a given uniform number: temperature, top-k,
+// top-p and min-p, then a draw by rank.
+//
+// A row's tokens are ranked by (logit descending, index ascending) and weighted by
+// w = exp((logit - largest) / T). Every filter keeps a prefix of that ranking:
+// top-k its first k, top-p the tokens with at most p of the first k's mass before
+// them, min-p those of at least p of the largest weight. The drawn token is the
+// first whose inclusive mass exceeds u times the kept mass. So all of it is
+// positions in one running sum, and no sort is needed: the row is binned by
+// logit, finely (256 bins to a factor e of weight), the bins in which a boundary
+// lies are found from the bins' counts and masses, and only those bins' tokens
+// are ranked.
+//
+// Exactness. A boundary between two tokens must fall where 64-bit arithmetic puts
+// it, in sums over a whole vocabulary. A bin's mass is T_b (n - sum q) with T_b the
+// weight at the bin's top, n its count and q = 1 - w / T_b < 2^-8. The q are formed
+// in fp64 by a polynomial (error 2^-47) and added as integers, count and sum in one
+// 64-bit LDS add, so the sums do not depend on their order. One is rounded to
+// 2^-QS, QS = 71 - 2 log2(vocabulary), at most 40: 2^-37 at 131,072 tokens.
+// Weights below e^-32 of the largest logit seen first (1e-14) count as nothing.
+//
+// Bins reach from 28 factors e above the largest logit of the row's first piece to
+// 32 below it, so one pass serves whatever follows; a row with a logit above that
+// range is binned again from its true maximum.
+#include <algorithm>
+
+#include "mf_common.h"
+
+namespace mf {
+namespace {
+
+constexpr int kThreads = 1024;
+constexpr int kOwn = 15;                 // consecutive bins of one thread (odd: no LDS bank twice)
+constexpr int kBins = kOwn * kThreads;
+constexpr double kPerE = 256.0;          // bins to a factor e of weight
+constexpr int kTop = kBins - 32 * 256;   // the bin of the reference logit
+constexpr int kList = 2048;              // tokens of boundary bins that are ranked in LDS
+constexpr int kSegs = 128;               // boundary bins
+constexpr int kFirst = 8192;             // tokens of a row whose maximum is the reference
+
+struct SampleArgs {
+    const char* logits;
+    int64_t stride_row;
+    int vocab;
+    int num_rows;
+    const float* uniforms;
+    const float* temp;
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    float temp0, top_p0, min_p0;
+    int top_k0;
+    int count_shift;  // a bin's word: count << count_shift | sum of q * 2^qs
+    double q_scale, q_unit;  // 2^qs, 2^-qs
+    int64_t* tokens;
+    float* probs;
+};
+
+struct Seg {
+    double mass_before;  // of the bins before it
+    double top;          // T_b
+    uint64_t total;      // sum of its tokens' 2^qs (1 - q)
+    int bin, base, n, count_before, cursor;
+};
+
+// A bin that a search found (bin < 0: none).
+struct Found {
+    int bin, n, count_before;
+    double mass_before, mass;
+};
+
+struct Shared {
+    uint64_t words[kBins];   // the bins; then ranked[kList], mass[kList]
+    uint64_t list[kList];
+    uint8_t list_seg[kList];
+    Seg seg[kSegs];
+    double wave_mass[16];
+    int wave_count[16];
+    float wave_max[16];
+    unsigned long long best;
+    int found[4];
+    Found at[4];
+    int segs, listed;
+    double d0, d1;
+    uint64_t u0;
+    int i0;
+};
+
+template <int DT>
+__device__ __forceinline__ float value_of(uint32_t bits) {
+    const float v = bits_to_f32<DT>(bits);
+    return v == v ? v : -__builtin_huge_valf();  // NaN: never drawn
+}
+
+// f(index, logit) for the tokens [e0, e1) of a row, each by one of the
+// workgroup's threads: 16-byte loads from the first aligned token on.
+template <int DT, class F>
+__device__ __forceinline__ void scan_row(const char* row, int e0, int e1, F f) {
+    constexpr int ES = DT == MF_F32 ? 4 : 2, VE = 16 / ES;
+    const int tid = threadIdx.x;
+    auto one = [&](int i) {
+        f(i, value_of<DT>(ES == 4 ? ((const uint32_t*)row)[i] : (uint32_t)((const uint16_t*)row)[i]));
+    };
+    const int head = min((int)((16 - ((uintptr_t)(row + (int64_t)e0 * ES) & 15)) & 15) / ES, e1 - e0);
+    if (tid < head) one(e0 + tid);
+    const int v0 = e0 + head, nv = (e1 - v0) / VE;
+    const uint4* vec = (const uint4*)(row + (int64_t)v0 * ES);
+    uint4 next[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) next[u] = tid + u * kThreads < nv ? vec[tid + u * kThreads] : make_uint4(0, 0, 0, 0);
+    for (int v = tid; v < nv; v += 2 * kThreads) {
+        uint4 cur[2] = {next[0], next[1]};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int w = v + (2 + u) * kThreads;
+            if (w < nv) next[u] = vec[w];
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int w = v + u * kThreads;
+            if (w >= nv) break;
+            const uint32_t x[4] = {cur[u].x, cur[u].y, cur[u].z, cur[u].w};
+#pragma unroll
+            for (int k = 0; k < VE; ++k) {
+                const uint32_t bits = ES == 4 ? x[k] : (k & 1 ? x[k >> 1] >> 16 : x[k >> 1] & 0xffffu);
+                f(v0 + w * VE + k, value_of<DT>(bits));
+            }
+        }
+    }
+    const int tail = v0 + nv * VE;
+    if (tid < e1 - tail) one(tail + tid);
+}
+
+// Larger for a larger logit; -0 as 0.
+__device__ __forceinline__ uint32_t order_key(float v) {
+    const uint32_t u = __float_as_uint(v + 0.f);
+    return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+
+// A token's bin and q below the reference; false where its weight is nothing.
+struct Binner {
+    double ref, per, q_scale;
+    float ref_f;
+    __device__ __forceinline__ Binner(const SampleArgs& a, float reference, float temp)
+        : ref(reference), per(kPerE / (double)temp), q_scale(a.q_scale), ref_f(reference) {}
+    __device__ __forceinline__ bool place(float v, double& y) const {
+        y = v == ref_f ? (double)kTop : __builtin_fma(ref - (double)v, per, (double)kTop);
+        return y >= 0.0 && y < (double)kBins;
+    }
+    // 2^qs q, q = 1 - exp(-r / 256) for the part r in [0, 1) of y inside its bin
+    __device__ __forceinline__ uint32_t q_of(double y, int bin) const {
+        const double t = (y - (double)bin) * (1.0 / kPerE);
+        const double q = t * __builtin_fma(t, __builtin_fma(t, __builtin_fma(t, -1.0 / 24.0, 1.0 / 6.0), -0.5), 1.0);
+        return (uint32_t)__builtin_fma(q, q_scale, 0.5);
+    }
+};
+
+__device__ __forceinline__ double bin_top(int bin) { return exp((double)(kTop - bin) * (1.0 / kPerE)); }
+
+__device__ __forceinline__ float block_max(Shared& sh, float v) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.wave_max[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float m = sh.wave_max[0];
+#pragma unroll
+    for (int w = 1; w < kThreads / 64; ++w) m = fmaxf(m, sh.wave_max[w]);
+    return m;
+}
+
+__device__ __forceinline__ void clear_words(Shared& sh) {
+    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.words[i] = 0;
+}
+
+// Exclusive sums of the threads' counts and masses, and the totals.
+__device__ __forceinline__ void block_sums(Shared& sh, int& n, double& mass, int& n_all, double& mass_all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int ni = n;
+    double mi = mass;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int nu = __shfl_up(ni, o, 64);
+        const double mu = __shfl_up(mi, o, 64);
+        if (lane >= o) {
+            ni += nu;
+            mi += mu;
+        }
+    }
+    double before = __shfl_up(mi, 1, 64);
+    if (lane == 0) before = 0.0;
+    __syncthreads();
+    if (lane == 63) {
+        sh.wave_count[wave] = ni;
+        sh.wave_mass[wave] = mi;
+    }
+    __syncthreads();
+    int nb = 0;
+    double mb = 0.0;
+    n_all = 0;
+    mass_all = 0.0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) {
+        if (w == wave) {
+            nb = n_all;
+            mb = mass_all;
+        }
+        n_all += sh.wave_count[w];
+        mass_all += sh.wave_mass[w];
+    }
+    n = nb + ni - n;
+    mass = mb + before;
+}
+
+// The bins of one thread: counts and masses by walking its kOwn words.
+struct Owner {
+    int count_shift;
+    double q_scale, q_unit;
+    int count_before;      // of the bins before this thread's
+    double mass_before, mass_end;
+    int count_end;
+    double top0;           // T_b of its first bin
+
+    __device__ __forceinline__ static double step() { return 0.9961013694701175; }  // exp(-1/256)
+    __device__ __forceinline__ int count(uint64_t w) const { return (int)(w >> count_shift); }
+    __device__ __forceinline__ uint64_t parts(uint64_t w) const {
+        const uint64_t n = w >> count_shift;
+        return n * (uint64_t)q_scale - (w & ((1ull << count_shift) - 1));
+    }
+    // g(bin, word, T_b, count before, mass before, mass): true ends the walk
+    template <class G>
+    __device__ __forceinline__ void walk(const Shared& sh, G g) const {
+        double top = top0, before = mass_before;
+        int n = count_before;
+        for (int j = 0; j < kOwn; ++j) {
+            const int bin = (int)threadIdx.x * kOwn + j;
+            const uint64_t w = sh.words[bin];
+            if (w) {
+                const double mass = top * ((double)parts(w) * q_unit);
+                if (g(bin, w, top, n, before, mass)) return;
+                before += mass;
+                n += count(w);
+            }
+            top *= step();
+        }
+    }
+};
+
+// The first bin whose inclusive mass exceeds x (COUNT: whose inclusive count does),
+// into sh.at[k]; none: bin -1. All threads call it.
+template <bool COUNT>
+__device__ __forceinline__ void find(Shared& sh, const Owner& o, double x, int k) {
+    if (threadIdx.x == 0) {
+        sh.found[k] = kBins;
+        sh.at[k].bin = -1;
+    }
+    __syncthreads();
+    Found f;
+    f.bin = -1;
+    if (COUNT ? (double)o.count_end > x : o.mass_end > x) {
+        o.walk(sh, [&](int bin, uint64_t w, double, int n, double before, double mass) {
+            if (COUNT ? (double)(n + o.count(w)) > x : before + mass > x) {
+                f = Found{bin, o.count(w), n, before, mass};
+                return true;
+            }
+            return false;
+        });
+    }
+    if (f.bin >= 0) atomicMin(&sh.found[k], f.bin);
+    __syncthreads();
+    if (f.bin >= 0 && f.bin == sh.found[k]) sh.at[k] = f;
+    __syncthreads();
+}
+
+// A prefix of the ranking: whole bins before `bin`, then the first n tokens of it.
+struct Limit {
+    int bin, n;
+    double mass;  // of the prefix
+    __device__ __forceinline__ bool before(const Limit& o) const { return bin < o.bin || (bin == o.bin && n < o.n); }
+};
+
+// Boundary bins too full for the list: the token at which a running sum over the
+// bin's ranking passes a target is found digit by digit, from 64-bit rank keys
+// (logit key inverted, then index) of which every level bins the next 12 bits. Six
+// passes over the row; rows of many equal logits and extreme temperatures.
+struct Ranked {
+    uint64_t key;          // of the token found
+    int before;            // tokens of the bin ranked before it
+    double parts_before;   // and their sum of 2^qs (1 - q)
+    double parts;          // its own
+    bool found;
+};
+
+__device__ __forceinline__ uint64_t parts_in(const SampleArgs& a, uint64_t w) {
+    return (w >> a.count_shift) * (uint64_t)a.q_scale - (w & ((1ull << a.count_shift) - 1));
+}
+
+template <int DT>
+__device__ Ranked descend(const SampleArgs& a, Shared& sh, const char* row, const Binner& bn, int bin, bool by_count,
+                          double target) {
+    // target: tokens (by_count) or parts; found is the first whose inclusive sum exceeds it
+    Ranked r{0, 0, 0.0, 0.0, true};
+    uint64_t prefix = 0;
+    for (int level = 0; level < 6; ++level) {
+        const int shift = level < 5 ? 52 - 12 * level : 0;
+        const int width = level < 5 ? 12 : 4;
+        __syncthreads();
+        for (int i = threadIdx.x; i < 4096; i += kThreads) sh.words[i] = 0;
+        __syncthreads();
+        scan_row<DT>(row, 0, a.vocab, [&](int i, float v) {
+            double y;
+            if (!bn.place(v, y) || (int)y != bin) return;
+            const uint64_t key = (uint64_t)~order_key(v) << 32 | (uint32_t)i;
+            if (level > 0 && (key >> (shift + width)) != prefix) return;
+            atomicAdd((unsigned long long*)&sh.words[(key >> shift) & ((1u << width) - 1)],
+                      (unsigned long long)((1ull << a.count_shift) + bn.q_of(y, bin)));
+        });
+        __syncthreads();
+        // four digits to a thread: the first whose inclusive sum passes the target, else the last
+        int n = 0, n_before, n_all;
+        double parts = 0.0, parts_before, parts_all;
+        uint64_t w[4];
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            w[d] = sh.words[4 * threadIdx.x + d];
+            n += (int)(w[d] >> a.count_shift);
+            parts += (double)parts_in(a, w[d]);
+        }
+        n_before = n;
+        parts_before = parts;
+        block_sums(sh, n_before, parts_before, n_all, parts_all);
+        if (threadIdx.x == 0) {
+            sh.found[0] = 4096;
+            sh.found[1] = -1;
+        }
+        __syncthreads();
+        n_before += r.before;
+        parts_before += r.parts_before;
+        int pick = 4096, last = -1, at_n = 0;
+        double at_parts = 0.0, own = 0.0, last_parts = 0.0, last_own = 0.0;
+        int last_n = 0;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            if (!w[d]) continue;
+            const int dn = (int)(w[d] >> a.count_shift);
+            const double dp = (double)parts_in(a, w[d]);
+            last = 4 * threadIdx.x + d;
+            last_n = n_before;
+            last_parts = parts_before;
+            last_own = dp;
+            if (pick == 4096 && (by_count ? (double)(n_before + dn) > target : parts_before + dp > target)) {
+                pick = last;
+                at_n = n_before;
+                at_parts = parts_before;
+                own = dp;
+            }
+            n_before += dn;
+            parts_before += dp;
+        }
+        if (pick < 4096) atomicMin(&sh.found[0], pick);
+        if (last >= 0) atomicMax(&sh.found[1], last);
+        __syncthreads();
+        const bool passed = sh.found[0] < 4096;
+        if (sh.found[1] < 0 || (level == 0 && !passed)) {
+            r.found = false;
+            return r;
+        }
+        const int digit = passed ? sh.found[0] : sh.found[1];
+        if (passed ? pick == digit : last == digit) {
+            sh.i0 = passed ? at_n : last_n;
+            sh.d0 = passed ? at_parts : last_parts;
+            sh.d1 = passed ? own : last_own;
+        }
+        __syncthreads();
+        prefix = prefix << width | (uint64_t)digit;
+        r.before = sh.i0;
+        r.parts_before = sh.d0;
+        r.parts = sh.d1;
+    }
+    r.key = prefix;
+    return r;
+}
+
+// The finish of one row, whose bins are in sh.words.
+template <int DT>
+__device__ void finish_row(const SampleArgs& a, Shared& sh, const char* row, int r, const Binner& bn, float largest,
+                           float temp) {
+    const int tid = threadIdx.x;
+    Owner own;
+    own.count_shift = a.count_shift;
+    own.q_scale = a.q_scale;
+    own.q_unit = a.q_unit;
+    own.count_before = 0;
+    own.mass_before = 0.0;
+    own.top0 = bin_top(tid * kOwn);
+    int n = 0;
+    double mass = 0.0;
+    own.walk(sh, [&](int, uint64_t w, double, int, double, double m) {
+        n += own.count(w);
+        mass += m;
+        return false;
+    });
+    int n_before = n, n_all;
+    double mass_before = mass, mass_all;
+    block_sums(sh, n_before, mass_before, n_all, mass_all);
+    own.count_before = n_before;
+    own.mass_before = mass_before;
+    own.count_end = n_before + n;
+    own.mass_end = mass_before + mass;
+
+    const int top_k = a.top_k ? a.top_k[r] : a.top_k0;
+    const double top_p = a.top_p ? a.top_p[r] : a.top_p0;
+    const double min_p = a.min_p ? a.min_p[r] : a.min_p0;
+    double u = a.uniforms[r];
+    u = u > 0.0 ? fmin(u, 1.0 - 0x1p-24) : 0.0;
+
+    // ---- the bins in which the boundaries lie. Exact masses need a bin's tokens:
+    // until then a boundary is an interval of bins.
+    const bool by_k = top_k > 0 && top_k < n_all;
+    const bool by_p = !(top_p >= 1.0);
+    const bool by_m = min_p > 0.0;
+    const int none = kBins;
+    // the least weight that min_p lets pass, in the bins' unit
+    const double least = largest == bn.ref_f ? min_p : min_p * exp((largest - bn.ref) * bn.per * (1.0 / kPerE));
+    int kb = none, p_lo = none, p_hi = none, mb = none;
+    double lo = mass_all, hi = mass_all;
+    if (by_k) {
+        find<true>(sh, own, (double)(top_k - 1), 0);
+        kb = sh.at[0].bin;
+        lo = sh.at[0].mass_before;
+        hi = lo + sh.at[0].mass;
+    }
+    const double p_of = top_p > 0.0 ? top_p : 0.0;
+    if (by_p) {
+        find<false>(sh, own, p_of * lo, 1);
+        find<false>(sh, own, p_of * hi, 2);
+        p_lo = sh.at[1].bin >= 0 ? sh.at[1].bin : none;
+        p_hi = sh.at[2].bin >= 0 ? sh.at[2].bin : kBins - 1;
+        if (p_lo != none) lo = fmin(lo, sh.at[1].mass_before);
+        if (sh.at[2].bin >= 0) hi = fmin(hi, sh.at[2].mass_before + sh.at[2].mass);
+    }
+    if (by_m) {
+        // w >= min_p: places down to -ln(min_p) below the largest logit
+        double y;
+        bn.place(largest, y);
+        const double edge = y - log(min_p) * kPerE;
+        mb = edge < 0.0 ? 0 : edge < (double)kBins ? (int)edge : none;
+        if (min_p > 1.0) mb = (int)y;
+        if (mb != none) {
+            // the masses around that bin
+            if (tid == 0) sh.d0 = -1.0;
+            __syncthreads();
+            if (tid == mb / kOwn) {
+                double before = own.mass_before, m = 0.0;
+                own.walk(sh, [&](int bin, uint64_t, double, int, double b, double mm) {
+                    if (bin < mb) before = b + mm;
+                    if (bin == mb) m = mm;
+                    return bin >= mb;
+                });
+                sh.at[3] = Found{mb, 0, 0, before, m};
+            }
+            __syncthreads();
+            lo = fmin(lo, sh.at[3].mass_before);
+            hi = fmin(hi, sh.at[3].mass_before + sh.at[3].mass);
+        }
+    }
+    find<false>(sh, own, 0.0, 0);  // the first bin that holds anything
+    const int first_bin = sh.at[0].bin;
+    find<false>(sh, own, u * lo, 1);
+    find<false>(sh, own, u * hi, 2);
+    const int d_lo = sh.at[1].bin >= 0 ? sh.at[1].bin : 0;
+    const int d_hi = sh.at[2].bin >= 0 ? sh.at[2].bin : kBins - 1;
+
+    // ---- their tokens, bin by bin
+    if (tid == 0) {
+        sh.segs = 0;
+        sh.listed = 0;
+    }
+    __syncthreads();
+    auto wanted = [&](int bin) {
+        return bin == kb || (bin >= p_lo && bin <= p_hi) || bin == mb || (bin >= d_lo && bin <= d_hi) || bin == first_bin;
+    };
+    own.walk(sh, [&](int bin, uint64_t w, double top, int nb, double before, double) {
+        if (wanted(bin)) {
+            const int k = atomicAdd(&sh.segs, 1), base = atomicAdd(&sh.listed, own.count(w));
+            if (k < kSegs) sh.seg[k] = Seg{before, top, own.parts(w), bin, base, own.count(w), nb, 0};
+        }
+        return false;
+    });
+    __syncthreads();
+    const int segs = sh.segs, listed = sh.listed;
+    const bool fits = segs <= kSegs && listed <= kList;
+    auto seg_of = [&](int bin) -> int {
+        for (int k = 0; k < segs; ++k)
+            if (sh.seg[k].bin == bin) return k;
+        return -1;
+    };
+    Limit limit{none, 0, mass_all};
+    if (fits) {
+        // bins' words become their segment + 1 (0: not wanted)
+        for (int j = 0; j < kOwn; ++j) sh.words[tid * kOwn + j] = 0;
+        __syncthreads();
+        if (tid < segs) sh.words[sh.seg[tid].bin] = tid + 1;
+        __syncthreads();
+        int b0 = kBins, b1 = -1;
+        for (int k = 0; k < segs; ++k) {
+            b0 = min(b0, sh.seg[k].bin);
+            b1 = max(b1, sh.seg[k].bin);
+        }
+        const double y0 = b0, y1 = b1 + 1;
+        scan_row<DT>(row, 0, a.vocab, [&](int i, float v) {
+            double y;
+            bn.place(v, y);
+            if (!(y >= y0 && y < y1)) return;
+            const int k = (int)sh.words[(int)y] - 1;
+            if (k < 0) return;
+            const int at = sh.seg[k].base + atomicAdd(&sh.seg[k].cursor, 1);
+            sh.list[at] = (uint64_t)~order_key(v) << 32 | (uint32_t)i;
+            sh.list_seg[at] = (uint8_t)k;
+        });
+        __syncthreads();
+        // ---- ranked inside their bins, with the parts before each
+        uint64_t* ranked = sh.words;
+        uint64_t* before = sh.words + kList;
+        auto parts_of = [&](uint64_t key, int bin) -> uint64_t {
+            double y;
+            bn.place(key_value(~(uint32_t)(key >> 32)), y);
+            return (uint64_t)a.q_scale - bn.q_of(y, bin);
+        };
+        uint64_t keys[kList / kThreads], sums[kList / kThreads];
+        int ranks[kList / kThreads];
+#pragma unroll
+        for (int c = 0; c < kList / kThreads; ++c) {
+            const int i = tid + c * kThreads;
+            if (i >= listed) break;
+            const Seg& s = sh.seg[sh.list_seg[i]];
+            keys[c] = sh.list[i];
+            ranks[c] = 0;
+        }
+        // each token's own parts, so that the ranking loop only adds
+        uint64_t* parts = sh.words + 2 * kList;
+#pragma unroll
+        for (int c = 0; c < kList / kThreads; ++c) {
+            const int i = tid + c * kThreads;
+            if (i < listed) parts[i] = parts_of(keys[c], sh.seg[sh.list_seg[i]].bin);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < kList / kThreads; ++c) {
+            const int i = tid + c * kThreads;
+            if (i >= listed) break;
+            const Seg& s = sh.seg[sh.list_seg[i]];
+            const int j0 = s.base, j1 = s.base + s.n;
+            int rank = 0;
+            uint64_t sum = 0;
+            for (int j = j0; j < j1; ++j) {
+                const bool ahead = sh.list[j] < keys[c];
+                rank += ahead;
+                sum += ahead ? parts[j] : 0;
+            }
+            ranks[c] = s.base + rank;
+            sums[c] = sum;
+        }
+#pragma unroll
+        for (int c = 0; c < kList / kThreads; ++c) {
+            const int i = tid + c * kThreads;
+            if (i >= listed) break;
+            ranked[ranks[c]] = keys[c];
+            before[ranks[c]] = sums[c];
+        }
+        __syncthreads();
+        auto sum_to = [&](const Seg& s, int j) -> uint64_t { return j < s.n ? before[s.base + j] : s.total; };
+        auto mass_to = [&](const Seg& s, int j) -> double {
+            return s.mass_before + s.top * ((double)sum_to(s, j) * a.q_unit);
+        };
+        // how many of a segment's tokens satisfy g(position): g is true, then false
+        auto many = [&](const Seg& s, auto g) -> int {
+            int lo_ = 0, hi_ = s.n;
+            while (lo_ < hi_) {
+                const int mid = (lo_ + hi_) >> 1;
+                if (g(mid)) lo_ = mid + 1;
+                else hi_ = mid;
+            }
+            return lo_;
+        };
+        double mass_k = mass_all;
+        if (by_k) {
+            const Seg& s = sh.seg[seg_of(kb)];
+            limit = Limit{kb, top_k - s.count_before, mass_to(s, top_k - s.count_before)};
+            mass_k = limit.mass;
+        }
+        if (by_p) {
+            const double x = p_of * mass_k;
+            int pick = -1;
+            for (int k = 0; k < segs; ++k) {
+                const Seg& s = sh.seg[k];
+                if (s.bin >= p_lo && s.bin <= p_hi && mass_to(s, s.n) > x && (pick < 0 || s.bin < sh.seg[pick].bin)) pick = k;
+            }
+            if (pick >= 0) {
+                const Seg& s = sh.seg[pick];
+                const int m = max(1, many(s, [&](int j) { return mass_to(s, j) <= x; }));
+                const Limit l{s.bin, m, mass_to(s, m)};
+                if (l.before(limit)) limit = l;
+            }
+        }
+        if (by_m && mb != none) {
+            const int k = seg_of(mb);
+            Limit l{mb, 0, sh.at[3].mass_before};
+            if (k >= 0) {
+                const Seg& s = sh.seg[k];
+                l.n = many(s, [&](int j) {
+                    return s.top * ((double)(sum_to(s, j + 1) - sum_to(s, j)) * a.q_unit) >= least;
+                });
+                l.mass = mass_to(s, l.n);
+            }
+            if (l.before(limit)) limit = l;
+        }
+        {  // the first token is always kept
+            const Seg& s = sh.seg[seg_of(first_bin)];
+            const Limit one{first_bin, 1, mass_to(s, 1)};
+            if (limit.before(one)) limit = one;
+        }
+        const double x = u * limit.mass;
+        int pick = -1, last = -1;
+        for (int k = 0; k < segs; ++k) {
+            const Seg& s = sh.seg[k];
+            if (s.bin > limit.bin || (s.bin == limit.bin && limit.n == 0)) continue;
+            if (last < 0 || s.bin > sh.seg[last].bin) last = k;
+            const int m = s.bin == limit.bin ? limit.n : s.n;
+            if (mass_to(s, m) > x && (pick < 0 || s.bin < sh.seg[pick].bin)) pick = k;
+        }
+        if (pick < 0) pick = last;
+        if (tid == 0) {
+            const Seg& s = sh.seg[pick];
+            const int m = s.bin == limit.bin ? limit.n : s.n;
+            const int j = min(m - 1, many(s, [&](int i) { return mass_to(s, i + 1) <= x; }));
+            a.tokens[r] = (int64_t)(uint32_t)ranked[s.base + j];
+            if (a.probs)
+                a.probs[r] = (float)(s.top * ((double)(sum_to(s, j + 1) - sum_to(s, j)) * a.q_unit) / limit.mass);
+        }
+        __syncthreads();
+        return;
+    }
+    // ---- full bins: each boundary by itself, in the same order. The searches keep to
+    // the intervals found above, so the bins' words are formed again after each.
+    // (not reached by the list; see descend)
+    Binner again = bn;
+    auto rebin = [&]() {
+        __syncthreads();
+        clear_words(sh);
+        __syncthreads();
+        scan_row<DT>(row, 0, a.vocab, [&](int, float v) {
+            double y;
+            if (again.place(v, y))
+                atomicAdd((unsigned long long*)&sh.words[(int)y],
+                          (unsigned long long)((1ull << a.count_shift) + again.q_of(y, (int)y)));
+        });
+        __syncthreads();
+    };
+    auto top_of = [&](int bin) -> double {  // T_b as its owner forms it
+        double t = bin_top(bin / kOwn * kOwn);
+        for (int j = 0; j < bin % kOwn; ++j) t *= Owner::step();
+        return t;
+    };
+    double mass_k = mass_all;
+    if (by_k) {
+        find<true>(sh, own, (double)(top_k - 1), 0);
+        const Found f = sh.at[0];
+        const Ranked e = descend<DT>(a, sh, row, bn, f.bin, true, (double)(top_k - 1 - f.count_before));
+        limit = Limit{f.bin, e.before + 1, f.mass_before + top_of(f.bin) * ((e.parts_before + e.parts) * a.q_unit)};
+        mass_k = limit.mass;
+        rebin();
+    }
+    if (by_p) {
+        const double x = p_of * mass_k;
+        find<false>(sh, own, x, 0);
+        const Found f = sh.at[0];
+        if (f.bin >= 0) {
+            const double top = top_of(f.bin);
+            const Ranked e = descend<DT>(a, sh, row, bn, f.bin, false, (x - f.mass_before) / top * a.q_scale);
+            Limit l{f.bin, f.n, f.mass_before + f.mass};
+            if (e.found)
+                l = Limit{f.bin, e.before + 1, f.mass_before + top * ((e.parts_before + e.parts) * a.q_unit)};
+            if (l.before(limit)) limit = l;
+            rebin();
+        }
+    }
+    if (by_m && mb != none) {
+        const double top = top_of(mb);
+        if (tid == 0) {
+            sh.u0 = 0;
+            sh.i0 = 0;
+        }
+        __syncthreads();
+        scan_row<DT>(row, 0, a.vocab, [&](int, float v) {
+            double yy;
+            if (!bn.place(v, yy) || (int)yy != mb) return;
+            const uint64_t p = (uint64_t)a.q_scale - bn.q_of(yy, mb);
+            if (top * ((double)p * a.q_unit) < least) return;
+            atomicAdd((unsigned long long*)&sh.u0, (unsigned long long)p);
+            atomicAdd(&sh.i0, 1);
+        });
+        __syncthreads();
+        const Limit l{mb, sh.i0, sh.at[3].mass_before + top * ((double)sh.u0 * a.q_unit)};
+        if (l.before(limit)) limit = l;
+        __syncthreads();
+    }
+    {
+        const Ranked e = descend<DT>(a, sh, row, bn, first_bin, true, 0.0);
+        const Limit one{first_bin, 1, top_of(first_bin) * (e.parts * a.q_unit)};
+        if (limit.before(one)) limit = one;
+        rebin();
+    }
+    const double x = u * limit.mass;
+    find<false>(sh, own, x, 0);
+    Found f = sh.at[0];
+    double by_count = -1.0;  // >= 0: this token of the bin, the limit's last
+    if (f.bin < 0 || f.bin > limit.bin) {
+        f.bin = limit.bin;
+        by_count = limit.n - 1;
+    }
+    const double top = top_of(f.bin);
+    Ranked e{};
+    if (by_count < 0.0) {
+        e = descend<DT>(a, sh, row, bn, f.bin, false, (x - f.mass_before) / top * a.q_scale);
+        if (!e.found || (f.bin == limit.bin && e.before >= limit.n)) by_count = f.bin == limit.bin ? limit.n - 1 : f.n - 1;
+    }
+    if (by_count >= 0.0) e = descend<DT>(a, sh, row, bn, f.bin, true, by_count);
+    if (tid == 0) {
+        a.tokens[r] = (int64_t)(uint32_t)e.key;
+        if (a.probs) a.probs[r] = (float)(top * (e.parts * a.q_unit) / limit.mass);
+    }
+    __syncthreads();
+}
+
+// The first largest logit.
+template <int DT>
+__device__ void greedy_row(const SampleArgs& a, Shared& sh, const char* row, int r) {
+    uint64_t best = 0;
+    scan_row<DT>(row, 0, a.vocab, [&](int i, float v) {
+        const uint64_t k = (uint64_t)order_key(v) << 32 | (uint32_t)~i;
+        best = k > best ? k : best;
+    });
+    if (threadIdx.x == 0) sh.best = 0;
+    __syncthreads();
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        const uint64_t x = __shfl_xor((unsigned long long)best, o, 64);
+        best = x > best ? x : best;
+    }
+    if ((threadIdx.x & 63) == 0) atomicMax(&sh.best, (unsigned long long)best);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        a.tokens[r] = (int64_t)(uint32_t)~(uint32_t)sh.best;
+        if (a.probs) a.probs[r] = 1.f;
+    }
+    __syncthreads();
+}
+
+// Bins of the tokens [e0, e1) into sh.words; their largest logit.
+template <int DT>
+__device__ float bin_range(const SampleArgs& a, Shared& sh, const char* row, const Binner& bn, int e0, int e1) {
+    float m = -__builtin_huge_valf();
+    scan_row<DT>(row, e0, e1, [&](int, float v) {
+        m = fmaxf(m, v);
+        double y;
+        if (bn.place(v, y))
+            atomicAdd((unsigned long long*)&sh.words[(int)y],
+                      (unsigned long long)((1ull << a.count_shift) + bn.q_of(y, (int)y)));
+    });
+    return block_max(sh, m);
+}
+
+template <int DT>
+__device__ float range_max(Shared& sh, const char* row, int e0, int e1) {
+    float m = -__builtin_huge_valf();
+    scan_row<DT>(row, e0, e1, [&](int, float v) { m = fmaxf(m, v); });
+    return block_max(sh, m);
+}
+
+// One workgroup a row.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
+    __shared__ Shared sh;
+    const int r = blockIdx.x;
+    const char* row = a.logits + (int64_t)r * a.stride_row * (DT == MF_F32 ? 4 : 2);
+    const float temp = a.temp ? a.temp[r] : a.temp0;
+    if (!(temp > 0.f)) {
+        greedy_row<DT>(a, sh, row, r);
+        return;
+    }
+    clear_words(sh);
+    float ref = range_max<DT>(sh, row, 0, min(a.vocab, kFirst));
+    Binner bn(a, ref, temp);
+    float largest = bin_range<DT>(a, sh, row, bn, 0, a.vocab);
+    double y;
+    if (!bn.place(largest, y)) {  // above the bins: again from the true maximum
+        bn = Binner(a, largest, temp);
+        __syncthreads();
+        clear_words(sh);
+        __syncthreads();
+        bin_range<DT>(a, sh, row, bn, 0, a.vocab);
+    }
+    finish_row<DT>(a, sh, row, r, bn, largest, temp);
+}
+
+}  // namespace
+}  // namespace mf
+
+extern "C" int mf_sample(const void* logits, int dtype, int64_t stride_row, int num_rows, int vocab,
+                         const float* uniforms, const float* temperature, float temperature0, const int32_t* top_k,
+                         int top_k0, const float* top_p, float top_p0, const float* min_p, float min_p0,
+                         int64_t* tokens, float* probs, mf_stream_t stream) {
+    using namespace mf;
+    if (!dtype_ok(dtype) || num_rows < 0 || vocab < 1 || vocab > MF_SAMPLE_MAX_VOCAB || stride_row < 0) return MF_ERR_ARG;
+    if (num_rows == 0) return MF_OK;
+    if (!logits || !uniforms || !tokens) return MF_ERR_ARG;
+    int lv = 0;
+    while ((1 << lv) < vocab) ++lv;
+    const int qs = std::min(40, 71 - 2 * lv);
+    SampleArgs a{(const char*)logits, stride_row, vocab, num_rows, uniforms, temperature, top_k, top_p, min_p,
+                 temperature0, top_p0, min_p0, top_k0, 63 - lv, (double)(1ull << qs), 1.0 / (double)(1ull << qs),
+                 tokens, probs};
+    static_assert(sizeof(Shared) <= 160 * 1024, "LDS of one compute unit");
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == MF_F32)
+        hipLaunchKernelGGL(sample_kernel<MF_F32>, dim3((unsigned)num_rows), dim3(kThreads), 0, st, a);
+    else if (dtype == MF_F16)
+        hipLaunchKernelGGL(sample_kernel<MF_F16>, dim3((unsigned)num_rows), dim3(kThreads), 0, st, a);
+    else
+        hipLaunchKernelGGL(sample_kernel<MF_BF16>, dim3((unsigned)num_rows), dim3(kThreads), 0, st, a);
+    return check_launch();
+}

@@ -26,10 +26,12 @@ from __future__ import annotations
 
 import dataclasses
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Tuple, Union
 
 import torch
 import torch.nn.functional as F
+
+from memforge_amd import _native as nat
 
 
 @dataclass
@@ -94,3 +96,27 @@ def sample_logits(logits: torch.Tensor, params: SamplingParams,
     if params.greedy:
         return int(logits.float().argmax())
     return sample_from_probs(logits_to_probs(logits, params.temperature, params.top_p), generator)
+
+
+def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Union[float, torch.Tensor] = 1.0,
+                  top_k: Union[int, torch.Tensor] = 0, top_p: Union[float, torch.Tensor] = 1.0,
+                  min_p: Union[float, torch.Tensor] = 0.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The next token of every row of a batch, on the device, from given random numbers.
+
+    ``logits``: (rows, vocab) in fp32, fp16 or bf16, up to 2^20 tokens, any row stride.
+    ``uniforms``: fp32 (rows), in [0, 1). The settings are numbers for all rows or
+    tensors with one per row (fp32; ``top_k`` int32), held in 32 bits. Returns the
+    tokens (int64) and the probability each was drawn with (fp32).
+
+    A row's tokens are ranked by (logit descending, index ascending) and weighted by
+    the softmax of logit / temperature. Kept are the first ``top_k`` (0: all), of those
+    the ones with at most ``top_p`` of their mass before them, as ``apply_top_p``
+    keeps them, and those of at least ``min_p`` times the largest weight; the first
+    always is. The token is the first kept one, in rank order, whose inclusive mass
+    exceeds ``uniform`` times the kept mass. A temperature of 0 or less takes the first
+    largest logit. A logit of -infinity is never drawn while the row holds any other
+    (NaN counts as one); a row without any is drawn from uniformly, and so is what
+    +infinity is held by. Unlike ``sample_logits`` it consumes no generator and waits for
+    nothing, so it can be captured into a graph; its draws are others than
+    ``torch.multinomial``'s."""
+    return nat.sample(logits, uniforms, temperature, top_k, top_p, min_p)
