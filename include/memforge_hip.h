@@ -664,6 +664,49 @@ int mf_sample(const void* logits, int dtype, int64_t stride_row, int num_rows, i
               const float* min_p, float min_p0, int64_t* tokens, float* probs,
               mf_stream_t stream);
 
+/* ---------------------------------------------------- attention for drafted trees
+ * Sequence s has context_lens[s] keys in the pool (through its row of the block
+ * tables) and the nodes of a tree, rows cu_nodes[s] .. cu_nodes[s+1] - 1 of q, out,
+ * new_k and new_v: node i's parent is node parents[row] < i of the same tree
+ * (anything else: none). A node sees the whole context, itself and its ancestors:
+ *     out = softmax(scale q.k) v over those keys,
+ * heads grouped as everywhere (query head h reads kv head h / (q heads / kv heads)).
+ * Nothing is written to the pool.
+ *
+ * mf_tree_plan, once for all layers of a step, works out on the device which keys
+ * each node sees, how the keys are split over the launch, and every node's position
+ * (context length + number of ancestors; int64, one per row). context_lens,
+ * cu_nodes and parents are read by it alone and only then. Contexts are taken to
+ * be at most max_context, trees max_nodes; a tree whose rows are not within
+ * num_rows has none. mf_tree_plan_sizes gives the int32 words of the plan (16-byte
+ * aligned) and the fp32 partials that a launch on num_cus compute units needs; the
+ * four shape arguments, num_seqs, num_rows and num_cus are the same in all three
+ * calls, and every block table row holds at least max_context / block_size entries.
+ * Block numbers past num_blocks read the last block. Rows that belong to no tree
+ * are left as they are. head_dim 32, 64, 128 or 256; rows and strides in whole 16
+ * bytes.
+ * Beyond paged_attention_varlen (memforge_ml/kernels/varlen_attention.py:78-235),
+ * whose rows see the rows before them.
+ */
+int mf_tree_plan_sizes(int num_seqs, int64_t num_rows, int max_nodes, int num_q_heads,
+                       int num_kv_heads, int head_dim, int dtype, int num_cus,
+                       int64_t* plan_words, int64_t* partials_floats);
+int mf_tree_plan(const int32_t* parents, const int32_t* cu_nodes, const int32_t* context_lens,
+                 int num_seqs, int64_t num_rows, int max_nodes, int64_t max_context,
+                 int num_q_heads, int num_kv_heads, int head_dim, int dtype, int num_cus,
+                 int32_t* plan, int64_t plan_words, int64_t* positions, mf_stream_t stream);
+int mf_tree_attention(const void* q, int64_t q_stride_row, int64_t q_stride_head, void* out,
+                      int64_t out_stride_row, int64_t out_stride_head, int dtype,
+                      const void* k_pool, const void* v_pool, int64_t pool_stride_block,
+                      int64_t pool_stride_slot, int64_t pool_stride_head, int block_size,
+                      int64_t num_blocks, const int32_t* block_tables,
+                      int64_t block_table_stride, const void* new_k, const void* new_v,
+                      int64_t new_stride_row, int64_t new_stride_head, int num_seqs,
+                      int64_t num_rows, int max_nodes, int num_q_heads, int num_kv_heads,
+                      int head_dim, float scale, int num_cus, const int32_t* plan,
+                      int64_t plan_words, float* partials, int64_t partials_floats,
+                      mf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

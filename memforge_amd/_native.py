@@ -106,6 +106,13 @@ _SIGNATURES = {
     "mf_tree_accept": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_i64, _c_int, _vp, _vp, _vp, _vp]),
     "mf_sample": (_c_int, [_vp, _c_int, _c_i64, _c_int, _c_int, _vp, _vp, _c_f32, _vp, _c_int, _vp, _c_f32, _vp,
                            _c_f32, _vp, _vp, _vp]),
+    "mf_tree_plan_sizes": (_c_int, [_c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _vp]),
+    "mf_tree_plan": (_c_int, [_vp, _vp, _vp, _c_int, _c_i64, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int,
+                              _vp, _c_i64, _vp, _vp]),
+    "mf_tree_attention": (_c_int, [
+        _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_int, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_int, _c_i64, _vp, _c_i64,
+        _vp, _vp, _c_i64, _c_i64, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_f32, _c_int, _vp, _c_i64, _vp,
+        _c_i64, _vp]),
 }
 
 _LIB: Optional[ctypes.CDLL] = None
@@ -1617,3 +1624,97 @@ def tree_accept(tokens: torch.Tensor, targets: torch.Tensor, parents: torch.Tens
     _launch(dev, "mf_tree_accept", lib().mf_tree_accept, tokens.data_ptr(), targets.data_ptr(), parents.data_ptr(),
             cu_nodes.data_ptr(), seqs, rows, max_nodes, path.data_ptr(), out.data_ptr(), count.data_ptr())
     return path, out, count
+
+
+TREE_HEAD_DIMS = (32, 64, 128, 256)
+_TREE_SIZES = {}  # shape of a call -> mf_tree_plan_sizes
+
+
+@dataclass
+class TreePlan:
+    """One step's trees as ``tree_attention`` reads them (mf_tree_plan)."""
+
+    buffer: torch.Tensor      # int32
+    positions: torch.Tensor   # int64 per row: context length + number of ancestors
+    num_seqs: int
+    num_rows: int
+    max_nodes: int
+    max_context: int
+    num_q_heads: int
+    num_kv_heads: int
+    head_dim: int
+    dtype: torch.dtype
+    num_cus: int
+    partials_floats: int
+
+
+def tree_plan(parents: torch.Tensor, cu_nodes: torch.Tensor, context_lens: torch.Tensor, max_nodes: int, max_context: int,
+              num_q_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype) -> TreePlan:
+    """mf_tree_plan into new buffers."""
+    require_device(parents, cu_nodes, context_lens)
+    dev, rows, seqs = parents.device, parents.numel(), context_lens.numel()
+    for name, x, n in (("parents", parents, rows), ("cu_nodes", cu_nodes, seqs + 1), ("context_lens", context_lens, seqs)):
+        check_index(name, x, torch.int32, dev, (n,))
+    if not 1 <= max_nodes <= TREE_MAX_NODES:
+        raise ValueError(f"max_nodes must be 1 to {TREE_MAX_NODES}, got {max_nodes}")
+    if not 0 <= max_context <= 1 << 30:
+        raise ValueError(f"max_context must be 0 to 2^30, got {max_context}")
+    if num_kv_heads < 1 or num_q_heads < 1 or num_q_heads % num_kv_heads:
+        raise ValueError(f"{num_q_heads} query heads is not a multiple of {num_kv_heads} kv heads")
+    if head_dim not in TREE_HEAD_DIMS:
+        raise ValueError(f"tree attention takes head_dims {TREE_HEAD_DIMS}, got {head_dim}")
+    cus = device_cus(dev)
+    shape = (seqs, rows, max_nodes, num_q_heads, num_kv_heads, head_dim, dtype_code(dtype), cus)
+    sizes = _TREE_SIZES.get(shape)
+    if sizes is None:
+        got = np.zeros(2, dtype=np.int64)
+        _check(lib().mf_tree_plan_sizes(*shape, got.ctypes.data, got.ctypes.data + 8), "mf_tree_plan_sizes")
+        if len(_TREE_SIZES) >= 4096:
+            _TREE_SIZES.clear()
+        sizes = _TREE_SIZES[shape] = (int(got[0]), int(got[1]))
+    buffer = torch.empty(sizes[0], dtype=torch.int32, device=dev)
+    positions = torch.empty(rows, dtype=torch.int64, device=dev)
+    _launch(dev, "mf_tree_plan", lib().mf_tree_plan, parents.data_ptr(), cu_nodes.data_ptr(), context_lens.data_ptr(),
+            seqs, rows, max_nodes, max_context, num_q_heads, num_kv_heads, head_dim, shape[6], cus, buffer.data_ptr(),
+            sizes[0], positions.data_ptr())
+    return TreePlan(buffer, positions, seqs, rows, max_nodes, max_context, num_q_heads, num_kv_heads, head_dim, dtype, cus,
+                    sizes[1])
+
+
+def tree_attention(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: PoolView, block_tables: torch.Tensor, plan: TreePlan,
+                   new_k_rows: torch.Tensor, new_v_rows: torch.Tensor, scale: float,
+                   partials: Optional[torch.Tensor] = None) -> None:
+    """mf_tree_attention into ``out_rows`` ((rows, Hq, D) views, device)."""
+    require_device(q_rows, out_rows, pool.k, block_tables, new_k_rows, new_v_rows)
+    dev, dtype = plan.buffer.device, plan.dtype
+    for name, x, heads in (("q_rows", q_rows, plan.num_q_heads), ("out_rows", out_rows, plan.num_q_heads),
+                           ("new_k_rows", new_k_rows, plan.num_kv_heads), ("new_v_rows", new_v_rows, plan.num_kv_heads)):
+        if x.shape != (plan.num_rows, heads, plan.head_dim) or x.dtype != dtype or x.device != dev:
+            raise ValueError(f"{name} must be {(plan.num_rows, heads, plan.head_dim)} in {dtype} on {dev}, got "
+                             f"{tuple(x.shape)} in {x.dtype} on {x.device}")
+        _rows_ok(x, name)
+    if not same_layout(new_k_rows, new_v_rows):
+        new_k_rows, new_v_rows = new_k_rows.contiguous(), new_v_rows.contiguous()
+    if pool.k.dtype != dtype or pool.num_heads != plan.num_kv_heads or pool.head_dim != plan.head_dim or pool.k.device != dev:
+        raise ValueError(f"a pool of {pool.num_heads} heads x {pool.head_dim} in {pool.k.dtype} on {pool.k.device} does not "
+                         f"match a plan for {plan.num_kv_heads} x {plan.head_dim} in {dtype} on {dev}")
+    check_index("block_tables", block_tables, torch.int32, dev)
+    width = block_tables.shape[1] if block_tables.dim() == 2 else 0
+    if block_tables.dim() != 2 or block_tables.shape[0] != plan.num_seqs or width * pool.block_size < plan.max_context:
+        raise ValueError(f"block_tables {tuple(block_tables.shape)} do not hold {plan.num_seqs} contexts of up to "
+                         f"{plan.max_context} tokens in blocks of {pool.block_size}")
+    if not abs(scale) < float("inf"):
+        raise ValueError(f"scale must be finite, got {scale}")
+    if plan.num_rows == 0 or plan.num_seqs == 0:
+        return
+    if partials is None:
+        partials = _WORKSPACE.partials(plan.partials_floats, dev)
+    elif partials.dtype != torch.float32 or not partials.is_contiguous() or partials.device != dev:
+        raise ValueError(f"partials must be contiguous fp32 on {dev}, got {partials.dtype} on {partials.device}")
+    _launch(dev, "mf_tree_attention", lib().mf_tree_attention,
+            q_rows.data_ptr(), q_rows.stride(0), q_rows.stride(1), out_rows.data_ptr(), out_rows.stride(0),
+            out_rows.stride(1), dtype_code(dtype), pool.k.data_ptr(), pool.v.data_ptr(), pool.stride_block, pool.stride_slot,
+            pool.stride_head, pool.block_size, pool.num_blocks, block_tables.data_ptr(), width,
+            new_k_rows.data_ptr(), new_v_rows.data_ptr(), new_k_rows.stride(0), new_k_rows.stride(1), plan.num_seqs,
+            plan.num_rows, plan.max_nodes, plan.num_q_heads, plan.num_kv_heads, plan.head_dim, float(scale), plan.num_cus,
+            plan.buffer.data_ptr(), plan.buffer.numel(), partials.data_ptr(), partials.numel())

@@ -1,0 +1,835 @@
+// Attention for trees of drafted tokens over the paged cache.
+//
+// Sequence s has ctx tokens in the pool and n nodes whose keys and values are rows
+// of the call. Node i sees the context, itself and its ancestors:
+//     out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q.k_j)
+// with grouped heads. A (node, head) pair is a column; the G heads of a kv head
+// share its K/V rows, so a kv head's n G columns are one matrix product with them.
+//
+// Work. A kv head's keys are tiles of 32: the context's, then the nodes'. The tiles
+// of every (sequence, kv head, column group) stand in one line, which the launch's
+// workgroups cut into equal shares: a workgroup runs the pieces of up to several
+// (sequence, kv head)s that its share covers, writes the whole ones out and leaves
+// the others' unnormalised sums for merge_tree_kernel. So one long context and a
+// batch of uneven ones both fill the GPU, from lengths that only the device knows:
+// the plan (tree_plan_kernel, once for all layers of a step) is made there.
+//
+// Tiles. Four waves, WC side by side on columns (NB blocks of 32 each) and 4 / WC on
+// keys, so a stage of 4 / WC tiles goes from global memory straight into LDS once
+// for all columns; a ring of stages keeps loads in flight. S^T = K Q^T, softmax with
+// a lazily moved maximum, O^T += V^T P^T in 32x32 MFMA blocks whose operands need no
+// move between lanes: as attn_wide_body (attn_kernels.h) lays them out.
+#include <algorithm>
+#include <cmath>
+
+#include "attn_kernels.h"
+
+namespace mf {
+namespace {
+
+constexpr int kTreeThreads = 256;
+constexpr int kTile = 32;            // keys
+constexpr int kMaxSeqs = 4096;
+constexpr int kWindow = 1024;        // block-table entries held in LDS
+constexpr int kSeqInts = 8;          // ctx, nodes, first row, tiles, column groups, context tiles, -, -
+
+struct TreePlanArgs {
+    const int32_t* parents;
+    const int32_t* cu_nodes;
+    const int32_t* ctx_lens;
+    int num_seqs;
+    int64_t num_rows;
+    int max_nodes, mask_words;
+    int64_t max_context;
+    int group;        // query heads of a kv head
+    int num_kv_heads;
+    int group_cols;   // columns of one column group
+    int num_workers, min_share;
+    int64_t* head;      // share, all tiles
+    int32_t* seqs;
+    int64_t* seq_first; // first tile of each sequence in the line
+    int32_t* work;      // (seq, unit, tile, -) at which each worker starts
+    uint32_t* masks;
+    int64_t* positions;
+};
+
+__device__ __forceinline__ void seq_shape(const TreePlanArgs& a, int s, int& ctx, int& n, int64_t& row0) {
+    row0 = a.cu_nodes[s];
+    const int64_t rows = a.cu_nodes[s + 1] - row0;
+    n = (int)min(rows, (int64_t)a.max_nodes);
+    if (row0 < 0 || rows < 0 || row0 + n > a.num_rows) n = 0;
+    ctx = (int)min((int64_t)max(a.ctx_lens[s], 0), a.max_context);
+}
+
+// Block 0 lays the tiles out; block 1 + s writes sequence s's masks and positions.
+__global__ __launch_bounds__(kTreeThreads) void tree_plan_kernel(TreePlanArgs a) {
+    __shared__ int64_t first[kMaxSeqs + 1];
+    __shared__ int64_t waves[kTreeThreads / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (blockIdx.x > 0) {
+        int* up = (int*)first;
+        const int s = blockIdx.x - 1;
+        int ctx, n;
+        int64_t row0;
+        seq_shape(a, s, ctx, n, row0);
+        for (int i = tid; i < n; i += kTreeThreads) {
+            const int p = a.parents[row0 + i];
+            up[i] = p >= 0 && p < i ? p : -1;
+        }
+        __syncthreads();
+        // ancestors come in falling order, so a node's words are finished one after the other
+        for (int i = tid; i < n; i += kTreeThreads) {
+            uint32_t* row = a.masks + (row0 + i) * a.mask_words;
+            for (int w = a.mask_words - 1; w > i >> 5; --w) row[w] = 0;
+            int depth = 0, word = i >> 5;
+            uint32_t bits = 0;
+            for (int at = i;; at = up[at]) {
+                while (at < 0 ? word >= 0 : at >> 5 < word) {
+                    row[word--] = bits;
+                    bits = 0;
+                }
+                if (at < 0) break;
+                bits |= 1u << (at & 31);
+                ++depth;
+            }
+            a.positions[row0 + i] = (int64_t)ctx + depth - 1;
+        }
+        return;
+    }
+    const int per = (a.num_seqs + kTreeThreads - 1) / kTreeThreads;
+    const int s0 = min(tid * per, a.num_seqs), s1 = min(s0 + per, a.num_seqs);
+    int64_t mine = 0;
+    for (int s = s0; s < s1; ++s) {
+        int ctx, n;
+        int64_t row0;
+        seq_shape(a, s, ctx, n, row0);
+        const int held = (ctx + kTile - 1) / kTile;
+        const int tiles = n > 0 ? held + (n + kTile - 1) / kTile : 0;
+        const int groups = (n * a.group + a.group_cols - 1) / a.group_cols;
+        int32_t* q = a.seqs + (int64_t)s * kSeqInts;
+        q[0] = ctx;
+        q[1] = n;
+        q[2] = (int)row0;
+        q[3] = tiles;
+        q[4] = groups;
+        q[5] = held;
+        first[s] = mine;
+        mine += (int64_t)tiles * groups * a.num_kv_heads;
+    }
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t up = __shfl_up(incl, o, 64);
+        if (lane >= o) incl += up;
+    }
+    if (lane == 63) waves[wave] = incl;
+    __syncthreads();
+    int64_t base = incl - mine, total = 0;
+    for (int w = 0; w < kTreeThreads / 64; ++w) {
+        if (w < wave) base += waves[w];
+        total += waves[w];
+    }
+    for (int s = s0; s < s1; ++s) {
+        first[s] += base;
+        a.seq_first[s] = first[s];
+    }
+    if (tid == 0) first[a.num_seqs] = total;
+    const int64_t share = max((total + a.num_workers - 1) / a.num_workers, (int64_t)a.min_share);
+    if (tid == 0) {
+        a.head[0] = share;
+        a.head[1] = total;
+    }
+    __syncthreads();
+    for (int w = tid; w < a.num_workers; w += kTreeThreads) {
+        const int64_t at = (int64_t)w * share;
+        if (at >= total) break;
+        int lo = 0, hi = a.num_seqs - 1;  // the last sequence that starts at or before `at`: it has tiles
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (first[mid] <= at) lo = mid;
+            else hi = mid - 1;
+        }
+        const int tiles = a.seqs[(int64_t)lo * kSeqInts + 3];
+        const int64_t in = at - first[lo];
+        *(int4*)(a.work + 4 * w) = make_int4(lo, (int)(in / tiles), (int)(in % tiles), 0);
+    }
+}
+
+struct TreeArgs {
+    const int64_t* head;
+    const int32_t* work;
+    const int32_t* seqs;
+    const int64_t* seq_first;
+    const uint32_t* masks;
+    int mask_words;
+    int num_seqs;
+    const char* q;
+    int64_t q_sr, q_sh;
+    char* out;
+    int64_t o_sr, o_sh;
+    const char *k_pool, *v_pool;
+    int64_t p_sb, p_ss, p_sh;
+    int block_size, block_shift;  // shift -1: not a power of two
+    uint32_t num_blocks;
+    const int32_t* tables;
+    int64_t table_stride;
+    const char *new_k, *new_v;
+    int64_t n_sr, n_sh;
+    int group, num_kv_heads;
+    float scale_log2, inv_scale_log2;
+    uint32_t q_sign;
+    float* partials;
+};
+
+template <int DT, int D, int WC, int NB>
+struct TreeShape {
+    static constexpr int ES = DT == MF_F32 ? 4 : 2;
+    static constexpr int RB = D * ES;                      // bytes of a key row
+    static constexpr int NCH = RB / 16;                    // its 16-byte chunks
+    static constexpr int RPB = RB >= 256 ? 1 : 256 / RB;   // rows in 256 bytes (every LDS bank once)
+    static constexpr int WK = 4 / WC;                      // waves along the keys
+    static constexpr int TILE = kTile * RB;
+    static constexpr int HALF = WK * TILE;                 // K rows of a stage, then its V rows
+    static constexpr int STG = 2 * HALF;
+    static constexpr int RING = STG * 4 <= 64 * 1024 ? 4 : STG * 3 <= 64 * 1024 ? 3 : 2;
+    static constexpr int NLD = STG / 1024 / 4;             // 1 KB pieces of a stage per wave
+    static constexpr int NQ = RB / 32;                     // 16-byte pieces of a query row per lane half
+    static constexpr int ND = D / 32;
+    static constexpr int COLS = WC * NB * 32;
+    static constexpr int SLOT = COLS * (D + 2);            // floats of a piece's sums
+};
+
+// Sum and maximum of a column live in two lanes (lane halves); O^T's lane (hf, column)
+// holds head_dim elements 32 d + 8 b + 4 hf + 0..3 in acc[d][4 b ..].
+template <int DT, int ND>
+__device__ __forceinline__ void store_column(char* dst, bool live, const f32x16 (&acc)[ND], float inv, int hf) {
+    if constexpr (DT == MF_F32) {
+        if (!live) return;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+                *(float4*)(dst + (32 * d + 8 * b + 4 * hf) * 4) =
+                    make_float4(acc[d][4 * b] * inv, acc[d][4 * b + 1] * inv, acc[d][4 * b + 2] * inv, acc[d][4 * b + 3] * inv);
+    } else {
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int b = 0; b < 4; b += 2) {
+                uint32_t w[2][2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        w[e][k] = f32_to_bits<DT>(acc[d][4 * (b + e) + 2 * k] * inv) |
+                                  (f32_to_bits<DT>(acc[d][4 * (b + e) + 2 * k + 1] * inv) << 16);
+                auto x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+                auto y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+                if (live) *(uint4*)(dst + (32 * d + 8 * (b + hf)) * 2) = make_uint4(x[0], y[0], x[1], y[1]);
+            }
+    }
+}
+
+__device__ __forceinline__ f32x16 mfma32_f32(float a, float b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
+}
+
+// The sum over both lane halves, in both.
+__device__ __forceinline__ float both_halves_sum(float v) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <int DT, int D, int WC, int NB>
+__global__ __launch_bounds__(kTreeThreads) void tree_kernel(TreeArgs a) {
+    using S = TreeShape<DT, D, WC, NB>;
+    constexpr int ES = S::ES, RB = S::RB, NCH = S::NCH, RPB = S::RPB, WK = S::WK, NQ = S::NQ, ND = S::ND, NLD = S::NLD;
+    constexpr float kNegInf = -__builtin_huge_valf();
+    __shared__ __align__(1024) char ring[S::RING * S::STG];
+    __shared__ int tab[kWindow];
+    static_assert(WK == 1 || (WK - 1) * WC * NB * (ND * 16 + 2) * 256 <= S::RING * S::STG, "the key waves' sums fit the ring");
+
+    const int64_t share = a.head[0], total = a.head[1];
+    const int64_t begin = (int64_t)blockIdx.x * share;
+    if (begin >= total) return;
+    int64_t left = min(share, total - begin);
+    const int4 at = *(const int4*)(a.work + 4 * blockIdx.x);
+    int s = at.x, unit = at.y, tile0 = at.z;
+    const int tid = threadIdx.x, lane = tid & 63, hf = lane >> 5, j = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wc = wave % WC, wk = wave / WC;
+    const uint32_t ring_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)ring;
+    auto sync = [&]() {
+        __builtin_amdgcn_s_waitcnt((15) | (3 << 14) | (7 << 4) | (0 << 8));  // lgkmcnt(0)
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    // lane addresses inside a wave's tile: K rows (key lane & 31), V rows
+    uint32_t kaddr[NQ], vaddr[ND];
+#pragma unroll
+    for (int c = 0; c < NQ; ++c)
+        kaddr[c] = (uint32_t)(wk * S::TILE + (lane & 31) * RB + (((2 * c + hf) ^ ((j / RPB) & (NCH - 1))) << 4));
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+        if constexpr (DT == MF_F32)
+            vaddr[d] = (uint32_t)(S::HALF + wk * S::TILE + 4 * hf * RB + (32 * d + (lane & 31)) * 4);
+        else
+            vaddr[d] = (uint32_t)(S::HALF + wk * S::TILE + (4 * hf + (j >> 2)) * RB +
+                                  (((4 * d + 2 * ((lane & 31) >> 4) + ((j & 3) >> 1)) ^ (((j >> 2) / RPB) << 2)) << 4) +
+                                  8 * (j & 1));
+    }
+
+    bool first = true;
+    while (left > 0) {
+        const int32_t* info = a.seqs + (int64_t)s * kSeqInts;
+        const int ctx = info[0], n = info[1], row0 = info[2], tiles = info[3], groups = info[4], held = info[5];
+        if (tiles == 0) {
+            ++s;
+            unit = 0;
+            tile0 = 0;
+            continue;
+        }
+        const int h = unit / groups, grp = unit - h * groups;
+        const int t0 = tile0, t1 = (int)min((int64_t)tiles, t0 + left);
+        const int nst = (t1 - t0 + WK - 1) / WK;
+
+        // ---- this lane's columns
+        int cidx[NB];
+        bool valid[NB];
+        int64_t prow[NB];
+        int qhead[NB];
+        uint4 qf[NB][NQ];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            cidx[b] = grp * S::COLS + (wc * NB + b) * 32 + (lane & 31);
+            valid[b] = cidx[b] < n * a.group;
+            const int c = valid[b] ? cidx[b] : 0;
+            const int node = (int)((unsigned)c / (unsigned)a.group);
+            prow[b] = row0 + node;
+            qhead[b] = h * a.group + c - node * a.group;
+            const char* qp = a.q + (prow[b] * a.q_sr + (int64_t)qhead[b] * a.q_sh) * ES;
+#pragma unroll
+            for (int c2 = 0; c2 < NQ; ++c2) {
+                const uint4 v = *(const uint4*)(qp + (2 * c2 + hf) * 16);
+                qf[b][c2] = make_uint4(v.x ^ a.q_sign, v.y ^ a.q_sign, v.z ^ a.q_sign, v.w ^ a.q_sign);
+            }
+        }
+        const bool busy = grp * S::COLS + wc * NB * 32 < n * a.group;  // a wave of padding columns only loads
+
+        // ---- block-table entries of the piece's keys, a window of them in LDS
+        const int32_t* trow = a.tables + (int64_t)s * a.table_stride;
+        auto block_of = [&](int key) -> int {
+            return a.block_shift >= 0 ? key >> a.block_shift : (int)((unsigned)key / (unsigned)a.block_size);
+        };
+        int window = 0;
+        const int key_end = min(t1 * kTile, ctx);
+        auto fill_window = [&](int from_key) {
+            window = block_of(from_key);
+            const int end = min(window + kWindow, block_of(key_end - 1) + 1);
+            for (int i = window + tid; i < end; i += kTreeThreads) tab[i - window] = trow[i];
+        };
+        if (t0 * kTile < key_end) fill_window(t0 * kTile);
+        sync();
+
+        auto fetch = [&](int u, int buf) __attribute__((always_inline)) {
+            const int st0 = t0 + u * WK;
+            {
+                const int last = min((st0 + WK) * kTile, key_end) - 1;
+                if (st0 * kTile < key_end && block_of(last) >= window + kWindow) {
+                    sync();
+                    fill_window(st0 * kTile);
+                    sync();
+                }
+            }
+            const uint32_t dst0 = ring_at + (uint32_t)(buf * S::STG);
+#pragma unroll
+            for (int i = 0; i < NLD; ++i) {
+                const int x = wave + 4 * i;
+                constexpr int P = S::STG / 2048;  // pieces of the K half
+                const bool isv = x >= P;
+                const int r = (isv ? x - P : x) * (1024 / RB) + lane * 16 / RB;  // row of the stage
+                const int t = min(st0 + (r >> 5), t1 - 1), in = r & 31;
+                const int swz = !isv ? ((in & 15) / RPB) & (NCH - 1) : DT == MF_F32 ? 0 : ((in & 3) / RPB) << 2;
+                const char* src;
+                if (t < held) {
+                    // rows past the context's end read its last one: masked, and every column sees that row
+                    const int key = min(t * kTile + in, ctx - 1);
+                    const int blk = block_of(key);
+                    const uint32_t e = min((uint32_t)tab[blk - window], a.num_blocks - 1);
+                    const int slot = key - blk * a.block_size;
+                    src = (isv ? a.v_pool : a.k_pool) + ((int64_t)e * a.p_sb + (int64_t)slot * a.p_ss + (int64_t)h * a.p_sh) * ES;
+                } else {
+                    const int node = min((t - held) * kTile + in, n - 1);
+                    src = (isv ? a.new_v : a.new_k) + ((int64_t)(row0 + node) * a.n_sr + (int64_t)h * a.n_sh) * ES;
+                }
+                ld_lds16(src + (((lane & (NCH - 1)) ^ swz) << 4), dst0 + (uint32_t)(x * 1024));
+            }
+        };
+
+        float m[NB], l[NB], thr[NB];
+        f32x16 acc[NB][ND];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            m[b] = kMinM;
+            l[b] = 0.f;
+            thr[b] = (kMinM + kLazyLog2) * a.inv_scale_log2;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[b][d][i] = 0.f;
+        }
+
+        auto tile = [&](const char* stg, int t) __attribute__((always_inline)) {
+            f32x16 st[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) st[b][i] = 0.f;
+#pragma unroll
+            for (int c = 0; c < NQ; ++c) {
+                const uint4 kf = *(const uint4*)(stg + kaddr[c]);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    if constexpr (DT == MF_F32) {
+                        st[b] = mfma32_f32(__uint_as_float(kf.x), __uint_as_float(qf[b][c].x), st[b]);
+                        st[b] = mfma32_f32(__uint_as_float(kf.y), __uint_as_float(qf[b][c].y), st[b]);
+                        st[b] = mfma32_f32(__uint_as_float(kf.z), __uint_as_float(qf[b][c].z), st[b]);
+                        st[b] = mfma32_f32(__uint_as_float(kf.w), __uint_as_float(qf[b][c].w), st[b]);
+                    } else {
+                        st[b] = mfma32<DT>(kf, qf[b][c], st[b]);
+                    }
+                }
+            }
+            if (t >= held || (t + 1) * kTile > ctx) {  // the context's last tile, and the nodes'
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    uint32_t seen;
+                    if (t < held) seen = 0xffffffffu >> ((t + 1) * kTile - ctx);
+                    else seen = valid[b] ? a.masks[prow[b] * a.mask_words + (t - held)] : 0u;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int key = 8 * (i >> 2) + 4 * hf + (i & 3);
+                        st[b][i] = seen >> key & 1u ? st[b][i] : kNegInf;
+                    }
+                }
+            }
+            // lazy rescale: the maximum moves when a score passes it by more than 2^8
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                float lmax = st[b][0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) lmax = fmax_prop(lmax, st[b][i]);
+                if (__builtin_amdgcn_ballot_w64(lmax > thr[b]) != 0) {
+                    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(lmax), __float_as_uint(lmax), false, false);
+                    const float mn = fmaxf(m[b], fmax_prop(__uint_as_float(r[0]), __uint_as_float(r[1])) * a.scale_log2);
+                    const float alpha = __builtin_amdgcn_exp2f(m[b] - mn);
+                    l[b] *= alpha;
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[b][d][i] *= alpha;
+                    m[b] = mn;
+                    thr[b] = (mn + kLazyLog2) * a.inv_scale_log2;
+                }
+            }
+            uint32_t pw[NB][8];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    st[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[b][i], a.scale_log2, -m[b]));
+                    sum += st[b][i];
+                }
+                l[b] += sum;
+                if constexpr (DT != MF_F32) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        // 16-bit operands of the second product: each weight off by half a step of the type
+                        if constexpr (DT == MF_BF16)
+                            pw[b][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){st[b][2 * i], st[b][2 * i + 1]}, bf16x2));
+                        else
+                            pw[b][i] = f32_to_bits<DT>(st[b][2 * i]) | (f32_to_bits<DT>(st[b][2 * i + 1]) << 16);
+                    }
+                }
+            }
+            if constexpr (DT == MF_F32) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        const float v = *(const float*)(stg + vaddr[d] + (8 * (i >> 2) + (i & 3)) * RB);
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) acc[b][d] = mfma32_f32(v, st[b][i], acc[b][d]);
+                    }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        const uint2 v0 = ld_tr16(stg + vaddr[d] + 16 * k * RB);
+                        const uint2 v1 = ld_tr16(stg + vaddr[d] + (16 * k + 8) * RB);
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+                            acc[b][d] = mfma32<DT>(make_uint4(v0.x, v0.y, v1.x, v1.y),
+                                                   make_uint4(pw[b][4 * k], pw[b][4 * k + 1], pw[b][4 * k + 2], pw[b][4 * k + 3]),
+                                                   acc[b][d]);
+                    }
+            }
+        };
+
+        // ---- stages
+        constexpr int AHEAD = S::RING - 1;
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+            if (u < nst) fetch(u, u);
+        int buf = 0;
+        for (int u = 0; u < nst; ++u) {
+            if (nst - 1 - u >= AHEAD - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((AHEAD - 1) * NLD) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            sync();  // stage u is whole, and the one before has been read
+            if (u + AHEAD < nst) fetch(u + AHEAD, buf == 0 ? S::RING - 1 : buf - 1);
+            const int t = t0 + u * WK + wk;
+            if (busy && t < t1) tile(ring + buf * S::STG, t);
+            buf = buf + 1 == S::RING ? 0 : buf + 1;
+        }
+        sync();
+
+        // ---- the key waves' sums in one, then the piece's result
+#pragma unroll
+        for (int b = 0; b < NB; ++b) l[b] = both_halves_sum(l[b]);
+        if constexpr (WK > 1) {
+            constexpr int PART = NB * (ND * 16 + 2) * 64;
+            float* mine = (float*)ring + ((wk - 1) * WC + wc) * PART;
+            if (wk > 0) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    float* to = mine + b * (ND * 16 + 2) * 64;
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4)
+                            *(float4*)(to + (d * 16 + i) * 64 + 4 * lane) =
+                                make_float4(acc[b][d][i], acc[b][d][i + 1], acc[b][d][i + 2], acc[b][d][i + 3]);
+                    to[ND * 1024 + lane] = m[b];
+                    to[ND * 1024 + 64 + lane] = l[b];
+                }
+            }
+            sync();
+            if (wk == 0) {
+#pragma unroll
+                for (int o = 0; o < WK - 1; ++o)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const float* from = (const float*)ring + (o * WC + wc) * PART + b * (ND * 16 + 2) * 64;
+                        const float m1 = from[ND * 1024 + lane], l1 = from[ND * 1024 + 64 + lane];
+                        const float mn = fmaxf(m[b], m1);
+                        const float w0 = __builtin_amdgcn_exp2f(m[b] - mn), w1 = __builtin_amdgcn_exp2f(m1 - mn);
+                        m[b] = mn;
+                        l[b] = l[b] * w0 + l1 * w1;
+#pragma unroll
+                        for (int d = 0; d < ND; ++d)
+#pragma unroll
+                            for (int i = 0; i < 16; i += 4) {
+                                const float4 v = *(const float4*)(from + (d * 16 + i) * 64 + 4 * lane);
+                                acc[b][d][i] = acc[b][d][i] * w0 + v.x * w1;
+                                acc[b][d][i + 1] = acc[b][d][i + 1] * w0 + v.y * w1;
+                                acc[b][d][i + 2] = acc[b][d][i + 2] * w0 + v.z * w1;
+                                acc[b][d][i + 3] = acc[b][d][i + 3] * w0 + v.w * w1;
+                            }
+                    }
+            }
+        }
+        if (wk == 0 && busy) {
+            const bool whole = t0 == 0 && t1 == tiles;
+            if (whole) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+                    store_column<DT, ND>(a.out + (prow[b] * a.o_sr + (int64_t)qhead[b] * a.o_sh) * ES, valid[b], acc[b],
+                                         1.f / l[b], hf);
+            } else {
+                float* slot = a.partials + (2 * (int64_t)blockIdx.x + (first ? 0 : 1)) * S::SLOT;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    float* to = slot + (wc * NB + b) * 32 * (D + 2);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4)
+                            *(float4*)(to + (d * 16 + i) * 64 + 4 * lane) =
+                                make_float4(acc[b][d][i], acc[b][d][i + 1], acc[b][d][i + 2], acc[b][d][i + 3]);
+                    if (hf == 0) {
+                        to[32 * D + lane] = m[b];
+                        to[32 * D + 32 + lane] = l[b];
+                    }
+                }
+            }
+        }
+        sync();  // the ring and the window are free
+        left -= t1 - t0;
+        first = false;
+        tile0 = 0;
+        if (++unit == groups * a.num_kv_heads) {
+            unit = 0;
+            ++s;
+        }
+    }
+}
+
+// One workgroup for (32 columns, 32 head_dim elements) of a cut (sequence, kv head,
+// column group): its four waves take every fourth piece.
+template <int DT, int D, int WC, int NB>
+__global__ __launch_bounds__(kTreeThreads) void merge_tree_kernel(TreeArgs a, int units_per_seq) {
+    using S = TreeShape<DT, D, WC, NB>;
+    constexpr int ES = S::ES;
+    __shared__ float sums[3][18 * 64];
+    const int64_t share = a.head[0];
+    const int u = blockIdx.x, s = u / units_per_seq, unit = u - s * units_per_seq;
+    const int blk = blockIdx.y / S::ND, d = blockIdx.y % S::ND;
+    const int32_t* info = a.seqs + (int64_t)s * kSeqInts;
+    const int n = info[1], row0 = info[2], tiles = info[3], groups = info[4];
+    if (tiles == 0 || unit >= groups * a.num_kv_heads) return;
+    const int h = unit / groups, grp = unit - h * groups;
+    if (grp * S::COLS + blk * 32 >= n * a.group) return;
+    const int64_t begin = a.seq_first[s] + (int64_t)unit * tiles;
+    const int64_t w0 = begin / share, w1 = (begin + tiles - 1) / share;
+    if (w0 == w1) return;
+    const int lane = threadIdx.x & 63, hf = lane >> 5, wave = threadIdx.x >> 6;
+    float m = kMinM, l = 0.f;
+    f32x16 acc[1];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[0][i] = 0.f;
+    for (int64_t w = w0 + wave; w <= w1; w += 4) {
+        const float* from = a.partials + (2 * w + (w * share < begin ? 1 : 0)) * S::SLOT + blk * 32 * (D + 2);
+        const float m1 = from[32 * D + (lane & 31)], l1 = from[32 * D + 32 + (lane & 31)];
+        float4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = *(const float4*)(from + (d * 16 + 4 * i) * 64 + 4 * lane);
+        const float mn = fmaxf(m, m1);
+        const float e0 = __builtin_amdgcn_exp2f(m - mn), e1 = __builtin_amdgcn_exp2f(m1 - mn);
+        m = mn;
+        l = l * e0 + l1 * e1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            acc[0][4 * i] = acc[0][4 * i] * e0 + v[i].x * e1;
+            acc[0][4 * i + 1] = acc[0][4 * i + 1] * e0 + v[i].y * e1;
+            acc[0][4 * i + 2] = acc[0][4 * i + 2] * e0 + v[i].z * e1;
+            acc[0][4 * i + 3] = acc[0][4 * i + 3] * e0 + v[i].w * e1;
+        }
+    }
+    if (wave > 0) {
+        float* to = sums[wave - 1];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) to[i * 64 + lane] = acc[0][i];
+        to[16 * 64 + lane] = m;
+        to[17 * 64 + lane] = l;
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int o = 0; o < 3; ++o) {
+        const float m1 = sums[o][16 * 64 + lane], l1 = sums[o][17 * 64 + lane];
+        const float mn = fmaxf(m, m1);
+        const float e0 = __builtin_amdgcn_exp2f(m - mn), e1 = __builtin_amdgcn_exp2f(m1 - mn);
+        m = mn;
+        l = l * e0 + l1 * e1;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[0][i] = acc[0][i] * e0 + sums[o][i * 64 + lane] * e1;
+    }
+    const int c = grp * S::COLS + blk * 32 + (lane & 31);
+    const bool valid = c < n * a.group;
+    const int node = (int)((unsigned)(valid ? c : 0) / (unsigned)a.group);
+    const int qhead = h * a.group + (valid ? c : 0) - node * a.group;
+    store_column<DT, 1>(a.out + ((int64_t)(row0 + node) * a.o_sr + (int64_t)qhead * a.o_sh + 32 * d) * ES, valid, acc,
+                        1.f / l, hf);
+}
+
+// The waves' arrangement for a call: WC side by side on blocks of 32 columns.
+struct TreeConfig {
+    int wc, nb, wgs_per_cu, min_share;
+};
+
+TreeConfig tree_config(int dtype, int head_dim, int max_nodes, int group) {
+    const int64_t cols = (int64_t)max_nodes * group;
+    const int rb = head_dim * dtype_size(dtype);
+    if (dtype == MF_F32 || rb > 256) return {4, 1, rb > 512 ? 1 : 2, 8};
+    if (cols <= 32) return {1, 1, rb > 128 ? 1 : 2, 8};
+    if (cols <= 64) return {2, 1, 2, 8};
+    if (cols <= 128) return {4, 1, 2, 8};
+    return {4, 2, 1, 8};
+}
+
+template <int DT, int D, int WC, int NB>
+int launch_tree(const TreeArgs& a, int workers, int units_per_seq, hipStream_t st) {
+    hipLaunchKernelGGL((tree_kernel<DT, D, WC, NB>), dim3((unsigned)workers), dim3(kTreeThreads), 0, st, a);
+    if (int e = check_launch()) return e;
+    hipLaunchKernelGGL((merge_tree_kernel<DT, D, WC, NB>), dim3((unsigned)(a.num_seqs * units_per_seq), WC * NB * (D / 32)),
+                       dim3(kTreeThreads), 0, st, a, units_per_seq);
+    return check_launch();
+}
+
+template <int DT, int D>
+int launch_tree(const TreeArgs& a, const TreeConfig& c, int workers, int units_per_seq, hipStream_t st) {
+    if constexpr (DT != MF_F32 && D <= 128) {
+        if (c.wc == 1) return launch_tree<DT, D, 1, 1>(a, workers, units_per_seq, st);
+        if (c.wc == 2) return launch_tree<DT, D, 2, 1>(a, workers, units_per_seq, st);
+        if (c.nb == 2) return launch_tree<DT, D, 4, 2>(a, workers, units_per_seq, st);
+    }
+    return launch_tree<DT, D, 4, 1>(a, workers, units_per_seq, st);
+}
+
+bool tree_shape_ok(int num_seqs, int64_t num_rows, int max_nodes, int num_q_heads, int num_kv_heads, int head_dim, int dtype) {
+    return num_seqs >= 0 && num_seqs <= kMaxSeqs && num_rows >= 0 && num_rows <= INT_MAX && max_nodes >= 1 &&
+           max_nodes <= MF_TREE_MAX_NODES && num_kv_heads >= 1 && num_q_heads >= num_kv_heads &&
+           num_q_heads % num_kv_heads == 0 && num_q_heads <= (1 << 16) && dtype_ok(dtype) && head_dim > 0;
+}
+bool tree_dim_ok(int head_dim) { return head_dim == 32 || head_dim == 64 || head_dim == 128 || head_dim == 256; }
+
+// Where a plan's parts lie in its buffer, in 32-bit words.
+struct TreeLayout {
+    int64_t head, seq_first, work, seqs, masks, total;
+    int workers, mask_words;
+};
+TreeLayout tree_layout(int num_seqs, int64_t num_rows, int max_nodes, const TreeConfig& c, int num_cus) {
+    TreeLayout l;
+    l.workers = num_cus * c.wgs_per_cu;
+    l.mask_words = (max_nodes + 31) / 32;
+    l.head = 0;
+    l.seq_first = 4;
+    l.work = l.seq_first + 2 * (((int64_t)num_seqs + 1) & ~1ll);
+    l.seqs = l.work + 4 * (int64_t)l.workers;
+    l.masks = l.seqs + (int64_t)kSeqInts * num_seqs;
+    l.total = l.masks + num_rows * l.mask_words;
+    return l;
+}
+
+}  // namespace
+}  // namespace mf
+
+extern "C" int mf_tree_plan_sizes(int num_seqs, int64_t num_rows, int max_nodes, int num_q_heads, int num_kv_heads,
+                                  int head_dim, int dtype, int num_cus, int64_t* plan_words, int64_t* partials_floats) {
+    using namespace mf;
+    if (!tree_shape_ok(num_seqs, num_rows, max_nodes, num_q_heads, num_kv_heads, head_dim, dtype) || num_cus < 1 ||
+        num_cus > 4096 || !plan_words || !partials_floats)
+        return MF_ERR_ARG;
+    if (!tree_dim_ok(head_dim)) return MF_ERR_UNSUPPORTED;
+    const TreeConfig c = tree_config(dtype, head_dim, max_nodes, num_q_heads / num_kv_heads);
+    const TreeLayout l = tree_layout(num_seqs, num_rows, max_nodes, c, num_cus);
+    *plan_words = l.total;
+    *partials_floats = 2 * (int64_t)l.workers * (c.wc * c.nb * 32) * (head_dim + 2);
+    return MF_OK;
+}
+
+extern "C" int mf_tree_plan(const int32_t* parents, const int32_t* cu_nodes, const int32_t* context_lens, int num_seqs,
+                            int64_t num_rows, int max_nodes, int64_t max_context, int num_q_heads, int num_kv_heads,
+                            int head_dim, int dtype, int num_cus, int32_t* plan, int64_t plan_words, int64_t* positions,
+                            mf_stream_t stream) {
+    using namespace mf;
+    int64_t words = 0, floats = 0;
+    if (int e = mf_tree_plan_sizes(num_seqs, num_rows, max_nodes, num_q_heads, num_kv_heads, head_dim, dtype, num_cus,
+                                   &words, &floats))
+        return e;
+    if (max_context < 0 || max_context > (1 << 30)) return MF_ERR_ARG;
+    if (num_seqs == 0) return MF_OK;
+    if (!cu_nodes || !context_lens || !plan || ((uintptr_t)plan & 15) || (num_rows > 0 && (!parents || !positions)))
+        return MF_ERR_ARG;
+    if (plan_words < words) return MF_ERR_WORKSPACE;
+    const int group = num_q_heads / num_kv_heads;
+    const TreeConfig c = tree_config(dtype, head_dim, max_nodes, group);
+    const TreeLayout l = tree_layout(num_seqs, num_rows, max_nodes, c, num_cus);
+    TreePlanArgs a{parents, cu_nodes, context_lens, num_seqs, num_rows, max_nodes, l.mask_words, max_context, group,
+                   num_kv_heads, c.wc * c.nb * 32, l.workers, c.min_share, (int64_t*)(plan + l.head), plan + l.seqs,
+                   (int64_t*)(plan + l.seq_first), plan + l.work, (uint32_t*)(plan + l.masks), positions};
+    hipLaunchKernelGGL(tree_plan_kernel, dim3((unsigned)num_seqs + 1), dim3(kTreeThreads), 0, (hipStream_t)stream, a);
+    return check_launch();
+}
+
+extern "C" int mf_tree_attention(const void* q, int64_t q_stride_row, int64_t q_stride_head, void* out,
+                                 int64_t out_stride_row, int64_t out_stride_head, int dtype, const void* k_pool,
+                                 const void* v_pool, int64_t pool_stride_block, int64_t pool_stride_slot,
+                                 int64_t pool_stride_head, int block_size, int64_t num_blocks,
+                                 const int32_t* block_tables, int64_t block_table_stride, const void* new_k,
+                                 const void* new_v, int64_t new_stride_row, int64_t new_stride_head, int num_seqs,
+                                 int64_t num_rows, int max_nodes, int num_q_heads, int num_kv_heads, int head_dim,
+                                 float scale, int num_cus, const int32_t* plan, int64_t plan_words, float* partials,
+                                 int64_t partials_floats, mf_stream_t stream) {
+    using namespace mf;
+    if (!(std::fabs(scale) < INFINITY)) return MF_ERR_ARG;
+    int64_t words = 0, floats = 0;
+    if (int e = mf_tree_plan_sizes(num_seqs, num_rows, max_nodes, num_q_heads, num_kv_heads, head_dim, dtype, num_cus,
+                                   &words, &floats))
+        return e;
+    if (block_size < 1 || num_blocks < 1 || num_blocks > INT_MAX || block_table_stride < 0) return MF_ERR_ARG;
+    if (num_seqs == 0 || num_rows == 0) return MF_OK;
+    if (!q || !out || !k_pool || !v_pool || !block_tables || !new_k || !new_v || !plan || !partials) return MF_ERR_ARG;
+    if (plan_words < words || partials_floats < floats) return MF_ERR_WORKSPACE;
+    const int es = dtype_size(dtype);
+    const int64_t strides[] = {q_stride_row, q_stride_head, out_stride_row, out_stride_head, pool_stride_block,
+                               pool_stride_slot, pool_stride_head, new_stride_row, new_stride_head};
+    for (int64_t x : strides)
+        if (x % (16 / es)) return MF_ERR_ARG;  // rows are read and written in 16-byte pieces
+    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)new_k | (uintptr_t)new_v |
+         (uintptr_t)plan | (uintptr_t)partials) & 15)
+        return MF_ERR_ARG;
+    const int group = num_q_heads / num_kv_heads;
+    const TreeConfig c = tree_config(dtype, head_dim, max_nodes, group);
+    const TreeLayout l = tree_layout(num_seqs, num_rows, max_nodes, c, num_cus);
+    TreeArgs a{};
+    a.head = (const int64_t*)(plan + l.head);
+    a.work = plan + l.work;
+    a.seqs = plan + l.seqs;
+    a.seq_first = (const int64_t*)(plan + l.seq_first);
+    a.masks = (const uint32_t*)(plan + l.masks);
+    a.mask_words = l.mask_words;
+    a.num_seqs = num_seqs;
+    a.q = (const char*)q;
+    a.q_sr = q_stride_row;
+    a.q_sh = q_stride_head;
+    a.out = (char*)out;
+    a.o_sr = out_stride_row;
+    a.o_sh = out_stride_head;
+    a.k_pool = (const char*)k_pool;
+    a.v_pool = (const char*)v_pool;
+    a.p_sb = pool_stride_block;
+    a.p_ss = pool_stride_slot;
+    a.p_sh = pool_stride_head;
+    a.block_size = block_size;
+    a.block_shift = -1;
+    for (int b = 0; b < 31; ++b)
+        if (1 << b == block_size) a.block_shift = b;
+    a.num_blocks = (uint32_t)num_blocks;
+    a.tables = block_tables;
+    a.table_stride = block_table_stride;
+    a.new_k = (const char*)new_k;
+    a.new_v = (const char*)new_v;
+    a.n_sr = new_stride_row;
+    a.n_sh = new_stride_head;
+    a.group = group;
+    a.num_kv_heads = num_kv_heads;
+    // a negative scale flips the queries' signs; 2^-100 for 0 makes every weight exactly 1
+    a.q_sign = scale < 0.f ? (es == 4 ? 0x80000000u : 0x80008000u) : 0u;
+    a.scale_log2 = scale == 0.f ? 0x1p-100f : std::fabs(scale) * 1.4426950408889634f;
+    a.inv_scale_log2 = 1.f / a.scale_log2;
+    a.partials = partials;
+    const int64_t cols = (int64_t)max_nodes * group;
+    const int units = num_kv_heads * (int)((cols + c.wc * c.nb * 32 - 1) / (c.wc * c.nb * 32));
+    if ((int64_t)num_seqs * units > INT_MAX) return MF_ERR_ARG;
+    hipStream_t st = (hipStream_t)stream;
+#define MF_TREE_CASE(DT, DV) \
+    if (dtype == DT && head_dim == DV) return launch_tree<DT, DV>(a, c, l.workers, units, st);
+    MF_TREE_CASE(MF_BF16, 32)
+    MF_TREE_CASE(MF_BF16, 64)
+    MF_TREE_CASE(MF_BF16, 128)
+    MF_TREE_CASE(MF_BF16, 256)
+    MF_TREE_CASE(MF_F16, 32)
+    MF_TREE_CASE(MF_F16, 64)
+    MF_TREE_CASE(MF_F16, 128)
+    MF_TREE_CASE(MF_F16, 256)
+    MF_TREE_CASE(MF_F32, 32)
+    MF_TREE_CASE(MF_F32, 64)
+    MF_TREE_CASE(MF_F32, 128)
+    MF_TREE_CASE(MF_F32, 256)
+#undef MF_TREE_CASE
+    return MF_ERR_UNSUPPORTED;
+}

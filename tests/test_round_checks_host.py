@@ -116,3 +116,94 @@ def test_sample_and_accept_entry_points_check_sizes():
         args = list(accept)
         args[at] = bad
         assert L.mf_tree_accept(*args) == -1, (at, bad)
+
+
+# ------------------------------------------------------------------------- trees
+
+def _plan(**change):
+    from memforge_amd.kernels.tree_attention import plan_tree
+
+    call = dict(parents=ints(-1, 0, 0), cu_nodes=ints(0, 2, 3), context_lens=ints(5, 9), max_nodes=2, num_q_heads=4,
+                num_kv_heads=2, head_dim=64, dtype=torch.bfloat16, max_context=16)
+    return plan_tree(**{**call, **change})
+
+
+@pytest.mark.parametrize("change", [
+    dict(parents=torch.tensor([-1, 0, 0])), dict(parents=torch.zeros(3)), dict(cu_nodes=ints(0, 3)),
+    dict(cu_nodes=torch.tensor([0, 2, 3])), dict(context_lens=ints(5)), dict(context_lens=torch.tensor([5, 9])),
+    dict(max_nodes=0), dict(max_nodes=1025), dict(max_context=-1), dict(max_context=(1 << 30) + 1), dict(num_kv_heads=0),
+    dict(num_q_heads=5), dict(num_q_heads=0), dict(head_dim=80), dict(head_dim=16), dict(dtype=torch.float64),
+    dict(dtype=torch.int32), dict(context_lens=torch.zeros(2, dtype=torch.int32, device="meta"))])
+def test_tree_plans_refuse(no_gpu_check, monkeypatch, change):
+    monkeypatch.setattr(nat, "device_cus", lambda _: 256)
+    with pytest.raises((ValueError, TypeError)):
+        _plan(**change)
+
+
+def test_tree_plan_needs_the_gpu():
+    with pytest.raises(ValueError):
+        _plan()
+
+
+TREE_CALL = dict(query=torch.zeros((1, 4, 3, 64), dtype=torch.bfloat16),
+                 key_pool=torch.zeros((1, 4, 16, 2, 64), dtype=torch.bfloat16),
+                 value_pool=torch.zeros((1, 4, 16, 2, 64), dtype=torch.bfloat16), layer_idx=0,
+                 block_tables=torch.zeros((2, 1), dtype=torch.int32),
+                 new_keys=torch.zeros((1, 2, 3, 64), dtype=torch.bfloat16),
+                 new_values=torch.zeros((1, 2, 3, 64), dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("change", [
+    dict(query=TREE_CALL["query"][0]), dict(query=TREE_CALL["query"][:, :3]), dict(query=TREE_CALL["query"][:, :, :2]),
+    dict(query=TREE_CALL["query"].float()), dict(query=TREE_CALL["query"].repeat(2, 1, 1, 1)),
+    dict(new_keys=TREE_CALL["new_keys"][:, :1]), dict(new_values=TREE_CALL["new_values"].half()),
+    dict(new_keys=TREE_CALL["new_keys"][..., :32]), dict(block_tables=torch.zeros((1, 1), dtype=torch.int32)),
+    dict(block_tables=torch.zeros((2, 0), dtype=torch.int32)), dict(block_tables=torch.zeros((2, 1))),
+    dict(block_tables=torch.zeros(2, dtype=torch.int32)), dict(block_tables=torch.zeros((2, 2), dtype=torch.int32)[:, ::2]),
+    dict(key_pool=TREE_CALL["key_pool"].float(), value_pool=TREE_CALL["value_pool"].float()),
+    dict(key_pool=TREE_CALL["key_pool"].float()), dict(key_pool=TREE_CALL["key_pool"][:, :, :, :1]),
+    dict(key_pool=TREE_CALL["key_pool"][:, :, :8], value_pool=TREE_CALL["value_pool"][:, :, :8]),
+    dict(scale=float("nan")), dict(scale=float("inf")), dict(new_keys=TREE_CALL["new_keys"].to("meta"))])
+def test_tree_attention_refuses(no_gpu_check, monkeypatch, change):
+    from memforge_amd.kernels.tree_attention import paged_attention_tree
+
+    monkeypatch.setattr(nat, "device_cus", lambda _: 256)
+    launches = []
+    monkeypatch.setattr(nat, "_launch", lambda dev, what, *_: launches.append(what))
+    plan = _plan()
+    paged_attention_tree(**{**TREE_CALL, "plan": plan})
+    assert launches == ["mf_tree_plan", "mf_tree_attention"]
+    with pytest.raises((ValueError, TypeError)):
+        paged_attention_tree(**{**TREE_CALL, "plan": plan, **change})
+    assert len(launches) == 2
+
+
+def test_tree_entry_points_check_sizes():
+    import ctypes
+
+    L, p = nat.lib(), 4096
+    out = (ctypes.c_int64 * 2)()
+    at = ctypes.addressof(out)
+    shape = [2, 3, 2, 4, 2, 64, 2, 256]
+    assert L.mf_tree_plan_sizes(*shape, at, at + 8) == 0 and out[0] > 0 and out[1] > 0
+    words, floats = out[0], out[1]
+    for i, bad, status in ((0, -1, -1), (0, 4097, -1), (1, -1, -1), (2, 0, -1), (2, 1025, -1), (3, 3, -1), (4, 0, -1),
+                           (5, 80, -2), (5, 0, -1), (6, 3, -1), (7, 0, -1), (7, 5000, -1)):
+        args = list(shape)
+        args[i] = bad
+        assert L.mf_tree_plan_sizes(*args, at, at + 8) == status, (i, bad)
+    plan = [p, p, p, 2, 3, 2, 16, 4, 2, 64, 2, 256, p, words, p, None]
+    for i, bad, status in ((0, None, -1), (1, None, -1), (2, None, -1), (6, -1, -1), (12, None, -1), (12, p + 4, -1),
+                           (13, words - 1, -3), (14, None, -1), (9, 48, -2)):
+        args = list(plan)
+        args[i] = bad
+        assert L.mf_tree_plan(*args) == status, (i, bad)
+    call = [p, 256, 64, p, 256, 64, 2, p, p, 2048, 128, 64, 16, 4, p, 1, p, p, 128, 64, 2, 3, 2, 4, 2, 64, 0.125, 256, p, words,
+            p, floats, None]
+    for i, bad, status in ((0, None, -1), (0, p + 2, -1), (1, 257, -1), (3, p + 8, -1), (5, 65, -1), (9, 2049, -1),
+                           (10, 100, -1), (12, 0, -1), (13, 0, -1), (14, None, -1), (15, -1, -1), (16, None, -1),
+                           (18, 4, -1), (25, 48, -2), (26, float("nan"), -1), (26, float("inf"), -1), (28, None, -1),
+                           (29, words - 1, -3), (30, None, -1), (31, floats - 1, -3)):
+        args = list(call)
+        args[i] = bad
+        assert L.mf_tree_attention(*args) == status, (i, bad)
