@@ -168,6 +168,7 @@ def test_tree_attention_refuses(no_gpu_check, monkeypatch, change):
     from memforge_amd.kernels.tree_attention import paged_attention_tree
 
     monkeypatch.setattr(nat, "device_cus", lambda _: 256)
+    monkeypatch.setattr(nat._WORKSPACE, "partials", lambda n, dev: torch.empty(n))
     launches = []
     monkeypatch.setattr(nat, "_launch", lambda dev, what, *_: launches.append(what))
     plan = _plan()
