@@ -193,8 +193,11 @@ struct TreeShape {
     static constexpr int STG = 2 * HALF;
     static constexpr int RING = STG * 4 <= 64 * 1024 ? 4 : STG * 3 <= 64 * 1024 ? 3 : 2;
     static constexpr int NLD = STG / 1024 / 4;             // 1 KB pieces of a stage per wave
+    static constexpr bool SPLIT = NLD == 1;                // two waves load K, two V (otherwise each both)
+    static constexpr int PAIRS = SPLIT ? 1 : NLD / 2;
     static constexpr int NQ = RB / 32;                     // 16-byte pieces of a query row per lane half
     static constexpr int ND = D / 32;
+    static constexpr int WGS = NB == 2 || RB > 256 || RING * STG > 72 * 1024 ? 1 : 2;  // workgroups per CU
     static constexpr int COLS = WC * NB * 32;
     static constexpr int SLOT = COLS * (D + 2);            // floats of a piece's sums
 };
@@ -241,7 +244,7 @@ __device__ __forceinline__ float both_halves_sum(float v) {
 }
 
 template <int DT, int D, int WC, int NB>
-__global__ __launch_bounds__(kTreeThreads) void tree_kernel(TreeArgs a) {
+__global__ __launch_bounds__(kTreeThreads, (TreeShape<DT, D, WC, NB>::WGS)) void tree_kernel(TreeArgs a) {
     using S = TreeShape<DT, D, WC, NB>;
     constexpr int ES = S::ES, RB = S::RB, NCH = S::NCH, RPB = S::RPB, WK = S::WK, NQ = S::NQ, ND = S::ND, NLD = S::NLD;
     constexpr float kNegInf = -__builtin_huge_valf();
@@ -279,6 +282,15 @@ __global__ __launch_bounds__(kTreeThreads) void tree_kernel(TreeArgs a) {
                                   (((4 * d + 2 * ((lane & 31) >> 4) + ((j & 3) >> 1)) ^ (((j >> 2) / RPB) << 2)) << 4) +
                                   8 * (j & 1));
     }
+
+    // 1 KB pieces of a stage: this wave's i-th K piece holds row_of(i) of the stage in this
+    // lane's 16 bytes, its V piece the same row; rows are swizzled in 16-byte chunks
+    auto k_swizzle = [](int in) { return ((in & 15) / RPB) & (NCH - 1); };
+    auto v_swizzle = [](int in) { return DT == MF_F32 ? 0 : ((in & 3) / RPB) << 2; };
+    auto row_of = [&](int i) { return (S::SPLIT ? wave & 1 : wave + 4 * i) * (1024 / RB) + lane * 16 / RB; };
+    auto k_piece = [&](int i) { return ((lane & (NCH - 1)) ^ k_swizzle(row_of(i))) << 4; };
+    auto v_piece = [&](int i) { return ((lane & (NCH - 1)) ^ v_swizzle(row_of(i))) << 4; };
+    const int64_t v_delta = a.v_pool - a.k_pool, nv_delta = a.new_v - a.new_k;
 
     bool first = true;
     while (left > 0) {
@@ -332,38 +344,50 @@ __global__ __launch_bounds__(kTreeThreads) void tree_kernel(TreeArgs a) {
         if (t0 * kTile < key_end) fill_window(t0 * kTile);
         sync();
 
+        const int64_t new_base = (int64_t)row0 * a.n_sr + (int64_t)h * a.n_sh;
         auto fetch = [&](int u, int buf) __attribute__((always_inline)) {
             const int st0 = t0 + u * WK;
-            {
-                const int last = min((st0 + WK) * kTile, key_end) - 1;
-                if (st0 * kTile < key_end && block_of(last) >= window + kWindow) {
-                    sync();
-                    fill_window(st0 * kTile);
-                    sync();
-                }
-            }
             const uint32_t dst0 = ring_at + (uint32_t)(buf * S::STG);
+            if (st0 * kTile < key_end && block_of(min((st0 + WK) * kTile, key_end) - 1) >= window + kWindow) {
+                sync();
+                fill_window(st0 * kTile);
+                sync();
+            }
+            if (st0 + WK <= min(held, t1) && a.block_shift >= 0) {
+                // all keys in the pool; rows past the context's end read its last one: masked, and every
+                // column sees that row
+                const char* kh = a.k_pool + (int64_t)h * a.p_sh * ES;
 #pragma unroll
-            for (int i = 0; i < NLD; ++i) {
-                const int x = wave + 4 * i;
-                constexpr int P = S::STG / 2048;  // pieces of the K half
-                const bool isv = x >= P;
-                const int r = (isv ? x - P : x) * (1024 / RB) + lane * 16 / RB;  // row of the stage
+                for (int i = 0; i < S::PAIRS; ++i) {
+                    const int key = min(st0 * kTile + row_of(i), ctx - 1);
+                    const uint32_t e = min((uint32_t)tab[(key >> a.block_shift) - window], a.num_blocks - 1);
+                    const char* at = kh + ((int64_t)e * a.p_sb + (int64_t)((key & (a.block_size - 1)) * a.p_ss)) * ES;
+                    if constexpr (S::SPLIT) {
+                        ld_lds16(at + (wave & 2 ? v_delta : 0) + (wave & 2 ? v_piece(i) : k_piece(i)),
+                                 dst0 + (uint32_t)(wave * 1024));
+                    } else {
+                        ld_lds16(at + k_piece(i), dst0 + (uint32_t)((wave + 4 * i) * 1024));
+                        ld_lds16(at + v_delta + v_piece(i), dst0 + (uint32_t)(S::HALF + (wave + 4 * i) * 1024));
+                    }
+                }
+                return;
+            }
+#pragma unroll 1
+            for (int x = wave; x < S::STG / 1024; x += 4) {
+                const bool isv = x >= S::STG / 2048;
+                const int r = (isv ? x - S::STG / 2048 : x) * (1024 / RB) + lane * 16 / RB;
                 const int t = min(st0 + (r >> 5), t1 - 1), in = r & 31;
-                const int swz = !isv ? ((in & 15) / RPB) & (NCH - 1) : DT == MF_F32 ? 0 : ((in & 3) / RPB) << 2;
                 const char* src;
                 if (t < held) {
-                    // rows past the context's end read its last one: masked, and every column sees that row
-                    const int key = min(t * kTile + in, ctx - 1);
-                    const int blk = block_of(key);
+                    const int key = min(t * kTile + in, ctx - 1), blk = block_of(key);
                     const uint32_t e = min((uint32_t)tab[blk - window], a.num_blocks - 1);
-                    const int slot = key - blk * a.block_size;
-                    src = (isv ? a.v_pool : a.k_pool) + ((int64_t)e * a.p_sb + (int64_t)slot * a.p_ss + (int64_t)h * a.p_sh) * ES;
+                    src = a.k_pool + ((int64_t)e * a.p_sb + (int64_t)(key - blk * a.block_size) * a.p_ss + (int64_t)h * a.p_sh) * ES +
+                          (isv ? v_delta : 0);
                 } else {
                     const int node = min((t - held) * kTile + in, n - 1);
-                    src = (isv ? a.new_v : a.new_k) + ((int64_t)(row0 + node) * a.n_sr + (int64_t)h * a.n_sh) * ES;
+                    src = a.new_k + (new_base + (int64_t)node * a.n_sr) * ES + (isv ? nv_delta : 0);
                 }
-                ld_lds16(src + (((lane & (NCH - 1)) ^ swz) << 4), dst0 + (uint32_t)(x * 1024));
+                ld_lds16(src + (((lane & (NCH - 1)) ^ (isv ? v_swizzle(in) : k_swizzle(in))) << 4), dst0 + (uint32_t)(x * 1024));
             }
         };
 
@@ -481,9 +505,8 @@ __global__ __launch_bounds__(kTreeThreads) void tree_kernel(TreeArgs a) {
 
         // ---- stages
         constexpr int AHEAD = S::RING - 1;
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u)
-            if (u < nst) fetch(u, u);
+#pragma unroll 1
+        for (int u = 0; u < min(AHEAD, nst); ++u) fetch(u, u);
         int buf = 0;
         for (int u = 0; u < nst; ++u) {
             if (nst - 1 - u >= AHEAD - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((AHEAD - 1) * NLD) : "memory");
