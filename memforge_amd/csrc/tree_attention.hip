@@ -14,8 +14,8 @@
 // batch of uneven ones both fill the GPU, from lengths that only the device knows:
 // the plan (tree_plan_kernel, once for all layers of a step) is made there.
 //
-// Tiles. Four waves, WC side by side on columns (NB blocks of 32 each) and 4 / WC on
-// keys, so a stage of 4 / WC tiles goes from global memory straight into LDS once
+// Tiles. Four or eight waves, WC side by side on blocks of 32 columns and WK along
+// the keys: a stage of WK or more tiles goes from global memory straight into LDS once
 // for all columns; a ring of stages keeps loads in flight. S^T = K Q^T, softmax with
 // a lazily moved maximum, O^T += V^T P^T in 32x32 MFMA blocks whose operands need no
 // move between lanes: as attn_wide_body (attn_kernels.h) lays them out.
@@ -27,11 +27,14 @@
 namespace mf {
 namespace {
 
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+
 constexpr int kTreeThreads = 256;
 constexpr int kTile = 32;            // keys
 constexpr int kMaxSeqs = 4096;
 constexpr int kWindow = 1024;        // block-table entries held in LDS
-constexpr int kSeqInts = 8;          // ctx, nodes, first row, tiles, column groups, context tiles, -, -
+constexpr int kSeqInts = 8;          // context, nodes, first row, tiles, column groups, context tiles, -, -
+constexpr int kWorkInts = 16;        // sequence, unit, tile at which a worker starts, its tiles, and the sequence's first six
 
 struct TreePlanArgs {
     const int32_t* parents;
@@ -48,7 +51,7 @@ struct TreePlanArgs {
     int64_t* head;      // share, all tiles
     int32_t* seqs;
     int64_t* seq_first; // first tile of each sequence in the line
-    int32_t* work;      // (seq, unit, tile, -) at which each worker starts
+    int32_t* work;
     uint32_t* masks;
     int64_t* positions;
 };
@@ -134,7 +137,8 @@ __global__ __launch_bounds__(kTreeThreads) void tree_plan_kernel(TreePlanArgs a)
         a.seq_first[s] = first[s];
     }
     if (tid == 0) first[a.num_seqs] = total;
-    const int64_t share = max((total + a.num_workers - 1) / a.num_workers, (int64_t)a.min_share);
+    // (a worker's tiles fit 32 bits: fewer than 2^26 in a sequence of one kv head, spread over all of them)
+    const int64_t share = min(max((total + a.num_workers - 1) / a.num_workers, (int64_t)a.min_share), (int64_t)INT_MAX);
     if (tid == 0) {
         a.head[0] = share;
         a.head[1] = total;
@@ -142,7 +146,10 @@ __global__ __launch_bounds__(kTreeThreads) void tree_plan_kernel(TreePlanArgs a)
     __syncthreads();
     for (int w = tid; w < a.num_workers; w += kTreeThreads) {
         const int64_t at = (int64_t)w * share;
-        if (at >= total) break;
+        if (at >= total) {
+            a.work[(int64_t)w * kWorkInts + 3] = 0;
+            continue;
+        }
         int lo = 0, hi = a.num_seqs - 1;  // the last sequence that starts at or before `at`: it has tiles
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
@@ -151,7 +158,11 @@ __global__ __launch_bounds__(kTreeThreads) void tree_plan_kernel(TreePlanArgs a)
         }
         const int tiles = a.seqs[(int64_t)lo * kSeqInts + 3];
         const int64_t in = at - first[lo];
-        *(int4*)(a.work + 4 * w) = make_int4(lo, (int)(in / tiles), (int)(in % tiles), 0);
+        const int32_t* q = a.seqs + (int64_t)lo * kSeqInts;
+        int4* to = (int4*)(a.work + (int64_t)w * kWorkInts);
+        to[0] = make_int4(lo, (int)(in / tiles), (int)(in % tiles), (int)min(share, total - at));
+        to[1] = make_int4(q[0], q[1], q[2], tiles);
+        to[2] = make_int4(q[4], q[5], 0, 0);
     }
 }
 
@@ -181,25 +192,27 @@ struct TreeArgs {
     float* partials;
 };
 
-template <int DT, int D, int WC, int NB>
+template <int DT, int D, int WC, int WK>
 struct TreeShape {
     static constexpr int ES = DT == MF_F32 ? 4 : 2;
+    static constexpr int WAVES = WC * WK;
     static constexpr int RB = D * ES;                      // bytes of a key row
     static constexpr int NCH = RB / 16;                    // its 16-byte chunks
     static constexpr int RPB = RB >= 256 ? 1 : 256 / RB;   // rows in 256 bytes (every LDS bank once)
-    static constexpr int WK = 4 / WC;                      // waves along the keys
     static constexpr int TILE = kTile * RB;
-    static constexpr int HALF = WK * TILE;                 // K rows of a stage, then its V rows
+    static constexpr int SUB = WK * TILE >= 8192 ? 1 : 8192 / (WK * TILE);  // tiles of a wave in a stage
+    static constexpr int ST = WK * SUB;                    // tiles of a stage
+    static constexpr int HALF = ST * TILE;                 // its K rows, then its V rows
     static constexpr int STG = 2 * HALF;
-    static constexpr int RING = STG * 4 <= 64 * 1024 ? 4 : STG * 3 <= 64 * 1024 ? 3 : 2;
-    static constexpr int NLD = STG / 1024 / 4;             // 1 KB pieces of a stage per wave
-    static constexpr bool SPLIT = NLD == 1;                // two waves load K, two V (otherwise each both)
-    static constexpr int PAIRS = SPLIT ? 1 : NLD / 2;
+    static constexpr int RING = STG * 4 <= 64 * 1024 ? 4 : 2;
+    static constexpr int PAIRS = HALF / 1024 / WAVES;      // 1 KB pieces of K, and of V, per wave and stage
+    static constexpr int NLD = 2 * PAIRS;
     static constexpr int NQ = RB / 32;                     // 16-byte pieces of a query row per lane half
     static constexpr int ND = D / 32;
-    static constexpr int WGS = NB == 2 || RB > 256 || RING * STG > 72 * 1024 ? 1 : 2;  // workgroups per CU
-    static constexpr int COLS = WC * NB * 32;
+    static constexpr int PER_CU = WAVES == 8 || RB > 256 || RING * STG > 72 * 1024 ? 1 : 2;  // workgroups
+    static constexpr int COLS = WC * 32;
     static constexpr int SLOT = COLS * (D + 2);            // floats of a piece's sums
+    static_assert(PAIRS >= 1 && HALF % (1024 * WAVES) == 0, "whole pieces for every wave");
 };
 
 // Sum and maximum of a column live in two lanes (lane halves); O^T's lane (hf, column)
@@ -243,21 +256,20 @@ __device__ __forceinline__ float both_halves_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-template <int DT, int D, int WC, int NB>
-__global__ __launch_bounds__(kTreeThreads, (TreeShape<DT, D, WC, NB>::WGS)) void tree_kernel(TreeArgs a) {
-    using S = TreeShape<DT, D, WC, NB>;
-    constexpr int ES = S::ES, RB = S::RB, NCH = S::NCH, RPB = S::RPB, WK = S::WK, NQ = S::NQ, ND = S::ND, NLD = S::NLD;
+template <int DT, int D, int WC, int WK>
+__global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * WC * WK / 4)) void tree_kernel(TreeArgs a) {
+    using S = TreeShape<DT, D, WC, WK>;
+    constexpr int ES = S::ES, RB = S::RB, NCH = S::NCH, RPB = S::RPB, NQ = S::NQ, ND = S::ND, ST = S::ST;
+    constexpr int AHEAD = S::RING - 1;  // stages in flight
     constexpr float kNegInf = -__builtin_huge_valf();
     __shared__ __align__(1024) char ring[S::RING * S::STG];
     __shared__ int tab[kWindow];
-    static_assert(WK == 1 || (WK - 1) * WC * NB * (ND * 16 + 2) * 256 <= S::RING * S::STG, "the key waves' sums fit the ring");
+    static_assert(WK == 1 || (WK - 1) * WC * (ND * 16 + 2) * 256 <= S::RING * S::STG, "the key waves' sums fit the ring");
 
-    const int64_t share = a.head[0], total = a.head[1];
-    const int64_t begin = (int64_t)blockIdx.x * share;
-    if (begin >= total) return;
-    int64_t left = min(share, total - begin);
-    const int4 at = *(const int4*)(a.work + 4 * blockIdx.x);
-    int s = at.x, unit = at.y, tile0 = at.z;
+    const int32_t* at = a.work + (int64_t)blockIdx.x * kWorkInts;
+    int s = at[0], unit = at[1], tile0 = at[2], left = at[3];
+    int ctx = at[4], n = at[5], row0 = at[6], tiles = at[7], groups = at[8], held = at[9];
+    if (left <= 0) return;
     const int tid = threadIdx.x, lane = tid & 63, hf = lane >> 5, j = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wc = wave % WC, wk = wave / WC;
@@ -268,343 +280,318 @@ __global__ __launch_bounds__(kTreeThreads, (TreeShape<DT, D, WC, NB>::WGS)) void
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    // lane addresses inside a wave's tile: K rows (key lane & 31), V rows
+    // lane addresses inside a tile: K rows (key lane & 31), V rows
     uint32_t kaddr[NQ], vaddr[ND];
 #pragma unroll
     for (int c = 0; c < NQ; ++c)
-        kaddr[c] = (uint32_t)(wk * S::TILE + (lane & 31) * RB + (((2 * c + hf) ^ ((j / RPB) & (NCH - 1))) << 4));
+        kaddr[c] = (uint32_t)((lane & 31) * RB + (((2 * c + hf) ^ ((j / RPB) & (NCH - 1))) << 4));
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
         if constexpr (DT == MF_F32)
-            vaddr[d] = (uint32_t)(S::HALF + wk * S::TILE + 4 * hf * RB + (32 * d + (lane & 31)) * 4);
+            vaddr[d] = (uint32_t)(S::HALF + 4 * hf * RB + (32 * d + (lane & 31)) * 4);
         else
-            vaddr[d] = (uint32_t)(S::HALF + wk * S::TILE + (4 * hf + (j >> 2)) * RB +
+            vaddr[d] = (uint32_t)(S::HALF + (4 * hf + (j >> 2)) * RB +
                                   (((4 * d + 2 * ((lane & 31) >> 4) + ((j & 3) >> 1)) ^ (((j >> 2) / RPB) << 2)) << 4) +
                                   8 * (j & 1));
     }
-
     // 1 KB pieces of a stage: this wave's i-th K piece holds row_of(i) of the stage in this
     // lane's 16 bytes, its V piece the same row; rows are swizzled in 16-byte chunks
     auto k_swizzle = [](int in) { return ((in & 15) / RPB) & (NCH - 1); };
     auto v_swizzle = [](int in) { return DT == MF_F32 ? 0 : ((in & 3) / RPB) << 2; };
-    auto row_of = [&](int i) { return (S::SPLIT ? wave & 1 : wave + 4 * i) * (1024 / RB) + lane * 16 / RB; };
+    auto row_of = [&](int i) { return (wave + S::WAVES * i) * (1024 / RB) + lane * 16 / RB; };
     auto k_piece = [&](int i) { return ((lane & (NCH - 1)) ^ k_swizzle(row_of(i))) << 4; };
     auto v_piece = [&](int i) { return ((lane & (NCH - 1)) ^ v_swizzle(row_of(i))) << 4; };
     const int64_t v_delta = a.v_pool - a.k_pool, nv_delta = a.new_v - a.new_k;
+    auto block_of = [&](int key) -> int {
+        return a.block_shift >= 0 ? key >> a.block_shift : (int)((unsigned)key / (unsigned)a.block_size);
+    };
 
     bool first = true;
-    while (left > 0) {
-        const int32_t* info = a.seqs + (int64_t)s * kSeqInts;
-        const int ctx = info[0], n = info[1], row0 = info[2], tiles = info[3], groups = info[4], held = info[5];
-        if (tiles == 0) {
-            ++s;
-            unit = 0;
-            tile0 = 0;
-            continue;
-        }
-        const int h = unit / groups, grp = unit - h * groups;
-        const int t0 = tile0, t1 = (int)min((int64_t)tiles, t0 + left);
-        const int nst = (t1 - t0 + WK - 1) / WK;
-
-        // ---- this lane's columns
-        int cidx[NB];
-        bool valid[NB];
-        int64_t prow[NB];
-        int qhead[NB];
-        uint4 qf[NB][NQ];
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            cidx[b] = grp * S::COLS + (wc * NB + b) * 32 + (lane & 31);
-            valid[b] = cidx[b] < n * a.group;
-            const int c = valid[b] ? cidx[b] : 0;
-            const int node = (int)((unsigned)c / (unsigned)a.group);
-            prow[b] = row0 + node;
-            qhead[b] = h * a.group + c - node * a.group;
-            const char* qp = a.q + (prow[b] * a.q_sr + (int64_t)qhead[b] * a.q_sh) * ES;
-#pragma unroll
-            for (int c2 = 0; c2 < NQ; ++c2) {
-                const uint4 v = *(const uint4*)(qp + (2 * c2 + hf) * 16);
-                qf[b][c2] = make_uint4(v.x ^ a.q_sign, v.y ^ a.q_sign, v.z ^ a.q_sign, v.w ^ a.q_sign);
-            }
-        }
-        const bool busy = grp * S::COLS + wc * NB * 32 < n * a.group;  // a wave of padding columns only loads
-
-        // ---- block-table entries of the piece's keys, a window of them in LDS
+    for (;;) {
+        // ---- one sequence: its block-table entries, or a window of them, in LDS
         const int32_t* trow = a.tables + (int64_t)s * a.table_stride;
-        auto block_of = [&](int key) -> int {
-            return a.block_shift >= 0 ? key >> a.block_shift : (int)((unsigned)key / (unsigned)a.block_size);
-        };
-        int window = 0;
-        const int key_end = min(t1 * kTile, ctx);
+        int window = 0, window_lo = 0, window_hi = 0;  // first block, and the keys it covers
         auto fill_window = [&](int from_key) {
-            window = block_of(from_key);
-            const int end = min(window + kWindow, block_of(key_end - 1) + 1);
-            for (int i = window + tid; i < end; i += kTreeThreads) tab[i - window] = trow[i];
+            const int blocks = ctx > 0 ? block_of(ctx - 1) + 1 : 0;
+            window = blocks <= kWindow ? 0 : block_of(from_key);
+            window_lo = window * a.block_size;
+            window_hi = blocks - window <= kWindow ? ctx : (window + kWindow) * a.block_size;
+            const int end = min(window + kWindow, blocks);
+            for (int i = window + tid; i < end; i += S::WAVES * 64) tab[i - window] = trow[i];
         };
-        if (t0 * kTile < key_end) fill_window(t0 * kTile);
+        fill_window(tile0 * kTile);
         sync();
 
-        const int64_t new_base = (int64_t)row0 * a.n_sr + (int64_t)h * a.n_sh;
-        auto fetch = [&](int u, int buf) __attribute__((always_inline)) {
-            const int st0 = t0 + u * WK;
-            const uint32_t dst0 = ring_at + (uint32_t)(buf * S::STG);
-            if (st0 * kTile < key_end && block_of(min((st0 + WK) * kTile, key_end) - 1) >= window + kWindow) {
+        // ---- stages in the order of the line: across the sequence's units where every
+        // wave has columns of its own (WK 1); the key waves' sums need the ring at a unit's end
+        const int units = groups * a.num_kv_heads;
+        int f_unit = unit, f_tile = tile0;
+        int f_left = WK == 1 ? (int)min((int64_t)left, (int64_t)(units - unit) * tiles - tile0) : min(left, tiles - tile0);
+        const int run = f_left;
+        int in_flight = 0, head_buf = 0, next_buf = 0;
+        auto fetch = [&]() __attribute__((always_inline)) {
+            const int take = min(min(ST, f_left), tiles - f_tile);
+            const int h = f_unit / groups, st0 = f_tile, t_end = st0 + take;
+            const uint32_t dst0 = ring_at + (uint32_t)(next_buf * S::STG);
+            const int first_key = st0 * kTile, end_key = min(t_end * kTile, ctx);
+            if (first_key < end_key && (first_key < window_lo || end_key > window_hi)) {
                 sync();
-                fill_window(st0 * kTile);
+                fill_window(first_key);
                 sync();
             }
-            if (st0 + WK <= min(held, t1) && a.block_shift >= 0) {
+            if (st0 + ST <= min(held, t_end) && a.block_shift >= 0) {
                 // all keys in the pool; rows past the context's end read its last one: masked, and every
                 // column sees that row
                 const char* kh = a.k_pool + (int64_t)h * a.p_sh * ES;
+                uint32_t e[S::PAIRS];
+                int key[S::PAIRS];
 #pragma unroll
                 for (int i = 0; i < S::PAIRS; ++i) {
-                    const int key = min(st0 * kTile + row_of(i), ctx - 1);
-                    const uint32_t e = min((uint32_t)tab[(key >> a.block_shift) - window], a.num_blocks - 1);
-                    const char* at = kh + ((int64_t)e * a.p_sb + (int64_t)((key & (a.block_size - 1)) * a.p_ss)) * ES;
-                    if constexpr (S::SPLIT) {
-                        ld_lds16(at + (wave & 2 ? v_delta : 0) + (wave & 2 ? v_piece(i) : k_piece(i)),
-                                 dst0 + (uint32_t)(wave * 1024));
-                    } else {
-                        ld_lds16(at + k_piece(i), dst0 + (uint32_t)((wave + 4 * i) * 1024));
-                        ld_lds16(at + v_delta + v_piece(i), dst0 + (uint32_t)(S::HALF + (wave + 4 * i) * 1024));
-                    }
+                    key[i] = min(first_key + row_of(i), ctx - 1);
+                    e[i] = (uint32_t)tab[(key[i] >> a.block_shift) - window];
                 }
-                return;
-            }
-#pragma unroll 1
-            for (int x = wave; x < S::STG / 1024; x += 4) {
-                const bool isv = x >= S::STG / 2048;
-                const int r = (isv ? x - S::STG / 2048 : x) * (1024 / RB) + lane * 16 / RB;
-                const int t = min(st0 + (r >> 5), t1 - 1), in = r & 31;
-                const char* src;
-                if (t < held) {
-                    const int key = min(t * kTile + in, ctx - 1), blk = block_of(key);
-                    const uint32_t e = min((uint32_t)tab[blk - window], a.num_blocks - 1);
-                    src = a.k_pool + ((int64_t)e * a.p_sb + (int64_t)(key - blk * a.block_size) * a.p_ss + (int64_t)h * a.p_sh) * ES +
-                          (isv ? v_delta : 0);
-                } else {
-                    const int node = min((t - held) * kTile + in, n - 1);
-                    src = a.new_k + (new_base + (int64_t)node * a.n_sr) * ES + (isv ? nv_delta : 0);
-                }
-                ld_lds16(src + (((lane & (NCH - 1)) ^ (isv ? v_swizzle(in) : k_swizzle(in))) << 4), dst0 + (uint32_t)(x * 1024));
-            }
-        };
-
-        float m[NB], l[NB], thr[NB];
-        f32x16 acc[NB][ND];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            m[b] = kMinM;
-            l[b] = 0.f;
-            thr[b] = (kMinM + kLazyLog2) * a.inv_scale_log2;
+                for (int i = 0; i < S::PAIRS; ++i) {
+                    const char* src = kh + ((int64_t)min(e[i], a.num_blocks - 1) * a.p_sb +
+                                            (int64_t)(key[i] & (a.block_size - 1)) * a.p_ss) * ES;
+                    ld_lds16(src + k_piece(i), dst0 + (uint32_t)((wave + S::WAVES * i) * 1024));
+                    ld_lds16(src + v_delta + v_piece(i), dst0 + (uint32_t)(S::HALF + (wave + S::WAVES * i) * 1024));
+                }
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < S::PAIRS; ++i) {
+                    const int r = row_of(i), in = r & 31;
+                    const int t = min(st0 + (r >> 5), t_end - 1);
+                    const char* src;
+                    int64_t to_v;
+                    if (t < held) {
+                        const int key = min(t * kTile + in, ctx - 1), blk = block_of(key);
+                        const uint32_t e = min((uint32_t)tab[blk - window], a.num_blocks - 1);
+                        src = a.k_pool + ((int64_t)e * a.p_sb + (int64_t)(key - blk * a.block_size) * a.p_ss + (int64_t)h * a.p_sh) * ES;
+                        to_v = v_delta;
+                    } else {
+                        const int node = min((t - held) * kTile + in, n - 1);
+                        src = a.new_k + ((int64_t)(row0 + node) * a.n_sr + (int64_t)h * a.n_sh) * ES;
+                        to_v = nv_delta;
+                    }
+                    ld_lds16(src + k_piece(i), dst0 + (uint32_t)((wave + S::WAVES * i) * 1024));
+                    ld_lds16(src + to_v + v_piece(i), dst0 + (uint32_t)(S::HALF + (wave + S::WAVES * i) * 1024));
+                }
+            }
+            f_left -= take;
+            f_tile += take;
+            if (f_tile == tiles) {
+                f_tile = 0;
+                ++f_unit;
+            }
+            ++in_flight;
+            next_buf = next_buf + 1 == S::RING ? 0 : next_buf + 1;
+        };
+#pragma unroll 1
+        for (int u = 0; u < AHEAD && f_left > 0; ++u) fetch();
+
+        int done = 0;
+        while (done < run) {
+            // ---- one (kv head, column group): this lane's column and query
+            const int h = unit / groups, grp = unit - h * groups;
+            const int t0 = tile0, t1 = min(tiles, t0 + run - done);
+            const int cidx = grp * S::COLS + wc * 32 + (lane & 31);
+            const bool valid = cidx < n * a.group;
+            const int node = (int)((unsigned)(valid ? cidx : 0) / (unsigned)a.group);
+            const int64_t prow = row0 + node;
+            const int qhead = h * a.group + (valid ? cidx : 0) - node * a.group;
+            const bool busy = grp * S::COLS + wc * 32 < n * a.group;  // a wave of padding columns only loads
+            uint4 qf[NQ];
+            const char* qp = a.q + (prow * a.q_sr + (int64_t)qhead * a.q_sh) * ES;
+#pragma unroll
+            for (int c = 0; c < NQ; ++c) {
+                const uint4 v = *(const uint4*)(qp + (2 * c + hf) * 16);
+                qf[c] = make_uint4(v.x ^ a.q_sign, v.y ^ a.q_sign, v.z ^ a.q_sign, v.w ^ a.q_sign);
+            }
+            float m = kMinM, l = 0.f, thr = (kMinM + kLazyLog2) * a.inv_scale_log2;
+            f32x16 acc[ND];
 #pragma unroll
             for (int d = 0; d < ND; ++d)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc[b][d][i] = 0.f;
-        }
+                for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
 
-        auto tile = [&](const char* stg, int t) __attribute__((always_inline)) {
-            f32x16 st[NB];
+            auto tile = [&](const char* stg, int t) __attribute__((always_inline)) {
+                f32x16 st;
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+                for (int i = 0; i < 16; ++i) st[i] = 0.f;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) st[b][i] = 0.f;
-#pragma unroll
-            for (int c = 0; c < NQ; ++c) {
-                const uint4 kf = *(const uint4*)(stg + kaddr[c]);
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
+                for (int c = 0; c < NQ; ++c) {
+                    const uint4 kf = *(const uint4*)(stg + kaddr[c]);
                     if constexpr (DT == MF_F32) {
-                        st[b] = mfma32_f32(__uint_as_float(kf.x), __uint_as_float(qf[b][c].x), st[b]);
-                        st[b] = mfma32_f32(__uint_as_float(kf.y), __uint_as_float(qf[b][c].y), st[b]);
-                        st[b] = mfma32_f32(__uint_as_float(kf.z), __uint_as_float(qf[b][c].z), st[b]);
-                        st[b] = mfma32_f32(__uint_as_float(kf.w), __uint_as_float(qf[b][c].w), st[b]);
+                        st = mfma32_f32(__uint_as_float(kf.x), __uint_as_float(qf[c].x), st);
+                        st = mfma32_f32(__uint_as_float(kf.y), __uint_as_float(qf[c].y), st);
+                        st = mfma32_f32(__uint_as_float(kf.z), __uint_as_float(qf[c].z), st);
+                        st = mfma32_f32(__uint_as_float(kf.w), __uint_as_float(qf[c].w), st);
                     } else {
-                        st[b] = mfma32<DT>(kf, qf[b][c], st[b]);
+                        st = mfma32<DT>(kf, qf[c], st);
                     }
                 }
-            }
-            if (t >= held || (t + 1) * kTile > ctx) {  // the context's last tile, and the nodes'
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
+                if ((t + 1) * kTile > ctx) {  // the context's last tile, and the nodes'
                     uint32_t seen;
                     if (t < held) seen = 0xffffffffu >> ((t + 1) * kTile - ctx);
-                    else seen = valid[b] ? a.masks[prow[b] * a.mask_words + (t - held)] : 0u;
+                    else seen = valid ? a.masks[prow * a.mask_words + (t - held)] : 0u;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int key = 8 * (i >> 2) + 4 * hf + (i & 3);
-                        st[b][i] = seen >> key & 1u ? st[b][i] : kNegInf;
+                        st[i] = seen >> key & 1u ? st[i] : kNegInf;
                     }
                 }
-            }
-            // lazy rescale: the maximum moves when a score passes it by more than 2^8
+                // lazy rescale: the maximum moves when a score passes it by more than 2^8
+                float lmax = st[0];
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                float lmax = st[b][0];
-#pragma unroll
-                for (int i = 1; i < 16; ++i) lmax = fmax_prop(lmax, st[b][i]);
-                if (__builtin_amdgcn_ballot_w64(lmax > thr[b]) != 0) {
+                for (int i = 1; i < 16; ++i) lmax = fmax_prop(lmax, st[i]);
+                if (__builtin_amdgcn_ballot_w64(lmax > thr) != 0) {
                     auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(lmax), __float_as_uint(lmax), false, false);
-                    const float mn = fmaxf(m[b], fmax_prop(__uint_as_float(r[0]), __uint_as_float(r[1])) * a.scale_log2);
-                    const float alpha = __builtin_amdgcn_exp2f(m[b] - mn);
-                    l[b] *= alpha;
+                    const float mn = fmaxf(m, fmax_prop(__uint_as_float(r[0]), __uint_as_float(r[1])) * a.scale_log2);
+                    const float alpha = __builtin_amdgcn_exp2f(m - mn);
+                    l *= alpha;
 #pragma unroll
                     for (int d = 0; d < ND; ++d)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) acc[b][d][i] *= alpha;
-                    m[b] = mn;
-                    thr[b] = (mn + kLazyLog2) * a.inv_scale_log2;
+                        for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
+                    m = mn;
+                    thr = (mn + kLazyLog2) * a.inv_scale_log2;
                 }
-            }
-            uint32_t pw[NB][8];
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
                 float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    st[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[b][i], a.scale_log2, -m[b]));
-                    sum += st[b][i];
+                    st[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i], a.scale_log2, -m));
+                    sum += st[i];
                 }
-                l[b] += sum;
-                if constexpr (DT != MF_F32) {
+                l += sum;
+                if constexpr (DT == MF_F32) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+#pragma unroll
+                        for (int d = 0; d < ND; ++d)
+                            acc[d] = mfma32_f32(*(const float*)(stg + vaddr[d] + (8 * (i >> 2) + (i & 3)) * RB), st[i], acc[d]);
+                } else {
+                    // 16-bit operands of the second product: each weight off by half a step of the type
+                    uint32_t pw[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        // 16-bit operands of the second product: each weight off by half a step of the type
                         if constexpr (DT == MF_BF16)
-                            pw[b][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){st[b][2 * i], st[b][2 * i + 1]}, bf16x2));
+                            pw[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){st[2 * i], st[2 * i + 1]}, bf16x2));
                         else
-                            pw[b][i] = f32_to_bits<DT>(st[b][2 * i]) | (f32_to_bits<DT>(st[b][2 * i + 1]) << 16);
+                            pw[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){st[2 * i], st[2 * i + 1]}, f16x2));
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int d = 0; d < ND; ++d) {
+                            const uint2 v0 = ld_tr16(stg + vaddr[d] + 16 * k * RB);
+                            const uint2 v1 = ld_tr16(stg + vaddr[d] + (16 * k + 8) * RB);
+                            acc[d] = mfma32<DT>(make_uint4(v0.x, v0.y, v1.x, v1.y),
+                                                make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]), acc[d]);
+                        }
+                }
+            };
+
+            for (int st0 = t0; st0 < t1; st0 += ST) {
+                if (in_flight == AHEAD) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((AHEAD - 1) * S::NLD) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                --in_flight;
+                sync();  // the oldest stage is whole, and the one before it has been read
+                if (f_left > 0) fetch();
+                if (busy) {
+                    const char* stg = ring + head_buf * S::STG;
+#pragma unroll 1
+                    for (int x = 0; x < S::SUB; ++x) {
+                        const int t = st0 + x * WK + wk;
+                        if (t < t1) tile(stg + (x * WK + wk) * S::TILE, t);
                     }
                 }
+                head_buf = head_buf + 1 == S::RING ? 0 : head_buf + 1;
             }
-            if constexpr (DT == MF_F32) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-#pragma unroll
-                    for (int d = 0; d < ND; ++d) {
-                        const float v = *(const float*)(stg + vaddr[d] + (8 * (i >> 2) + (i & 3)) * RB);
-#pragma unroll
-                        for (int b = 0; b < NB; ++b) acc[b][d] = mfma32_f32(v, st[b][i], acc[b][d]);
-                    }
-            } else {
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-#pragma unroll
-                    for (int d = 0; d < ND; ++d) {
-                        const uint2 v0 = ld_tr16(stg + vaddr[d] + 16 * k * RB);
-                        const uint2 v1 = ld_tr16(stg + vaddr[d] + (16 * k + 8) * RB);
-#pragma unroll
-                        for (int b = 0; b < NB; ++b)
-                            acc[b][d] = mfma32<DT>(make_uint4(v0.x, v0.y, v1.x, v1.y),
-                                                   make_uint4(pw[b][4 * k], pw[b][4 * k + 1], pw[b][4 * k + 2], pw[b][4 * k + 3]),
-                                                   acc[b][d]);
-                    }
-            }
-        };
 
-        // ---- stages
-        constexpr int AHEAD = S::RING - 1;
-#pragma unroll 1
-        for (int u = 0; u < min(AHEAD, nst); ++u) fetch(u, u);
-        int buf = 0;
-        for (int u = 0; u < nst; ++u) {
-            if (nst - 1 - u >= AHEAD - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((AHEAD - 1) * NLD) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            sync();  // stage u is whole, and the one before has been read
-            if (u + AHEAD < nst) fetch(u + AHEAD, buf == 0 ? S::RING - 1 : buf - 1);
-            const int t = t0 + u * WK + wk;
-            if (busy && t < t1) tile(ring + buf * S::STG, t);
-            buf = buf + 1 == S::RING ? 0 : buf + 1;
-        }
-        sync();
-
-        // ---- the key waves' sums in one, then the piece's result
-#pragma unroll
-        for (int b = 0; b < NB; ++b) l[b] = both_halves_sum(l[b]);
-        if constexpr (WK > 1) {
-            constexpr int PART = NB * (ND * 16 + 2) * 64;
-            float* mine = (float*)ring + ((wk - 1) * WC + wc) * PART;
-            if (wk > 0) {
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    float* to = mine + b * (ND * 16 + 2) * 64;
+            // ---- the key waves' sums in one, then the piece's result
+            l = both_halves_sum(l);
+            if constexpr (WK > 1) {
+                constexpr int PART = (ND * 16 + 2) * 64;
+                sync();
+                if (wk > 0) {
+                    float* to = (float*)ring + ((wk - 1) * WC + wc) * PART;
 #pragma unroll
                     for (int d = 0; d < ND; ++d)
 #pragma unroll
                         for (int i = 0; i < 16; i += 4)
-                            *(float4*)(to + (d * 16 + i) * 64 + 4 * lane) =
-                                make_float4(acc[b][d][i], acc[b][d][i + 1], acc[b][d][i + 2], acc[b][d][i + 3]);
-                    to[ND * 1024 + lane] = m[b];
-                    to[ND * 1024 + 64 + lane] = l[b];
+                            *(float4*)(to + (d * 16 + i) * 64 + 4 * lane) = make_float4(acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]);
+                    to[ND * 1024 + lane] = m;
+                    to[ND * 1024 + 64 + lane] = l;
                 }
-            }
-            sync();
-            if (wk == 0) {
+                sync();
+                if (wk == 0) {
 #pragma unroll
-                for (int o = 0; o < WK - 1; ++o)
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        const float* from = (const float*)ring + (o * WC + wc) * PART + b * (ND * 16 + 2) * 64;
+                    for (int o = 0; o < WK - 1; ++o) {
+                        const float* from = (const float*)ring + (o * WC + wc) * PART;
                         const float m1 = from[ND * 1024 + lane], l1 = from[ND * 1024 + 64 + lane];
-                        const float mn = fmaxf(m[b], m1);
-                        const float w0 = __builtin_amdgcn_exp2f(m[b] - mn), w1 = __builtin_amdgcn_exp2f(m1 - mn);
-                        m[b] = mn;
-                        l[b] = l[b] * w0 + l1 * w1;
+                        const float mn = fmaxf(m, m1);
+                        const float w0 = __builtin_amdgcn_exp2f(m - mn), w1 = __builtin_amdgcn_exp2f(m1 - mn);
+                        m = mn;
+                        l = l * w0 + l1 * w1;
 #pragma unroll
                         for (int d = 0; d < ND; ++d)
 #pragma unroll
                             for (int i = 0; i < 16; i += 4) {
                                 const float4 v = *(const float4*)(from + (d * 16 + i) * 64 + 4 * lane);
-                                acc[b][d][i] = acc[b][d][i] * w0 + v.x * w1;
-                                acc[b][d][i + 1] = acc[b][d][i + 1] * w0 + v.y * w1;
-                                acc[b][d][i + 2] = acc[b][d][i + 2] * w0 + v.z * w1;
-                                acc[b][d][i + 3] = acc[b][d][i + 3] * w0 + v.w * w1;
+                                acc[d][i] = acc[d][i] * w0 + v.x * w1;
+                                acc[d][i + 1] = acc[d][i + 1] * w0 + v.y * w1;
+                                acc[d][i + 2] = acc[d][i + 2] * w0 + v.z * w1;
+                                acc[d][i + 3] = acc[d][i + 3] * w0 + v.w * w1;
                             }
                     }
+                }
             }
-        }
-        if (wk == 0 && busy) {
-            const bool whole = t0 == 0 && t1 == tiles;
-            if (whole) {
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-                    store_column<DT, ND>(a.out + (prow[b] * a.o_sr + (int64_t)qhead[b] * a.o_sh) * ES, valid[b], acc[b],
-                                         1.f / l[b], hf);
-            } else {
-                float* slot = a.partials + (2 * (int64_t)blockIdx.x + (first ? 0 : 1)) * S::SLOT;
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    float* to = slot + (wc * NB + b) * 32 * (D + 2);
+            if (wk == 0 && busy) {
+                if (t0 == 0 && t1 == tiles) {
+                    store_column<DT, ND>(a.out + (prow * a.o_sr + (int64_t)qhead * a.o_sh) * ES, valid, acc, 1.f / l, hf);
+                } else {
+                    float* to = a.partials + (2 * (int64_t)blockIdx.x + (first ? 0 : 1)) * S::SLOT + wc * 32 * (D + 2);
 #pragma unroll
                     for (int d = 0; d < ND; ++d)
 #pragma unroll
                         for (int i = 0; i < 16; i += 4)
-                            *(float4*)(to + (d * 16 + i) * 64 + 4 * lane) =
-                                make_float4(acc[b][d][i], acc[b][d][i + 1], acc[b][d][i + 2], acc[b][d][i + 3]);
+                            *(float4*)(to + (d * 16 + i) * 64 + 4 * lane) = make_float4(acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]);
                     if (hf == 0) {
-                        to[32 * D + lane] = m[b];
-                        to[32 * D + 32 + lane] = l[b];
+                        to[32 * D + lane] = m;
+                        to[32 * D + 32 + lane] = l;
                     }
                 }
             }
+            first = false;
+            done += t1 - t0;
+            tile0 = t1 == tiles ? 0 : t1;
+            unit += t1 == tiles;
         }
-        sync();  // the ring and the window are free
-        left -= t1 - t0;
-        first = false;
-        tile0 = 0;
-        if (++unit == groups * a.num_kv_heads) {
+        left -= run;
+        if (left <= 0) return;
+        sync();  // the ring and the window have been read
+        if (unit == units) {
             unit = 0;
-            ++s;
+            do {
+                ++s;
+                const int32_t* info = a.seqs + (int64_t)s * kSeqInts;
+                ctx = info[0];
+                n = info[1];
+                row0 = info[2];
+                tiles = info[3];
+                groups = info[4];
+                held = info[5];
+            } while (tiles == 0);  // the line has `left` more tiles, so a sequence with tiles comes
         }
     }
 }
 
 // One workgroup for (32 columns, 32 head_dim elements) of a cut (sequence, kv head,
 // column group): its four waves take every fourth piece.
-template <int DT, int D, int WC, int NB>
+template <int DT, int D, int WC, int WK>
 __global__ __launch_bounds__(kTreeThreads) void merge_tree_kernel(TreeArgs a, int units_per_seq) {
-    using S = TreeShape<DT, D, WC, NB>;
+    using S = TreeShape<DT, D, WC, WK>;
     constexpr int ES = S::ES;
     __shared__ float sums[3][18 * 64];
     const int64_t share = a.head[0];
@@ -668,26 +655,27 @@ __global__ __launch_bounds__(kTreeThreads) void merge_tree_kernel(TreeArgs a, in
                         1.f / l, hf);
 }
 
-// The waves' arrangement for a call: WC side by side on blocks of 32 columns.
+// The waves' arrangement for a call: wc side by side on blocks of 32 columns, 4 / wc along
+// the keys (8 waves where 8 blocks share their keys).
 struct TreeConfig {
-    int wc, nb, wgs_per_cu, min_share;
+    int wc, per_cu, min_share;
 };
 
 TreeConfig tree_config(int dtype, int head_dim, int max_nodes, int group) {
     const int64_t cols = (int64_t)max_nodes * group;
     const int rb = head_dim * dtype_size(dtype);
-    if (dtype == MF_F32 || rb > 256) return {4, 1, rb > 512 ? 1 : 2, 8};
-    if (cols <= 32) return {1, 1, rb > 128 ? 1 : 2, 8};
-    if (cols <= 64) return {2, 1, 2, 8};
-    if (cols <= 128) return {4, 1, 2, 8};
-    return {4, 2, 1, 8};
+    if (dtype == MF_F32 || rb > 256) return {4, rb > 256 ? 1 : 2, 8};
+    if (cols <= 32) return {1, rb == 256 ? 1 : 2, 8};
+    if (cols <= 64) return {2, 2, 8};
+    if (cols <= 128) return {4, 2, 8};
+    return {8, 1, 8};
 }
 
-template <int DT, int D, int WC, int NB>
+template <int DT, int D, int WC, int WK>
 int launch_tree(const TreeArgs& a, int workers, int units_per_seq, hipStream_t st) {
-    hipLaunchKernelGGL((tree_kernel<DT, D, WC, NB>), dim3((unsigned)workers), dim3(kTreeThreads), 0, st, a);
+    hipLaunchKernelGGL((tree_kernel<DT, D, WC, WK>), dim3((unsigned)workers), dim3(WC * WK * 64), 0, st, a);
     if (int e = check_launch()) return e;
-    hipLaunchKernelGGL((merge_tree_kernel<DT, D, WC, NB>), dim3((unsigned)(a.num_seqs * units_per_seq), WC * NB * (D / 32)),
+    hipLaunchKernelGGL((merge_tree_kernel<DT, D, WC, WK>), dim3((unsigned)(a.num_seqs * units_per_seq), WC * (D / 32)),
                        dim3(kTreeThreads), 0, st, a, units_per_seq);
     return check_launch();
 }
@@ -695,9 +683,9 @@ int launch_tree(const TreeArgs& a, int workers, int units_per_seq, hipStream_t s
 template <int DT, int D>
 int launch_tree(const TreeArgs& a, const TreeConfig& c, int workers, int units_per_seq, hipStream_t st) {
     if constexpr (DT != MF_F32 && D <= 128) {
-        if (c.wc == 1) return launch_tree<DT, D, 1, 1>(a, workers, units_per_seq, st);
-        if (c.wc == 2) return launch_tree<DT, D, 2, 1>(a, workers, units_per_seq, st);
-        if (c.nb == 2) return launch_tree<DT, D, 4, 2>(a, workers, units_per_seq, st);
+        if (c.wc == 1) return launch_tree<DT, D, 1, 4>(a, workers, units_per_seq, st);
+        if (c.wc == 2) return launch_tree<DT, D, 2, 2>(a, workers, units_per_seq, st);
+        if (c.wc == 8) return launch_tree<DT, D, 8, 1>(a, workers, units_per_seq, st);
     }
     return launch_tree<DT, D, 4, 1>(a, workers, units_per_seq, st);
 }
@@ -716,12 +704,12 @@ struct TreeLayout {
 };
 TreeLayout tree_layout(int num_seqs, int64_t num_rows, int max_nodes, const TreeConfig& c, int num_cus) {
     TreeLayout l;
-    l.workers = num_cus * c.wgs_per_cu;
+    l.workers = num_cus * c.per_cu;
     l.mask_words = (max_nodes + 31) / 32;
     l.head = 0;
     l.seq_first = 4;
     l.work = l.seq_first + 2 * (((int64_t)num_seqs + 1) & ~1ll);
-    l.seqs = l.work + 4 * (int64_t)l.workers;
+    l.seqs = l.work + kWorkInts * (int64_t)l.workers;
     l.masks = l.seqs + (int64_t)kSeqInts * num_seqs;
     l.total = l.masks + num_rows * l.mask_words;
     return l;
@@ -740,7 +728,7 @@ extern "C" int mf_tree_plan_sizes(int num_seqs, int64_t num_rows, int max_nodes,
     const TreeConfig c = tree_config(dtype, head_dim, max_nodes, num_q_heads / num_kv_heads);
     const TreeLayout l = tree_layout(num_seqs, num_rows, max_nodes, c, num_cus);
     *plan_words = l.total;
-    *partials_floats = 2 * (int64_t)l.workers * (c.wc * c.nb * 32) * (head_dim + 2);
+    *partials_floats = 2 * (int64_t)l.workers * (c.wc * 32) * (head_dim + 2);
     return MF_OK;
 }
 
@@ -762,7 +750,7 @@ extern "C" int mf_tree_plan(const int32_t* parents, const int32_t* cu_nodes, con
     const TreeConfig c = tree_config(dtype, head_dim, max_nodes, group);
     const TreeLayout l = tree_layout(num_seqs, num_rows, max_nodes, c, num_cus);
     TreePlanArgs a{parents, cu_nodes, context_lens, num_seqs, num_rows, max_nodes, l.mask_words, max_context, group,
-                   num_kv_heads, c.wc * c.nb * 32, l.workers, c.min_share, (int64_t*)(plan + l.head), plan + l.seqs,
+                   num_kv_heads, c.wc * 32, l.workers, c.min_share, (int64_t*)(plan + l.head), plan + l.seqs,
                    (int64_t*)(plan + l.seq_first), plan + l.work, (uint32_t*)(plan + l.masks), positions};
     hipLaunchKernelGGL(tree_plan_kernel, dim3((unsigned)num_seqs + 1), dim3(kTreeThreads), 0, (hipStream_t)stream, a);
     return check_launch();
@@ -836,7 +824,7 @@ extern "C" int mf_tree_attention(const void* q, int64_t q_stride_row, int64_t q_
     a.inv_scale_log2 = 1.f / a.scale_log2;
     a.partials = partials;
     const int64_t cols = (int64_t)max_nodes * group;
-    const int units = num_kv_heads * (int)((cols + c.wc * c.nb * 32 - 1) / (c.wc * c.nb * 32));
+    const int units = num_kv_heads * (int)((cols + c.wc * 32 - 1) / (c.wc * 32));
     if ((int64_t)num_seqs * units > INT_MAX) return MF_ERR_ARG;
     hipStream_t st = (hipStream_t)stream;
 #define MF_TREE_CASE(DT, DV) \
