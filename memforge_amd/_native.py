@@ -1681,28 +1681,33 @@ def tree_plan(parents: torch.Tensor, cu_nodes: torch.Tensor, context_lens: torch
                     sizes[1])
 
 
-def tree_attention(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: PoolView, block_tables: torch.Tensor, plan: TreePlan,
-                   new_k_rows: torch.Tensor, new_v_rows: torch.Tensor, scale: float,
-                   partials: Optional[torch.Tensor] = None) -> None:
-    """mf_tree_attention into ``out_rows`` ((rows, Hq, D) views, device)."""
-    require_device(q_rows, out_rows, pool.k, block_tables, new_k_rows, new_v_rows)
-    dev, dtype = plan.buffer.device, plan.dtype
-    for name, x, heads in (("q_rows", q_rows, plan.num_q_heads), ("out_rows", out_rows, plan.num_q_heads),
-                           ("new_k_rows", new_k_rows, plan.num_kv_heads), ("new_v_rows", new_v_rows, plan.num_kv_heads)):
-        if x.shape != (plan.num_rows, heads, plan.head_dim) or x.dtype != dtype or x.device != dev:
-            raise ValueError(f"{name} must be {(plan.num_rows, heads, plan.head_dim)} in {dtype} on {dev}, got "
-                             f"{tuple(x.shape)} in {x.dtype} on {x.device}")
-        _rows_ok(x, name)
-    if not same_layout(new_k_rows, new_v_rows):
-        new_k_rows, new_v_rows = new_k_rows.contiguous(), new_v_rows.contiguous()
-    if pool.k.dtype != dtype or pool.num_heads != plan.num_kv_heads or pool.head_dim != plan.head_dim or pool.k.device != dev:
-        raise ValueError(f"a pool of {pool.num_heads} heads x {pool.head_dim} in {pool.k.dtype} on {pool.k.device} does not "
-                         f"match a plan for {plan.num_kv_heads} x {plan.head_dim} in {dtype} on {dev}")
+def _tree_rows(name: str, x: torch.Tensor, heads: int, plan: "TreePlan", rows: int, head: int) -> Tuple[int, int, int]:
+    """(address, row stride, head stride) of a call's rows, whose axes ``rows`` and ``head`` are the rows and heads."""
+    shape, stride = x.shape, x.stride()
+    if shape[rows] != plan.num_rows or shape[head] != heads or shape[-1] != plan.head_dim or x.dtype != plan.dtype \
+            or x.device != plan.buffer.device:
+        raise ValueError(f"{name} must be {plan.num_rows} rows of {heads} heads x {plan.head_dim} in {plan.dtype} on "
+                         f"{plan.buffer.device}, got {tuple(shape)} in {x.dtype} on {x.device}")
+    if stride[-1] != 1:
+        raise ValueError(f"{name} head_dim axis must be contiguous")
+    return x.data_ptr(), stride[rows], stride[head]
+
+
+def tree_attention_at(q: Tuple[int, int, int], out: Tuple[int, int, int], pool: Tuple[int, int, int, int, int, int, int],
+                      pool_shape: Tuple[int, int], pool_dtype: torch.dtype, pool_device: torch.device,
+                      block_tables: torch.Tensor, plan: "TreePlan", new_k: Tuple[int, int, int], new_v: int, scale: float,
+                      partials: Optional[torch.Tensor] = None) -> None:
+    """mf_tree_attention on addresses: rows as ``_tree_rows`` gives them (``new_v`` laid out as ``new_k``), ``pool`` = (K
+    address, V address, strides of blocks, slots and heads, block size, blocks), ``pool_shape`` = (kv heads, head_dim)."""
+    dev = plan.buffer.device
+    if pool_dtype != plan.dtype or pool_shape != (plan.num_kv_heads, plan.head_dim) or pool_device != dev:
+        raise ValueError(f"a pool of {pool_shape[0]} heads x {pool_shape[1]} in {pool_dtype} on {pool_device} does not match a "
+                         f"plan for {plan.num_kv_heads} x {plan.head_dim} in {plan.dtype} on {dev}")
     check_index("block_tables", block_tables, torch.int32, dev)
-    width = block_tables.shape[1] if block_tables.dim() == 2 else 0
-    if block_tables.dim() != 2 or block_tables.shape[0] != plan.num_seqs or width * pool.block_size < plan.max_context:
-        raise ValueError(f"block_tables {tuple(block_tables.shape)} do not hold {plan.num_seqs} contexts of up to "
-                         f"{plan.max_context} tokens in blocks of {pool.block_size}")
+    shape, block_size = block_tables.shape, pool[5]
+    if len(shape) != 2 or shape[0] != plan.num_seqs or shape[1] * block_size < plan.max_context:
+        raise ValueError(f"block_tables {tuple(shape)} do not hold {plan.num_seqs} contexts of up to {plan.max_context} tokens "
+                         f"in blocks of {block_size}")
     if not abs(scale) < float("inf"):
         raise ValueError(f"scale must be finite, got {scale}")
     if plan.num_rows == 0 or plan.num_seqs == 0:
@@ -1711,10 +1716,24 @@ def tree_attention(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: PoolView,
         partials = _WORKSPACE.partials(plan.partials_floats, dev)
     elif partials.dtype != torch.float32 or not partials.is_contiguous() or partials.device != dev:
         raise ValueError(f"partials must be contiguous fp32 on {dev}, got {partials.dtype} on {partials.device}")
-    _launch(dev, "mf_tree_attention", lib().mf_tree_attention,
-            q_rows.data_ptr(), q_rows.stride(0), q_rows.stride(1), out_rows.data_ptr(), out_rows.stride(0),
-            out_rows.stride(1), dtype_code(dtype), pool.k.data_ptr(), pool.v.data_ptr(), pool.stride_block, pool.stride_slot,
-            pool.stride_head, pool.block_size, pool.num_blocks, block_tables.data_ptr(), width,
-            new_k_rows.data_ptr(), new_v_rows.data_ptr(), new_k_rows.stride(0), new_k_rows.stride(1), plan.num_seqs,
-            plan.num_rows, plan.max_nodes, plan.num_q_heads, plan.num_kv_heads, plan.head_dim, float(scale), plan.num_cus,
-            plan.buffer.data_ptr(), plan.buffer.numel(), partials.data_ptr(), partials.numel())
+    _launch(dev, "mf_tree_attention", lib().mf_tree_attention, *q, *out, DTYPE_CODES[plan.dtype], *pool,
+            block_tables.data_ptr(), shape[1], new_k[0], new_v, new_k[1], new_k[2], plan.num_seqs, plan.num_rows,
+            plan.max_nodes, plan.num_q_heads, plan.num_kv_heads, plan.head_dim, scale, plan.num_cus, plan.buffer.data_ptr(),
+            plan.buffer.numel(), partials.data_ptr(), partials.numel())
+
+
+def tree_attention(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: PoolView, block_tables: torch.Tensor, plan: TreePlan,
+                   new_k_rows: torch.Tensor, new_v_rows: torch.Tensor, scale: float,
+                   partials: Optional[torch.Tensor] = None) -> None:
+    """mf_tree_attention into ``out_rows`` ((rows, Hq, D) views, device)."""
+    require_device(q_rows, out_rows, pool.k, block_tables, new_k_rows, new_v_rows)
+    for name, x in (("q_rows", q_rows), ("out_rows", out_rows), ("new_k_rows", new_k_rows), ("new_v_rows", new_v_rows)):
+        _rows_ok(x, name)
+    if not same_layout(new_k_rows, new_v_rows):
+        new_k_rows, new_v_rows = new_k_rows.contiguous(), new_v_rows.contiguous()
+    tree_attention_at(_tree_rows("q_rows", q_rows, plan.num_q_heads, plan, 0, 1),
+                      _tree_rows("out_rows", out_rows, plan.num_q_heads, plan, 0, 1),
+                      (pool.k.data_ptr(), pool.v.data_ptr(), pool.stride_block, pool.stride_slot, pool.stride_head,
+                       pool.block_size, pool.num_blocks), (pool.num_heads, pool.head_dim), pool.k.dtype, pool.k.device,
+                      block_tables, plan, _tree_rows("new_k_rows", new_k_rows, plan.num_kv_heads, plan, 0, 1),
+                      _tree_rows("new_v_rows", new_v_rows, plan.num_kv_heads, plan, 0, 1)[0], float(scale), partials)

@@ -29,6 +29,12 @@ namespace {
 
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 
+// As ld_lds16, for rows that are read once: past what the caches hold (two layers of 64
+// contexts of a median of 2048 at 40/8 x 128: 428 -> 381 us with plan and merges).
+__device__ __forceinline__ void ld_lds16_nt(const void* gsrc, uint32_t lds_addr) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"{m0}"(lds_addr), "v"(gsrc) : "memory");
+}
+
 constexpr int kTreeThreads = 256;
 constexpr int kTile = 32;            // keys
 constexpr int kMaxSeqs = 4096;
@@ -354,8 +360,8 @@ __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * W
                 for (int i = 0; i < S::PAIRS; ++i) {
                     const char* src = kh + ((int64_t)min(e[i], a.num_blocks - 1) * a.p_sb +
                                             (int64_t)(key[i] & (a.block_size - 1)) * a.p_ss) * ES;
-                    ld_lds16(src + k_piece(i), dst0 + (uint32_t)((wave + S::WAVES * i) * 1024));
-                    ld_lds16(src + v_delta + v_piece(i), dst0 + (uint32_t)(S::HALF + (wave + S::WAVES * i) * 1024));
+                    ld_lds16_nt(src + k_piece(i), dst0 + (uint32_t)((wave + S::WAVES * i) * 1024));
+                    ld_lds16_nt(src + v_delta + v_piece(i), dst0 + (uint32_t)(S::HALF + (wave + S::WAVES * i) * 1024));
                 }
             } else {
 #pragma unroll 1
@@ -374,8 +380,8 @@ __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * W
                         src = a.new_k + ((int64_t)(row0 + node) * a.n_sr + (int64_t)h * a.n_sh) * ES;
                         to_v = nv_delta;
                     }
-                    ld_lds16(src + k_piece(i), dst0 + (uint32_t)((wave + S::WAVES * i) * 1024));
-                    ld_lds16(src + to_v + v_piece(i), dst0 + (uint32_t)(S::HALF + (wave + S::WAVES * i) * 1024));
+                    ld_lds16_nt(src + k_piece(i), dst0 + (uint32_t)((wave + S::WAVES * i) * 1024));
+                    ld_lds16_nt(src + to_v + v_piece(i), dst0 + (uint32_t)(S::HALF + (wave + S::WAVES * i) * 1024));
                 }
             }
             f_left -= take;
@@ -556,7 +562,8 @@ __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * W
                     for (int d = 0; d < ND; ++d)
 #pragma unroll
                         for (int i = 0; i < 16; i += 4)
-                            *(float4*)(to + (d * 16 + i) * 64 + 4 * lane) = make_float4(acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]);
+                            if (valid)
+                                *(float4*)(to + (d * 16 + i) * 64 + 4 * lane) = make_float4(acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]);
                     if (hf == 0) {
                         to[32 * D + lane] = m;
                         to[32 * D + 32 + lane] = l;
@@ -587,72 +594,78 @@ __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * W
     }
 }
 
-// One workgroup for (32 columns, 32 head_dim elements) of a cut (sequence, kv head,
-// column group): its four waves take every fourth piece.
-template <int DT, int D, int WC, int WK>
+// The cut (sequence, kv head, column group)s' results. SPLIT: a workgroup for 32 columns and
+// 32 head_dim elements, whose four waves take every fourth piece; otherwise one for 32
+// columns, a wave for every 32 elements, which walks the two or three pieces itself.
+template <int DT, int D, int WC, int WK, bool SPLIT>
 __global__ __launch_bounds__(kTreeThreads) void merge_tree_kernel(TreeArgs a, int units_per_seq) {
     using S = TreeShape<DT, D, WC, WK>;
     constexpr int ES = S::ES;
-    __shared__ float sums[3][18 * 64];
+    __shared__ float sums[SPLIT ? 3 : 1][SPLIT ? 18 * 64 : 1];
     const int64_t share = a.head[0];
     const int u = blockIdx.x, s = u / units_per_seq, unit = u - s * units_per_seq;
-    const int blk = blockIdx.y / S::ND, d = blockIdx.y % S::ND;
+    const int lane = threadIdx.x & 63, hf = lane >> 5, wave = threadIdx.x >> 6;
+    const int blk = SPLIT ? blockIdx.y / S::ND : blockIdx.y;
     const int32_t* info = a.seqs + (int64_t)s * kSeqInts;
     const int n = info[1], row0 = info[2], tiles = info[3], groups = info[4];
+    const int64_t begin = a.seq_first[s] + (int64_t)unit * tiles;
     if (tiles == 0 || unit >= groups * a.num_kv_heads) return;
     const int h = unit / groups, grp = unit - h * groups;
     if (grp * S::COLS + blk * 32 >= n * a.group) return;
-    const int64_t begin = a.seq_first[s] + (int64_t)unit * tiles;
     const int64_t w0 = begin / share, w1 = (begin + tiles - 1) / share;
     if (w0 == w1) return;
-    const int lane = threadIdx.x & 63, hf = lane >> 5, wave = threadIdx.x >> 6;
-    float m = kMinM, l = 0.f;
-    f32x16 acc[1];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) acc[0][i] = 0.f;
-    for (int64_t w = w0 + wave; w <= w1; w += 4) {
-        const float* from = a.partials + (2 * w + (w * share < begin ? 1 : 0)) * S::SLOT + blk * 32 * (D + 2);
-        const float m1 = from[32 * D + (lane & 31)], l1 = from[32 * D + 32 + (lane & 31)];
-        float4 v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = *(const float4*)(from + (d * 16 + 4 * i) * 64 + 4 * lane);
-        const float mn = fmaxf(m, m1);
-        const float e0 = __builtin_amdgcn_exp2f(m - mn), e1 = __builtin_amdgcn_exp2f(m1 - mn);
-        m = mn;
-        l = l * e0 + l1 * e1;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            acc[0][4 * i] = acc[0][4 * i] * e0 + v[i].x * e1;
-            acc[0][4 * i + 1] = acc[0][4 * i + 1] * e0 + v[i].y * e1;
-            acc[0][4 * i + 2] = acc[0][4 * i + 2] * e0 + v[i].z * e1;
-            acc[0][4 * i + 3] = acc[0][4 * i + 3] * e0 + v[i].w * e1;
-        }
-    }
-    if (wave > 0) {
-        float* to = sums[wave - 1];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) to[i * 64 + lane] = acc[0][i];
-        to[16 * 64 + lane] = m;
-        to[17 * 64 + lane] = l;
-    }
-    __syncthreads();
-    if (wave > 0) return;
-#pragma unroll
-    for (int o = 0; o < 3; ++o) {
-        const float m1 = sums[o][16 * 64 + lane], l1 = sums[o][17 * 64 + lane];
-        const float mn = fmaxf(m, m1);
-        const float e0 = __builtin_amdgcn_exp2f(m - mn), e1 = __builtin_amdgcn_exp2f(m1 - mn);
-        m = mn;
-        l = l * e0 + l1 * e1;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[0][i] = acc[0][i] * e0 + sums[o][i * 64 + lane] * e1;
-    }
     const int c = grp * S::COLS + blk * 32 + (lane & 31);
     const bool valid = c < n * a.group;
-    const int node = (int)((unsigned)(valid ? c : 0) / (unsigned)a.group);
-    const int qhead = h * a.group + (valid ? c : 0) - node * a.group;
-    store_column<DT, 1>(a.out + ((int64_t)(row0 + node) * a.o_sr + (int64_t)qhead * a.o_sh + 32 * d) * ES, valid, acc,
-                        1.f / l, hf);
+    for (int d = SPLIT ? blockIdx.y % S::ND : wave; d < S::ND; d += SPLIT ? S::ND : 4) {
+        float m = kMinM, l = 0.f;
+        f32x16 acc[1];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[0][i] = 0.f;
+#pragma unroll 2
+        for (int64_t w = w0 + (SPLIT ? wave : 0); w <= w1; w += SPLIT ? 4 : 1) {
+            const float* from = a.partials + (2 * w + (w * share < begin ? 1 : 0)) * S::SLOT + blk * 32 * (D + 2);
+            const float m1 = from[32 * D + (lane & 31)], l1 = from[32 * D + 32 + (lane & 31)];
+            float4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = *(const float4*)(from + (d * 16 + 4 * i) * 64 + 4 * lane);
+            const float mn = fmaxf(m, m1);
+            const float e0 = __builtin_amdgcn_exp2f(m - mn), e1 = __builtin_amdgcn_exp2f(m1 - mn);
+            m = mn;
+            l = l * e0 + l1 * e1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                acc[0][4 * i] = acc[0][4 * i] * e0 + v[i].x * e1;
+                acc[0][4 * i + 1] = acc[0][4 * i + 1] * e0 + v[i].y * e1;
+                acc[0][4 * i + 2] = acc[0][4 * i + 2] * e0 + v[i].z * e1;
+                acc[0][4 * i + 3] = acc[0][4 * i + 3] * e0 + v[i].w * e1;
+            }
+        }
+        if constexpr (SPLIT) {
+            if (wave > 0) {
+                float* to = sums[wave - 1];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) to[i * 64 + lane] = acc[0][i];
+                to[16 * 64 + lane] = m;
+                to[17 * 64 + lane] = l;
+            }
+            __syncthreads();
+            if (wave > 0) return;
+#pragma unroll
+            for (int o = 0; o < 3; ++o) {
+                const float m1 = sums[o][16 * 64 + lane], l1 = sums[o][17 * 64 + lane];
+                const float mn = fmaxf(m, m1);
+                const float e0 = __builtin_amdgcn_exp2f(m - mn), e1 = __builtin_amdgcn_exp2f(m1 - mn);
+                m = mn;
+                l = l * e0 + l1 * e1;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[0][i] = acc[0][i] * e0 + sums[o][i * 64 + lane] * e1;
+            }
+        }
+        const int node = (int)((unsigned)(valid ? c : 0) / (unsigned)a.group);
+        const int qhead = h * a.group + (valid ? c : 0) - node * a.group;
+        store_column<DT, 1>(a.out + ((int64_t)(row0 + node) * a.o_sr + (int64_t)qhead * a.o_sh + 32 * d) * ES, valid, acc,
+                            1.f / l, hf);
+    }
 }
 
 // The waves' arrangement for a call: wc side by side on blocks of 32 columns, 4 / wc along
@@ -665,8 +678,10 @@ TreeConfig tree_config(int dtype, int head_dim, int max_nodes, int group) {
     const int64_t cols = (int64_t)max_nodes * group;
     const int rb = head_dim * dtype_size(dtype);
     if (dtype == MF_F32 || rb > 256) return {4, rb > 256 ? 1 : 2, 8};
-    if (cols <= 32) return {1, rb == 256 ? 1 : 2, 8};
-    if (cols <= 64) return {2, 2, 8};
+    // few columns: one stage is a share (4 contexts of up to 700 with 8 nodes at 15/5 x 64: four layers 74 us at 8
+    // tiles, 58 at 4)
+    if (cols <= 32) return {1, rb == 256 ? 1 : 2, 4};
+    if (cols <= 64) return {2, 2, 4};
     if (cols <= 128) return {4, 2, 8};
     return {8, 1, 8};
 }
@@ -675,8 +690,14 @@ template <int DT, int D, int WC, int WK>
 int launch_tree(const TreeArgs& a, int workers, int units_per_seq, hipStream_t st) {
     hipLaunchKernelGGL((tree_kernel<DT, D, WC, WK>), dim3((unsigned)workers), dim3(WC * WK * 64), 0, st, a);
     if (int e = check_launch()) return e;
-    hipLaunchKernelGGL((merge_tree_kernel<DT, D, WC, WK>), dim3((unsigned)(a.num_seqs * units_per_seq), WC * (D / 32)),
-                       dim3(kTreeThreads), 0, st, a, units_per_seq);
+    const int units = a.num_seqs * units_per_seq;
+    // many pieces to a unit where there are few units for the workers
+    if ((int64_t)units * 8 <= workers)
+        hipLaunchKernelGGL((merge_tree_kernel<DT, D, WC, WK, true>), dim3((unsigned)units, WC * (D / 32)), dim3(kTreeThreads), 0,
+                           st, a, units_per_seq);
+    else
+        hipLaunchKernelGGL((merge_tree_kernel<DT, D, WC, WK, false>), dim3((unsigned)units, WC), dim3(kTreeThreads), 0, st, a,
+                           units_per_seq);
     return check_launch();
 }
 

@@ -46,19 +46,37 @@ def paged_attention_tree(query: torch.Tensor, key_pool: torch.Tensor, value_pool
     belong to no tree are not computed and hold anything. A value that is not finite
     reaches the nodes of its tree that do not see it too, as zero times it does in a
     product."""
-    nat.require_device(query, key_pool)
+    nat.require_device(query, key_pool, new_keys, new_values)
     for name, x in (("query", query), ("new_keys", new_keys), ("new_values", new_values)):
         if x.dim() != 4 or x.shape[0] != 1:
             raise ValueError(f"{name} must be (1, heads, rows, head_dim), got {tuple(x.shape)}")
-
-    def rows(x):
-        x = x[0].permute(1, 0, 2)
-        aligned = x.stride(2) == 1 and not (x.stride(0) * x.element_size() % 16 or x.stride(1) * x.element_size() % 16
-                                            or x.data_ptr() % 16)
-        return x if aligned else x.contiguous()
-
+    if key_pool.dim() != 5 or key_pool.shape != value_pool.shape or key_pool.stride() != value_pool.stride() \
+            or key_pool.dtype != value_pool.dtype or key_pool.stride(4) != 1 or value_pool.device != key_pool.device:
+        raise ValueError("K and V pools must be (layers, blocks, slots, kv_heads, head_dim) of one shape, layout, dtype and "
+                         f"device, got {tuple(key_pool.shape)} in {key_pool.dtype} and {tuple(value_pool.shape)} in "
+                         f"{value_pool.dtype}")
+    layers, blocks, block_size, kv_heads, dim = key_pool.shape
+    if not -layers <= layer_idx < layers:
+        raise IndexError(f"layer {layer_idx} of pools of {layers}")
+    query, new_keys, new_values = _whole_pieces(query), _whole_pieces(new_keys), _whole_pieces(new_values)
+    if new_keys.stride() != new_values.stride():
+        new_keys, new_values = new_keys.contiguous(), new_values.contiguous()
     out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    nat.tree_attention(rows(query), out[0].permute(1, 0, 2), nat.PoolView.from_bshd(key_pool[layer_idx], value_pool[layer_idx]),
-                       block_tables, plan, rows(new_keys), rows(new_values),
-                       scale if scale is not None else 1.0 / math.sqrt(query.shape[3]))
+    stride = key_pool.stride()
+    at = (layer_idx % layers) * stride[0] * key_pool.element_size()
+    nat.tree_attention_at(
+        nat._tree_rows("query", query, plan.num_q_heads, plan, 2, 1), nat._tree_rows("out", out, plan.num_q_heads, plan, 2, 1),
+        (key_pool.data_ptr() + at, value_pool.data_ptr() + at, stride[1], stride[2], stride[3], block_size, blocks),
+        (kv_heads, dim), key_pool.dtype, key_pool.device, block_tables, plan,
+        nat._tree_rows("new_keys", new_keys, plan.num_kv_heads, plan, 2, 1),
+        nat._tree_rows("new_values", new_values, plan.num_kv_heads, plan, 2, 1)[0],
+        float(scale) if scale is not None else 1.0 / math.sqrt(dim))
     return out
+
+
+def _whole_pieces(x: torch.Tensor) -> torch.Tensor:
+    """``x`` itself where its rows and heads begin at whole 16 bytes (as the kernel reads them), else a copy."""
+    stride, per = x.stride(), 16 // x.element_size() if x.element_size() < 16 else 1
+    if stride[3] == 1 and not (stride[1] % per or stride[2] % per or x.data_ptr() & 15):
+        return x
+    return x.contiguous()
