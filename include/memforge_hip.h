@@ -587,9 +587,9 @@ int mf_spec_verify(int num_rows, int num_draft, int vocab,
  *
  * mf_tables_extend grows request s by new_tokens[s] (int32; negative: none). In
  * request order each takes the blocks it lacks from the stack's top. A request
- * is refused, and keeps what it has, when its table row is too short, its rows
- * end past max_rows, or the blocks asked for up to and including it (those of
- * requests that are refused for the first two reasons not counted) are more than
+ * is refused, and keeps what it has, when its table row or 31 bits are too short for
+ * its length, its rows end past max_rows, or the blocks asked for up to and including it (those of
+ * requests that are refused for another reason not counted) are more than
  * the stack holds and it lacks any. Outputs: cu_seqlens (num_requests + 1) sums of
  * new_tokens, kv_lens the new lengths, *refused their number, and for every row
  * r < max_rows slot_mapping / positions (int64): row cu_seqlens[s] + i is the

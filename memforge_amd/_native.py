@@ -1554,12 +1554,13 @@ def spec_verify(draft_tokens: torch.Tensor, draft_probs: torch.Tensor, target_lo
 
 def check_index(name: str, x: torch.Tensor, dtype: torch.dtype, device: torch.device, shape: Optional[tuple] = None) -> None:
     """An index tensor of a call: its type, its device, contiguous, and its shape when given."""
+    if x.dtype is dtype and x.device == device and x.is_contiguous() and (shape is None or x.shape == shape):
+        return
     if x.dtype != dtype or not x.is_contiguous():
         raise TypeError(f"{name} must be a contiguous {dtype} tensor, got {x.dtype} with strides {x.stride()}")
     if shape is not None and tuple(x.shape) != shape:
         raise ValueError(f"{name} must be of shape {shape}, got {tuple(x.shape)}")
-    if x.device != device:
-        raise ValueError(f"{name} is on {x.device}, the call's other tensors on {device}")
+    raise ValueError(f"{name} is on {x.device}, the call's other tensors on {device}")
 
 
 # ---------------------------------------------------------------- sampling
@@ -1611,9 +1612,11 @@ def tree_accept(tokens: torch.Tensor, targets: torch.Tensor, parents: torch.Tens
     """mf_tree_accept: (path int32 (B, max_nodes), tokens int64 (B, max_nodes), count int32 (B))."""
     require_device(tokens, targets, parents, cu_nodes)
     dev, rows, seqs = parents.device, parents.numel(), cu_nodes.numel() - 1
-    for name, x, dt, n in (("tokens", tokens, torch.int64, rows), ("targets", targets, torch.int64, rows),
-                           ("parents", parents, torch.int32, rows), ("cu_nodes", cu_nodes, torch.int32, seqs + 1)):
-        check_index(name, x, dt, dev, (n,))
+    shape = (rows,)
+    check_index("parents", parents, torch.int32, dev, shape)
+    check_index("tokens", tokens, torch.int64, dev, shape)
+    check_index("targets", targets, torch.int64, dev, shape)
+    check_index("cu_nodes", cu_nodes, torch.int32, dev, (seqs + 1,))
     if seqs < 0:
         raise ValueError("cu_nodes must have one more entry than sequences")
     if not 1 <= max_nodes <= TREE_MAX_NODES:
@@ -1646,6 +1649,7 @@ class TreePlan:
     dtype: torch.dtype
     num_cus: int
     partials_floats: int
+    device: torch.device
 
 
 def tree_plan(parents: torch.Tensor, cu_nodes: torch.Tensor, context_lens: torch.Tensor, max_nodes: int, max_context: int,
@@ -1653,8 +1657,9 @@ def tree_plan(parents: torch.Tensor, cu_nodes: torch.Tensor, context_lens: torch
     """mf_tree_plan into new buffers."""
     require_device(parents, cu_nodes, context_lens)
     dev, rows, seqs = parents.device, parents.numel(), context_lens.numel()
-    for name, x, n in (("parents", parents, rows), ("cu_nodes", cu_nodes, seqs + 1), ("context_lens", context_lens, seqs)):
-        check_index(name, x, torch.int32, dev, (n,))
+    check_index("parents", parents, torch.int32, dev, (rows,))
+    check_index("cu_nodes", cu_nodes, torch.int32, dev, (seqs + 1,))
+    check_index("context_lens", context_lens, torch.int32, dev, (seqs,))
     if not 1 <= max_nodes <= TREE_MAX_NODES:
         raise ValueError(f"max_nodes must be 1 to {TREE_MAX_NODES}, got {max_nodes}")
     if not 0 <= max_context <= 1 << 30:
@@ -1678,40 +1683,36 @@ def tree_plan(parents: torch.Tensor, cu_nodes: torch.Tensor, context_lens: torch
             seqs, rows, max_nodes, max_context, num_q_heads, num_kv_heads, head_dim, shape[6], cus, buffer.data_ptr(),
             sizes[0], positions.data_ptr())
     return TreePlan(buffer, positions, seqs, rows, max_nodes, max_context, num_q_heads, num_kv_heads, head_dim, dtype, cus,
-                    sizes[1])
+                    sizes[1], dev)
 
 
 def _tree_rows(name: str, x: torch.Tensor, heads: int, plan: "TreePlan", rows: int, head: int) -> Tuple[int, int, int]:
     """(address, row stride, head stride) of a call's rows, whose axes ``rows`` and ``head`` are the rows and heads."""
     shape, stride = x.shape, x.stride()
-    if shape[rows] != plan.num_rows or shape[head] != heads or shape[-1] != plan.head_dim or x.dtype != plan.dtype \
-            or x.device != plan.buffer.device:
+    if shape[rows] != plan.num_rows or shape[head] != heads or shape[-1] != plan.head_dim or x.dtype is not plan.dtype \
+            or x.device != plan.device:
         raise ValueError(f"{name} must be {plan.num_rows} rows of {heads} heads x {plan.head_dim} in {plan.dtype} on "
-                         f"{plan.buffer.device}, got {tuple(shape)} in {x.dtype} on {x.device}")
+                         f"{plan.device}, got {tuple(shape)} in {x.dtype} on {x.device}")
     if stride[-1] != 1:
         raise ValueError(f"{name} head_dim axis must be contiguous")
     return x.data_ptr(), stride[rows], stride[head]
 
 
 def tree_attention_at(q: Tuple[int, int, int], out: Tuple[int, int, int], pool: Tuple[int, int, int, int, int, int, int],
-                      pool_shape: Tuple[int, int], pool_dtype: torch.dtype, pool_device: torch.device,
                       block_tables: torch.Tensor, plan: "TreePlan", new_k: Tuple[int, int, int], new_v: int, scale: float,
                       partials: Optional[torch.Tensor] = None) -> None:
-    """mf_tree_attention on addresses: rows as ``_tree_rows`` gives them (``new_v`` laid out as ``new_k``), ``pool`` = (K
-    address, V address, strides of blocks, slots and heads, block size, blocks), ``pool_shape`` = (kv heads, head_dim)."""
-    dev = plan.buffer.device
-    if pool_dtype != plan.dtype or pool_shape != (plan.num_kv_heads, plan.head_dim) or pool_device != dev:
-        raise ValueError(f"a pool of {pool_shape[0]} heads x {pool_shape[1]} in {pool_dtype} on {pool_device} does not match a "
-                         f"plan for {plan.num_kv_heads} x {plan.head_dim} in {plan.dtype} on {dev}")
-    check_index("block_tables", block_tables, torch.int32, dev)
-    shape, block_size = block_tables.shape, pool[5]
-    if len(shape) != 2 or shape[0] != plan.num_seqs or shape[1] * block_size < plan.max_context:
+    """mf_tree_attention on addresses that the caller has checked: rows as ``_tree_rows`` gives them (``new_v`` laid out
+    as ``new_k``), ``pool`` = (K address, V address, strides of blocks, slots and heads, block size, blocks)."""
+    check_index("block_tables", block_tables, torch.int32, plan.device)
+    shape = block_tables.shape
+    if len(shape) != 2 or shape[0] != plan.num_seqs or shape[1] * pool[5] < plan.max_context:
         raise ValueError(f"block_tables {tuple(shape)} do not hold {plan.num_seqs} contexts of up to {plan.max_context} tokens "
-                         f"in blocks of {block_size}")
+                         f"in blocks of {pool[5]}")
     if not abs(scale) < float("inf"):
         raise ValueError(f"scale must be finite, got {scale}")
     if plan.num_rows == 0 or plan.num_seqs == 0:
         return
+    dev = plan.device
     if partials is None:
         partials = _WORKSPACE.partials(plan.partials_floats, dev)
     elif partials.dtype != torch.float32 or not partials.is_contiguous() or partials.device != dev:
@@ -1720,6 +1721,13 @@ def tree_attention_at(q: Tuple[int, int, int], out: Tuple[int, int, int], pool: 
             block_tables.data_ptr(), shape[1], new_k[0], new_v, new_k[1], new_k[2], plan.num_seqs, plan.num_rows,
             plan.max_nodes, plan.num_q_heads, plan.num_kv_heads, plan.head_dim, scale, plan.num_cus, plan.buffer.data_ptr(),
             plan.buffer.numel(), partials.data_ptr(), partials.numel())
+
+
+def check_tree_pool(key_pool: torch.Tensor, num_heads: int, head_dim: int, plan: "TreePlan") -> None:
+    if key_pool.dtype is not plan.dtype or num_heads != plan.num_kv_heads or head_dim != plan.head_dim \
+            or key_pool.device != plan.device:
+        raise ValueError(f"a pool of {num_heads} heads x {head_dim} in {key_pool.dtype} on {key_pool.device} does not match a "
+                         f"plan for {plan.num_kv_heads} x {plan.head_dim} in {plan.dtype} on {plan.device}")
 
 
 def tree_attention(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: PoolView, block_tables: torch.Tensor, plan: TreePlan,
@@ -1731,9 +1739,9 @@ def tree_attention(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: PoolView,
         _rows_ok(x, name)
     if not same_layout(new_k_rows, new_v_rows):
         new_k_rows, new_v_rows = new_k_rows.contiguous(), new_v_rows.contiguous()
+    check_tree_pool(pool.k, pool.num_heads, pool.head_dim, plan)
     tree_attention_at(_tree_rows("q_rows", q_rows, plan.num_q_heads, plan, 0, 1),
                       _tree_rows("out_rows", out_rows, plan.num_q_heads, plan, 0, 1),
                       (pool.k.data_ptr(), pool.v.data_ptr(), pool.stride_block, pool.stride_slot, pool.stride_head,
-                       pool.block_size, pool.num_blocks), (pool.num_heads, pool.head_dim), pool.k.dtype, pool.k.device,
-                      block_tables, plan, _tree_rows("new_k_rows", new_k_rows, plan.num_kv_heads, plan, 0, 1),
+                       pool.block_size, pool.num_blocks), block_tables, plan, _tree_rows("new_k_rows", new_k_rows, plan.num_kv_heads, plan, 0, 1),
                       _tree_rows("new_v_rows", new_v_rows, plan.num_kv_heads, plan, 0, 1)[0], float(scale), partials)

@@ -47,36 +47,40 @@ def paged_attention_tree(query: torch.Tensor, key_pool: torch.Tensor, value_pool
     reaches the nodes of its tree that do not see it too, as zero times it does in a
     product."""
     nat.require_device(query, key_pool, new_keys, new_values)
-    for name, x in (("query", query), ("new_keys", new_keys), ("new_values", new_values)):
-        if x.dim() != 4 or x.shape[0] != 1:
-            raise ValueError(f"{name} must be (1, heads, rows, head_dim), got {tuple(x.shape)}")
-    if key_pool.dim() != 5 or key_pool.shape != value_pool.shape or key_pool.stride() != value_pool.stride() \
-            or key_pool.dtype != value_pool.dtype or key_pool.stride(4) != 1 or value_pool.device != key_pool.device:
+    shape, stride = key_pool.shape, key_pool.stride()
+    if len(shape) != 5 or shape != value_pool.shape or stride != value_pool.stride() or key_pool.dtype is not value_pool.dtype \
+            or stride[4] != 1 or key_pool.device != value_pool.device:
         raise ValueError("K and V pools must be (layers, blocks, slots, kv_heads, head_dim) of one shape, layout, dtype and "
-                         f"device, got {tuple(key_pool.shape)} in {key_pool.dtype} and {tuple(value_pool.shape)} in "
-                         f"{value_pool.dtype}")
-    layers, blocks, block_size, kv_heads, dim = key_pool.shape
+                         f"device, got {tuple(shape)} in {key_pool.dtype} and {tuple(value_pool.shape)} in {value_pool.dtype}")
+    layers, blocks, block_size, kv_heads, dim = shape
+    nat.check_tree_pool(key_pool, kv_heads, dim, plan)
     if not -layers <= layer_idx < layers:
         raise IndexError(f"layer {layer_idx} of pools of {layers}")
-    query, new_keys, new_values = _whole_pieces(query), _whole_pieces(new_keys), _whole_pieces(new_values)
-    if new_keys.stride() != new_values.stride():
-        new_keys, new_values = new_keys.contiguous(), new_values.contiguous()
-    out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    stride = key_pool.stride()
+    q, q_copy = _rows("query", query, plan.num_q_heads, plan)
+    k, k_copy = _rows("new_keys", new_keys, plan.num_kv_heads, plan)
+    v, v_copy = _rows("new_values", new_values, plan.num_kv_heads, plan)
+    if k[1:] != v[1:]:
+        k, k_copy = _rows("new_keys", new_keys.contiguous(), plan.num_kv_heads, plan, True)
+        v, v_copy = _rows("new_values", new_values.contiguous(), plan.num_kv_heads, plan, True)
+    out = torch.empty((1, plan.num_q_heads, plan.num_rows, dim), dtype=plan.dtype, device=plan.device)
     at = (layer_idx % layers) * stride[0] * key_pool.element_size()
-    nat.tree_attention_at(
-        nat._tree_rows("query", query, plan.num_q_heads, plan, 2, 1), nat._tree_rows("out", out, plan.num_q_heads, plan, 2, 1),
-        (key_pool.data_ptr() + at, value_pool.data_ptr() + at, stride[1], stride[2], stride[3], block_size, blocks),
-        (kv_heads, dim), key_pool.dtype, key_pool.device, block_tables, plan,
-        nat._tree_rows("new_keys", new_keys, plan.num_kv_heads, plan, 2, 1),
-        nat._tree_rows("new_values", new_values, plan.num_kv_heads, plan, 2, 1)[0],
-        float(scale) if scale is not None else 1.0 / math.sqrt(dim))
+    nat.tree_attention_at(q, (out.data_ptr(), dim, plan.num_rows * dim),
+                          (key_pool.data_ptr() + at, value_pool.data_ptr() + at, stride[1], stride[2], stride[3], block_size,
+                           blocks), block_tables, plan, k, v[0], float(scale) if scale is not None else 1.0 / math.sqrt(dim))
     return out
 
 
-def _whole_pieces(x: torch.Tensor) -> torch.Tensor:
-    """``x`` itself where its rows and heads begin at whole 16 bytes (as the kernel reads them), else a copy."""
-    stride, per = x.stride(), 16 // x.element_size() if x.element_size() < 16 else 1
-    if stride[3] == 1 and not (stride[1] % per or stride[2] % per or x.data_ptr() & 15):
-        return x
-    return x.contiguous()
+def _rows(name: str, x: torch.Tensor, heads: int, plan: TreePlan, keep: bool = False):
+    """((address, row stride, head stride), what has to live until the launch) of ``(1, heads, rows, head_dim)``: of a
+    copy where rows or heads do not begin at whole 16 bytes, as the kernel reads them."""
+    if x.shape != (1, heads, plan.num_rows, plan.head_dim) or x.dtype is not plan.dtype or x.device != plan.device:
+        raise ValueError(f"{name} must be {(1, heads, plan.num_rows, plan.head_dim)} in {plan.dtype} on {plan.device}, got "
+                         f"{tuple(x.shape)} in {x.dtype} on {x.device}")
+    _, head, row, last = x.stride()
+    at = x.data_ptr()
+    per = 4 if plan.dtype is torch.float32 else 8
+    if last != 1 or head % per or row % per or at & 15:
+        x, keep = x.contiguous(), True
+        _, head, row, _ = x.stride()
+        at = x.data_ptr()
+    return (at, row, head), x if keep else None

@@ -60,18 +60,21 @@ class DeviceBlockTables:
 
     def _state(self, name: str, want: torch.Tensor):
         """The tensors' checks, and the C arguments that both entry points begin with."""
-        dev, n = self.tables.device, self.tables.shape[0]
-        nat.require_device(self.tables, want)
-        if self.tables.dim() != 2:
-            raise ValueError(f"tables must be (requests, max_blocks), got {tuple(self.tables.shape)}")
-        nat.check_index("tables", self.tables, torch.int32, dev)
-        for what, x, shape in (("lens", self.lens, (n,)), ("held", self.held, (n,)), ("free", self.free, None),
-                               ("free_count", self.free_count, (1,)), (name, want, (n,))):
-            nat.check_index(what, x, torch.int32, dev, shape)
-        width = self.tables.shape[1]
-        return dev, n, (self.tables.data_ptr(), width, width, self.lens.data_ptr(), self.held.data_ptr(),
-                        self.free.data_ptr(), self.free.numel(), self.free_count.data_ptr(), want.data_ptr(), n,
-                        self.block_size)
+        tables = self.tables
+        nat.require_device(tables, want)
+        if tables.dim() != 2:
+            raise ValueError(f"tables must be (requests, max_blocks), got {tuple(tables.shape)}")
+        (n, width), dev = tables.shape, tables.device
+        shape = (n,)
+        nat.check_index("tables", tables, torch.int32, dev)
+        nat.check_index("lens", self.lens, torch.int32, dev, shape)
+        nat.check_index("held", self.held, torch.int32, dev, shape)
+        nat.check_index("free", self.free, torch.int32, dev)
+        nat.check_index("free_count", self.free_count, torch.int32, dev, (1,))
+        nat.check_index(name, want, torch.int32, dev, shape)
+        return dev, n, (tables.data_ptr(), width, width, self.lens.data_ptr(), self.held.data_ptr(),
+                                  self.free.data_ptr(), self.free.numel(), self.free_count.data_ptr(), want.data_ptr(), n,
+                                  self.block_size)
 
     def extend(self, new_tokens: torch.Tensor, max_rows: int, rows: Optional[torch.Tensor] = None) -> SlotMap:
         """Grow request s by ``new_tokens[s]`` (int32, on the device). In request order each
@@ -90,15 +93,17 @@ class DeviceBlockTables:
             nat.check_index("rows", rows, torch.int32, dev)
             if rows.dim() != 2 or rows.shape[0] != n:
                 raise ValueError(f"rows must be ({n}, most new tokens), got {tuple(rows.shape)}")
-        places = torch.empty((2, max_rows), dtype=torch.int64, device=dev)
-        sums = torch.empty(2 * n + 2, dtype=torch.int32, device=dev)
-        at = sums.data_ptr()
-        nat._launch(dev, "mf_tables_extend", nat.lib().mf_tables_extend, *state, max_rows,
-                    None if rows is None else rows.data_ptr(), 0 if rows is None else rows.shape[1],
-                    0 if rows is None else rows.shape[1], places.data_ptr(), places.data_ptr() + 8 * max_rows,
-                    at, at + 4 * (n + 1), at + 4 * (2 * n + 1), nat._WORKSPACE.counters(1, dev).data_ptr())
-        slots, positions = places.unbind()
-        cu, lens, refused = sums.split((n + 1, n, 1))
+            at, width = rows.data_ptr(), rows.shape[1]
+        else:
+            at, width = None, 0
+        slots = torch.empty(max_rows, dtype=torch.int64, device=dev)
+        positions = torch.empty(max_rows, dtype=torch.int64, device=dev)
+        cu = torch.empty(n + 1, dtype=torch.int32, device=dev)
+        lens = torch.empty(n, dtype=torch.int32, device=dev)
+        refused = torch.empty(1, dtype=torch.int32, device=dev)
+        nat._launch(dev, "mf_tables_extend", nat.lib().mf_tables_extend, *state, max_rows, at, width, width,
+                    slots.data_ptr(), positions.data_ptr(), cu.data_ptr(), lens.data_ptr(), refused.data_ptr(),
+                    nat._WORKSPACE.counters(1, dev).data_ptr())
         return SlotMap(slots, positions, cu, lens, refused)
 
     def truncate(self, lengths: torch.Tensor) -> None:
