@@ -69,6 +69,9 @@ struct Found {
     double mass_before, mass;
 };
 
+// Places of the searches' results.
+enum { AT_K, AT_FIRST, AT_P_LO, AT_P_HI, AT_M, AT_D_LO, AT_D_HI, kFinds };
+
 struct Shared {
     uint64_t words[kBins];   // the bins; then ranked[kList], mass[kList]
     uint64_t list[kList];
@@ -78,8 +81,8 @@ struct Shared {
     int wave_count[16];
     float wave_max[16];
     unsigned long long best;
-    int found[4];
-    Found at[4];
+    int found[2];
+    Found at[kFinds];
     int segs, listed;
     double d0, d1;
     uint64_t u0;
@@ -105,25 +108,22 @@ __device__ __forceinline__ void scan_row(const char* row, int e0, int e1, F f) {
     if (tid < head) one(e0 + tid);
     const int v0 = e0 + head, nv = (e1 - v0) / VE;
     const uint4* vec = (const uint4*)(row + (int64_t)v0 * ES);
-    uint4 next[2];
+    constexpr int U = 4;  // loads in flight
+    uint4 next[U];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) next[u] = tid + u * kThreads < nv ? vec[tid + u * kThreads] : make_uint4(0, 0, 0, 0);
-    for (int v = tid; v < nv; v += 2 * kThreads) {
-        uint4 cur[2] = {next[0], next[1]};
+    for (int u = 0; u < U; ++u) next[u] = tid + u * kThreads < nv ? vec[tid + u * kThreads] : make_uint4(0, 0, 0, 0);
+    for (int v = tid; v < nv; v += U * kThreads) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int w = v + (2 + u) * kThreads;
-            if (w < nv) next[u] = vec[w];
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < U; ++u) {
             const int w = v + u * kThreads;
-            if (w >= nv) break;
-            const uint32_t x[4] = {cur[u].x, cur[u].y, cur[u].z, cur[u].w};
+            const uint32_t x[4] = {next[u].x, next[u].y, next[u].z, next[u].w};
+            if (w + U * kThreads < nv) next[u] = vec[w + U * kThreads];
+            if (w < nv) {
 #pragma unroll
-            for (int k = 0; k < VE; ++k) {
-                const uint32_t bits = ES == 4 ? x[k] : (k & 1 ? x[k >> 1] >> 16 : x[k >> 1] & 0xffffu);
-                f(v0 + w * VE + k, value_of<DT>(bits));
+                for (int k = 0; k < VE; ++k) {
+                    const uint32_t bits = ES == 4 ? x[k] : (k & 1 ? x[k >> 1] >> 16 : x[k >> 1] & 0xffffu);
+                    f(v0 + w * VE + k, value_of<DT>(bits));
+                }
             }
         }
     }
@@ -149,6 +149,11 @@ struct Binner {
     __device__ __forceinline__ bool place(float v, double& y) const {
         y = v == ref_f ? (double)kTop : __builtin_fma(ref - (double)v, per, (double)kTop);
         return y >= 0.0 && y < (double)kBins;
+    }
+    // a number below every logit whose place is above y
+    __device__ __forceinline__ float value_below(int y) const {
+        const double v = ref - ((double)(y - kTop) + 0.01) / per;
+        return (float)(v - fabs(v) * 1e-6);  // NaN where the reference is infinite: nothing is below it
     }
     // 2^qs q, q = 1 - exp(-r / 256) for the part r in [0, 1) of y inside its bin
     __device__ __forceinline__ uint32_t q_of(double y, int bin) const {
@@ -176,8 +181,9 @@ __device__ __forceinline__ void clear_words(Shared& sh) {
     for (int i = threadIdx.x; i < kBins; i += kThreads) sh.words[i] = 0;
 }
 
-// Exclusive sums of the threads' counts and masses, and the totals.
-__device__ __forceinline__ void block_sums(Shared& sh, int& n, double& mass, int& n_all, double& mass_all) {
+// Exclusive sums of the threads' counts and masses, and the totals; mass_end: the inclusive
+// sum, to the bit the next thread's exclusive one.
+__device__ __forceinline__ void block_sums(Shared& sh, int& n, double& mass, double& mass_end, int& n_all, double& mass_all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int ni = n;
     double mi = mass;
@@ -213,16 +219,38 @@ __device__ __forceinline__ void block_sums(Shared& sh, int& n, double& mass, int
     }
     n = nb + ni - n;
     mass = mb + before;
+    mass_end = mb + mi;
 }
 
-// The bins of one thread: counts and masses by walking its kOwn words.
+// The bins of one thread.
 struct Owner {
     int count_shift;
     double q_scale, q_unit;
-    int count_before;      // of the bins before this thread's
+    int count_before, count_end;      // of the bins before this thread's, and with them
     double mass_before, mass_end;
-    int count_end;
-    double top0;           // T_b of its first bin
+    double top0;                      // T_b of its first bin
+
+    // from the bins in sh.words, with the totals; empties the searches' places
+    __device__ __forceinline__ void build(const SampleArgs& a, Shared& sh, int& n_all, double& mass_all) {
+        count_shift = a.count_shift;
+        q_scale = a.q_scale;
+        q_unit = a.q_unit;
+        count_before = 0;
+        mass_before = 0.0;
+        top0 = bin_top(threadIdx.x * kOwn);
+        int n = 0;
+        double mass = 0.0;
+        walk(sh, [&](int, uint64_t w, double, int, double, double m) {
+            n += count(w);
+            mass += m;
+        });
+        if (threadIdx.x < kFinds) sh.at[threadIdx.x].bin = -1;
+        int before = n;
+        block_sums(sh, before, mass, mass_end, n_all, mass_all);
+        count_before = before;
+        mass_before = mass;
+        count_end = before + n;
+    }
 
     __device__ __forceinline__ static double step() { return 0.9961013694701175; }  // exp(-1/256)
     __device__ __forceinline__ int count(uint64_t w) const { return (int)(w >> count_shift); }
@@ -230,17 +258,17 @@ struct Owner {
         const uint64_t n = w >> count_shift;
         return n * (uint64_t)q_scale - (w & ((1ull << count_shift) - 1));
     }
-    // g(bin, word, T_b, count before, mass before, mass): true ends the walk
+    // g(bin, word, T_b, count before, mass before, mass) for every bin that holds anything
     template <class G>
     __device__ __forceinline__ void walk(const Shared& sh, G g) const {
         double top = top0, before = mass_before;
         int n = count_before;
+#pragma unroll 5
         for (int j = 0; j < kOwn; ++j) {
-            const int bin = (int)threadIdx.x * kOwn + j;
-            const uint64_t w = sh.words[bin];
+            const uint64_t w = sh.words[threadIdx.x * kOwn + j];
             if (w) {
                 const double mass = top * ((double)parts(w) * q_unit);
-                if (g(bin, w, top, n, before, mass)) return;
+                g((int)threadIdx.x * kOwn + j, w, top, n, before, mass);
                 before += mass;
                 n += count(w);
             }
@@ -249,30 +277,21 @@ struct Owner {
     }
 };
 
-// The first bin whose inclusive mass exceeds x (COUNT: whose inclusive count does),
-// into sh.at[k]; none: bin -1. All threads call it.
+// The first bin whose inclusive mass exceeds x (COUNT: whose inclusive count does), into
+// sh.at[k], which holds bin -1 before and where there is none. One thread's bins hold the
+// crossing, so nothing is compared between threads; the caller's next barrier publishes it.
 template <bool COUNT>
 __device__ __forceinline__ void find(Shared& sh, const Owner& o, double x, int k) {
-    if (threadIdx.x == 0) {
-        sh.found[k] = kBins;
-        sh.at[k].bin = -1;
-    }
-    __syncthreads();
+    if (COUNT ? !((double)o.count_before <= x && (double)o.count_end > x) : !(o.mass_before <= x && o.mass_end > x)) return;
     Found f;
     f.bin = -1;
-    if (COUNT ? (double)o.count_end > x : o.mass_end > x) {
-        o.walk(sh, [&](int bin, uint64_t w, double, int n, double before, double mass) {
-            if (COUNT ? (double)(n + o.count(w)) > x : before + mass > x) {
-                f = Found{bin, o.count(w), n, before, mass};
-                return true;
-            }
-            return false;
-        });
-    }
-    if (f.bin >= 0) atomicMin(&sh.found[k], f.bin);
-    __syncthreads();
-    if (f.bin >= 0 && f.bin == sh.found[k]) sh.at[k] = f;
-    __syncthreads();
+    bool done = false;
+    o.walk(sh, [&](int bin, uint64_t w, double, int n, double before, double mass) {
+        if (done) return;  // (the sums walked here round differently: the last bin stands in)
+        f = Found{bin, o.count(w), n, before, mass};
+        done = COUNT ? (double)(n + o.count(w)) > x : before + mass > x;
+    });
+    sh.at[k] = f;
 }
 
 // A prefix of the ranking: whole bins before `bin`, then the first n tokens of it.
@@ -299,7 +318,7 @@ __device__ __forceinline__ uint64_t parts_in(const SampleArgs& a, uint64_t w) {
 }
 
 template <int DT>
-__device__ Ranked descend(const SampleArgs& a, Shared& sh, const char* row, const Binner& bn, int bin, bool by_count,
+__device__ __forceinline__ Ranked descend(const SampleArgs& a, Shared& sh, const char* row, const Binner& bn, int bin, bool by_count,
                           double target) {
     // target: tokens (by_count) or parts; found is the first whose inclusive sum exceeds it
     Ranked r{0, 0, 0.0, 0.0, true};
@@ -321,7 +340,7 @@ __device__ Ranked descend(const SampleArgs& a, Shared& sh, const char* row, cons
         __syncthreads();
         // four digits to a thread: the first whose inclusive sum passes the target, else the last
         int n = 0, n_before, n_all;
-        double parts = 0.0, parts_before, parts_all;
+        double parts = 0.0, parts_before, parts_end, parts_all;
         uint64_t w[4];
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
@@ -331,7 +350,7 @@ __device__ Ranked descend(const SampleArgs& a, Shared& sh, const char* row, cons
         }
         n_before = n;
         parts_before = parts;
-        block_sums(sh, n_before, parts_before, n_all, parts_all);
+        block_sums(sh, n_before, parts_before, parts_end, n_all, parts_all);
         if (threadIdx.x == 0) {
             sh.found[0] = 4096;
             sh.found[1] = -1;
@@ -384,32 +403,139 @@ __device__ Ranked descend(const SampleArgs& a, Shared& sh, const char* row, cons
     return r;
 }
 
+// Bins of the tokens [e0, e1) into sh.words; their largest logit.
+template <int DT>
+__device__ float bin_range(const SampleArgs& a, Shared& sh, const char* row, const Binner& bn, int e0, int e1) {
+    float m = -__builtin_huge_valf();
+    scan_row<DT>(row, e0, e1, [&](int, float v) {
+        m = fmaxf(m, v);
+        double y;
+        if (bn.place(v, y))
+            atomicAdd((unsigned long long*)&sh.words[(int)y],
+                      (unsigned long long)((1ull << a.count_shift) + bn.q_of(y, (int)y)));
+    });
+    return block_max(sh, m);
+}
+
+// The finish of a row whose boundary bins are too full for the list: each boundary by itself,
+// in the same order (see descend). Rows of many equal logits and extreme temperatures.
+// top_k 0, p_of -1, mb kBins: no such filter; sh.at holds the searches for k, m and the first.
+template <int DT>
+__device__ __forceinline__ void finish_full(const SampleArgs& a, Shared& sh, const char* row, int r, const Binner& bn, double u,
+                                            int top_k, double p_of, double least, int mb, double mass_all) {
+    const int tid = threadIdx.x;
+    const Found at_k = sh.at[AT_K], at_m = sh.at[AT_M];
+    const int first_bin = sh.at[AT_FIRST].bin;
+    auto top_of = [&](int bin) -> double {  // T_b as its owner forms it
+        double t = bin_top(bin / kOwn * kOwn);
+        for (int j = 0; j < bin % kOwn; ++j) t *= Owner::step();
+        return t;
+    };
+    Limit limit{kBins, 0, mass_all};
+    if (mb != kBins) {
+        const double top = top_of(mb);
+        __syncthreads();
+        if (tid == 0) {
+            sh.u0 = 0;
+            sh.i0 = 0;
+        }
+        __syncthreads();
+        scan_row<DT>(row, 0, a.vocab, [&](int, float v) {
+            double y;
+            if (!bn.place(v, y) || (int)y != mb) return;
+            const uint64_t p = (uint64_t)a.q_scale - bn.q_of(y, mb);
+            if (top * ((double)p * a.q_unit) < least) return;
+            atomicAdd((unsigned long long*)&sh.u0, (unsigned long long)p);
+            atomicAdd(&sh.i0, 1);
+        });
+        __syncthreads();
+        limit = Limit{mb, sh.i0, at_m.mass_before + top * ((double)sh.u0 * a.q_unit)};
+    }
+    double mass_k = mass_all;
+    enum { BY_K, BY_P, ONE, DRAW, LAST };
+    bool clobbered = false;  // a descent has used the bins' memory
+    for (int stage = BY_K; stage <= LAST; ++stage) {
+        // ---- the bin, and the count or mass whose passing is looked for
+        Found f{-1, 0, 0, 0.0, 0.0};
+        bool by_count = false;
+        double target = 0.0;
+        if (stage == BY_K) {
+            if (top_k == 0) continue;
+            f = at_k;
+            by_count = true;
+            target = (double)(top_k - 1 - f.count_before);
+        } else if (stage == ONE) {
+            f.bin = first_bin;
+            by_count = true;
+        } else {
+            if (stage == BY_P && p_of < 0.0) continue;
+            if (stage != LAST) {
+                const double x = stage == BY_P ? p_of * mass_k : u * limit.mass;
+                __syncthreads();
+                if (clobbered) {
+                    clear_words(sh);
+                    __syncthreads();
+                    bin_range<DT>(a, sh, row, bn, 0, a.vocab);
+                    __syncthreads();
+                }
+                Owner own;
+                int n_all;
+                double m_all;
+                own.build(a, sh, n_all, m_all);
+                __syncthreads();
+                find<false>(sh, own, x, AT_D_LO);
+                __syncthreads();
+                f = sh.at[AT_D_LO];
+                target = (x - f.mass_before) / top_of(max(f.bin, 0)) * a.q_scale;
+                if (stage == BY_P && f.bin < 0) continue;
+                if (stage == DRAW && (f.bin < 0 || f.bin > limit.bin)) continue;  // the limit's last token
+            } else {
+                f.bin = limit.bin;
+                by_count = true;
+                target = (double)(limit.n - 1);
+            }
+        }
+        const double top = top_of(f.bin);
+        const Ranked e = descend<DT>(a, sh, row, bn, f.bin, by_count, target);
+        clobbered = true;
+        const double upto = f.mass_before + top * ((e.parts_before + e.parts) * a.q_unit);
+        if (stage == BY_K) {
+            const Limit l{f.bin, e.before + 1, upto};
+            mass_k = l.mass;
+            if (l.before(limit)) limit = l;
+        } else if (stage == BY_P) {
+            const Limit l = e.found ? Limit{f.bin, e.before + 1, upto} : Limit{f.bin, f.n, f.mass_before + f.mass};
+            if (l.before(limit)) limit = l;
+        } else if (stage == ONE) {
+            const Limit l{f.bin, 1, top * (e.parts * a.q_unit)};
+            if (limit.before(l)) limit = l;
+        } else {
+            if (stage == DRAW) {
+                if (!e.found && f.bin != limit.bin) {  // the bin's last token, by a rounding
+                    limit = Limit{f.bin, f.n, limit.mass};
+                    continue;
+                }
+                if (!e.found || (f.bin == limit.bin && e.before >= limit.n)) continue;
+            }
+            if (tid == 0) {
+                a.tokens[r] = (int64_t)(uint32_t)e.key;
+                if (a.probs) a.probs[r] = (float)(top * (e.parts * a.q_unit) / limit.mass);
+            }
+            __syncthreads();
+            return;
+        }
+    }
+}
+
 // The finish of one row, whose bins are in sh.words.
 template <int DT>
-__device__ void finish_row(const SampleArgs& a, Shared& sh, const char* row, int r, const Binner& bn, float largest,
+__device__ __forceinline__ void finish_row(const SampleArgs& a, Shared& sh, const char* row, int r, const Binner& bn, float largest,
                            float temp) {
     const int tid = threadIdx.x;
     Owner own;
-    own.count_shift = a.count_shift;
-    own.q_scale = a.q_scale;
-    own.q_unit = a.q_unit;
-    own.count_before = 0;
-    own.mass_before = 0.0;
-    own.top0 = bin_top(tid * kOwn);
-    int n = 0;
-    double mass = 0.0;
-    own.walk(sh, [&](int, uint64_t w, double, int, double, double m) {
-        n += own.count(w);
-        mass += m;
-        return false;
-    });
-    int n_before = n, n_all;
-    double mass_before = mass, mass_all;
-    block_sums(sh, n_before, mass_before, n_all, mass_all);
-    own.count_before = n_before;
-    own.mass_before = mass_before;
-    own.count_end = n_before + n;
-    own.mass_end = mass_before + mass;
+    int n_all;
+    double mass_all;
+    own.build(a, sh, n_all, mass_all);
 
     const int top_k = a.top_k ? a.top_k[r] : a.top_k0;
     const double top_p = a.top_p ? a.top_p[r] : a.top_p0;
@@ -427,59 +553,56 @@ __device__ void finish_row(const SampleArgs& a, Shared& sh, const char* row, int
     const double least = largest == bn.ref_f ? min_p : min_p * exp((largest - bn.ref) * bn.per * (1.0 / kPerE));
     int kb = none, p_lo = none, p_hi = none, mb = none;
     double lo = mass_all, hi = mass_all;
-    if (by_k) {
-        find<true>(sh, own, (double)(top_k - 1), 0);
-        kb = sh.at[0].bin;
-        lo = sh.at[0].mass_before;
-        hi = lo + sh.at[0].mass;
-    }
-    const double p_of = top_p > 0.0 ? top_p : 0.0;
-    if (by_p) {
-        find<false>(sh, own, p_of * lo, 1);
-        find<false>(sh, own, p_of * hi, 2);
-        p_lo = sh.at[1].bin >= 0 ? sh.at[1].bin : none;
-        p_hi = sh.at[2].bin >= 0 ? sh.at[2].bin : kBins - 1;
-        if (p_lo != none) lo = fmin(lo, sh.at[1].mass_before);
-        if (sh.at[2].bin >= 0) hi = fmin(hi, sh.at[2].mass_before + sh.at[2].mass);
-    }
+    if (by_k) find<true>(sh, own, (double)(top_k - 1), AT_K);
+    find<true>(sh, own, 0.0, AT_FIRST);  // the first bin that holds anything
     if (by_m) {
         // w >= min_p: places down to -ln(min_p) below the largest logit
         double y;
         bn.place(largest, y);
         const double edge = y - log(min_p) * kPerE;
-        mb = edge < 0.0 ? 0 : edge < (double)kBins ? (int)edge : none;
-        if (min_p > 1.0) mb = (int)y;
-        if (mb != none) {
-            // the masses around that bin
-            if (tid == 0) sh.d0 = -1.0;
-            __syncthreads();
-            if (tid == mb / kOwn) {
-                double before = own.mass_before, m = 0.0;
-                own.walk(sh, [&](int bin, uint64_t, double, int, double b, double mm) {
-                    if (bin < mb) before = b + mm;
-                    if (bin == mb) m = mm;
-                    return bin >= mb;
-                });
-                sh.at[3] = Found{mb, 0, 0, before, m};
-            }
-            __syncthreads();
-            lo = fmin(lo, sh.at[3].mass_before);
-            hi = fmin(hi, sh.at[3].mass_before + sh.at[3].mass);
+        mb = min_p > 1.0 ? (int)y : edge < 0.0 ? 0 : edge < (double)kBins ? (int)edge : none;
+        if (mb != none && tid == mb / kOwn) {  // the masses around that bin
+            double before = own.mass_before, m = 0.0;
+            own.walk(sh, [&](int bin, uint64_t, double, int, double b, double mm) {
+                if (bin < mb) before = b + mm;
+                if (bin == mb) m = mm;
+            });
+            sh.at[AT_M] = Found{mb, 0, 0, before, m};
         }
     }
-    find<false>(sh, own, 0.0, 0);  // the first bin that holds anything
-    const int first_bin = sh.at[0].bin;
-    find<false>(sh, own, u * lo, 1);
-    find<false>(sh, own, u * hi, 2);
-    const int d_lo = sh.at[1].bin >= 0 ? sh.at[1].bin : 0;
-    const int d_hi = sh.at[2].bin >= 0 ? sh.at[2].bin : kBins - 1;
-
-    // ---- their tokens, bin by bin
+    __syncthreads();
+    const int first_bin = sh.at[AT_FIRST].bin;
+    if (by_k) {
+        kb = sh.at[AT_K].bin;
+        lo = sh.at[AT_K].mass_before;
+        hi = lo + sh.at[AT_K].mass;
+    }
+    const double p_of = top_p > 0.0 ? top_p : 0.0;
+    if (by_p) {
+        find<false>(sh, own, p_of * lo, AT_P_LO);
+        find<false>(sh, own, p_of * hi, AT_P_HI);
+        __syncthreads();
+        p_lo = sh.at[AT_P_LO].bin >= 0 ? sh.at[AT_P_LO].bin : none;
+        p_hi = sh.at[AT_P_HI].bin >= 0 ? sh.at[AT_P_HI].bin : kBins - 1;
+        if (p_lo != none) lo = fmin(lo, sh.at[AT_P_LO].mass_before);
+        if (sh.at[AT_P_HI].bin >= 0) hi = fmin(hi, sh.at[AT_P_HI].mass_before + sh.at[AT_P_HI].mass);
+    }
+    if (mb != none) {
+        lo = fmin(lo, sh.at[AT_M].mass_before);
+        hi = fmin(hi, sh.at[AT_M].mass_before + sh.at[AT_M].mass);
+    }
+    hi = fmax(hi, sh.at[AT_FIRST].mass);  // (the first token is kept whatever the filters say)
+    find<false>(sh, own, u * lo, AT_D_LO);
+    find<false>(sh, own, u * hi, AT_D_HI);
     if (tid == 0) {
         sh.segs = 0;
         sh.listed = 0;
     }
     __syncthreads();
+    const int d_lo = sh.at[AT_D_LO].bin >= 0 ? sh.at[AT_D_LO].bin : 0;
+    const int d_hi = sh.at[AT_D_HI].bin >= 0 ? sh.at[AT_D_HI].bin : kBins - 1;
+
+    // ---- their tokens, bin by bin
     auto wanted = [&](int bin) {
         return bin == kb || (bin >= p_lo && bin <= p_hi) || bin == mb || (bin >= d_lo && bin <= d_hi) || bin == first_bin;
     };
@@ -488,7 +611,6 @@ __device__ void finish_row(const SampleArgs& a, Shared& sh, const char* row, int
             const int k = atomicAdd(&sh.segs, 1), base = atomicAdd(&sh.listed, own.count(w));
             if (k < kSegs) sh.seg[k] = Seg{before, top, own.parts(w), bin, base, own.count(w), nb, 0};
         }
-        return false;
     });
     __syncthreads();
     const int segs = sh.segs, listed = sh.listed;
@@ -511,7 +633,10 @@ __device__ void finish_row(const SampleArgs& a, Shared& sh, const char* row, int
             b1 = max(b1, sh.seg[k].bin);
         }
         const double y0 = b0, y1 = b1 + 1;
+        // no logit below this reaches those bins (the margin is far above the roundings of both sides)
+        const float least_v = bn.value_below(b1 + 1);
         scan_row<DT>(row, 0, a.vocab, [&](int i, float v) {
+            if (v < least_v) return;
             double y;
             bn.place(v, y);
             if (!(y >= y0 && y < y1)) return;
@@ -556,6 +681,7 @@ __device__ void finish_row(const SampleArgs& a, Shared& sh, const char* row, int
             const int j0 = s.base, j1 = s.base + s.n;
             int rank = 0;
             uint64_t sum = 0;
+#pragma unroll 8
             for (int j = j0; j < j1; ++j) {
                 const bool ahead = sh.list[j] < keys[c];
                 rank += ahead;
@@ -608,7 +734,7 @@ __device__ void finish_row(const SampleArgs& a, Shared& sh, const char* row, int
         }
         if (by_m && mb != none) {
             const int k = seg_of(mb);
-            Limit l{mb, 0, sh.at[3].mass_before};
+            Limit l{mb, 0, sh.at[AT_M].mass_before};
             if (k >= 0) {
                 const Seg& s = sh.seg[k];
                 l.n = many(s, [&](int j) {
@@ -644,96 +770,7 @@ __device__ void finish_row(const SampleArgs& a, Shared& sh, const char* row, int
         __syncthreads();
         return;
     }
-    // ---- full bins: each boundary by itself, in the same order. The searches keep to
-    // the intervals found above, so the bins' words are formed again after each.
-    // (not reached by the list; see descend)
-    Binner again = bn;
-    auto rebin = [&]() {
-        __syncthreads();
-        clear_words(sh);
-        __syncthreads();
-        scan_row<DT>(row, 0, a.vocab, [&](int, float v) {
-            double y;
-            if (again.place(v, y))
-                atomicAdd((unsigned long long*)&sh.words[(int)y],
-                          (unsigned long long)((1ull << a.count_shift) + again.q_of(y, (int)y)));
-        });
-        __syncthreads();
-    };
-    auto top_of = [&](int bin) -> double {  // T_b as its owner forms it
-        double t = bin_top(bin / kOwn * kOwn);
-        for (int j = 0; j < bin % kOwn; ++j) t *= Owner::step();
-        return t;
-    };
-    double mass_k = mass_all;
-    if (by_k) {
-        find<true>(sh, own, (double)(top_k - 1), 0);
-        const Found f = sh.at[0];
-        const Ranked e = descend<DT>(a, sh, row, bn, f.bin, true, (double)(top_k - 1 - f.count_before));
-        limit = Limit{f.bin, e.before + 1, f.mass_before + top_of(f.bin) * ((e.parts_before + e.parts) * a.q_unit)};
-        mass_k = limit.mass;
-        rebin();
-    }
-    if (by_p) {
-        const double x = p_of * mass_k;
-        find<false>(sh, own, x, 0);
-        const Found f = sh.at[0];
-        if (f.bin >= 0) {
-            const double top = top_of(f.bin);
-            const Ranked e = descend<DT>(a, sh, row, bn, f.bin, false, (x - f.mass_before) / top * a.q_scale);
-            Limit l{f.bin, f.n, f.mass_before + f.mass};
-            if (e.found)
-                l = Limit{f.bin, e.before + 1, f.mass_before + top * ((e.parts_before + e.parts) * a.q_unit)};
-            if (l.before(limit)) limit = l;
-            rebin();
-        }
-    }
-    if (by_m && mb != none) {
-        const double top = top_of(mb);
-        if (tid == 0) {
-            sh.u0 = 0;
-            sh.i0 = 0;
-        }
-        __syncthreads();
-        scan_row<DT>(row, 0, a.vocab, [&](int, float v) {
-            double yy;
-            if (!bn.place(v, yy) || (int)yy != mb) return;
-            const uint64_t p = (uint64_t)a.q_scale - bn.q_of(yy, mb);
-            if (top * ((double)p * a.q_unit) < least) return;
-            atomicAdd((unsigned long long*)&sh.u0, (unsigned long long)p);
-            atomicAdd(&sh.i0, 1);
-        });
-        __syncthreads();
-        const Limit l{mb, sh.i0, sh.at[3].mass_before + top * ((double)sh.u0 * a.q_unit)};
-        if (l.before(limit)) limit = l;
-        __syncthreads();
-    }
-    {
-        const Ranked e = descend<DT>(a, sh, row, bn, first_bin, true, 0.0);
-        const Limit one{first_bin, 1, top_of(first_bin) * (e.parts * a.q_unit)};
-        if (limit.before(one)) limit = one;
-        rebin();
-    }
-    const double x = u * limit.mass;
-    find<false>(sh, own, x, 0);
-    Found f = sh.at[0];
-    double by_count = -1.0;  // >= 0: this token of the bin, the limit's last
-    if (f.bin < 0 || f.bin > limit.bin) {
-        f.bin = limit.bin;
-        by_count = limit.n - 1;
-    }
-    const double top = top_of(f.bin);
-    Ranked e{};
-    if (by_count < 0.0) {
-        e = descend<DT>(a, sh, row, bn, f.bin, false, (x - f.mass_before) / top * a.q_scale);
-        if (!e.found || (f.bin == limit.bin && e.before >= limit.n)) by_count = f.bin == limit.bin ? limit.n - 1 : f.n - 1;
-    }
-    if (by_count >= 0.0) e = descend<DT>(a, sh, row, bn, f.bin, true, by_count);
-    if (tid == 0) {
-        a.tokens[r] = (int64_t)(uint32_t)e.key;
-        if (a.probs) a.probs[r] = (float)(top * (e.parts * a.q_unit) / limit.mass);
-    }
-    __syncthreads();
+    finish_full<DT>(a, sh, row, r, bn, u, by_k ? top_k : 0, by_p ? p_of : -1.0, by_m ? least : 0.0, mb, mass_all);
 }
 
 // The first largest logit.
@@ -758,20 +795,6 @@ __device__ void greedy_row(const SampleArgs& a, Shared& sh, const char* row, int
         if (a.probs) a.probs[r] = 1.f;
     }
     __syncthreads();
-}
-
-// Bins of the tokens [e0, e1) into sh.words; their largest logit.
-template <int DT>
-__device__ float bin_range(const SampleArgs& a, Shared& sh, const char* row, const Binner& bn, int e0, int e1) {
-    float m = -__builtin_huge_valf();
-    scan_row<DT>(row, e0, e1, [&](int, float v) {
-        m = fmaxf(m, v);
-        double y;
-        if (bn.place(v, y))
-            atomicAdd((unsigned long long*)&sh.words[(int)y],
-                      (unsigned long long)((1ull << a.count_shift) + bn.q_of(y, (int)y)));
-    });
-    return block_max(sh, m);
 }
 
 template <int DT>
