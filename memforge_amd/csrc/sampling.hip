@@ -33,7 +33,10 @@ constexpr int kThreads = 1024;
 constexpr int kOwn = 15;                 // consecutive bins of one thread (odd: no LDS bank twice)
 constexpr int kBins = kOwn * kThreads;
 constexpr double kPerE = 256.0;          // bins to a factor e of weight
-constexpr int kTop = kBins - 32 * 256;   // the bin of the reference logit
+// The bin of the reference logit: 32 factors e below it have bins. Even and its thread's first,
+// so that equal logits at the reference weigh exactly 1 (Binner, Owner).
+constexpr int kTop = (kBins - 32 * 256 + 5) / kOwn * kOwn;
+static_assert(kTop % 2 == 0 && kTop % kOwn == 0 && kBins - kTop >= 8190, "the reference's bin");
 constexpr int kList = 2048;              // tokens of boundary bins that are ranked in LDS
 constexpr int kSegs = 128;               // boundary bins
 constexpr int kFirst = 8192;             // tokens of a row whose maximum is the reference
@@ -73,7 +76,7 @@ struct Found {
 enum { AT_K, AT_FIRST, AT_P_LO, AT_P_HI, AT_M, AT_D_LO, AT_D_HI, kFinds };
 
 struct Shared {
-    uint64_t words[kBins];   // the bins; then ranked[kList], mass[kList]
+    uint64_t words[kBins + 64];  // the bins, and words that are never read; then the ranking's arrays
     uint64_t list[kList];
     uint8_t list_seg[kList];
     Seg seg[kSegs];
@@ -91,14 +94,14 @@ struct Shared {
 
 template <int DT>
 __device__ __forceinline__ float value_of(uint32_t bits) {
-    const float v = bits_to_f32<DT>(bits);
-    return v == v ? v : -__builtin_huge_valf();  // NaN: never drawn
+    return bits_to_f32<DT>(bits);
 }
 
-// f(index, logit) for the tokens [e0, e1) of a row, each by one of the
-// workgroup's threads: 16-byte loads from the first aligned token on.
-template <int DT, class F>
-__device__ __forceinline__ void scan_row(const char* row, int e0, int e1, F f) {
+// g(first index, 16 bytes of consecutive logits) for the tokens [e0, e1) of a row, each by one
+// of the workgroup's threads, from the first aligned token on; f(index, logit) for the few
+// around them.
+template <int DT, class F, class G>
+__device__ __forceinline__ void scan_row(const char* row, int e0, int e1, F f, G g) {
     constexpr int ES = DT == MF_F32 ? 4 : 2, VE = 16 / ES;
     const int tid = threadIdx.x;
     auto one = [&](int i) {
@@ -108,58 +111,96 @@ __device__ __forceinline__ void scan_row(const char* row, int e0, int e1, F f) {
     if (tid < head) one(e0 + tid);
     const int v0 = e0 + head, nv = (e1 - v0) / VE;
     const uint4* vec = (const uint4*)(row + (int64_t)v0 * ES);
-    constexpr int U = 4;  // loads in flight
-    uint4 next[U];
+    // loads two rounds of U ahead, none of them behind a branch (the compiler waits for every
+    // load in flight where a branch joins); past the end the last piece is read again
+    constexpr int U = 2;
+    if (nv > 0) {
+        auto piece = [&](int w) { return vec[min(w, nv - 1)]; };
+        uint4 one_ahead[U], two_ahead[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) next[u] = tid + u * kThreads < nv ? vec[tid + u * kThreads] : make_uint4(0, 0, 0, 0);
-    for (int v = tid; v < nv; v += U * kThreads) {
+        for (int u = 0; u < U; ++u) one_ahead[u] = piece(tid + u * kThreads);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int w = v + u * kThreads;
-            const uint32_t x[4] = {next[u].x, next[u].y, next[u].z, next[u].w};
-            if (w + U * kThreads < nv) next[u] = vec[w + U * kThreads];
-            if (w < nv) {
+        for (int u = 0; u < U; ++u) two_ahead[u] = piece(tid + (U + u) * kThreads);
+        for (int v = tid; v < nv; v += U * kThreads) {
+            uint4 cur[U];
 #pragma unroll
-                for (int k = 0; k < VE; ++k) {
-                    const uint32_t bits = ES == 4 ? x[k] : (k & 1 ? x[k >> 1] >> 16 : x[k >> 1] & 0xffffu);
-                    f(v0 + w * VE + k, value_of<DT>(bits));
-                }
+            for (int u = 0; u < U; ++u) {
+                cur[u] = one_ahead[u];
+                one_ahead[u] = two_ahead[u];
+                two_ahead[u] = piece(v + (2 * U + u) * kThreads);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t x[4] = {cur[u].x, cur[u].y, cur[u].z, cur[u].w};
+                float v_[VE];
+#pragma unroll
+                for (int k = 0; k < VE; ++k)
+                    v_[k] = value_of<DT>(ES == 4 ? x[k] : (k & 1 ? x[k >> 1] >> 16 : x[k >> 1] & 0xffffu));
+                if (v + u * kThreads < nv) g(v0 + (v + u * kThreads) * VE, v_);
             }
         }
     }
     const int tail = v0 + nv * VE;
     if (tid < e1 - tail) one(tail + tid);
 }
+template <int DT, class F>
+__device__ __forceinline__ void scan_row(const char* row, int e0, int e1, F f) {
+    scan_row<DT>(row, e0, e1, f, [&](int i, const auto& v) {
+#pragma unroll
+        for (int k = 0; k < (int)(sizeof(v) / 4); ++k) f(i + k, v[k]);
+    });
+}
 
-// Larger for a larger logit; -0 as 0.
+// Larger for a larger logit; -0 as 0, NaN as -infinity.
 __device__ __forceinline__ uint32_t order_key(float v) {
-    const uint32_t u = __float_as_uint(v + 0.f);
+    const uint32_t u = v == v ? __float_as_uint(v + 0.f) : 0xff800000u;
     return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
-// A token's bin and q below the reference; false where its weight is nothing.
+// Places of logits below a finite reference: y = kTop + 256 (reference - logit) / T, whose whole
+// part is the bin: y - 1/2 rounded to the nearest, which leaves the whole number in the low
+// bits of a sum and costs a quarter of the conversions (a y that is whole may fall to the
+// bin above, with the same weight; the even kTop itself does not).
 struct Binner {
-    double ref, per, q_scale;
-    float ref_f;
+    double ref, per, c1, c2, c3, c4;
+    uint32_t one_hi;  // a token's count in its word
+    float lo, hi;     // the logits that have a bin
+
+    static constexpr double kWhole = 6755399441055744.0;  // 1.5 * 2^52
     __device__ __forceinline__ Binner(const SampleArgs& a, float reference, float temp)
-        : ref(reference), per(kPerE / (double)temp), q_scale(a.q_scale), ref_f(reference) {}
-    __device__ __forceinline__ bool place(float v, double& y) const {
-        y = v == ref_f ? (double)kTop : __builtin_fma(ref - (double)v, per, (double)kTop);
-        return y >= 0.0 && y < (double)kBins;
+        : ref(reference), per(kPerE / (double)temp), c1(a.q_scale), c2(-0.5 * a.q_scale), c3(a.q_scale / 6.0),
+          c4(a.q_scale / -24.0), one_hi(1u << (a.count_shift - 32)) {
+        lo = fmaxf((float)(ref - (kBins - kTop - 0.02) / per), -3.4028234663852886e38f);
+        hi = fminf((float)(ref + (kTop - 0.02) / per), 3.4028234663852886e38f);
+        while (!(y_of(lo) < kBins - 0.01)) lo = nextafterf(lo, __builtin_huge_valf());  // rounded outwards: a step or two
+        while (!(y_of(hi) > 0.01)) hi = nextafterf(hi, -__builtin_huge_valf());
     }
-    // a number below every logit whose place is above y
-    __device__ __forceinline__ float value_below(int y) const {
-        const double v = ref - ((double)(y - kTop) + 0.01) / per;
-        return (float)(v - fabs(v) * 1e-6);  // NaN where the reference is infinite: nothing is below it
+    __device__ __forceinline__ double y_of(float v) const { return __builtin_fma(ref - (double)v, per, (double)kTop); }
+    // a token's bin and its place below the bin's top in factors e; false where it has none
+    __device__ __forceinline__ bool has_bin(float v) const { return v >= lo && v <= hi; }
+    __device__ __forceinline__ void place_any(float v, int& bin, double& t) const {
+        const double y = __builtin_fma(ref - (double)v, per, kTop - 0.5), whole = y + kWhole;
+        bin = (int)(uint32_t)__double_as_longlong(whole);
+        t = __builtin_fma(y - (whole - kWhole), 1.0 / kPerE, 0.5 / kPerE);
     }
-    // 2^qs q, q = 1 - exp(-r / 256) for the part r in [0, 1) of y inside its bin
-    __device__ __forceinline__ uint32_t q_of(double y, int bin) const {
-        const double t = (y - (double)bin) * (1.0 / kPerE);
-        const double q = t * __builtin_fma(t, __builtin_fma(t, __builtin_fma(t, -1.0 / 24.0, 1.0 / 6.0), -0.5), 1.0);
-        return (uint32_t)__builtin_fma(q, q_scale, 0.5);
+    __device__ __forceinline__ bool place(float v, int& bin, double& t) const {
+        if (!has_bin(v)) return false;
+        place_any(v, bin, t);
+        return true;
+    }
+    // 2^qs q, q = 1 - exp(-t)
+    __device__ __forceinline__ uint32_t q_of(double t) const {
+        return (uint32_t)__double_as_longlong(
+            __builtin_fma(t, __builtin_fma(t, __builtin_fma(t, __builtin_fma(t, c4, c3), c2), c1), 4503599627370496.0));
+    }
+    __device__ __forceinline__ unsigned long long word(double t) const { return (unsigned long long)one_hi << 32 | q_of(t); }
+    // a number below every logit of bins up to `bin`
+    __device__ __forceinline__ float value_below(int bin) const {
+        const double v = ref - ((double)(bin - kTop) + 1.1) / per;
+        return (float)(v - fabs(v) * 1e-6);
     }
 };
 
@@ -258,6 +299,11 @@ struct Owner {
         const uint64_t n = w >> count_shift;
         return n * (uint64_t)q_scale - (w & ((1ull << count_shift) - 1));
     }
+    // n - sum of q: the word's weight in units of T_b (its sum is below 2^52)
+    __device__ __forceinline__ double weight(uint64_t w) const {
+        const double q = __longlong_as_double((long long)((w & ((1ull << count_shift) - 1)) | 0x4330000000000000ull)) - 4503599627370496.0;
+        return __builtin_fma(q, -q_unit, (double)(uint32_t)(w >> count_shift));
+    }
     // g(bin, word, T_b, count before, mass before, mass) for every bin that holds anything
     template <class G>
     __device__ __forceinline__ void walk(const Shared& sh, G g) const {
@@ -267,7 +313,7 @@ struct Owner {
         for (int j = 0; j < kOwn; ++j) {
             const uint64_t w = sh.words[threadIdx.x * kOwn + j];
             if (w) {
-                const double mass = top * ((double)parts(w) * q_unit);
+                const double mass = top * weight(w);
                 g((int)threadIdx.x * kOwn + j, w, top, n, before, mass);
                 before += mass;
                 n += count(w);
@@ -276,6 +322,12 @@ struct Owner {
         }
     }
 };
+
+__device__ __forceinline__ double top_of(int bin) {  // T_b as its owner forms it
+    double t = bin_top(bin / kOwn * kOwn);
+    for (int j = 0; j < bin % kOwn; ++j) t *= Owner::step();
+    return t;
+}
 
 // The first bin whose inclusive mass exceeds x (COUNT: whose inclusive count does), into
 // sh.at[k], which holds bin -1 before and where there is none. One thread's bins hold the
@@ -330,12 +382,13 @@ __device__ __forceinline__ Ranked descend(const SampleArgs& a, Shared& sh, const
         for (int i = threadIdx.x; i < 4096; i += kThreads) sh.words[i] = 0;
         __syncthreads();
         scan_row<DT>(row, 0, a.vocab, [&](int i, float v) {
-            double y;
-            if (!bn.place(v, y) || (int)y != bin) return;
+            int at;
+            double part;
+            if (!bn.place(v, at, part) || at != bin) return;
             const uint64_t key = (uint64_t)~order_key(v) << 32 | (uint32_t)i;
             if (level > 0 && (key >> (shift + width)) != prefix) return;
             atomicAdd((unsigned long long*)&sh.words[(key >> shift) & ((1u << width) - 1)],
-                      (unsigned long long)((1ull << a.count_shift) + bn.q_of(y, bin)));
+                      bn.word(part));
         });
         __syncthreads();
         // four digits to a thread: the first whose inclusive sum passes the target, else the last
@@ -407,13 +460,32 @@ __device__ __forceinline__ Ranked descend(const SampleArgs& a, Shared& sh, const
 template <int DT>
 __device__ float bin_range(const SampleArgs& a, Shared& sh, const char* row, const Binner& bn, int e0, int e1) {
     float m = -__builtin_huge_valf();
-    scan_row<DT>(row, e0, e1, [&](int, float v) {
-        m = fmaxf(m, v);
-        double y;
-        if (bn.place(v, y))
-            atomicAdd((unsigned long long*)&sh.words[(int)y],
-                      (unsigned long long)((1ull << a.count_shift) + bn.q_of(y, (int)y)));
-    });
+    auto add = [&](int bin, double part) { atomicAdd((unsigned long long*)&sh.words[bin], bn.word(part)); };
+    scan_row<DT>(
+        row, e0, e1,
+        [&](int, float v) {
+            m = fmaxf(m, v);
+            int bin;
+            double part;
+            if (bn.place(v, bin, part)) add(bin, part);
+        },
+        [&](int, const auto& v) {
+            // without a branch between them, so that their chains of fp64 operations run side by
+            // side; what has no bin adds to a word of the lane's own
+            constexpr int N = sizeof(v) / 4;
+            int bin[N];
+            unsigned long long word[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                m = fmaxf(m, v[k]);
+                double part;
+                bn.place_any(v[k], bin[k], part);
+                bin[k] = bn.has_bin(v[k]) ? bin[k] : kBins + (int)(threadIdx.x & 63);
+                word[k] = bn.word(part);
+            }
+#pragma unroll
+            for (int k = 0; k < N; ++k) atomicAdd((unsigned long long*)&sh.words[bin[k]], word[k]);
+        });
     return block_max(sh, m);
 }
 
@@ -426,11 +498,6 @@ __device__ __forceinline__ void finish_full(const SampleArgs& a, Shared& sh, con
     const int tid = threadIdx.x;
     const Found at_k = sh.at[AT_K], at_m = sh.at[AT_M];
     const int first_bin = sh.at[AT_FIRST].bin;
-    auto top_of = [&](int bin) -> double {  // T_b as its owner forms it
-        double t = bin_top(bin / kOwn * kOwn);
-        for (int j = 0; j < bin % kOwn; ++j) t *= Owner::step();
-        return t;
-    };
     Limit limit{kBins, 0, mass_all};
     if (mb != kBins) {
         const double top = top_of(mb);
@@ -441,9 +508,10 @@ __device__ __forceinline__ void finish_full(const SampleArgs& a, Shared& sh, con
         }
         __syncthreads();
         scan_row<DT>(row, 0, a.vocab, [&](int, float v) {
-            double y;
-            if (!bn.place(v, y) || (int)y != mb) return;
-            const uint64_t p = (uint64_t)a.q_scale - bn.q_of(y, mb);
+            int at;
+            double part;
+            if (!bn.place(v, at, part) || at != mb) return;
+            const uint64_t p = (uint64_t)a.q_scale - bn.q_of(part);
             if (top * ((double)p * a.q_unit) < least) return;
             atomicAdd((unsigned long long*)&sh.u0, (unsigned long long)p);
             atomicAdd(&sh.i0, 1);
@@ -528,9 +596,8 @@ __device__ __forceinline__ void finish_full(const SampleArgs& a, Shared& sh, con
 }
 
 // The finish of one row, whose bins are in sh.words.
-template <int DT>
-__device__ __forceinline__ void finish_row(const SampleArgs& a, Shared& sh, const char* row, int r, const Binner& bn, float largest,
-                           float temp) {
+template <int DT, bool FULL>
+__device__ __forceinline__ void finish_row(const SampleArgs& a, Shared& sh, const char* row, int r, const Binner& bn, float largest) {
     const int tid = threadIdx.x;
     Owner own;
     int n_all;
@@ -550,17 +617,19 @@ __device__ __forceinline__ void finish_row(const SampleArgs& a, Shared& sh, cons
     const bool by_m = min_p > 0.0;
     const int none = kBins;
     // the least weight that min_p lets pass, in the bins' unit
-    const double least = largest == bn.ref_f ? min_p : min_p * exp((largest - bn.ref) * bn.per * (1.0 / kPerE));
+    // (formed as the tokens' own weights are, so that one passes at 1)
+    int top_bin = 0;
+    double top_part = 0.0;
+    bn.place(largest, top_bin, top_part);
+    const double least = min_p * (top_of(top_bin) * ((double)((uint64_t)a.q_scale - bn.q_of(top_part)) * a.q_unit));
     int kb = none, p_lo = none, p_hi = none, mb = none;
     double lo = mass_all, hi = mass_all;
     if (by_k) find<true>(sh, own, (double)(top_k - 1), AT_K);
     find<true>(sh, own, 0.0, AT_FIRST);  // the first bin that holds anything
     if (by_m) {
         // w >= min_p: places down to -ln(min_p) below the largest logit
-        double y;
-        bn.place(largest, y);
-        const double edge = y - log(min_p) * kPerE;
-        mb = min_p > 1.0 ? (int)y : edge < 0.0 ? 0 : edge < (double)kBins ? (int)edge : none;
+        const double y = bn.y_of(largest), edge = min_p > 1.0 ? y : y - log(min_p) * kPerE;
+        mb = edge < kBins - 1 ? max((int)floor(edge), 0) : none;
         if (mb != none && tid == mb / kOwn) {  // the masses around that bin
             double before = own.mass_before, m = 0.0;
             own.walk(sh, [&](int bin, uint64_t, double, int, double b, double mm) {
@@ -602,11 +671,18 @@ __device__ __forceinline__ void finish_row(const SampleArgs& a, Shared& sh, cons
     const int d_lo = sh.at[AT_D_LO].bin >= 0 ? sh.at[AT_D_LO].bin : 0;
     const int d_hi = sh.at[AT_D_HI].bin >= 0 ? sh.at[AT_D_HI].bin : kBins - 1;
 
+    if constexpr (FULL) {
+        finish_full<DT>(a, sh, row, r, bn, u, by_k ? top_k : 0, by_p ? p_of : -1.0, least, mb, mass_all);
+        return;
+    }
     // ---- their tokens, bin by bin
     auto wanted = [&](int bin) {
         return bin == kb || (bin >= p_lo && bin <= p_hi) || bin == mb || (bin >= d_lo && bin <= d_hi) || bin == first_bin;
     };
-    own.walk(sh, [&](int bin, uint64_t w, double top, int nb, double before, double) {
+    const int own0 = tid * kOwn, own1 = own0 + kOwn - 1;
+    auto near = [&](int b0, int b1) { return b0 <= own1 && b1 >= own0; };
+    if (near(kb, kb) || near(p_lo, p_hi) || near(mb, mb) || near(d_lo, d_hi) || near(first_bin, first_bin))
+        own.walk(sh, [&](int bin, uint64_t w, double top, int nb, double before, double) {
         if (wanted(bin)) {
             const int k = atomicAdd(&sh.segs, 1), base = atomicAdd(&sh.listed, own.count(w));
             if (k < kSegs) sh.seg[k] = Seg{before, top, own.parts(w), bin, base, own.count(w), nb, 0};
@@ -632,15 +708,14 @@ __device__ __forceinline__ void finish_row(const SampleArgs& a, Shared& sh, cons
             b0 = min(b0, sh.seg[k].bin);
             b1 = max(b1, sh.seg[k].bin);
         }
-        const double y0 = b0, y1 = b1 + 1;
         // no logit below this reaches those bins (the margin is far above the roundings of both sides)
-        const float least_v = bn.value_below(b1 + 1);
+        const float least_v = bn.value_below(b1);
         scan_row<DT>(row, 0, a.vocab, [&](int i, float v) {
-            if (v < least_v) return;
-            double y;
-            bn.place(v, y);
-            if (!(y >= y0 && y < y1)) return;
-            const int k = (int)sh.words[(int)y] - 1;
+            if (!(v >= least_v)) return;
+            int bin;
+            double part;
+            if (!bn.place(v, bin, part) || bin < b0 || bin > b1) return;
+            const int k = (int)sh.words[bin] - 1;
             if (k < 0) return;
             const int at = sh.seg[k].base + atomicAdd(&sh.seg[k].cursor, 1);
             sh.list[at] = (uint64_t)~order_key(v) << 32 | (uint32_t)i;
@@ -650,52 +725,45 @@ __device__ __forceinline__ void finish_row(const SampleArgs& a, Shared& sh, cons
         // ---- ranked inside their bins, with the parts before each
         uint64_t* ranked = sh.words;
         uint64_t* before = sh.words + kList;
-        auto parts_of = [&](uint64_t key, int bin) -> uint64_t {
-            double y;
-            bn.place(key_value(~(uint32_t)(key >> 32)), y);
-            return (uint64_t)a.q_scale - bn.q_of(y, bin);
+        auto parts_of = [&](uint64_t key) -> uint64_t {
+            int bin;
+            double part = 0.0;
+            bn.place(key_value(~(uint32_t)(key >> 32)), bin, part);
+            return (uint64_t)a.q_scale - bn.q_of(part);
         };
-        uint64_t keys[kList / kThreads], sums[kList / kThreads];
-        int ranks[kList / kThreads];
-#pragma unroll
-        for (int c = 0; c < kList / kThreads; ++c) {
-            const int i = tid + c * kThreads;
-            if (i >= listed) break;
-            const Seg& s = sh.seg[sh.list_seg[i]];
-            keys[c] = sh.list[i];
-            ranks[c] = 0;
-        }
-        // each token's own parts, so that the ranking loop only adds
-        uint64_t* parts = sh.words + 2 * kList;
-#pragma unroll
-        for (int c = 0; c < kList / kThreads; ++c) {
-            const int i = tid + c * kThreads;
-            if (i < listed) parts[i] = parts_of(keys[c], sh.seg[sh.list_seg[i]].bin);
+        uint64_t* parts = sh.words + 2 * kList;            // each token's own
+        uint64_t* sums = sh.words + 3 * kList;             // those of the tokens ahead of it in its bin
+        uint32_t* ranks = (uint32_t*)(sh.words + 4 * kList);  // their number
+        for (int i = tid; i < listed; i += kThreads) {
+            parts[i] = parts_of(sh.list[i]);
+            sums[i] = 0;
+            ranks[i] = 0;
         }
         __syncthreads();
-#pragma unroll
-        for (int c = 0; c < kList / kThreads; ++c) {
-            const int i = tid + c * kThreads;
-            if (i >= listed) break;
+        // the comparisons of a bin's tokens, shared out over the threads
+        const int shares = max(1, kThreads / max(listed, 1));
+        for (int x = tid; x < listed * shares; x += kThreads) {
+            const int i = x / shares, from = x - i * shares;
             const Seg& s = sh.seg[sh.list_seg[i]];
-            const int j0 = s.base, j1 = s.base + s.n;
+            const uint64_t key = sh.list[i];
             int rank = 0;
             uint64_t sum = 0;
-#pragma unroll 8
-            for (int j = j0; j < j1; ++j) {
-                const bool ahead = sh.list[j] < keys[c];
+#pragma unroll 4
+            for (int j = s.base + from; j < s.base + s.n; j += shares) {
+                const bool ahead = sh.list[j] < key;
                 rank += ahead;
                 sum += ahead ? parts[j] : 0;
             }
-            ranks[c] = s.base + rank;
-            sums[c] = sum;
+            if (rank) {
+                atomicAdd(&ranks[i], (uint32_t)rank);
+                atomicAdd((unsigned long long*)&sums[i], (unsigned long long)sum);
+            }
         }
-#pragma unroll
-        for (int c = 0; c < kList / kThreads; ++c) {
-            const int i = tid + c * kThreads;
-            if (i >= listed) break;
-            ranked[ranks[c]] = keys[c];
-            before[ranks[c]] = sums[c];
+        __syncthreads();
+        for (int i = tid; i < listed; i += kThreads) {
+            const int to = sh.seg[sh.list_seg[i]].base + (int)ranks[i];
+            ranked[to] = sh.list[i];
+            before[to] = sums[i];
         }
         __syncthreads();
         auto sum_to = [&](const Seg& s, int j) -> uint64_t { return j < s.n ? before[s.base + j] : s.total; };
@@ -770,7 +838,7 @@ __device__ __forceinline__ void finish_row(const SampleArgs& a, Shared& sh, cons
         __syncthreads();
         return;
     }
-    finish_full<DT>(a, sh, row, r, bn, u, by_k ? top_k : 0, by_p ? p_of : -1.0, by_m ? least : 0.0, mb, mass_all);
+    if (tid == 0) a.tokens[r] = -1;  // left to full_kernel
 }
 
 // The first largest logit.
@@ -804,11 +872,47 @@ __device__ float range_max(Shared& sh, const char* row, int e0, int e1) {
     return block_max(sh, m);
 }
 
-// One workgroup a row.
+// A row whose largest logit is infinite: its tokens of that logit (all, where it is -infinity)
+// are alike, the others nothing. Every boundary is a number of them.
 template <int DT>
+__device__ void alike_row(const SampleArgs& a, Shared& sh, const char* row, int r, float largest) {
+    const int per = (a.vocab + kThreads - 1) / kThreads;
+    const int i0 = min((int)threadIdx.x * per, a.vocab), i1 = min(i0 + per, a.vocab);
+    auto is = [&](int i) {
+        const float v = value_of<DT>(DT == MF_F32 ? ((const uint32_t*)row)[i] : (uint32_t)((const uint16_t*)row)[i]);
+        return largest < 0.f || v == largest;
+    };
+    int n = 0, all;
+    for (int i = i0; i < i1; ++i) n += is(i);
+    int before = n;
+    double none = 0.0, end, sum;
+    block_sums(sh, before, none, end, all, sum);
+    const int top_k = a.top_k ? a.top_k[r] : a.top_k0;
+    const double top_p = a.top_p ? a.top_p[r] : a.top_p0;
+    const double min_p = a.min_p ? a.min_p[r] : a.min_p0;
+    double u = a.uniforms[r];
+    u = u > 0.0 ? fmin(u, 1.0 - 0x1p-24) : 0.0;
+    int kept = top_k > 0 ? min(top_k, all) : all;
+    if (!(top_p >= 1.0)) kept = min(kept, (int)floor((top_p > 0.0 ? top_p : 0.0) * kept) + 1);
+    if (min_p > 1.0) kept = 1;
+    int at = min((int)floor(u * kept), kept - 1) - before;
+    if (at >= 0 && at < n) {
+        for (int i = i0; i < i1; ++i)
+            if (is(i) && at-- == 0) {
+                a.tokens[r] = i;
+                if (a.probs) a.probs[r] = (float)(1.0 / kept);
+            }
+    }
+}
+
+// One workgroup a row. FULL: the rows that the first launch left (token -1), whose boundary bins
+// hold too many tokens; in a kernel of their own, since their code's registers cost every other
+// row 12 us of 55 (256 rows of 130021).
+template <int DT, bool FULL>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     __shared__ Shared sh;
     const int r = blockIdx.x;
+    if (FULL && a.tokens[r] >= 0) return;
     const char* row = a.logits + (int64_t)r * a.stride_row * (DT == MF_F32 ? 4 : 2);
     const float temp = a.temp ? a.temp[r] : a.temp0;
     if (!(temp > 0.f)) {
@@ -817,17 +921,29 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     }
     clear_words(sh);
     float ref = range_max<DT>(sh, row, 0, min(a.vocab, kFirst));
-    Binner bn(a, ref, temp);
-    float largest = bin_range<DT>(a, sh, row, bn, 0, a.vocab);
-    double y;
-    if (!bn.place(largest, y)) {  // above the bins: again from the true maximum
-        bn = Binner(a, largest, temp);
+    if (isinf(ref)) ref = range_max<DT>(sh, row, 0, a.vocab);
+    float largest = ref;
+    while (!isinf(ref)) {
+        const Binner bn(a, ref, temp);
+        largest = bin_range<DT>(a, sh, row, bn, 0, a.vocab);
+        if (largest <= bn.hi) {
+            finish_row<DT, FULL>(a, sh, row, r, bn, largest);
+            return;
+        }
+        ref = largest;  // above the bins: again from the true maximum
         __syncthreads();
         clear_words(sh);
         __syncthreads();
-        bin_range<DT>(a, sh, row, bn, 0, a.vocab);
     }
-    finish_row<DT>(a, sh, row, r, bn, largest, temp);
+    alike_row<DT>(a, sh, row, r, largest);
+}
+
+template <int DT>
+int launch_sample(const SampleArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL((sample_kernel<DT, false>), dim3((unsigned)a.num_rows), dim3(kThreads), 0, st, a);
+    if (int e = check_launch()) return e;
+    hipLaunchKernelGGL((sample_kernel<DT, true>), dim3((unsigned)a.num_rows), dim3(kThreads), 0, st, a);
+    return check_launch();
 }
 
 }  // namespace
@@ -849,11 +965,7 @@ extern "C" int mf_sample(const void* logits, int dtype, int64_t stride_row, int 
                  tokens, probs};
     static_assert(sizeof(Shared) <= 160 * 1024, "LDS of one compute unit");
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == MF_F32)
-        hipLaunchKernelGGL(sample_kernel<MF_F32>, dim3((unsigned)num_rows), dim3(kThreads), 0, st, a);
-    else if (dtype == MF_F16)
-        hipLaunchKernelGGL(sample_kernel<MF_F16>, dim3((unsigned)num_rows), dim3(kThreads), 0, st, a);
-    else
-        hipLaunchKernelGGL(sample_kernel<MF_BF16>, dim3((unsigned)num_rows), dim3(kThreads), 0, st, a);
-    return check_launch();
+    if (dtype == MF_F32) return launch_sample<MF_F32>(a, st);
+    if (dtype == MF_F16) return launch_sample<MF_F16>(a, st);
+    return launch_sample<MF_BF16>(a, st);
 }
