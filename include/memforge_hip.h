@@ -655,14 +655,18 @@ int mf_tree_accept(const int64_t* tokens, const int64_t* targets, const int32_t*
  * Weights below e^-32 of the largest count as 0; sums are exact to 2^-30 of a
  * weight or better, so tokens are those of 64-bit arithmetic but where the draw
  * falls that close to a border.
+ * num_cus: the device's compute units; few rows are split over them, through a
+ * workspace of mf_sample_workspace_size bytes (8-byte aligned; 0: none) that is
+ * all 0 before the call and after it.
  * Beyond sampling.sample_logits (memforge_ml/runtime/sampling.py:33-75).
  */
 #define MF_SAMPLE_MAX_VOCAB (1 << 20)
+int64_t mf_sample_workspace_size(int num_rows, int vocab, int num_cus);
 int mf_sample(const void* logits, int dtype, int64_t stride_row, int num_rows, int vocab,
               const float* uniforms, const float* temperature, float temperature0,
               const int32_t* top_k, int top_k0, const float* top_p, float top_p0,
-              const float* min_p, float min_p0, int64_t* tokens, float* probs,
-              mf_stream_t stream);
+              const float* min_p, float min_p0, int64_t* tokens, float* probs, int num_cus,
+              void* workspace, int64_t workspace_bytes, mf_stream_t stream);
 
 /* ---------------------------------------------------- attention for drafted trees
  * Sequence s has context_lens[s] keys in the pool (through its row of the block

@@ -105,7 +105,8 @@ _SIGNATURES = {
     "mf_tables_truncate": (_c_int, [_vp, _c_i64, _c_int, _vp, _vp, _vp, _c_i64, _vp, _vp, _c_int, _c_int, _vp, _vp]),
     "mf_tree_accept": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_i64, _c_int, _vp, _vp, _vp, _vp]),
     "mf_sample": (_c_int, [_vp, _c_int, _c_i64, _c_int, _c_int, _vp, _vp, _c_f32, _vp, _c_int, _vp, _c_f32, _vp,
-                           _c_f32, _vp, _vp, _vp]),
+                           _c_f32, _vp, _vp, _c_int, _vp, _c_i64, _vp]),
+    "mf_sample_workspace_size": (_c_i64, [_c_int, _c_int, _c_int]),
     "mf_tree_plan_sizes": (_c_int, [_c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _vp]),
     "mf_tree_plan": (_c_int, [_vp, _vp, _vp, _c_int, _c_i64, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int,
                               _vp, _c_i64, _vp, _vp]),
@@ -863,7 +864,8 @@ class CountedPlan:
 class Workspace:
     """Grow-only scratch for split-K partials (fp32), merge arrival counters
     (int32, kept all-zero between calls by the kernels) and the rejection
-    verify, one per (device, stream) so concurrent streams never share it.
+    verify, one per (device, stream) so concurrent streams never share it; likewise the
+    bins of split sampling rows (int64, kept all-zero).
 
     A call recorded into a graph gets memory of its own, which the graph's private
     pool holds: a shared buffer would be freed under the graph when a later call
@@ -876,6 +878,7 @@ class Workspace:
         self._partials = {}
         self._counters = {}
         self._verify = {}
+        self._bins = {}
 
     def partials(self, floats: int, device) -> Optional[torch.Tensor]:
         if floats <= 0:
@@ -914,6 +917,18 @@ class Workspace:
         if buf is None or buf.numel() < n:
             buf = torch.zeros(max(n, 1 << 12), dtype=torch.int32, device=device)
             self._counters[key] = buf
+        return buf
+
+    def bins(self, n: int, device) -> Optional[torch.Tensor]:
+        """mf_sample's words for rows split over workgroups, all zero between calls like the counters."""
+        if n <= 0:
+            return None
+        if torch.cuda.is_current_stream_capturing():
+            return torch.zeros(n, dtype=torch.int64, device=device)
+        key = (device.index, _stream(device))
+        buf = self._bins.get(key)
+        if buf is None or buf.numel() < n:
+            buf = self._bins[key] = torch.zeros(n, dtype=torch.int64, device=device)
         return buf
 
 
@@ -1566,6 +1581,7 @@ def check_index(name: str, x: torch.Tensor, dtype: torch.dtype, device: torch.de
 # ---------------------------------------------------------------- sampling
 
 SAMPLE_MAX_VOCAB = 1 << 20
+_SAMPLE_WS_BYTES = {}  # (rows, vocab, compute units) -> mf_sample_workspace_size
 
 
 def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
@@ -1580,7 +1596,7 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=
     rows, vocab = logits.shape
     if not 1 <= vocab <= SAMPLE_MAX_VOCAB:
         raise ValueError(f"a vocabulary holds 1 to {SAMPLE_MAX_VOCAB} tokens, got {vocab}")
-    dev = logits.device
+    dev, code = logits.device, dtype_code(logits.dtype)
     check_index("uniforms", uniforms, torch.float32, dev, (rows,))
     settings = []
     for name, x, dt in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
@@ -1597,8 +1613,16 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=
             settings += [None, float(x)]
     tokens = torch.empty(rows, dtype=torch.int64, device=dev)
     probs = torch.empty(rows, dtype=torch.float32, device=dev)
-    _launch(dev, "mf_sample", lib().mf_sample, logits.data_ptr(), dtype_code(logits.dtype), logits.stride(0), rows,
-            vocab, uniforms.data_ptr(), *settings, tokens.data_ptr(), probs.data_ptr())
+    cus = device_cus(dev)
+    shape = (rows, vocab, cus)
+    nbytes = _SAMPLE_WS_BYTES.get(shape)
+    if nbytes is None:
+        if len(_SAMPLE_WS_BYTES) >= 4096:
+            _SAMPLE_WS_BYTES.clear()
+        nbytes = _SAMPLE_WS_BYTES[shape] = int(lib().mf_sample_workspace_size(*shape))
+    ws = _WORKSPACE.bins(nbytes // 8, dev)
+    _launch(dev, "mf_sample", lib().mf_sample, logits.data_ptr(), code, logits.stride(0), rows,
+            vocab, uniforms.data_ptr(), *settings, tokens.data_ptr(), probs.data_ptr(), cus, _ptr(ws), nbytes)
     return tokens, probs
 
 

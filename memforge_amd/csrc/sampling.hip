@@ -35,11 +35,12 @@ constexpr int kBins = kOwn * kThreads;
 constexpr double kPerE = 256.0;          // bins to a factor e of weight
 // The bin of the reference logit: 32 factors e below it have bins. Even and its thread's first,
 // so that equal logits at the reference weigh exactly 1 (Binner, Owner).
-constexpr int kTop = (kBins - 32 * 256 + 5) / kOwn * kOwn;
-static_assert(kTop % 2 == 0 && kTop % kOwn == 0 && kBins - kTop >= 8190, "the reference's bin");
+constexpr int kTop = (kBins - 32 * 256) / (2 * kOwn) * (2 * kOwn);
+static_assert(kTop % 2 == 0 && kTop % kOwn == 0 && kBins - kTop >= 8192, "the reference's bin");
 constexpr int kList = 2048;              // tokens of boundary bins that are ranked in LDS
 constexpr int kSegs = 128;               // boundary bins
 constexpr int kFirst = 8192;             // tokens of a row whose maximum is the reference
+constexpr int kRowWords = kBins + 2;     // a split row's bins, its largest (key, index), and its reference
 
 struct SampleArgs {
     const char* logits;
@@ -57,6 +58,8 @@ struct SampleArgs {
     double q_scale, q_unit;  // 2^qs, 2^-qs
     int64_t* tokens;
     float* probs;
+    uint64_t* bins;  // rows split over workgroups: kRowWords words a row, all 0 between calls
+    int chunk;       // tokens of one workgroup's part
 };
 
 struct Seg {
@@ -270,6 +273,7 @@ struct Owner {
     int count_before, count_end;      // of the bins before this thread's, and with them
     double mass_before, mass_end;
     double top0;                      // T_b of its first bin
+    double down;                      // exp(-lane / 256)
 
     // from the bins in sh.words, with the totals; empties the searches' places
     __device__ __forceinline__ void build(const SampleArgs& a, Shared& sh, int& n_all, double& mass_all) {
@@ -279,6 +283,7 @@ struct Owner {
         count_before = 0;
         mass_before = 0.0;
         top0 = bin_top(threadIdx.x * kOwn);
+        down = exp((double)(threadIdx.x & 63) * (-1.0 / kPerE));
         int n = 0;
         double mass = 0.0;
         walk(sh, [&](int, uint64_t w, double, int, double, double m) {
@@ -332,18 +337,36 @@ __device__ __forceinline__ double top_of(int bin) {  // T_b as its owner forms i
 // The first bin whose inclusive mass exceeds x (COUNT: whose inclusive count does), into
 // sh.at[k], which holds bin -1 before and where there is none. One thread's bins hold the
 // crossing, so nothing is compared between threads; the caller's next barrier publishes it.
+// The owner's wave works out its bins side by side.
 template <bool COUNT>
 __device__ __forceinline__ void find(Shared& sh, const Owner& o, double x, int k) {
-    if (COUNT ? !((double)o.count_before <= x && (double)o.count_end > x) : !(o.mass_before <= x && o.mass_end > x)) return;
-    Found f;
-    f.bin = -1;
-    bool done = false;
-    o.walk(sh, [&](int bin, uint64_t w, double, int n, double before, double mass) {
-        if (done) return;  // (the sums walked here round differently: the last bin stands in)
-        f = Found{bin, o.count(w), n, before, mass};
-        done = COUNT ? (double)(n + o.count(w)) > x : before + mass > x;
-    });
-    sh.at[k] = f;
+    const uint64_t owner = __builtin_amdgcn_ballot_w64(
+        COUNT ? (double)o.count_before <= x && (double)o.count_end > x : o.mass_before <= x && o.mass_end > x);
+    if (owner == 0) return;
+    const int src = __ffsll((unsigned long long)owner) - 1, lane = threadIdx.x & 63;
+    const double base = __shfl(o.mass_before, src, 64);
+    const int base_n = __shfl(o.count_before, src, 64);
+    const int bin = ((int)threadIdx.x - lane + src) * kOwn + lane;
+    const uint64_t w = lane < kOwn ? sh.words[bin] : 0;
+    const double top = __shfl(o.top0, src, 64) * o.down;
+    const double mass = w ? top * o.weight(w) : 0.0;
+    const int n = o.count(w);
+    double upto = mass;
+    int upto_n = n;
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+        const double m1 = __shfl_up(upto, d, 64);
+        const int n1 = __shfl_up(upto_n, d, 64);
+        if (lane >= d) {
+            upto += m1;
+            upto_n += n1;
+        }
+    }
+    const uint64_t held = __builtin_amdgcn_ballot_w64(w != 0);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(w != 0 && (COUNT ? (double)(base_n + upto_n) > x : base + upto > x));
+    // (these sums round differently from the owner's: without a crossing the last bin stands in)
+    const int at = past ? __ffsll((unsigned long long)past) - 1 : 63 - __clzll((long long)held);
+    if (lane == at) sh.at[k] = Found{bin, n, base_n + upto_n - n, base + upto - mass, mass};
 }
 
 // A prefix of the ranking: whole bins before `bin`, then the first n tokens of it.
@@ -841,11 +864,11 @@ __device__ __forceinline__ void finish_row(const SampleArgs& a, Shared& sh, cons
     if (tid == 0) a.tokens[r] = -1;  // left to full_kernel
 }
 
-// The first largest logit.
+// The first largest logit of the tokens [e0, e1): its order key, and its index inverted.
 template <int DT>
-__device__ void greedy_row(const SampleArgs& a, Shared& sh, const char* row, int r) {
+__device__ uint64_t range_best(Shared& sh, const char* row, int e0, int e1) {
     uint64_t best = 0;
-    scan_row<DT>(row, 0, a.vocab, [&](int i, float v) {
+    scan_row<DT>(row, e0, e1, [&](int i, float v) {
         const uint64_t k = (uint64_t)order_key(v) << 32 | (uint32_t)~i;
         best = k > best ? k : best;
     });
@@ -858,11 +881,7 @@ __device__ void greedy_row(const SampleArgs& a, Shared& sh, const char* row, int
     }
     if ((threadIdx.x & 63) == 0) atomicMax(&sh.best, (unsigned long long)best);
     __syncthreads();
-    if (threadIdx.x == 0) {
-        a.tokens[r] = (int64_t)(uint32_t)~(uint32_t)sh.best;
-        if (a.probs) a.probs[r] = 1.f;
-    }
-    __syncthreads();
+    return sh.best;
 }
 
 template <int DT>
@@ -905,64 +924,160 @@ __device__ void alike_row(const SampleArgs& a, Shared& sh, const char* row, int 
     }
 }
 
-// One workgroup a row. FULL: the rows that the first launch left (token -1), whose boundary bins
-// hold too many tokens; in a kernel of their own, since their code's registers cost every other
-// row 12 us of 55 (256 rows of 130021).
-template <int DT, bool FULL>
-__global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
+// The bins of a part of a row, added to the row's in memory (few rows: their parts spread over
+// the GPU).
+template <int DT>
+__global__ __launch_bounds__(kThreads) void bins_kernel(SampleArgs a) {
     __shared__ Shared sh;
-    const int r = blockIdx.x;
-    if (FULL && a.tokens[r] >= 0) return;
+    const int r = blockIdx.y, e0 = blockIdx.x * a.chunk, e1 = min(e0 + a.chunk, a.vocab);
     const char* row = a.logits + (int64_t)r * a.stride_row * (DT == MF_F32 ? 4 : 2);
+    uint64_t* out = a.bins + (int64_t)r * kRowWords;
     const float temp = a.temp ? a.temp[r] : a.temp0;
     if (!(temp > 0.f)) {
-        greedy_row<DT>(a, sh, row, r);
+        const uint64_t best = range_best<DT>(sh, row, e0, e1);
+        if (threadIdx.x == 0) atomicMax((unsigned long long*)&out[kBins], (unsigned long long)best);
         return;
     }
     clear_words(sh);
     float ref = range_max<DT>(sh, row, 0, min(a.vocab, kFirst));
     if (isinf(ref)) ref = range_max<DT>(sh, row, 0, a.vocab);
     float largest = ref;
-    while (!isinf(ref)) {
-        const Binner bn(a, ref, temp);
-        largest = bin_range<DT>(a, sh, row, bn, 0, a.vocab);
-        if (largest <= bn.hi) {
-            finish_row<DT, FULL>(a, sh, row, r, bn, largest);
+    if (!isinf(ref)) {
+        largest = bin_range<DT>(a, sh, row, Binner(a, ref, temp), e0, e1);
+        for (int i = threadIdx.x; i < kBins; i += kThreads) {
+            const uint64_t w = sh.words[i];
+            if (w) atomicAdd((unsigned long long*)&out[i], (unsigned long long)w);
+        }
+    }
+    if (threadIdx.x == 0) {
+        atomicMax((unsigned long long*)&out[kBins], (unsigned long long)order_key(largest) << 32);
+        if (blockIdx.x == 0) out[kBins + 1] = __float_as_uint(ref);
+    }
+}
+
+// One workgroup a row. WHOLE: the row from its logits on. PARTS: from the bins that bins_kernel
+// left, which it clears. FULL: the rows that the launch before left (token -1), because their
+// boundary bins hold too many tokens or, of a split row, its reference was too small; in a
+// kernel of their own, since their code's registers cost every other row 12 us of 55 (256 rows
+// of 130021).
+enum { WHOLE, PARTS, FULL };
+
+template <int DT, int MODE>
+__global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
+    __shared__ Shared sh;
+    const int r = blockIdx.x;
+    if (MODE == FULL && a.tokens[r] >= 0) return;
+    const char* row = a.logits + (int64_t)r * a.stride_row * (DT == MF_F32 ? 4 : 2);
+    const float temp = a.temp ? a.temp[r] : a.temp0;
+    if constexpr (MODE == PARTS) {
+        uint64_t* in = a.bins + (int64_t)r * kRowWords;
+        const uint64_t best = in[kBins];
+        const float ref = __uint_as_float((uint32_t)in[kBins + 1]);
+        const float largest = key_value((uint32_t)(best >> 32));
+        const bool greedy = !(temp > 0.f);
+        if (!greedy) {
+            for (int i = threadIdx.x; i < kBins; i += kThreads) {
+                const uint64_t w = in[i];
+                sh.words[i] = w;
+                if (w) in[i] = 0;
+            }
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) in[kBins] = 0;
+        if (greedy) {
+            if (threadIdx.x == 0) {
+                a.tokens[r] = (int64_t)(uint32_t)~(uint32_t)best;
+                if (a.probs) a.probs[r] = 1.f;
+            }
             return;
         }
-        ref = largest;  // above the bins: again from the true maximum
-        __syncthreads();
+        if (!isinf(ref)) {
+            const Binner bn(a, ref, temp);
+            if (largest <= bn.hi) finish_row<DT, false>(a, sh, row, r, bn, largest);
+            else if (threadIdx.x == 0) a.tokens[r] = -1;
+            return;
+        }
+        alike_row<DT>(a, sh, row, r, largest);
+    } else {
+        if (!(temp > 0.f)) {
+            const uint64_t best = range_best<DT>(sh, row, 0, a.vocab);
+            if (threadIdx.x == 0) {
+                a.tokens[r] = (int64_t)(uint32_t)~(uint32_t)best;
+                if (a.probs) a.probs[r] = 1.f;
+            }
+            return;
+        }
         clear_words(sh);
-        __syncthreads();
+        float ref = range_max<DT>(sh, row, 0, min(a.vocab, kFirst));
+        if (isinf(ref)) ref = range_max<DT>(sh, row, 0, a.vocab);
+        float largest = ref;
+        while (!isinf(ref)) {
+            const Binner bn(a, ref, temp);
+            largest = bin_range<DT>(a, sh, row, bn, 0, a.vocab);
+            if (largest <= bn.hi) {
+                finish_row<DT, MODE == FULL>(a, sh, row, r, bn, largest);
+                return;
+            }
+            ref = largest;  // above the bins: again from the true maximum
+            __syncthreads();
+            clear_words(sh);
+            __syncthreads();
+        }
+        alike_row<DT>(a, sh, row, r, largest);
     }
-    alike_row<DT>(a, sh, row, r, largest);
+}
+
+// Tokens of one workgroup's part, 0 where rows are not split: about num_cus / 4 parts, of at
+// least 4096 tokens. More of them cost more in the memory's additions, a few thousand a part,
+// than they win: us a call, unsplit, and 16, 32 and 64 parts: one row of 130021 fp32 logits 68, 50,
+// 50, 50, 16 rows 69, 69, 60, 57, 32 rows 71, 71, 70, 63 (64 rows in 512 parts: 331 against 50).
+int chunk_for(int num_rows, int vocab, int num_cus) {
+    const int parts = std::min(num_cus / 4 / num_rows, (vocab + 4095) / 4096);
+    return parts < 2 ? 0 : ((vocab + parts - 1) / parts + 7) / 8 * 8;
 }
 
 template <int DT>
 int launch_sample(const SampleArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((sample_kernel<DT, false>), dim3((unsigned)a.num_rows), dim3(kThreads), 0, st, a);
+    const dim3 rows((unsigned)a.num_rows), threads(kThreads);
+    if (a.chunk > 0) {
+        const dim3 parts((unsigned)((a.vocab + a.chunk - 1) / a.chunk), (unsigned)a.num_rows);
+        hipLaunchKernelGGL((bins_kernel<DT>), parts, threads, 0, st, a);
+        if (int e = check_launch()) return e;
+        hipLaunchKernelGGL((sample_kernel<DT, PARTS>), rows, threads, 0, st, a);
+    } else {
+        hipLaunchKernelGGL((sample_kernel<DT, WHOLE>), rows, threads, 0, st, a);
+    }
     if (int e = check_launch()) return e;
-    hipLaunchKernelGGL((sample_kernel<DT, true>), dim3((unsigned)a.num_rows), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((sample_kernel<DT, FULL>), rows, threads, 0, st, a);
     return check_launch();
 }
 
 }  // namespace
 }  // namespace mf
 
+extern "C" int64_t mf_sample_workspace_size(int num_rows, int vocab, int num_cus) {
+    using namespace mf;
+    if (num_rows < 1 || vocab < 1 || vocab > MF_SAMPLE_MAX_VOCAB || num_cus < 1) return 0;
+    return chunk_for(num_rows, vocab, num_cus) > 0 ? (int64_t)num_rows * kRowWords * 8 : 0;
+}
+
 extern "C" int mf_sample(const void* logits, int dtype, int64_t stride_row, int num_rows, int vocab,
                          const float* uniforms, const float* temperature, float temperature0, const int32_t* top_k,
                          int top_k0, const float* top_p, float top_p0, const float* min_p, float min_p0,
-                         int64_t* tokens, float* probs, mf_stream_t stream) {
+                         int64_t* tokens, float* probs, int num_cus, void* workspace, int64_t workspace_bytes,
+                         mf_stream_t stream) {
     using namespace mf;
-    if (!dtype_ok(dtype) || num_rows < 0 || vocab < 1 || vocab > MF_SAMPLE_MAX_VOCAB || stride_row < 0) return MF_ERR_ARG;
+    if (!dtype_ok(dtype) || num_cus < 1 || num_rows < 0 || vocab < 1 || vocab > MF_SAMPLE_MAX_VOCAB || stride_row < 0) return MF_ERR_ARG;
     if (num_rows == 0) return MF_OK;
-    if (!logits || !uniforms || !tokens) return MF_ERR_ARG;
+    if (!logits || !uniforms || !tokens || ((uintptr_t)workspace & 7)) return MF_ERR_ARG;
+    const int64_t need = mf_sample_workspace_size(num_rows, vocab, num_cus);
+    if (need > 0 && (!workspace || workspace_bytes < need)) return MF_ERR_WORKSPACE;
     int lv = 0;
     while ((1 << lv) < vocab) ++lv;
     const int qs = std::min(40, 71 - 2 * lv);
     SampleArgs a{(const char*)logits, stride_row, vocab, num_rows, uniforms, temperature, top_k, top_p, min_p,
                  temperature0, top_p0, min_p0, top_k0, 63 - lv, (double)(1ull << qs), 1.0 / (double)(1ull << qs),
-                 tokens, probs};
+                 tokens, probs, (uint64_t*)workspace, need > 0 ? chunk_for(num_rows, vocab, num_cus) : 0};
     static_assert(sizeof(Shared) <= 160 * 1024, "LDS of one compute unit");
     hipStream_t st = (hipStream_t)stream;
     if (dtype == MF_F32) return launch_sample<MF_F32>(a, st);

@@ -106,11 +106,16 @@ def test_accept_refuses(no_gpu_check, change):
 
 def test_sample_and_accept_entry_points_check_sizes():
     L, p = nat.lib(), 4096
-    sample = [p, 0, 10, 2, 10, p, None, 1.0, None, 0, None, 1.0, None, 0.0, p, p, None]
-    for at, bad in ((0, None), (1, 3), (2, -1), (3, -1), (4, 0), (4, nat.SAMPLE_MAX_VOCAB + 1), (5, None), (14, None)):
+    sample = [p, 0, 10, 2, 10, p, None, 1.0, None, 0, None, 1.0, None, 0.0, p, p, 256, None, 0, None]
+    for at, bad in ((0, None), (1, 3), (2, -1), (3, -1), (4, 0), (4, nat.SAMPLE_MAX_VOCAB + 1), (5, None), (14, None),
+                    (16, 0), (17, 4)):
         args = list(sample)
         args[at] = bad
         assert L.mf_sample(*args) == -1, (at, bad)
+    need = L.mf_sample_workspace_size(2, 100000, 256)
+    assert need > 0 and L.mf_sample_workspace_size(2, 10, 256) == 0 and L.mf_sample_workspace_size(5000, 100000, 256) == 0
+    big = [*sample[:2], 100000, 2, 100000, *sample[5:]]
+    assert L.mf_sample(*big) == -3 and L.mf_sample(*big[:17], p, need - 1, None) == -3
     accept = [p, p, p, p, 2, 6, 4, p, p, p, None]
     for at, bad in ((0, None), (3, None), (4, -1), (5, -1), (6, 0), (6, 1025), (7, None), (9, None)):
         args = list(accept)
