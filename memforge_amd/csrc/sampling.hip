@@ -694,10 +694,6 @@ __device__ __forceinline__ void finish_row(const SampleArgs& a, Shared& sh, cons
     const int d_lo = sh.at[AT_D_LO].bin >= 0 ? sh.at[AT_D_LO].bin : 0;
     const int d_hi = sh.at[AT_D_HI].bin >= 0 ? sh.at[AT_D_HI].bin : kBins - 1;
 
-    if constexpr (FULL) {
-        finish_full<DT>(a, sh, row, r, bn, u, by_k ? top_k : 0, by_p ? p_of : -1.0, least, mb, mass_all);
-        return;
-    }
     // ---- their tokens, bin by bin
     auto wanted = [&](int bin) {
         return bin == kb || (bin >= p_lo && bin <= p_hi) || bin == mb || (bin >= d_lo && bin <= d_hi) || bin == first_bin;
@@ -861,7 +857,9 @@ __device__ __forceinline__ void finish_row(const SampleArgs& a, Shared& sh, cons
         __syncthreads();
         return;
     }
-    if (tid == 0) a.tokens[r] = -1;  // left to full_kernel
+    if constexpr (FULL)
+        finish_full<DT>(a, sh, row, r, bn, u, by_k ? top_k : 0, by_p ? p_of : -1.0, least, mb, mass_all);
+    else if (tid == 0) a.tokens[r] = -1;  // left to the next launch
 }
 
 // The first largest logit of the tokens [e0, e1): its order key, and its index inverted.
@@ -957,9 +955,9 @@ __global__ __launch_bounds__(kThreads) void bins_kernel(SampleArgs a) {
 
 // One workgroup a row. WHOLE: the row from its logits on. PARTS: from the bins that bins_kernel
 // left, which it clears. FULL: the rows that the launch before left (token -1), because their
-// boundary bins hold too many tokens or, of a split row, its reference was too small; in a
-// kernel of their own, since their code's registers cost every other row 12 us of 55 (256 rows
-// of 130021).
+// boundary bins hold too many tokens or a logit lies above the bins; in a kernel of their own,
+// since their code's registers made every other row's loops spill (256 rows of 130021: 127 us in
+// one kernel).
 enum { WHOLE, PARTS, FULL };
 
 template <int DT, int MODE>
@@ -1011,17 +1009,20 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
         float ref = range_max<DT>(sh, row, 0, min(a.vocab, kFirst));
         if (isinf(ref)) ref = range_max<DT>(sh, row, 0, a.vocab);
         float largest = ref;
-        while (!isinf(ref)) {
-            const Binner bn(a, ref, temp);
-            largest = bin_range<DT>(a, sh, row, bn, 0, a.vocab);
-            if (largest <= bn.hi) {
+        if (!isinf(ref)) {
+            Binner bn(a, ref, temp);
+            for (;;) {
+                largest = bin_range<DT>(a, sh, row, bn, 0, a.vocab);
+                if (largest <= bn.hi || isinf(largest)) break;
+                bn = Binner(a, largest, temp);  // above the bins: again from the true maximum
+                __syncthreads();
+                clear_words(sh);
+                __syncthreads();
+            }
+            if (!isinf(largest)) {
                 finish_row<DT, MODE == FULL>(a, sh, row, r, bn, largest);
                 return;
             }
-            ref = largest;  // above the bins: again from the true maximum
-            __syncthreads();
-            clear_words(sh);
-            __syncthreads();
         }
         alike_row<DT>(a, sh, row, r, largest);
     }
