@@ -4,7 +4,8 @@ memforge_ml/runtime/__init__.py exports the same names)."""
 
 from memforge_amd.runtime.kv_pool import ModelKVSpec, PagedKVPool, PagedKVPool4
 from memforge_amd.runtime.paged_cache import PagedCache, PagedCacheLayer
-from memforge_amd.runtime.sampling import SamplingParams, sample_logits
+from memforge_amd.runtime.sampling import SamplingParams, sample_logits, sample_tokens
+from memforge_amd.runtime.device_tables import DeviceBlockTables, SlotMap
 from memforge_amd.runtime.continuous_engine import (
     HAS_CPP_ENGINE,
     ContinuousBatchingEngine,
@@ -21,6 +22,9 @@ __all__ = [
     "PagedCacheLayer",
     "SamplingParams",
     "sample_logits",
+    "sample_tokens",
+    "DeviceBlockTables",
+    "SlotMap",
     "ContinuousBatchingEngine",
     "SequenceRuntime",
     "StepReport",
