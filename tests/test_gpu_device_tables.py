@@ -129,6 +129,26 @@ def test_rows_given_by_number(device, requests):
         host.check(state)
 
 
+def test_no_requests_and_no_rows(device):
+    state = DeviceBlockTables.allocate(0, 4, 9, 16, device)
+    got = state.extend(ints(device, []), 3)
+    assert got.slot_mapping.tolist() == [-1] * 3 and got.cu_seqlens.tolist() == [0] and got.refused.tolist() == [0]
+    state.truncate(ints(device, []))
+    state = DeviceBlockTables.allocate(2, 0, 0, 16, device)
+    got = state.extend(ints(device, [0, 3]), 0)
+    assert got.kv_lens.tolist() == [0, 0] and got.refused.tolist() == [1]
+
+
+def test_lengths_at_the_end_of_31_bits(device):
+    """A length that 32 bits do not hold is refused; the one just below is not."""
+    most = 2**31 - 1
+    state = DeviceBlockTables(torch.zeros((2, 40), dtype=torch.int32, device=device), ints(device, [most - 3, most - 3]),
+                              ints(device, [32, 32]), ints(device, [0]), ints(device, [0]), 1 << 26)
+    got = state.extend(ints(device, [3, 4]), 10)
+    assert got.kv_lens.tolist() == [most, most - 3] and got.refused.tolist() == [1]
+    assert got.positions[:3].tolist() == [most - 3, most - 2, most - 1]
+
+
 def test_largest_lengths(device):
     """Token counts whose sum passes 32 bits are refused, the requests before them served."""
     state = DeviceBlockTables.allocate(4, 6, 12, 16, device)

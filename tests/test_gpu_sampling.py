@@ -150,6 +150,41 @@ def test_same_result_every_time(device):
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
 
 
+@pytest.mark.parametrize("kind", ["normal", "equal"])
+def test_largest_vocabulary(device, kind):
+    vocab = 1 << 20
+    logits, u = rows_of(device, 3, vocab, torch.bfloat16, seed=2, pad=1)
+    if kind == "equal":
+        logits[:] = 1.0
+    check(logits, u)
+    check(logits, u, top_k=vocab - 5, top_p=0.999, min_p=1e-6)
+
+
+def test_expanded_and_distant_rows(device):
+    """One row for many draws, and rows further apart than 32 bits hold."""
+    logits, u = rows_of(device, 40, 3001, torch.float32, seed=4)
+    check(logits[:1].expand(40, -1), u, top_p=0.9)
+    far = torch.zeros((3, 1 << 30), dtype=torch.bfloat16, device=device)
+    far[:, 7:3008] = logits[:3].to(torch.bfloat16)
+    check(far[:, 7:3008], u[:3], top_k=500)
+
+
+def test_two_streams_at_once(device):
+    """Split rows on two streams keep memory of their own."""
+    sets = [rows_of(device, 3, 60000, torch.float32, seed=s) for s in (1, 2)]
+    want = [sample_tokens(*s, top_p=0.97) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for s, stream, out in zip(sets, streams, got):
+            with torch.cuda.stream(stream):
+                out.append(sample_tokens(*s, top_p=0.97))
+    torch.cuda.synchronize()
+    for outs, w in zip(got, want):
+        assert all(torch.equal(o[0], w[0]) and torch.equal(o[1], w[1]) for o in outs)
+
+
 def test_no_rows(device):
     tokens, probs = sample_tokens(torch.empty((0, 10), device=device), torch.empty(0, device=device))
     assert tokens.shape == probs.shape == (0,)
