@@ -40,7 +40,7 @@ constexpr int kTile = 32;            // keys
 constexpr int kMaxSeqs = 4096;
 constexpr int kWindow = 1024;        // block-table entries held in LDS
 constexpr int kSeqInts = 8;          // context, nodes, first row, tiles, column groups, context tiles, -, -
-constexpr int kWorkInts = 16;        // sequence, unit, tile at which a worker starts, its tiles, and the sequence's first six
+constexpr int kWorkInts = 16;        // a worker's first sequence, kv head, first tile, tiles, the sequence's six, column group
 
 struct TreePlanArgs {
     const int32_t* parents;
@@ -53,7 +53,8 @@ struct TreePlanArgs {
     int group;        // query heads of a kv head
     int num_kv_heads;
     int group_cols;   // columns of one column group
-    int num_workers, min_share;
+    int lanes;        // (kv head, column group)s: workers of one share
+    int num_shares, min_share;
     int64_t* head;      // share, all tiles
     int32_t* seqs;
     int64_t* seq_first; // first tile of each sequence in the line
@@ -123,7 +124,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_plan_kernel(TreePlanArgs a)
         q[4] = groups;
         q[5] = held;
         first[s] = mine;
-        mine += (int64_t)tiles * groups * a.num_kv_heads;
+        mine += tiles;
     }
     int64_t incl = mine;
 #pragma unroll
@@ -143,32 +144,29 @@ __global__ __launch_bounds__(kTreeThreads) void tree_plan_kernel(TreePlanArgs a)
         a.seq_first[s] = first[s];
     }
     if (tid == 0) first[a.num_seqs] = total;
-    // (a worker's tiles fit 32 bits: fewer than 2^26 in a sequence of one kv head, spread over all of them)
-    const int64_t share = min(max((total + a.num_workers - 1) / a.num_workers, (int64_t)a.min_share), (int64_t)INT_MAX);
+    const int64_t share = min(max((total + a.num_shares - 1) / a.num_shares, (int64_t)a.min_share), (int64_t)INT_MAX);
     if (tid == 0) {
         a.head[0] = share;
         a.head[1] = total;
     }
     __syncthreads();
-    for (int w = tid; w < a.num_workers; w += kTreeThreads) {
-        const int64_t at = (int64_t)w * share;
-        if (at >= total) {
-            a.work[(int64_t)w * kWorkInts + 3] = 0;
-            continue;
-        }
+    const int column_groups = a.lanes / a.num_kv_heads;
+    for (int i = tid; i < a.num_shares; i += kTreeThreads) {
+        const int64_t at = (int64_t)i * share;
         int lo = 0, hi = a.num_seqs - 1;  // the last sequence that starts at or before `at`: it has tiles
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
             if (first[mid] <= at) lo = mid;
             else hi = mid - 1;
         }
-        const int tiles = a.seqs[(int64_t)lo * kSeqInts + 3];
-        const int64_t in = at - first[lo];
         const int32_t* q = a.seqs + (int64_t)lo * kSeqInts;
-        int4* to = (int4*)(a.work + (int64_t)w * kWorkInts);
-        to[0] = make_int4(lo, (int)(in / tiles), (int)(in % tiles), (int)min(share, total - at));
-        to[1] = make_int4(q[0], q[1], q[2], tiles);
-        to[2] = make_int4(q[4], q[5], 0, 0);
+        const int left = (int)max(min(share, total - at), (int64_t)0);
+        for (int u = 0; u < a.lanes; ++u) {
+            int4* to = (int4*)(a.work + ((int64_t)i * a.lanes + u) * kWorkInts);
+            to[0] = make_int4(lo, u / column_groups, (int)(at - first[lo]), left);
+            to[1] = make_int4(q[0], q[1], q[2], q[3]);
+            to[2] = make_int4(q[4], q[5], u % column_groups, 0);
+        }
     }
 }
 
@@ -273,7 +271,8 @@ __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * W
     static_assert(WK == 1 || (WK - 1) * WC * (ND * 16 + 2) * 256 <= S::RING * S::STG, "the key waves' sums fit the ring");
 
     const int32_t* at = a.work + (int64_t)blockIdx.x * kWorkInts;
-    int s = at[0], unit = at[1], tile0 = at[2], left = at[3];
+    const int h = at[1], grp = at[10];
+    int s = at[0], tile0 = at[2], left = at[3];
     int ctx = at[4], n = at[5], row0 = at[6], tiles = at[7], groups = at[8], held = at[9];
     if (left <= 0) return;
     const int tid = threadIdx.x, lane = tid & 63, hf = lane >> 5, j = lane & 15;
@@ -314,6 +313,8 @@ __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * W
 
     bool first = true;
     for (;;) {
+        const int run = min(left, tiles - tile0);
+        if (grp < groups) {
         // ---- one sequence: its block-table entries, or a window of them, in LDS
         const int32_t* trow = a.tables + (int64_t)s * a.table_stride;
         int window = 0, window_lo = 0, window_hi = 0;  // first block, and the keys it covers
@@ -328,16 +329,11 @@ __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * W
         fill_window(tile0 * kTile);
         sync();
 
-        // ---- stages in the order of the line: across the sequence's units where every
-        // wave has columns of its own (WK 1); the key waves' sums need the ring at a unit's end
-        const int units = groups * a.num_kv_heads;
-        int f_unit = unit, f_tile = tile0;
-        int f_left = WK == 1 ? (int)min((int64_t)left, (int64_t)(units - unit) * tiles - tile0) : min(left, tiles - tile0);
-        const int run = f_left;
+        int f_tile = tile0, f_left = run;
         int in_flight = 0, head_buf = 0, next_buf = 0;
         auto fetch = [&]() __attribute__((always_inline)) {
-            const int take = min(min(ST, f_left), tiles - f_tile);
-            const int h = f_unit / groups, st0 = f_tile, t_end = st0 + take;
+            const int take = min(ST, f_left);
+            const int st0 = f_tile, t_end = st0 + take;
             const uint32_t dst0 = ring_at + (uint32_t)(next_buf * S::STG);
             const int first_key = st0 * kTile, end_key = min(t_end * kTile, ctx);
             if (first_key < end_key && (first_key < window_lo || end_key > window_hi)) {
@@ -386,21 +382,15 @@ __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * W
             }
             f_left -= take;
             f_tile += take;
-            if (f_tile == tiles) {
-                f_tile = 0;
-                ++f_unit;
-            }
             ++in_flight;
             next_buf = next_buf + 1 == S::RING ? 0 : next_buf + 1;
         };
 #pragma unroll 1
         for (int u = 0; u < AHEAD && f_left > 0; ++u) fetch();
 
-        int done = 0;
-        while (done < run) {
-            // ---- one (kv head, column group): this lane's column and query
-            const int h = unit / groups, grp = unit - h * groups;
-            const int t0 = tile0, t1 = min(tiles, t0 + run - done);
+        {
+            // ---- this lane's column and query
+            const int t0 = tile0, t1 = t0 + run;
             const int cidx = grp * S::COLS + wc * 32 + (lane & 31);
             const bool valid = cidx < n * a.group;
             const int node = (int)((unsigned)(valid ? cidx : 0) / (unsigned)a.group);
@@ -570,27 +560,23 @@ __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * W
                     }
                 }
             }
-            first = false;
-            done += t1 - t0;
-            tile0 = t1 == tiles ? 0 : t1;
-            unit += t1 == tiles;
+        }
+        sync();  // the ring and the window have been read
         }
         left -= run;
         if (left <= 0) return;
-        sync();  // the ring and the window have been read
-        if (unit == units) {
-            unit = 0;
-            do {
-                ++s;
-                const int32_t* info = a.seqs + (int64_t)s * kSeqInts;
-                ctx = info[0];
-                n = info[1];
-                row0 = info[2];
-                tiles = info[3];
-                groups = info[4];
-                held = info[5];
-            } while (tiles == 0);  // the line has `left` more tiles, so a sequence with tiles comes
-        }
+        first = false;
+        tile0 = 0;
+        do {
+            ++s;
+            const int32_t* info = a.seqs + (int64_t)s * kSeqInts;
+            ctx = info[0];
+            n = info[1];
+            row0 = info[2];
+            tiles = info[3];
+            groups = info[4];
+            held = info[5];
+        } while (tiles == 0);  // the line has `left` more tiles, so a sequence with tiles comes
     }
 }
 
@@ -608,9 +594,9 @@ __global__ __launch_bounds__(kTreeThreads) void merge_tree_kernel(TreeArgs a, in
     const int blk = SPLIT ? blockIdx.y / S::ND : blockIdx.y;
     const int32_t* info = a.seqs + (int64_t)s * kSeqInts;
     const int n = info[1], row0 = info[2], tiles = info[3], groups = info[4];
-    const int64_t begin = a.seq_first[s] + (int64_t)unit * tiles;
-    if (tiles == 0 || unit >= groups * a.num_kv_heads) return;
-    const int h = unit / groups, grp = unit - h * groups;
+    const int64_t begin = a.seq_first[s];
+    const int column_groups = units_per_seq / a.num_kv_heads, h = unit / column_groups, grp = unit - h * column_groups;
+    if (tiles == 0 || grp >= groups) return;
     if (grp * S::COLS + blk * 32 >= n * a.group) return;
     const int64_t w0 = begin / share, w1 = (begin + tiles - 1) / share;
     if (w0 == w1) return;
@@ -623,7 +609,7 @@ __global__ __launch_bounds__(kTreeThreads) void merge_tree_kernel(TreeArgs a, in
         for (int i = 0; i < 16; ++i) acc[0][i] = 0.f;
 #pragma unroll 2
         for (int64_t w = w0 + (SPLIT ? wave : 0); w <= w1; w += SPLIT ? 4 : 1) {
-            const float* from = a.partials + (2 * w + (w * share < begin ? 1 : 0)) * S::SLOT + blk * 32 * (D + 2);
+            const float* from = a.partials + (2 * (w * units_per_seq + unit) + (w * share < begin ? 1 : 0)) * S::SLOT + blk * 32 * (D + 2);
             const float m1 = from[32 * D + (lane & 31)], l1 = from[32 * D + 32 + (lane & 31)];
             float4 v[4];
 #pragma unroll
@@ -721,11 +707,15 @@ bool tree_dim_ok(int head_dim) { return head_dim == 32 || head_dim == 64 || head
 // Where a plan's parts lie in its buffer, in 32-bit words.
 struct TreeLayout {
     int64_t head, seq_first, work, seqs, masks, total;
-    int workers, mask_words;
+    int shares, lanes, workers, mask_words;
 };
-TreeLayout tree_layout(int num_seqs, int64_t num_rows, int max_nodes, const TreeConfig& c, int num_cus) {
+TreeLayout tree_layout(int num_seqs, int64_t num_rows, int max_nodes, int group, int num_kv_heads, const TreeConfig& c,
+                       int num_cus) {
     TreeLayout l;
-    l.workers = num_cus * c.per_cu;
+    const int64_t lanes = num_kv_heads * (((int64_t)max_nodes * group + c.wc * 32 - 1) / (c.wc * 32));
+    l.lanes = (int)lanes;
+    l.shares = (int)std::max<int64_t>(num_cus * c.per_cu / lanes, 1);
+    l.workers = l.shares * l.lanes;
     l.mask_words = (max_nodes + 31) / 32;
     l.head = 0;
     l.seq_first = 4;
@@ -747,7 +737,7 @@ extern "C" int mf_tree_plan_sizes(int num_seqs, int64_t num_rows, int max_nodes,
         return MF_ERR_ARG;
     if (!tree_dim_ok(head_dim)) return MF_ERR_UNSUPPORTED;
     const TreeConfig c = tree_config(dtype, head_dim, max_nodes, num_q_heads / num_kv_heads);
-    const TreeLayout l = tree_layout(num_seqs, num_rows, max_nodes, c, num_cus);
+    const TreeLayout l = tree_layout(num_seqs, num_rows, max_nodes, num_q_heads / num_kv_heads, num_kv_heads, c, num_cus);
     *plan_words = l.total;
     *partials_floats = 2 * (int64_t)l.workers * (c.wc * 32) * (head_dim + 2);
     return MF_OK;
@@ -769,9 +759,9 @@ extern "C" int mf_tree_plan(const int32_t* parents, const int32_t* cu_nodes, con
     if (plan_words < words) return MF_ERR_WORKSPACE;
     const int group = num_q_heads / num_kv_heads;
     const TreeConfig c = tree_config(dtype, head_dim, max_nodes, group);
-    const TreeLayout l = tree_layout(num_seqs, num_rows, max_nodes, c, num_cus);
+    const TreeLayout l = tree_layout(num_seqs, num_rows, max_nodes, num_q_heads / num_kv_heads, num_kv_heads, c, num_cus);
     TreePlanArgs a{parents, cu_nodes, context_lens, num_seqs, num_rows, max_nodes, l.mask_words, max_context, group,
-                   num_kv_heads, c.wc * 32, l.workers, c.min_share, (int64_t*)(plan + l.head), plan + l.seqs,
+                   num_kv_heads, c.wc * 32, l.lanes, l.shares, c.min_share, (int64_t*)(plan + l.head), plan + l.seqs,
                    (int64_t*)(plan + l.seq_first), plan + l.work, (uint32_t*)(plan + l.masks), positions};
     hipLaunchKernelGGL(tree_plan_kernel, dim3((unsigned)num_seqs + 1), dim3(kTreeThreads), 0, (hipStream_t)stream, a);
     return check_launch();
@@ -806,7 +796,7 @@ extern "C" int mf_tree_attention(const void* q, int64_t q_stride_row, int64_t q_
         return MF_ERR_ARG;
     const int group = num_q_heads / num_kv_heads;
     const TreeConfig c = tree_config(dtype, head_dim, max_nodes, group);
-    const TreeLayout l = tree_layout(num_seqs, num_rows, max_nodes, c, num_cus);
+    const TreeLayout l = tree_layout(num_seqs, num_rows, max_nodes, num_q_heads / num_kv_heads, num_kv_heads, c, num_cus);
     TreeArgs a{};
     a.head = (const int64_t*)(plan + l.head);
     a.work = plan + l.work;
@@ -844,12 +834,10 @@ extern "C" int mf_tree_attention(const void* q, int64_t q_stride_row, int64_t q_
     a.scale_log2 = scale == 0.f ? 0x1p-100f : std::fabs(scale) * 1.4426950408889634f;
     a.inv_scale_log2 = 1.f / a.scale_log2;
     a.partials = partials;
-    const int64_t cols = (int64_t)max_nodes * group;
-    const int units = num_kv_heads * (int)((cols + c.wc * 32 - 1) / (c.wc * 32));
-    if ((int64_t)num_seqs * units > INT_MAX) return MF_ERR_ARG;
+    if ((int64_t)num_seqs * l.lanes > INT_MAX) return MF_ERR_ARG;
     hipStream_t st = (hipStream_t)stream;
 #define MF_TREE_CASE(DT, DV) \
-    if (dtype == DT && head_dim == DV) return launch_tree<DT, DV>(a, c, l.workers, units, st);
+    if (dtype == DT && head_dim == DV) return launch_tree<DT, DV>(a, c, l.workers, l.lanes, st);
     MF_TREE_CASE(MF_BF16, 32)
     MF_TREE_CASE(MF_BF16, 64)
     MF_TREE_CASE(MF_BF16, 128)
