@@ -6,13 +6,23 @@
 // with grouped heads. A (node, head) pair is a column; the G heads of a kv head
 // share its K/V rows, so a kv head's n G columns are one matrix product with them.
 //
-// Work. A kv head's keys are tiles of 32: the context's, then the nodes'. The tiles
-// of every (sequence, kv head, column group) stand in one line, which the launch's
-// workgroups cut into equal shares: a workgroup runs the pieces of up to several
-// (sequence, kv head)s that its share covers, writes the whole ones out and leaves
-// the others' unnormalised sums for merge_tree_kernel. So one long context and a
-// batch of uneven ones both fill the GPU, from lengths that only the device knows:
-// the plan (tree_plan_kernel, once for all layers of a step) is made there.
+// Work. A sequence's keys are tiles of 32: the context's, then the nodes'. All
+// sequences' tiles stand in one line, which is cut into equal shares; each share has
+// a workgroup for every lane, a (kv head, group of columns). It runs the pieces of
+// the sequences that the share covers, writes the whole ones out and leaves the
+// others' unnormalised sums for merge_tree_kernel. So one long context and a batch
+// of uneven ones both fill the GPU, from lengths that only the device knows: the
+// plan (tree_plan_kernel, once for all layers of a step) is made there. The lanes of
+// a share stand side by side, so that the kv heads of a slot, which lie together in
+// memory, are read at the same time (a share of one head's tiles of its own: 377 us
+// for 358 in the first case below, 145 for 133 in the second).
+//
+// Bound. Two layers with their plan, by graph replay on an MI355X: 64 contexts (median
+// 2,048, 16 nodes each, bf16, 40/8 heads of 128) 358 us, 327 with loads and merges
+// alone; their keys and values at the 4.9 TB/s of a large copy take 304. One context
+// of 32,001 under 48 nodes (fp16, the same heads) 133 us, 93 without the products and
+// 123 without the loads, floor 54: 240 columns a kv head, whose chain of product,
+// softmax, product the two waves of a SIMD do not hide from each other.
 //
 // Tiles. Four or eight waves, WC side by side on blocks of 32 columns and WK along
 // the keys: a stage of WK or more tiles goes from global memory straight into LDS once
@@ -315,253 +325,258 @@ __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * W
     for (;;) {
         const int run = min(left, tiles - tile0);
         if (grp < groups) {
-        // ---- one sequence: its block-table entries, or a window of them, in LDS
-        const int32_t* trow = a.tables + (int64_t)s * a.table_stride;
-        int window = 0, window_lo = 0, window_hi = 0;  // first block, and the keys it covers
-        auto fill_window = [&](int from_key) {
-            const int blocks = ctx > 0 ? block_of(ctx - 1) + 1 : 0;
-            window = blocks <= kWindow ? 0 : block_of(from_key);
-            window_lo = window * a.block_size;
-            window_hi = blocks - window <= kWindow ? ctx : (window + kWindow) * a.block_size;
-            const int end = min(window + kWindow, blocks);
-            for (int i = window + tid; i < end; i += S::WAVES * 64) tab[i - window] = trow[i];
-        };
-        fill_window(tile0 * kTile);
-        sync();
+            // ---- one sequence: its block-table entries, or a window of them, in LDS
+            const int32_t* trow = a.tables + (int64_t)s * a.table_stride;
+            int window = 0, window_lo = 0, window_hi = 0;  // first block, and the keys it covers
+            auto fill_window = [&](int from_key) {
+                const int blocks = ctx > 0 ? block_of(ctx - 1) + 1 : 0;
+                window = blocks <= kWindow ? 0 : block_of(from_key);
+                window_lo = window * a.block_size;
+                window_hi = blocks - window <= kWindow ? ctx : (window + kWindow) * a.block_size;
+                const int end = min(window + kWindow, blocks);
+                for (int i = window + tid; i < end; i += S::WAVES * 64) tab[i - window] = trow[i];
+            };
+            fill_window(tile0 * kTile);
+            sync();
 
-        int f_tile = tile0, f_left = run;
-        int in_flight = 0, head_buf = 0, next_buf = 0;
-        auto fetch = [&]() __attribute__((always_inline)) {
-            const int take = min(ST, f_left);
-            const int st0 = f_tile, t_end = st0 + take;
-            const uint32_t dst0 = ring_at + (uint32_t)(next_buf * S::STG);
-            const int first_key = st0 * kTile, end_key = min(t_end * kTile, ctx);
-            if (first_key < end_key && (first_key < window_lo || end_key > window_hi)) {
-                sync();
-                fill_window(first_key);
-                sync();
-            }
-            if (st0 + ST <= min(held, t_end) && a.block_shift >= 0) {
-                // all keys in the pool; rows past the context's end read its last one: masked, and every
-                // column sees that row
-                const char* kh = a.k_pool + (int64_t)h * a.p_sh * ES;
-                uint32_t e[S::PAIRS];
-                int key[S::PAIRS];
-#pragma unroll
-                for (int i = 0; i < S::PAIRS; ++i) {
-                    key[i] = min(first_key + row_of(i), ctx - 1);
-                    e[i] = (uint32_t)tab[(key[i] >> a.block_shift) - window];
+            int f_tile = tile0, f_left = run;
+            int in_flight = 0, head_buf = 0, next_buf = 0;
+            auto fetch = [&]() __attribute__((always_inline)) {
+                const int take = min(ST, f_left);
+                const int st0 = f_tile, t_end = st0 + take;
+                const uint32_t dst0 = ring_at + (uint32_t)(next_buf * S::STG);
+                const int first_key = st0 * kTile, end_key = min(t_end * kTile, ctx);
+                if (first_key < end_key && (first_key < window_lo || end_key > window_hi)) {
+                    sync();
+                    fill_window(first_key);
+                    sync();
                 }
+                if (st0 + ST <= min(held, t_end) && a.block_shift >= 0) {
+                    // all keys in the pool; rows past the context's end read its last one: masked, and every
+                    // column sees that row
+                    const char* kh = a.k_pool + (int64_t)h * a.p_sh * ES;
+                    uint32_t e[S::PAIRS];
+                    int key[S::PAIRS];
 #pragma unroll
-                for (int i = 0; i < S::PAIRS; ++i) {
-                    const char* src = kh + ((int64_t)min(e[i], a.num_blocks - 1) * a.p_sb +
-                                            (int64_t)(key[i] & (a.block_size - 1)) * a.p_ss) * ES;
-                    ld_lds16_nt(src + k_piece(i), dst0 + (uint32_t)((wave + S::WAVES * i) * 1024));
-                    ld_lds16_nt(src + v_delta + v_piece(i), dst0 + (uint32_t)(S::HALF + (wave + S::WAVES * i) * 1024));
-                }
-            } else {
-#pragma unroll 1
-                for (int i = 0; i < S::PAIRS; ++i) {
-                    const int r = row_of(i), in = r & 31;
-                    const int t = min(st0 + (r >> 5), t_end - 1);
-                    const char* src;
-                    int64_t to_v;
-                    if (t < held) {
-                        const int key = min(t * kTile + in, ctx - 1), blk = block_of(key);
-                        const uint32_t e = min((uint32_t)tab[blk - window], a.num_blocks - 1);
-                        src = a.k_pool + ((int64_t)e * a.p_sb + (int64_t)(key - blk * a.block_size) * a.p_ss + (int64_t)h * a.p_sh) * ES;
-                        to_v = v_delta;
-                    } else {
-                        const int node = min((t - held) * kTile + in, n - 1);
-                        src = a.new_k + ((int64_t)(row0 + node) * a.n_sr + (int64_t)h * a.n_sh) * ES;
-                        to_v = nv_delta;
+                    for (int i = 0; i < S::PAIRS; ++i) {
+                        key[i] = min(first_key + row_of(i), ctx - 1);
+                        e[i] = (uint32_t)tab[(key[i] >> a.block_shift) - window];
                     }
-                    ld_lds16_nt(src + k_piece(i), dst0 + (uint32_t)((wave + S::WAVES * i) * 1024));
-                    ld_lds16_nt(src + to_v + v_piece(i), dst0 + (uint32_t)(S::HALF + (wave + S::WAVES * i) * 1024));
-                }
-            }
-            f_left -= take;
-            f_tile += take;
-            ++in_flight;
-            next_buf = next_buf + 1 == S::RING ? 0 : next_buf + 1;
-        };
+#pragma unroll
+                    for (int i = 0; i < S::PAIRS; ++i) {
+                        const char* src = kh + ((int64_t)min(e[i], a.num_blocks - 1) * a.p_sb +
+                                                (int64_t)(key[i] & (a.block_size - 1)) * a.p_ss) * ES;
+                        ld_lds16_nt(src + k_piece(i), dst0 + (uint32_t)((wave + S::WAVES * i) * 1024));
+                        ld_lds16_nt(src + v_delta + v_piece(i), dst0 + (uint32_t)(S::HALF + (wave + S::WAVES * i) * 1024));
+                    }
+                } else {
 #pragma unroll 1
-        for (int u = 0; u < AHEAD && f_left > 0; ++u) fetch();
+                    for (int i = 0; i < S::PAIRS; ++i) {
+                        const int r = row_of(i), in = r & 31;
+                        const int t = min(st0 + (r >> 5), t_end - 1);
+                        const char* src;
+                        int64_t to_v;
+                        if (t < held) {
+                            const int key = min(t * kTile + in, ctx - 1), blk = block_of(key);
+                            const uint32_t e = min((uint32_t)tab[blk - window], a.num_blocks - 1);
+                            src = a.k_pool + ((int64_t)e * a.p_sb + (int64_t)(key - blk * a.block_size) * a.p_ss +
+                                              (int64_t)h * a.p_sh) * ES;
+                            to_v = v_delta;
+                        } else {
+                            const int node = min((t - held) * kTile + in, n - 1);
+                            src = a.new_k + ((int64_t)(row0 + node) * a.n_sr + (int64_t)h * a.n_sh) * ES;
+                            to_v = nv_delta;
+                        }
+                        ld_lds16_nt(src + k_piece(i), dst0 + (uint32_t)((wave + S::WAVES * i) * 1024));
+                        ld_lds16_nt(src + to_v + v_piece(i), dst0 + (uint32_t)(S::HALF + (wave + S::WAVES * i) * 1024));
+                    }
+                }
+                f_left -= take;
+                f_tile += take;
+                ++in_flight;
+                next_buf = next_buf + 1 == S::RING ? 0 : next_buf + 1;
+            };
+#pragma unroll 1
+            for (int u = 0; u < AHEAD && f_left > 0; ++u) fetch();
 
-        {
-            // ---- this lane's column and query
-            const int t0 = tile0, t1 = t0 + run;
-            const int cidx = grp * S::COLS + wc * 32 + (lane & 31);
-            const bool valid = cidx < n * a.group;
-            const int node = (int)((unsigned)(valid ? cidx : 0) / (unsigned)a.group);
-            const int64_t prow = row0 + node;
-            const int qhead = h * a.group + (valid ? cidx : 0) - node * a.group;
-            const bool busy = grp * S::COLS + wc * 32 < n * a.group;  // a wave of padding columns only loads
-            uint4 qf[NQ];
-            const char* qp = a.q + (prow * a.q_sr + (int64_t)qhead * a.q_sh) * ES;
-#pragma unroll
-            for (int c = 0; c < NQ; ++c) {
-                const uint4 v = *(const uint4*)(qp + (2 * c + hf) * 16);
-                qf[c] = make_uint4(v.x ^ a.q_sign, v.y ^ a.q_sign, v.z ^ a.q_sign, v.w ^ a.q_sign);
-            }
-            float m = kMinM, l = 0.f, thr = (kMinM + kLazyLog2) * a.inv_scale_log2;
-            f32x16 acc[ND];
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
-
-            auto tile = [&](const char* stg, int t) __attribute__((always_inline)) {
-                f32x16 st;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) st[i] = 0.f;
+            {
+                // ---- this lane's column and query
+                const int t0 = tile0, t1 = t0 + run;
+                const int cidx = grp * S::COLS + wc * 32 + (lane & 31);
+                const bool valid = cidx < n * a.group;
+                const int node = (int)((unsigned)(valid ? cidx : 0) / (unsigned)a.group);
+                const int64_t prow = row0 + node;
+                const int qhead = h * a.group + (valid ? cidx : 0) - node * a.group;
+                const bool busy = grp * S::COLS + wc * 32 < n * a.group;  // a wave of padding columns only loads
+                uint4 qf[NQ];
+                const char* qp = a.q + (prow * a.q_sr + (int64_t)qhead * a.q_sh) * ES;
 #pragma unroll
                 for (int c = 0; c < NQ; ++c) {
-                    const uint4 kf = *(const uint4*)(stg + kaddr[c]);
-                    if constexpr (DT == MF_F32) {
-                        st = mfma32_f32(__uint_as_float(kf.x), __uint_as_float(qf[c].x), st);
-                        st = mfma32_f32(__uint_as_float(kf.y), __uint_as_float(qf[c].y), st);
-                        st = mfma32_f32(__uint_as_float(kf.z), __uint_as_float(qf[c].z), st);
-                        st = mfma32_f32(__uint_as_float(kf.w), __uint_as_float(qf[c].w), st);
-                    } else {
-                        st = mfma32<DT>(kf, qf[c], st);
-                    }
+                    const uint4 v = *(const uint4*)(qp + (2 * c + hf) * 16);
+                    qf[c] = make_uint4(v.x ^ a.q_sign, v.y ^ a.q_sign, v.z ^ a.q_sign, v.w ^ a.q_sign);
                 }
-                if ((t + 1) * kTile > ctx) {  // the context's last tile, and the nodes'
-                    uint32_t seen;
-                    if (t < held) seen = 0xffffffffu >> ((t + 1) * kTile - ctx);
-                    else seen = valid ? a.masks[prow * a.mask_words + (t - held)] : 0u;
+                float m = kMinM, l = 0.f, thr = (kMinM + kLazyLog2) * a.inv_scale_log2;
+                f32x16 acc[ND];
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+
+                auto tile = [&](const char* stg, int t) __attribute__((always_inline)) {
+                    f32x16 st;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) st[i] = 0.f;
+#pragma unroll
+                    for (int c = 0; c < NQ; ++c) {
+                        const uint4 kf = *(const uint4*)(stg + kaddr[c]);
+                        if constexpr (DT == MF_F32) {
+                            st = mfma32_f32(__uint_as_float(kf.x), __uint_as_float(qf[c].x), st);
+                            st = mfma32_f32(__uint_as_float(kf.y), __uint_as_float(qf[c].y), st);
+                            st = mfma32_f32(__uint_as_float(kf.z), __uint_as_float(qf[c].z), st);
+                            st = mfma32_f32(__uint_as_float(kf.w), __uint_as_float(qf[c].w), st);
+                        } else {
+                            st = mfma32<DT>(kf, qf[c], st);
+                        }
+                    }
+                    if ((t + 1) * kTile > ctx) {  // the context's last tile, and the nodes'
+                        uint32_t seen;
+                        if (t < held) seen = 0xffffffffu >> ((t + 1) * kTile - ctx);
+                        else seen = valid ? a.masks[prow * a.mask_words + (t - held)] : 0u;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int key = 8 * (i >> 2) + 4 * hf + (i & 3);
+                            st[i] = seen >> key & 1u ? st[i] : kNegInf;
+                        }
+                    }
+                    // lazy rescale: the maximum moves when a score passes it by more than 2^8
+                    float lmax = st[0];
+#pragma unroll
+                    for (int i = 1; i < 16; ++i) lmax = fmax_prop(lmax, st[i]);
+                    if (__builtin_amdgcn_ballot_w64(lmax > thr) != 0) {
+                        auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(lmax), __float_as_uint(lmax), false, false);
+                        const float mn = fmaxf(m, fmax_prop(__uint_as_float(r[0]), __uint_as_float(r[1])) * a.scale_log2);
+                        const float alpha = __builtin_amdgcn_exp2f(m - mn);
+                        l *= alpha;
+#pragma unroll
+                        for (int d = 0; d < ND; ++d)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
+                        m = mn;
+                        thr = (mn + kLazyLog2) * a.inv_scale_log2;
+                    }
+                    float sum = 0.f;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const int key = 8 * (i >> 2) + 4 * hf + (i & 3);
-                        st[i] = seen >> key & 1u ? st[i] : kNegInf;
+                        st[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i], a.scale_log2, -m));
+                        sum += st[i];
                     }
-                }
-                // lazy rescale: the maximum moves when a score passes it by more than 2^8
-                float lmax = st[0];
+                    l += sum;
+                    if constexpr (DT == MF_F32) {
 #pragma unroll
-                for (int i = 1; i < 16; ++i) lmax = fmax_prop(lmax, st[i]);
-                if (__builtin_amdgcn_ballot_w64(lmax > thr) != 0) {
-                    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(lmax), __float_as_uint(lmax), false, false);
-                    const float mn = fmaxf(m, fmax_prop(__uint_as_float(r[0]), __uint_as_float(r[1])) * a.scale_log2);
-                    const float alpha = __builtin_amdgcn_exp2f(m - mn);
-                    l *= alpha;
+                        for (int i = 0; i < 16; ++i)
 #pragma unroll
-                    for (int d = 0; d < ND; ++d)
+                            for (int d = 0; d < ND; ++d)
+                                acc[d] = mfma32_f32(*(const float*)(stg + vaddr[d] + (8 * (i >> 2) + (i & 3)) * RB), st[i],
+                                                    acc[d]);
+                    } else {
+                        // 16-bit operands of the second product: each weight off by half a step of the type
+                        uint32_t pw[8];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
-                    m = mn;
-                    thr = (mn + kLazyLog2) * a.inv_scale_log2;
-                }
-                float sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    st[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i], a.scale_log2, -m));
-                    sum += st[i];
-                }
-                l += sum;
-                if constexpr (DT == MF_F32) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-#pragma unroll
-                        for (int d = 0; d < ND; ++d)
-                            acc[d] = mfma32_f32(*(const float*)(stg + vaddr[d] + (8 * (i >> 2) + (i & 3)) * RB), st[i], acc[d]);
-                } else {
-                    // 16-bit operands of the second product: each weight off by half a step of the type
-                    uint32_t pw[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        if constexpr (DT == MF_BF16)
-                            pw[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){st[2 * i], st[2 * i + 1]}, bf16x2));
-                        else
-                            pw[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){st[2 * i], st[2 * i + 1]}, f16x2));
-                    }
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int d = 0; d < ND; ++d) {
-                            const uint2 v0 = ld_tr16(stg + vaddr[d] + 16 * k * RB);
-                            const uint2 v1 = ld_tr16(stg + vaddr[d] + (16 * k + 8) * RB);
-                            acc[d] = mfma32<DT>(make_uint4(v0.x, v0.y, v1.x, v1.y),
-                                                make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]), acc[d]);
+                        for (int i = 0; i < 8; ++i) {
+                            const f32x2 pair = {st[2 * i], st[2 * i + 1]};
+                            if constexpr (DT == MF_BF16)
+                                pw[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, bf16x2));
+                            else
+                                pw[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, f16x2));
                         }
-                }
-            };
-
-            for (int st0 = t0; st0 < t1; st0 += ST) {
-                if (in_flight == AHEAD) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((AHEAD - 1) * S::NLD) : "memory");
-                else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                --in_flight;
-                sync();  // the oldest stage is whole, and the one before it has been read
-                if (f_left > 0) fetch();
-                if (busy) {
-                    const char* stg = ring + head_buf * S::STG;
-#pragma unroll 1
-                    for (int x = 0; x < S::SUB; ++x) {
-                        const int t = st0 + x * WK + wk;
-                        if (t < t1) tile(stg + (x * WK + wk) * S::TILE, t);
-                    }
-                }
-                head_buf = head_buf + 1 == S::RING ? 0 : head_buf + 1;
-            }
-
-            // ---- the key waves' sums in one, then the piece's result
-            l = both_halves_sum(l);
-            if constexpr (WK > 1) {
-                constexpr int PART = (ND * 16 + 2) * 64;
-                sync();
-                if (wk > 0) {
-                    float* to = (float*)ring + ((wk - 1) * WC + wc) * PART;
 #pragma unroll
-                    for (int d = 0; d < ND; ++d)
+                        for (int k = 0; k < 2; ++k)
 #pragma unroll
-                        for (int i = 0; i < 16; i += 4)
-                            *(float4*)(to + (d * 16 + i) * 64 + 4 * lane) = make_float4(acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]);
-                    to[ND * 1024 + lane] = m;
-                    to[ND * 1024 + 64 + lane] = l;
-                }
-                sync();
-                if (wk == 0) {
-#pragma unroll
-                    for (int o = 0; o < WK - 1; ++o) {
-                        const float* from = (const float*)ring + (o * WC + wc) * PART;
-                        const float m1 = from[ND * 1024 + lane], l1 = from[ND * 1024 + 64 + lane];
-                        const float mn = fmaxf(m, m1);
-                        const float w0 = __builtin_amdgcn_exp2f(m - mn), w1 = __builtin_amdgcn_exp2f(m1 - mn);
-                        m = mn;
-                        l = l * w0 + l1 * w1;
-#pragma unroll
-                        for (int d = 0; d < ND; ++d)
-#pragma unroll
-                            for (int i = 0; i < 16; i += 4) {
-                                const float4 v = *(const float4*)(from + (d * 16 + i) * 64 + 4 * lane);
-                                acc[d][i] = acc[d][i] * w0 + v.x * w1;
-                                acc[d][i + 1] = acc[d][i + 1] * w0 + v.y * w1;
-                                acc[d][i + 2] = acc[d][i + 2] * w0 + v.z * w1;
-                                acc[d][i + 3] = acc[d][i + 3] * w0 + v.w * w1;
+                            for (int d = 0; d < ND; ++d) {
+                                const uint2 v0 = ld_tr16(stg + vaddr[d] + 16 * k * RB);
+                                const uint2 v1 = ld_tr16(stg + vaddr[d] + (16 * k + 8) * RB);
+                                acc[d] = mfma32<DT>(make_uint4(v0.x, v0.y, v1.x, v1.y),
+                                                    make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]), acc[d]);
                             }
                     }
+                };
+
+                for (int st0 = t0; st0 < t1; st0 += ST) {
+                    if (in_flight == AHEAD) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((AHEAD - 1) * S::NLD) : "memory");
+                    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    --in_flight;
+                    sync();  // the oldest stage is whole, and the one before it has been read
+                    if (f_left > 0) fetch();
+                    if (busy) {
+                        const char* stg = ring + head_buf * S::STG;
+#pragma unroll 1
+                        for (int x = 0; x < S::SUB; ++x) {
+                            const int t = st0 + x * WK + wk;
+                            if (t < t1) tile(stg + (x * WK + wk) * S::TILE, t);
+                        }
+                    }
+                    head_buf = head_buf + 1 == S::RING ? 0 : head_buf + 1;
                 }
-            }
-            if (wk == 0 && busy) {
-                if (t0 == 0 && t1 == tiles) {
-                    store_column<DT, ND>(a.out + (prow * a.o_sr + (int64_t)qhead * a.o_sh) * ES, valid, acc, 1.f / l, hf);
-                } else {
-                    float* to = a.partials + (2 * (int64_t)blockIdx.x + (first ? 0 : 1)) * S::SLOT + wc * 32 * (D + 2);
+
+                // ---- the key waves' sums in one, then the piece's result
+                l = both_halves_sum(l);
+                if constexpr (WK > 1) {
+                    constexpr int PART = (ND * 16 + 2) * 64;
+                    sync();
+                    if (wk > 0) {
+                        float* to = (float*)ring + ((wk - 1) * WC + wc) * PART;
 #pragma unroll
-                    for (int d = 0; d < ND; ++d)
+                        for (int d = 0; d < ND; ++d)
 #pragma unroll
-                        for (int i = 0; i < 16; i += 4)
-                            if (valid)
-                                *(float4*)(to + (d * 16 + i) * 64 + 4 * lane) = make_float4(acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]);
-                    if (hf == 0) {
-                        to[32 * D + lane] = m;
-                        to[32 * D + 32 + lane] = l;
+                            for (int i = 0; i < 16; i += 4)
+                                *(float4*)(to + (d * 16 + i) * 64 + 4 * lane) =
+                                    make_float4(acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]);
+                        to[ND * 1024 + lane] = m;
+                        to[ND * 1024 + 64 + lane] = l;
+                    }
+                    sync();
+                    if (wk == 0) {
+#pragma unroll
+                        for (int o = 0; o < WK - 1; ++o) {
+                            const float* from = (const float*)ring + (o * WC + wc) * PART;
+                            const float m1 = from[ND * 1024 + lane], l1 = from[ND * 1024 + 64 + lane];
+                            const float mn = fmaxf(m, m1);
+                            const float w0 = __builtin_amdgcn_exp2f(m - mn), w1 = __builtin_amdgcn_exp2f(m1 - mn);
+                            m = mn;
+                            l = l * w0 + l1 * w1;
+#pragma unroll
+                            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                                for (int i = 0; i < 16; i += 4) {
+                                    const float4 v = *(const float4*)(from + (d * 16 + i) * 64 + 4 * lane);
+                                    acc[d][i] = acc[d][i] * w0 + v.x * w1;
+                                    acc[d][i + 1] = acc[d][i + 1] * w0 + v.y * w1;
+                                    acc[d][i + 2] = acc[d][i + 2] * w0 + v.z * w1;
+                                    acc[d][i + 3] = acc[d][i + 3] * w0 + v.w * w1;
+                                }
+                        }
+                    }
+                }
+                if (wk == 0 && busy) {
+                    if (t0 == 0 && t1 == tiles) {
+                        store_column<DT, ND>(a.out + (prow * a.o_sr + (int64_t)qhead * a.o_sh) * ES, valid, acc, 1.f / l, hf);
+                    } else {
+                        float* to = a.partials + (2 * (int64_t)blockIdx.x + (first ? 0 : 1)) * S::SLOT + wc * 32 * (D + 2);
+#pragma unroll
+                        for (int d = 0; d < ND; ++d)
+#pragma unroll
+                            for (int i = 0; i < 16; i += 4)
+                                if (valid)
+                                    *(float4*)(to + (d * 16 + i) * 64 + 4 * lane) =
+                                        make_float4(acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]);
+                        if (hf == 0) {
+                            to[32 * D + lane] = m;
+                            to[32 * D + 32 + lane] = l;
+                        }
                     }
                 }
             }
-        }
-        sync();  // the ring and the window have been read
+            sync();  // the ring and the window have been read
         }
         left -= run;
         if (left <= 0) return;
@@ -609,7 +624,8 @@ __global__ __launch_bounds__(kTreeThreads) void merge_tree_kernel(TreeArgs a, in
         for (int i = 0; i < 16; ++i) acc[0][i] = 0.f;
 #pragma unroll 2
         for (int64_t w = w0 + (SPLIT ? wave : 0); w <= w1; w += SPLIT ? 4 : 1) {
-            const float* from = a.partials + (2 * (w * units_per_seq + unit) + (w * share < begin ? 1 : 0)) * S::SLOT + blk * 32 * (D + 2);
+            const int64_t slot = 2 * (w * units_per_seq + unit) + (w * share < begin ? 1 : 0);
+            const float* from = a.partials + slot * S::SLOT + blk * 32 * (D + 2);
             const float m1 = from[32 * D + (lane & 31)], l1 = from[32 * D + 32 + (lane & 31)];
             float4 v[4];
 #pragma unroll
@@ -654,8 +670,20 @@ __global__ __launch_bounds__(kTreeThreads) void merge_tree_kernel(TreeArgs a, in
     }
 }
 
-// The waves' arrangement for a call: wc side by side on blocks of 32 columns, 4 / wc along
-// the keys (8 waves where 8 blocks share their keys).
+// The waves' arrangement for a call and the least tiles of a share. wc waves stand side by
+// side on blocks of 32 columns, 4 / wc along the keys; 8 waves where 8 blocks share their keys.
+//
+// Each tile is loaded once for all columns of its group, so a group is as wide as the columns
+// are. The rule by its sides (layers as in the comment above, us a call with the plan):
+// 20 columns, 64 contexts of up to 4,000 at 40/8 x 128: two blocks 202, four 205, one block
+// with four waves along the keys 222; 60 columns there: two 232, four 237. 80 columns, the
+// first case above: four blocks 358, eight 400. 240 columns, the second: eight blocks 133,
+// two groups of four 153; 192 at 15/5 x 64, four layers: 116, 126.
+//
+// Shares of few tiles spread a short line over more of the GPU and leave more sums to merge.
+// 4 contexts of up to 700 tokens at 15/5 x 64, least shares of 8, 4, 2 and 1: 24 columns (four
+// layers) -, 53, 44, 48; 72 columns 71, 65, 63, -; 192 columns 82, 73, 77, -; 24 in fp32 (two
+// layers) 63, 46, 38, -.
 struct TreeConfig {
     int wc, per_cu, min_share;
 };
@@ -663,13 +691,10 @@ struct TreeConfig {
 TreeConfig tree_config(int dtype, int head_dim, int max_nodes, int group) {
     const int64_t cols = (int64_t)max_nodes * group;
     const int rb = head_dim * dtype_size(dtype);
-    if (dtype == MF_F32 || rb > 256) return {4, rb > 256 ? 1 : 2, 8};
-    // few columns: one stage is a share (4 contexts of up to 700 with 8 nodes at 15/5 x 64: four layers 74 us at 8
-    // tiles, 58 at 4)
-    if (cols <= 32) return {1, rb == 256 ? 1 : 2, 4};
-    if (cols <= 64) return {2, 2, 4};
-    if (cols <= 128) return {4, 2, 8};
-    return {8, 1, 8};
+    if (dtype == MF_F32 || rb > 256) return {4, rb > 256 ? 1 : 2, 2};
+    if (cols <= 64) return {2, 2, 2};
+    if (cols <= 128) return {4, 2, 2};
+    return {8, 1, 4};
 }
 
 template <int DT, int D, int WC, int WK>
@@ -677,10 +702,13 @@ int launch_tree(const TreeArgs& a, int workers, int units_per_seq, hipStream_t s
     hipLaunchKernelGGL((tree_kernel<DT, D, WC, WK>), dim3((unsigned)workers), dim3(WC * WK * 64), 0, st, a);
     if (int e = check_launch()) return e;
     const int units = a.num_seqs * units_per_seq;
-    // many pieces to a unit where there are few units for the workers
-    if ((int64_t)units * 8 <= workers)
-        hipLaunchKernelGGL((merge_tree_kernel<DT, D, WC, WK, true>), dim3((unsigned)units, WC * (D / 32)), dim3(kTreeThreads), 0,
-                           st, a, units_per_seq);
+    // Few units for the workers are cut into many pieces each: their sums are spread over more
+    // workgroups (4 contexts of up to 700, the 24 columns above: 43 us, unsplit 53; one of 32,001:
+    // 133, 146; 16 at 15/5 x 64 and 192 columns: 114, 116). Where most units are whole, the larger
+    // grid has nothing to do (1,024 contexts of up to 200 at 40/8 x 128, 20 columns: 492, unsplit 418).
+    if ((int64_t)units * 2 <= workers)
+        hipLaunchKernelGGL((merge_tree_kernel<DT, D, WC, WK, true>), dim3((unsigned)units, WC * (D / 32)),
+                           dim3(kTreeThreads), 0, st, a, units_per_seq);
     else
         hipLaunchKernelGGL((merge_tree_kernel<DT, D, WC, WK, false>), dim3((unsigned)units, WC), dim3(kTreeThreads), 0, st, a,
                            units_per_seq);
@@ -690,7 +718,6 @@ int launch_tree(const TreeArgs& a, int workers, int units_per_seq, hipStream_t s
 template <int DT, int D>
 int launch_tree(const TreeArgs& a, const TreeConfig& c, int workers, int units_per_seq, hipStream_t st) {
     if constexpr (DT != MF_F32 && D <= 128) {
-        if (c.wc == 1) return launch_tree<DT, D, 1, 4>(a, workers, units_per_seq, st);
         if (c.wc == 2) return launch_tree<DT, D, 2, 2>(a, workers, units_per_seq, st);
         if (c.wc == 8) return launch_tree<DT, D, 8, 1>(a, workers, units_per_seq, st);
     }
