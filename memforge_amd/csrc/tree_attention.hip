@@ -161,7 +161,8 @@ __global__ __launch_bounds__(kTreeThreads) void tree_plan_kernel(TreePlanArgs a)
     }
     __syncthreads();
     const int column_groups = a.lanes / a.num_kv_heads;
-    for (int i = tid; i < a.num_shares; i += kTreeThreads) {
+    for (int w = tid; w < a.num_shares * a.lanes; w += kTreeThreads) {
+        const int i = w / a.lanes, lane_of = w - i * a.lanes, h = lane_of / column_groups;
         const int64_t at = (int64_t)i * share;
         int lo = 0, hi = a.num_seqs - 1;  // the last sequence that starts at or before `at`: it has tiles
         while (lo < hi) {
@@ -171,12 +172,10 @@ __global__ __launch_bounds__(kTreeThreads) void tree_plan_kernel(TreePlanArgs a)
         }
         const int32_t* q = a.seqs + (int64_t)lo * kSeqInts;
         const int left = (int)max(min(share, total - at), (int64_t)0);
-        for (int u = 0; u < a.lanes; ++u) {
-            int4* to = (int4*)(a.work + ((int64_t)i * a.lanes + u) * kWorkInts);
-            to[0] = make_int4(lo, u / column_groups, (int)(at - first[lo]), left);
-            to[1] = make_int4(q[0], q[1], q[2], q[3]);
-            to[2] = make_int4(q[4], q[5], u % column_groups, 0);
-        }
+        int4* to = (int4*)(a.work + (int64_t)w * kWorkInts);
+        to[0] = make_int4(lo, h, (int)(at - first[lo]), left);
+        to[1] = make_int4(q[0], q[1], q[2], q[3]);
+        to[2] = make_int4(q[4], q[5], lane_of - h * column_groups, 0);
     }
 }
 

@@ -136,6 +136,19 @@ def test_kinds_of_trees(device, shape):
     assert plan.positions.tolist() == depth
 
 
+@pytest.mark.parametrize("shape", ["chain", "random"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_the_largest_trees(device, dtype, shape):
+    st = Trees(device, dtype, 6, 2, 32, 16, [70, 0, 33], [1024, 1, 1000], seed=8, shape=shape)
+    st.check(st.run())
+
+
+def test_plans_wider_than_their_trees(device):
+    """Trees of up to 1024 nodes are allowed for, few come: most groups of columns are empty."""
+    st = Trees(device, torch.bfloat16, 15, 5, 64, 16, [700, 31, 0, 64], [8, 1, 30, 90], seed=9)
+    st.check(st.run(st.plan(max_nodes=1024, max_context=st.width * 16)))
+
+
 @pytest.mark.parametrize("nodes", [1, 4, 17, 48])
 def test_one_long_context(device, nodes):
     """Cut over every workgroup, merged from many pieces."""
