@@ -1767,5 +1767,6 @@ def tree_attention(q_rows: torch.Tensor, out_rows: torch.Tensor, pool: PoolView,
     tree_attention_at(_tree_rows("q_rows", q_rows, plan.num_q_heads, plan, 0, 1),
                       _tree_rows("out_rows", out_rows, plan.num_q_heads, plan, 0, 1),
                       (pool.k.data_ptr(), pool.v.data_ptr(), pool.stride_block, pool.stride_slot, pool.stride_head,
-                       pool.block_size, pool.num_blocks), block_tables, plan, _tree_rows("new_k_rows", new_k_rows, plan.num_kv_heads, plan, 0, 1),
+                       pool.block_size, pool.num_blocks), block_tables, plan,
+                      _tree_rows("new_k_rows", new_k_rows, plan.num_kv_heads, plan, 0, 1),
                       _tree_rows("new_v_rows", new_v_rows, plan.num_kv_heads, plan, 0, 1)[0], float(scale), partials)

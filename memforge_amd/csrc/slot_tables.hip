@@ -3,7 +3,8 @@
 // slot for every new token), and its cut back to given lengths (blocks pushed
 // again).
 //
-// One launch each. Every workgroup scans the batch's lengths for itself (at most
+// One launch each (growth with rows given by number: one more, which clears all
+// rows first). Every workgroup scans the batch's lengths for itself (at most
 // 4,096 requests: 16 per thread, then a scan over the workgroup), which costs
 // less than a launch that hands the sums over, and does its share of the rows,
 // table entries or returned blocks from them. The state that the scan reads

@@ -5,7 +5,7 @@ The host's allocator (``memforge_c.BlockAllocator``) hands out blocks between
 steps; a program whose steps follow each other on the device -- a round of
 speculation whose number of accepted tokens only the device knows, steps replayed
 as HIP graphs -- keeps its tables here instead and reads them back when it wants
-to. One launch a call (mf_tables_extend, mf_tables_truncate), every sum in it
+to. One launch a call (mf_tables_extend, two with ``rows``; mf_tables_truncate), every sum in it
 whole numbers, so the results do not depend on the order of anything."""
 
 from __future__ import annotations
@@ -83,8 +83,8 @@ class DeviceBlockTables:
         rows get slot -1, and so does every later one that lacks blocks when it was the
         blocks. The new tokens are packed: row ``cu_seqlens[s] + i`` is token i of request
         s, rows past the last get slot -1. With ``rows`` (int32 (requests, most)) token i of
-        request s is row ``rows[s, i]`` of ``max_rows`` instead, negative entries none: the
-        accepted path of a tree's rows, whose keys and values ``_native.kv_write`` then
+        request s is row ``rows[s, i]`` of ``max_rows`` instead, negative entries none, and
+        no row named twice: the accepted path of a tree's rows, whose keys and values ``_native.kv_write`` then
         puts into the pool as they lie."""
         dev, n, state = self._state("new_tokens", new_tokens)
         if max_rows < 0:
