@@ -657,7 +657,8 @@ int mf_tree_accept(const int64_t* tokens, const int64_t* targets, const int32_t*
  * falls that close to a border.
  * num_cus: the device's compute units; few rows are split over them, through a
  * workspace of mf_sample_workspace_size bytes (8-byte aligned; 0: none) that is
- * all 0 before the call and after it.
+ * all 0 before the call and after it. The call is up to three launches: calls that host
+ * threads make at the same time must not share a workspace, on one stream neither.
  * Beyond sampling.sample_logits (memforge_ml/runtime/sampling.py:33-75).
  */
 #define MF_SAMPLE_MAX_VOCAB (1 << 20)
@@ -683,7 +684,9 @@ int mf_sample(const void* logits, int dtype, int64_t stride_row, int num_rows, i
  * cu_nodes and parents are read by it alone and only then. Contexts are taken to
  * be at most max_context, trees max_nodes; a tree whose rows are not within
  * num_rows has none. mf_tree_plan_sizes gives the int32 words of the plan (16-byte
- * aligned) and the fp32 partials that a launch on num_cus compute units needs; the
+ * aligned) and the fp32 partials that a launch on num_cus compute units needs (a call is two
+ * launches: calls that host threads make at the same time must not share partials, on one
+ * stream neither); the
  * four shape arguments, num_seqs, num_rows and num_cus are the same in all three
  * calls, and every block table row holds at least max_context / block_size entries.
  * Block numbers past num_blocks read the last block. Rows that belong to no tree

@@ -11,6 +11,7 @@ runs on the MI355X or not at all.
 from __future__ import annotations
 
 import ctypes
+import threading
 from collections import OrderedDict
 from dataclasses import dataclass
 from pathlib import Path
@@ -861,11 +862,17 @@ class CountedPlan:
         self._copied.record()
 
 
-class Workspace:
+class Workspace(threading.local):
     """Grow-only scratch for split-K partials (fp32), merge arrival counters
     (int32, kept all-zero between calls by the kernels) and the rejection
     verify, one per (device, stream) so concurrent streams never share it; likewise the
     bins of split sampling rows (int64, kept all-zero).
+
+    Every host thread has scratch of its own too (``threading.local``: each gets
+    these dictionaries when it first comes here, and they end with it). A call may be
+    several launches, the C entry points run without the interpreter's lock, and
+    threads share a stream unless told otherwise, so another thread's launches
+    can stand between those of one call.
 
     A call recorded into a graph gets memory of its own, which the graph's private
     pool holds: a shared buffer would be freed under the graph when a later call
