@@ -680,7 +680,8 @@ int mf_sample(const void* logits, int dtype, int64_t stride_row, int num_rows, i
  *
  * mf_tree_plan, once for all layers of a step, works out on the device which keys
  * each node sees, how the keys are split over the launch, and every node's position
- * (context length + number of ancestors; int64, one per row). context_lens,
+ * (context length + number of ancestors; int64, one per row, 0 for rows of no tree:
+ * past max_nodes, before and behind all trees, without sequences; cu_nodes does not fall). context_lens,
  * cu_nodes and parents are read by it alone and only then. Contexts are taken to
  * be at most max_context, trees max_nodes; a tree whose rows are not within
  * num_rows has none. mf_tree_plan_sizes gives the int32 words of the plan (16-byte

@@ -1669,7 +1669,7 @@ class TreePlan:
     """One step's trees as ``tree_attention`` reads them (mf_tree_plan)."""
 
     buffer: torch.Tensor      # int32
-    positions: torch.Tensor   # int64 per row: context length + number of ancestors
+    positions: torch.Tensor   # int64 per row: context length + number of ancestors; 0: no node's row
     num_seqs: int
     num_rows: int
     max_nodes: int

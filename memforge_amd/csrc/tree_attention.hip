@@ -81,10 +81,19 @@ __device__ __forceinline__ void seq_shape(const TreePlanArgs& a, int s, int& ctx
     ctx = (int)min((int64_t)max(a.ctx_lens[s], 0), a.max_context);
 }
 
-// Block 0 lays the tiles out; block 1 + s writes sequence s's masks and positions.
+// Positions of no sequence's rows.
+__global__ __launch_bounds__(kTreeThreads) void clear_positions_kernel(int64_t* positions, int64_t num_rows) {
+    for (int64_t r = (int64_t)blockIdx.x * kTreeThreads + threadIdx.x; r < num_rows; r += (int64_t)gridDim.x * kTreeThreads)
+        positions[r] = 0;
+}
+
+// Block 0 lays the tiles out; block 1 + s writes sequence s's masks and positions. Rows that are no
+// node's have position 0, so that what follows may look it up: block 1 + s writes those of its
+// own rows (past max_nodes, or of a tree that has none), block 0 those before and behind all trees.
 __global__ __launch_bounds__(kTreeThreads) void tree_plan_kernel(TreePlanArgs a) {
     __shared__ int64_t first[kMaxSeqs + 1];
     __shared__ int64_t waves[kTreeThreads / 64];
+    __shared__ int rows_lo[kTreeThreads / 64], rows_hi[kTreeThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if (blockIdx.x > 0) {
         int* up = (int*)first;
@@ -114,15 +123,21 @@ __global__ __launch_bounds__(kTreeThreads) void tree_plan_kernel(TreePlanArgs a)
             }
             a.positions[row0 + i] = (int64_t)ctx + depth - 1;
         }
+        const int64_t last = min((int64_t)a.cu_nodes[s + 1], a.num_rows);
+        for (int64_t r = max(row0, (int64_t)0) + n + tid; r < last; r += kTreeThreads) a.positions[r] = 0;
         return;
     }
     const int per = (a.num_seqs + kTreeThreads - 1) / kTreeThreads;
     const int s0 = min(tid * per, a.num_seqs), s1 = min(s0 + per, a.num_seqs);
     int64_t mine = 0;
+    int row_lo = INT_MAX, row_hi = INT_MIN;  // of the numbers in cu_nodes
     for (int s = s0; s < s1; ++s) {
         int ctx, n;
         int64_t row0;
         seq_shape(a, s, ctx, n, row0);
+        const int row1 = a.cu_nodes[s + 1];
+        row_lo = min(row_lo, min((int)row0, row1));
+        row_hi = max(row_hi, max((int)row0, row1));
         const int held = (ctx + kTile - 1) / kTile;
         const int tiles = n > 0 ? held + (n + kTile - 1) / kTile : 0;
         const int groups = (n * a.group + a.group_cols - 1) / a.group_cols;
@@ -141,13 +156,21 @@ __global__ __launch_bounds__(kTreeThreads) void tree_plan_kernel(TreePlanArgs a)
     for (int o = 1; o < 64; o <<= 1) {
         const int64_t up = __shfl_up(incl, o, 64);
         if (lane >= o) incl += up;
+        row_lo = min(row_lo, __shfl_xor(row_lo, o, 64));
+        row_hi = max(row_hi, __shfl_xor(row_hi, o, 64));
     }
-    if (lane == 63) waves[wave] = incl;
+    if (lane == 63) {
+        waves[wave] = incl;
+        rows_lo[wave] = row_lo;
+        rows_hi[wave] = row_hi;
+    }
     __syncthreads();
     int64_t base = incl - mine, total = 0;
     for (int w = 0; w < kTreeThreads / 64; ++w) {
         if (w < wave) base += waves[w];
         total += waves[w];
+        row_lo = min(row_lo, rows_lo[w]);
+        row_hi = max(row_hi, rows_hi[w]);
     }
     for (int s = s0; s < s1; ++s) {
         first[s] += base;
@@ -177,6 +200,9 @@ __global__ __launch_bounds__(kTreeThreads) void tree_plan_kernel(TreePlanArgs a)
         to[1] = make_int4(q[0], q[1], q[2], q[3]);
         to[2] = make_int4(q[4], q[5], lane_of - h * column_groups, 0);
     }
+    const int64_t before = min((int64_t)row_lo, a.num_rows);
+    for (int64_t r = tid; r < before; r += kTreeThreads) a.positions[r] = 0;
+    for (int64_t r = max((int64_t)row_hi, (int64_t)0) + tid; r < a.num_rows; r += kTreeThreads) a.positions[r] = 0;
 }
 
 struct TreeArgs {
@@ -779,7 +805,14 @@ extern "C" int mf_tree_plan(const int32_t* parents, const int32_t* cu_nodes, con
                                    &words, &floats))
         return e;
     if (max_context < 0 || max_context > (1 << 30)) return MF_ERR_ARG;
-    if (num_seqs == 0) return MF_OK;
+    if (num_seqs == 0) {
+        if (num_rows == 0) return MF_OK;
+        if (!positions) return MF_ERR_ARG;
+        const int64_t blocks = std::min<int64_t>((num_rows + kTreeThreads - 1) / kTreeThreads, 1024);
+        hipLaunchKernelGGL(clear_positions_kernel, dim3((unsigned)blocks), dim3(kTreeThreads), 0, (hipStream_t)stream,
+                           positions, num_rows);
+        return check_launch();
+    }
     if (!cu_nodes || !context_lens || !plan || ((uintptr_t)plan & 15) || (num_rows > 0 && (!parents || !positions)))
         return MF_ERR_ARG;
     if (plan_words < words) return MF_ERR_WORKSPACE;

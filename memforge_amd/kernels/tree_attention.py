@@ -30,7 +30,8 @@ def plan_tree(parents: torch.Tensor, cu_nodes: torch.Tensor, context_lens: torch
     ``context_lens`` (int32, B) the tokens it has in the pool, taken as at most
     ``max_context``. All are read here and not by the attention: a step with other
     lengths or trees has a plan of its own. ``positions`` of the plan (int64 per row) are
-    the nodes' positions, context length plus ancestors, as rotary embeddings take them."""
+    the nodes' positions, context length plus ancestors, as rotary embeddings take them, and 0
+    at rows that belong to no tree."""
     return nat.tree_plan(parents, cu_nodes, context_lens, max_nodes, max_context, num_q_heads, num_kv_heads, head_dim, dtype)
 
 
