@@ -1726,7 +1726,7 @@ def _tree_rows(name: str, x: torch.Tensor, heads: int, plan: "TreePlan", rows: i
                          f"{plan.device}, got {tuple(shape)} in {x.dtype} on {x.device}")
     if stride[-1] != 1:
         raise ValueError(f"{name} head_dim axis must be contiguous")
-    return x.data_ptr(), stride[rows], stride[head]
+    return x.data_ptr(), stride[rows] if shape[rows] > 1 else 0, stride[head] if heads > 1 else 0
 
 
 def tree_attention_at(q: Tuple[int, int, int], out: Tuple[int, int, int], pool: Tuple[int, int, int, int, int, int, int],

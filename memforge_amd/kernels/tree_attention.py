@@ -57,12 +57,12 @@ def paged_attention_tree(query: torch.Tensor, key_pool: torch.Tensor, value_pool
     nat.check_tree_pool(key_pool, kv_heads, dim, plan)
     if not -layers <= layer_idx < layers:
         raise IndexError(f"layer {layer_idx} of pools of {layers}")
-    q, q_copy = _rows("query", query, plan.num_q_heads, plan)
-    k, k_copy = _rows("new_keys", new_keys, plan.num_kv_heads, plan)
-    v, v_copy = _rows("new_values", new_values, plan.num_kv_heads, plan)
+    q, q_rows = _rows("query", query, plan.num_q_heads, plan)
+    k, k_rows = _rows("new_keys", new_keys, plan.num_kv_heads, plan)
+    v, v_rows = _rows("new_values", new_values, plan.num_kv_heads, plan)
     if k[1:] != v[1:]:
-        k, k_copy = _rows("new_keys", new_keys.contiguous(), plan.num_kv_heads, plan, True)
-        v, v_copy = _rows("new_values", new_values.contiguous(), plan.num_kv_heads, plan, True)
+        k, k_rows = _rows("new_keys", new_keys, plan.num_kv_heads, plan, copy=True)
+        v, v_rows = _rows("new_values", new_values, plan.num_kv_heads, plan, copy=True)
     out = torch.empty((1, plan.num_q_heads, plan.num_rows, dim), dtype=plan.dtype, device=plan.device)
     at = (layer_idx % layers) * stride[0] * key_pool.element_size()
     nat.tree_attention_at(q, (out.data_ptr(), dim, plan.num_rows * dim),
@@ -71,17 +71,17 @@ def paged_attention_tree(query: torch.Tensor, key_pool: torch.Tensor, value_pool
     return out
 
 
-def _rows(name: str, x: torch.Tensor, heads: int, plan: TreePlan, keep: bool = False):
+def _rows(name: str, x: torch.Tensor, heads: int, plan: TreePlan, copy: bool = False):
     """((address, row stride, head stride), what has to live until the launch) of ``(1, heads, rows, head_dim)``: of a
-    copy where rows or heads do not begin at whole 16 bytes, as the kernel reads them."""
+    copy where rows or heads do not begin at whole 16 bytes, as the kernel reads them. The stride of an axis of length
+    one addresses nothing, may be any number, and is given as 0."""
     if x.shape != (1, heads, plan.num_rows, plan.head_dim) or x.dtype is not plan.dtype or x.device != plan.device:
         raise ValueError(f"{name} must be {(1, heads, plan.num_rows, plan.head_dim)} in {plan.dtype} on {plan.device}, got "
                          f"{tuple(x.shape)} in {x.dtype} on {x.device}")
     _, head, row, last = x.stride()
-    at = x.data_ptr()
+    at, dim = x.data_ptr(), plan.head_dim
     per = 4 if plan.dtype is torch.float32 else 8
-    if last != 1 or head % per or row % per or at & 15:
-        x, keep = x.contiguous(), True
-        _, head, row, _ = x.stride()
-        at = x.data_ptr()
-    return (at, row, head), x if keep else None
+    if copy or last != 1 or (head % per and heads > 1) or (row % per and plan.num_rows > 1) or at & 15:
+        x = torch.empty((heads, plan.num_rows, dim), dtype=plan.dtype, device=plan.device).copy_(x[0])
+        at, head, row = x.data_ptr(), plan.num_rows * dim, dim
+    return (at, row if plan.num_rows > 1 else 0, head if heads > 1 else 0), x
