@@ -1748,8 +1748,9 @@ def tree_attention_at(q: Tuple[int, int, int], out: Tuple[int, int, int], pool: 
         partials = _WORKSPACE.partials(plan.partials_floats, dev)
     elif partials.dtype != torch.float32 or not partials.is_contiguous() or partials.device != dev:
         raise ValueError(f"partials must be contiguous fp32 on {dev}, got {partials.dtype} on {partials.device}")
+    # (tables of no columns have no address; no context reads them, and the entry point takes no null pointer)
     _launch(dev, "mf_tree_attention", lib().mf_tree_attention, *q, *out, DTYPE_CODES[plan.dtype], *pool,
-            block_tables.data_ptr(), shape[1], new_k[0], new_v, new_k[1], new_k[2], plan.num_seqs, plan.num_rows,
+            block_tables.data_ptr() if shape[1] else plan.buffer.data_ptr(), shape[1], new_k[0], new_v, new_k[1], new_k[2], plan.num_seqs, plan.num_rows,
             plan.max_nodes, plan.num_q_heads, plan.num_kv_heads, plan.head_dim, scale, plan.num_cus, plan.buffer.data_ptr(),
             plan.buffer.numel(), partials.data_ptr(), partials.numel())
 

@@ -32,3 +32,10 @@ def test_layouts(device, dtype, hq, hkv, nodes, lay):
     st.check(st.run())
     st.nv = lay(st.nv)
     st.check(st.run())
+
+
+@pytest.mark.parametrize("nodes", [[1], [5, 1, 40]])
+def test_trees_without_context_or_tables(device, nodes):
+    st = Trees(device, torch.bfloat16, 4, 2, 64, 16, [0] * len(nodes), nodes, seed=3)
+    st.table = st.table[:, :0].contiguous()
+    st.check(st.run())

@@ -94,3 +94,17 @@ def test_raw_rows_of_one(monkeypatch):
                        0.125)
     a = calls[-1]
     assert all(x % 8 == 0 for x in (a[1], a[2], a[4], a[5], a[18], a[19]))
+
+
+def test_tables_without_columns(monkeypatch):
+    """A step of trees that have no context: a null pointer is refused below, so none is handed in."""
+    calls = []
+    monkeypatch.setattr(nat, "require_device", lambda *_: None)
+    monkeypatch.setattr(nat, "device_cus", lambda _: 256)
+    monkeypatch.setattr(nat, "_launch", lambda dev, what, fn, *a: calls.append(a))
+    monkeypatch.setattr(nat._WORKSPACE, "partials", lambda n, dev: torch.empty(n))
+    plan = plan_tree(ints(-1, 0), ints(0, 2), ints(0), 2, 2, 1, 64, torch.bfloat16, max_context=0)
+    pool = torch.zeros((1, 4, 16, 1, 64), dtype=torch.bfloat16)
+    rows = torch.zeros((1, 2, 2, 64), dtype=torch.bfloat16)
+    paged_attention_tree(rows, pool, pool, 0, torch.zeros((1, 0), dtype=torch.int32), plan, rows[:, :1], rows[:, :1])
+    assert calls[-1][14] and calls[-1][15] == 0
