@@ -93,7 +93,8 @@ class DeviceBlockTables:
             nat.check_index("rows", rows, torch.int32, dev)
             if rows.dim() != 2 or rows.shape[0] != n:
                 raise ValueError(f"rows must be ({n}, most new tokens), got {tuple(rows.shape)}")
-            at, width = rows.data_ptr(), rows.shape[1]
+            # (an empty tensor has no address, and no address means packed rows; nothing is read of no columns)
+            at, width = rows.data_ptr() or self.lens.data_ptr(), rows.shape[1]
         else:
             at, width = None, 0
         slots = torch.empty(max_rows, dtype=torch.int64, device=dev)
