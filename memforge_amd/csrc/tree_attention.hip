@@ -249,6 +249,13 @@ struct TreeShape {
     static constexpr int NQ = RB / 32;                     // 16-byte pieces of a query row per lane half
     static constexpr int ND = D / 32;
     static constexpr int PER_CU = WAVES == 8 || RB > 256 || RING * STG > 72 * 1024 ? 1 : 2;  // workgroups
+    // Weights are 2^(score - maximum + UP), the maximum moved when a score passes it by more than
+    // 2^SLACK, and UP cancels in out = sum w v / sum w. fp16 keeps weights for the second product in
+    // steps of 2^-24 at the least, which are then 2^-34 of the largest: all rounded off together are
+    // at most keys * 2^-35 of the sum. (With UP 0 the tail of 32,001 keys could lose 2^-10 of
+    // it.) 2^13 at the most leave a factor 8 to the type's largest number.
+    static constexpr float UP = DT == MF_F16 ? 10.f : 0.f;
+    static constexpr float SLACK = DT == MF_F16 ? 3.f : kLazyLog2;
     static constexpr int COLS = WC * 32;
     static constexpr int SLOT = COLS * (D + 2);            // floats of a piece's sums
     static_assert(PAIRS >= 1 && HALF % (1024 * WAVES) == 0, "whole pieces for every wave");
@@ -440,7 +447,7 @@ __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * W
                     const uint4 v = *(const uint4*)(qp + (2 * c + hf) * 16);
                     qf[c] = make_uint4(v.x ^ a.q_sign, v.y ^ a.q_sign, v.z ^ a.q_sign, v.w ^ a.q_sign);
                 }
-                float m = kMinM, l = 0.f, thr = (kMinM + kLazyLog2) * a.inv_scale_log2;
+                float m = kMinM, l = 0.f, thr = (kMinM + S::SLACK) * a.inv_scale_log2;
                 f32x16 acc[ND];
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
@@ -473,7 +480,7 @@ __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * W
                             st[i] = seen >> key & 1u ? st[i] : kNegInf;
                         }
                     }
-                    // lazy rescale: the maximum moves when a score passes it by more than 2^8
+                    // lazy rescale: the maximum moves when a score passes it by more than 2^SLACK
                     float lmax = st[0];
 #pragma unroll
                     for (int i = 1; i < 16; ++i) lmax = fmax_prop(lmax, st[i]);
@@ -487,12 +494,13 @@ __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * W
 #pragma unroll
                             for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
                         m = mn;
-                        thr = (mn + kLazyLog2) * a.inv_scale_log2;
+                        thr = (mn + S::SLACK) * a.inv_scale_log2;
                     }
                     float sum = 0.f;
+                    const float zero = DT == MF_F16 ? S::UP - m : -m;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        st[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i], a.scale_log2, -m));
+                        st[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i], a.scale_log2, zero));
                         sum += st[i];
                     }
                     l += sum;
@@ -504,7 +512,8 @@ __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * W
                                 acc[d] = mfma32_f32(*(const float*)(stg + vaddr[d] + (8 * (i >> 2) + (i & 3)) * RB), st[i],
                                                     acc[d]);
                     } else {
-                        // 16-bit operands of the second product: each weight off by half a step of the type
+                        // 16-bit operands of the second product: each weight off by half a step of the type (fp16's
+                        // smallest weights by half of its least step, see UP)
                         uint32_t pw[8];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {

@@ -1,0 +1,44 @@
+"""How near paged_attention_tree comes to 64 bits: the small weights of fp16, and errors in the norm of a head's output."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from tests.test_gpu_tree_attention import Trees
+from tests.tree_reference import definition
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d,nodes", [(64, 1), (64, 20), (128, 48), (256, 2)])
+@pytest.mark.parametrize("sink", [0, 17000, 31999, "node"])
+def test_a_flat_tail_far_below_one_key(device, dtype, d, nodes, sink):
+    """One key that holds nearly all the mass and has values 0: what comes out is the tail of 32,000 keys, each 2^-25.6 of
+    it, and has to come out: all within half a step, and fp16's within keys * 2^-35 of the sum besides (at most keys
+    half steps of 2^-24, where the largest weight is 2^10 or more)."""
+    st = Trees(device, dtype, 4, 2, d, 16, [32000], [nodes], seed=1, scale=0.125, shape="star")
+    st.q.zero_()
+    st.q[..., 0] = 8.0
+    for x in (st.k, st.nk):
+        x.zero_()
+        x[..., 0] = -8.875
+    if sink == "node":  # node 0, an ancestor of all
+        st.nk[0, :, 0, 0], st.nv[0, :, 0] = 8.875, 0.0
+    else:
+        block, slot = st.tables[0][sink // 16], sink % 16
+        st.k[0, block, slot, :, 0], st.v[0, block, slot] = 8.875, 0.0
+    st.v.abs_()
+    st.nv.abs_()
+    got = st.run()
+    (rows, want, size), = definition(st)
+    eps = torch.finfo(dtype).eps
+    # a weight: half a step; scores exact but for roundings of 26 log2 units to 32 bits, in the product, the sum with the
+    # maximum and the exponential (3 * 26 * 2^-24 < 2^-17); sums of 32,020 terms in 32 bits
+    rel = (eps / 2 if eps > 1e-6 else 0.0) + 2.0 ** -17 + 32020 * 2.0 ** -24
+    tol = eps / 2 * want.abs() + 1.01 * rel * size + 32020 * 2.0 ** -35 * float(st.v.max()) + 2.0 ** -25
+    err = (got[0, :, rows].double().cpu() - want).abs()
+    assert (err <= tol).all(), (float(err.max()), float(tol.min()), float(want.mean()))
