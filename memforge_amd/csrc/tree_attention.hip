@@ -49,6 +49,7 @@ constexpr int kTreeThreads = 256;
 constexpr int kTile = 32;            // keys
 constexpr int kMaxSeqs = 4096;
 constexpr int kWindow = 1024;        // block-table entries held in LDS
+constexpr int kMaxWild = 1 + MF_TREE_MAX_NODES / kTile;  // a context's last tile, and the nodes' tiles
 constexpr int kSeqInts = 8;          // context, nodes, first row, tiles, column groups, context tiles, -, -
 constexpr int kWorkInts = 16;        // a worker's first sequence, kv head, first tile, tiles, the sequence's six, column group
 
@@ -302,6 +303,24 @@ __device__ __forceinline__ float both_halves_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// Infinities and NaN are the elements whose exponent is all ones.
+template <int DT>
+__device__ __forceinline__ bool not_finite(uint32_t element) {
+    constexpr uint32_t inf = DT == MF_F32 ? 0x7f800000u : DT == MF_BF16 ? 0x7f80u : 0x7c00u;
+    return (element & inf) == inf;
+}
+// 0 in their place, in an element or in a pair.
+template <int DT>
+__device__ __forceinline__ uint32_t finite_of(uint32_t x) {
+    if constexpr (DT == MF_F32) return not_finite<DT>(x) ? 0u : x;
+    else return (not_finite<DT>(x & 0xffffu) ? 0u : x & 0xffffu) | (not_finite<DT>(x >> 16) ? 0u : x & 0xffff0000u);
+}
+// Adds an element to a sum if it is not finite.
+template <int DT>
+__device__ __forceinline__ float with(float sum, uint32_t element) {
+    return not_finite<DT>(element) ? sum + bits_to_f32<DT>(element) : sum;
+}
+
 template <int DT, int D, int WC, int WK>
 __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * WC * WK / 4)) void tree_kernel(TreeArgs a) {
     using S = TreeShape<DT, D, WC, WK>;
@@ -310,6 +329,9 @@ __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * W
     constexpr float kNegInf = -__builtin_huge_valf();
     __shared__ __align__(1024) char ring[S::RING * S::STG];
     __shared__ int tab[kWindow];
+    // Rows of the tiles that not all columns see whole (the context's last, and the nodes') whose V is not all
+    // finite: a word of 32 rows for each tile, then whether there are any.
+    __shared__ uint32_t wild[kMaxWild + 1];
     static_assert(WK == 1 || (WK - 1) * WC * (ND * 16 + 2) * 256 <= S::RING * S::STG, "the key waves' sums fit the ring");
 
     const int32_t* at = a.work + (int64_t)blockIdx.x * kWorkInts;
@@ -369,7 +391,9 @@ __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * W
                 for (int i = window + tid; i < end; i += S::WAVES * 64) tab[i - window] = trow[i];
             };
             fill_window(tile0 * kTile);
+            if (tid <= kMaxWild) wild[tid] = 0;
             sync();
+            const int part_seen = ctx / kTile;  // the first of those tiles
 
             int f_tile = tile0, f_left = run;
             int in_flight = 0, head_buf = 0, next_buf = 0;
@@ -541,6 +565,24 @@ __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * W
                     --in_flight;
                     sync();  // the oldest stage is whole, and the one before it has been read
                     if (f_left > 0) fetch();
+                    if (st0 + ST > part_seen) {
+                        // the product below gives a column 0 times the rows it does not see, which would be NaN for
+                        // an infinity: there the rows hold 0 instead, and who sees them gets it at the end
+                        char* v = ring + head_buf * S::STG + S::HALF + wave * 1024 + lane * 16;
+#pragma unroll
+                        for (int i = 0; i < S::PAIRS; ++i) {
+                            uint4* at_v = (uint4*)(v + i * S::WAVES * 1024);
+                            const uint4 x = *at_v;
+                            const uint4 y = make_uint4(finite_of<DT>(x.x), finite_of<DT>(x.y), finite_of<DT>(x.z), finite_of<DT>(x.w));
+                            const int t = st0 + (row_of(i) >> 5);
+                            if (((x.x ^ y.x) | (x.y ^ y.y) | (x.z ^ y.z) | (x.w ^ y.w)) != 0 && t >= part_seen && t < t1) {
+                                *at_v = y;
+                                atomicOr(&wild[t - part_seen], 1u << (row_of(i) & 31));
+                                wild[kMaxWild] = 1;
+                            }
+                        }
+                        sync();
+                    }
                     if (busy) {
                         const char* stg = ring + head_buf * S::STG;
 #pragma unroll 1
@@ -587,6 +629,45 @@ __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * W
                                     acc[d][i + 1] = acc[d][i + 1] * w0 + v.y * w1;
                                     acc[d][i + 2] = acc[d][i + 2] * w0 + v.z * w1;
                                     acc[d][i + 3] = acc[d][i + 3] * w0 + v.w * w1;
+                                }
+                        }
+                    }
+                }
+                if (wild[kMaxWild] != 0 && wk == 0 && busy) {
+                    for (int t = max(t0, part_seen); t < t1; ++t) {
+                        uint32_t rows = __builtin_amdgcn_readfirstlane(wild[t - part_seen]);
+                        const uint32_t seen = !valid ? 0u : t >= held ? a.masks[prow * a.mask_words + (t - held)]
+                                                                      : 0xffffffffu >> ((t + 1) * kTile - ctx);
+                        for (; rows != 0; rows &= rows - 1) {
+                            const int r = __builtin_ctz(rows), key = t * kTile + r;
+                            if (!(seen >> r & 1u)) continue;
+                            const char* src;
+                            if (t < held) {
+                                const int blk = block_of(key);
+                                const uint32_t e = min((uint32_t)trow[blk], a.num_blocks - 1);
+                                src = a.v_pool + ((int64_t)e * a.p_sb + (int64_t)(key - blk * a.block_size) * a.p_ss +
+                                                  (int64_t)h * a.p_sh) * ES;
+                            } else {
+                                src = a.new_v + ((int64_t)(row0 + (key - held * kTile)) * a.n_sr + (int64_t)h * a.n_sh) * ES;
+                            }
+#pragma unroll
+                            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                                for (int b = 0; b < 4; ++b) {
+                                    const char* piece = src + (32 * d + 8 * b + 4 * hf) * ES;
+                                    if constexpr (DT == MF_F32) {
+                                        const uint4 x = *(const uint4*)piece;
+                                        acc[d][4 * b] = with<DT>(acc[d][4 * b], x.x);
+                                        acc[d][4 * b + 1] = with<DT>(acc[d][4 * b + 1], x.y);
+                                        acc[d][4 * b + 2] = with<DT>(acc[d][4 * b + 2], x.z);
+                                        acc[d][4 * b + 3] = with<DT>(acc[d][4 * b + 3], x.w);
+                                    } else {
+                                        const uint2 x = *(const uint2*)piece;
+                                        acc[d][4 * b] = with<DT>(acc[d][4 * b], x.x & 0xffffu);
+                                        acc[d][4 * b + 1] = with<DT>(acc[d][4 * b + 1], x.x >> 16);
+                                        acc[d][4 * b + 2] = with<DT>(acc[d][4 * b + 2], x.y & 0xffffu);
+                                        acc[d][4 * b + 3] = with<DT>(acc[d][4 * b + 3], x.y >> 16);
+                                    }
                                 }
                         }
                     }

@@ -44,9 +44,8 @@ def paged_attention_tree(query: torch.Tensor, key_pool: torch.Tensor, value_pool
     (B, width) on the device, a row for each sequence of the plan, wide enough for its
     ``max_context``; ``new_keys`` / ``new_values`` ``(1, kv_heads, rows, head_dim)`` the
     nodes' own. fp32, fp16 or bf16 throughout, head_dim 32, 64, 128 or 256. Rows that
-    belong to no tree are not computed and hold anything. A value that is not finite
-    reaches the nodes of its tree that do not see it too, as zero times it does in a
-    product."""
+    belong to no tree are not computed and hold anything. An infinity or NaN in a row
+    reaches the nodes that see it and no others."""
     nat.require_device(query, key_pool, new_keys, new_values)
     shape, stride = key_pool.shape, key_pool.stride()
     if len(shape) != 5 or shape != value_pool.shape or stride != value_pool.stride() or key_pool.dtype is not value_pool.dtype \
