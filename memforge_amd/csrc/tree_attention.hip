@@ -254,9 +254,10 @@ struct TreeShape {
     // 2^SLACK, and UP cancels in out = sum w v / sum w. fp16 keeps weights for the second product in
     // steps of 2^-24 at the least, which are then 2^-34 of the largest: all rounded off together are
     // at most keys * 2^-35 of the sum. (With UP 0 the tail of 32,001 keys could lose 2^-10 of
-    // it.) 2^13 at the most leave a factor 8 to the type's largest number.
+    // it.) The price is a maximum that moves more often: the second case above 117.8 us a call with
+    // SLACK 8 and UP 0, 120.8 so, 123.5 with SLACK 3.
     static constexpr float UP = DT == MF_F16 ? 10.f : 0.f;
-    static constexpr float SLACK = DT == MF_F16 ? 3.f : kLazyLog2;
+    static constexpr float SLACK = DT == MF_F16 ? 5.f : kLazyLog2;
     static constexpr int COLS = WC * 32;
     static constexpr int SLOT = COLS * (D + 2);            // floats of a piece's sums
     static_assert(PAIRS >= 1 && HALF % (1024 * WAVES) == 0, "whole pieces for every wave");
@@ -510,7 +511,10 @@ __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * W
                     for (int i = 1; i < 16; ++i) lmax = fmax_prop(lmax, st[i]);
                     if (__builtin_amdgcn_ballot_w64(lmax > thr) != 0) {
                         auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(lmax), __float_as_uint(lmax), false, false);
-                        const float mn = fmaxf(m, fmax_prop(__uint_as_float(r[0]), __uint_as_float(r[1])) * a.scale_log2);
+                        float mn = fmax_prop(__uint_as_float(r[0]), __uint_as_float(r[1])) * a.scale_log2;
+                        // fp16's weights end at 2^16: roundings of scores of any size (here, and four in thr) go the other way
+                        if constexpr (DT == MF_F16) mn += fabsf(mn) * 0x1p-23f;
+                        mn = fmaxf(m, mn);
                         const float alpha = __builtin_amdgcn_exp2f(m - mn);
                         l *= alpha;
 #pragma unroll
@@ -518,7 +522,7 @@ __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * W
 #pragma unroll
                             for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
                         m = mn;
-                        thr = (mn + S::SLACK) * a.inv_scale_log2;
+                        thr = (mn + S::SLACK - (DT == MF_F16 ? fabsf(mn) * 0x1p-21f : 0.f)) * a.inv_scale_log2;
                     }
                     float sum = 0.f;
                     const float zero = DT == MF_F16 ? S::UP - m : -m;
@@ -537,7 +541,7 @@ __global__ __launch_bounds__(WC * WK * 64, (TreeShape<DT, D, WC, WK>::PER_CU * W
                                                     acc[d]);
                     } else {
                         // 16-bit operands of the second product: each weight off by half a step of the type (fp16's
-                        // smallest weights by half of its least step, see UP)
+                        // smallest weights by half of its least step, see UP; its largest are 2^15)
                         uint32_t pw[8];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {

@@ -42,3 +42,15 @@ def test_a_flat_tail_far_below_one_key(device, dtype, d, nodes, sink):
     tol = eps / 2 * want.abs() + 1.01 * rel * size + 32020 * 2.0 ** -35 * float(st.v.max()) + 2.0 ** -25
     err = (got[0, :, rows].double().cpu() - want).abs()
     assert (err <= tol).all(), (float(err.max()), float(tol.min()), float(want.mean()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_scores_of_millions(device, dtype):
+    """Where scores' 32-bit roundings are several log2 units the weights are what they are, but finite: an average of the
+    values, all of them the same."""
+    st = Trees(device, dtype, 4, 2, 64, 16, [3000], [20], seed=2, scale=1000.0)
+    st.q.mul_(64)
+    st.k.mul_(32)
+    st.v.fill_(1.5)
+    st.nv.fill_(1.5)
+    assert torch.isclose(st.run().float(), torch.tensor(1.5, device=device), rtol=2.0 ** -7).all()
