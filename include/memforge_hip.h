@@ -603,7 +603,7 @@ int mf_spec_verify(int num_rows, int num_draft, int vocab,
  * mf_tables_truncate cuts request s back to min(lens[s], lengths[s]) tokens
  * (negative: 0) and gives back the blocks it then does not need, in an order
  * that makes the stack after an extend what it was before; their table entries
- * become 0.
+ * become 0. A block belongs to one request: one in two tables would be given back twice.
  *
  * arrivals: one uint32 that is 0 before the call and after it. Both are one
  * launch (extend with `rows`: two), at most 4096 requests.

@@ -22,8 +22,8 @@ from memforge_amd import _native as nat
 class SlotMap:
     """Where a call's new tokens go: ``slot_mapping`` and ``positions`` (int64, one per
     row; slot -1 writes nothing), ``cu_seqlens`` (int32, each request's first row),
-    ``kv_lens`` (int32, the requests' lengths now) and ``refused`` (int32 of one, how
-    many requests could not grow)."""
+    ``kv_lens`` (int32, the requests' lengths now: as before where a request was refused)
+    and ``refused`` (int32 of one, how many could not grow)."""
 
     slot_mapping: torch.Tensor
     positions: torch.Tensor
@@ -110,7 +110,8 @@ class DeviceBlockTables:
     def truncate(self, lengths: torch.Tensor) -> None:
         """Cut request s back to ``min(lens[s], lengths[s])`` tokens (int32, on the device;
         negative as 0) and give back the blocks that it then does not need: all of a
-        finished request's with 0. Their table entries become 0. After ``extend`` and
+        finished request's with 0. A block belongs to one request; one that stood in two tables
+        would be given back twice. Their table entries become 0. After ``extend`` and
         ``truncate`` to the lengths before, tables and stack are as they were."""
         dev, n, state = self._state("lengths", lengths)
         nat._launch(dev, "mf_tables_truncate", nat.lib().mf_tables_truncate, *state,

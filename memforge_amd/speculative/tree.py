@@ -38,5 +38,6 @@ def accept_tree(tokens: torch.Tensor, targets: torch.Tensor, parents: torch.Tens
     (int64). Node 0 is the sequence's newest token; of several children with the drawn
     token the first counts. ``max_nodes``: at least the largest tree's nodes (further
     ones are ignored), at most 1024. ``path`` and ``count`` are what
-    ``DeviceBlockTables.extend`` takes to place the accepted rows."""
+    ``DeviceBlockTables.extend`` takes to place the accepted rows; a request that it refuses has
+    no place for them, and its tokens of this round do not count."""
     return AcceptedPath(*nat.tree_accept(tokens, targets, parents, cu_nodes, max_nodes))
