@@ -54,3 +54,45 @@ def test_scores_of_millions(device, dtype):
     st.v.fill_(1.5)
     st.nv.fill_(1.5)
     assert torch.isclose(st.run().float(), torch.tensor(1.5, device=device), rtol=2.0 ** -7).all()
+
+
+def norm_error(st, out):
+    """The largest error of a head's output (all of its rows) relative to its norm."""
+    worst = 0.0
+    for rows, want, _ in definition(st):
+        err = (out[0, :, rows].double().cpu() - want).flatten(1).norm(dim=1) / want.flatten(1).norm(dim=1)
+        worst = max(worst, float(err.max()))
+    return worst
+
+
+def norm_bound(st):
+    """Roundings are of either sign and add up as a random walk does. The result and the 16-bit weights: each at most half
+    a step, eps / (2 sqrt 3) of the norm in the mean square, so sqrt(2 / 3) < 1 times eps / 2 together. In 32 bits: sums over
+    n keys in numerator and denominator, sqrt(n) 2^-24 each, and scores of a few units, 8 * 2^-24."""
+    eps = torch.finfo(st.dtype).eps
+    n = max(st.ctx) + max(st.nodes)
+    return (eps / 2 if eps > 1e-6 else 0.0) + (8 + 2 * math.sqrt(n)) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("hq,hkv,d", [(15, 5, 64), (40, 8, 128), (8, 8, 32), (6, 1, 256)])
+@pytest.mark.parametrize("ctx,nodes", [([33, 0, 700], [8, 8, 8]), ([200, 1500], [64, 20]), ([9001], [3]), ([40, 90], [70, 129])])
+def test_errors_in_the_norm(device, dtype, hq, hkv, d, ctx, nodes):
+    st = Trees(device, dtype, hq, hkv, d, 16, ctx, nodes, seed=sum(ctx) + d)
+    assert norm_error(st, st.run()) <= norm_bound(st)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_errors_in_the_norm_of_a_long_context(device, dtype):
+    st = Trees(device, dtype, 4, 1, 128, 16, [30001], [17], seed=3)
+    assert norm_error(st, st.run()) <= norm_bound(st)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("bs,ctx", [(3, 4000), (3, 9100), (7, 9000), (5, 5121), (6, 6144), (48, 50000)])
+def test_long_tables_of_odd_blocks(device, dtype, bs, ctx):
+    """More than 1,024 blocks of a size that is no power of two."""
+    st = Trees(device, dtype, 4, 2, 64, bs, [ctx, 10], [9, 3], seed=bs)
+    out = st.run()
+    st.check(out)
+    assert norm_error(st, out) <= norm_bound(st)
