@@ -18,9 +18,9 @@
 // for 358 in the first case below, 145 for 133 in the second).
 //
 // Bound. Two layers with their plan, by graph replay on an MI355X: 64 contexts (median
-// 2,048, 16 nodes each, bf16, 40/8 heads of 128) 358 us, 327 with loads and merges
+// 2,048, 16 nodes each, bf16, 40/8 heads of 128) 360 us, 327 with loads and merges
 // alone; their keys and values at the 4.9 TB/s of a large copy take 304. One context
-// of 32,001 under 48 nodes (fp16, the same heads) 133 us, 93 without the products and
+// of 32,001 under 48 nodes (fp16, the same heads) 132 us, 93 without the products and
 // 123 without the loads, floor 54: 240 columns a kv head, whose chain of product,
 // softmax, product the two waves of a SIMD do not hide from each other.
 //
